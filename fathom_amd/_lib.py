@@ -11,7 +11,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libfathom_hip.so")
 
 OK, ERR_INVALID, ERR_HIP, ERR_ALLOC, ERR_WORKSPACE = 0, 1, 2, 3, 4
-DT_F32, DT_F16, DT_BF16 = 0, 1, 2
+DT_F32, DT_F16, DT_BF16, DT_E4M3, DT_I8 = 0, 1, 2, 3, 4
 
 _vp, _i32, _i64, _sz = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_size_t
 
@@ -59,6 +59,15 @@ PROTOTYPES = {
     "fathom_gather_attention_workspace_bytes": (_sz, [_i64, _i64, _i64]),
     "fathom_gather_attention": (_i32, [_vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _i64, _vp, _vp, _i64,
                                        ctypes.c_float, _vp, _vp, _vp, _sz, _vp]),
+    "fathom_rows8_write": (_i32, [_vp, _vp, _i32, _i64, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _i64, _i64, _i32, _vp,
+                                  _vp, _vp, _vp, _vp]),
+    "fathom_rows8_read": (_i32, [_vp, _vp, _vp, _vp, _i32, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _i32, _vp, _vp, _vp]),
+    "fathom_rows8_attention_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64]),
+    "fathom_rows8_attention": (_i32, [_vp, _i32, _vp, _vp, _vp, _vp, _i32, _i64, _i64, _i64, _i64, _vp, _i64, _i64,
+                                      ctypes.c_float, ctypes.c_float, _vp, _vp, _vp, _sz, _vp]),
+    "fathom_rows8_gather_attention_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64]),
+    "fathom_rows8_gather_attention": (_i32, [_vp, _i32, _vp, _vp, _vp, _vp, _vp, _i32, _i64, _i64, _i64, _i64, _i64, _vp,
+                                             _i64, ctypes.c_float, ctypes.c_float, _vp, _vp, _vp, _sz, _vp]),
     "fathom_gather_runs": (_i32, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp]),
     "fathom_copy_index": (_i32, [_vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp]),
     "fathom_copy_index_range": (_i32, [_vp, _i64, _i64, _i64, _i64, _i64, _i64, _i32, _vp, _vp, _vp, _vp, _vp]),

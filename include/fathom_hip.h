@@ -40,6 +40,9 @@ extern "C" {
 #define FATHOM_DT_F32 0
 #define FATHOM_DT_F16 1
 #define FATHOM_DT_BF16 2
+/* code types of the 8-bit row store (fathom_rows8_*) */
+#define FATHOM_DT_E4M3 3 /* OCP float8 e4m3: no infinity, largest 448 */
+#define FATHOM_DT_I8 4   /* -127 .. 127 */
 
 /* Library version string and last error text (per calling thread). */
 const char *fathom_version(void);
@@ -346,6 +349,75 @@ int fathom_gather_attention(const float *q, const int64_t *idx, int64_t BH, int6
                             const void *Ksrc, const void *Vsrc, int64_t cap, const void *Krec, const void *Vrec,
                             int64_t nrec, float scale, float *out, int32_t *n_unique, void *workspace,
                             size_t workspace_bytes, void *stream);
+
+/*
+ * The 8-bit K/V row store (fathom_rows8_*).  It has no counterpart in the
+ * reference.  Per (batch, KV head) row, for K and V apart: codes k8, v8
+ * [BH, cap, D] of one byte (code_dtype FATHOM_DT_E4M3 or FATHOM_DT_I8) and
+ * scales k_scale, v_scale [BH, ceil(cap / 64)] float32, one per 64-token block;
+ * value = code * scale.  D = 64 or 128; codes 16-byte aligned; BH <= 65535.
+ */
+
+/*
+ * Quantise rows K, V (element (bh, t, d) at bh * row_stride + t * tok_stride + d,
+ * of dtype FATHOM_DT_F32/F16/BF16; base and strides multiples of 16 bytes) into
+ * tokens [p, p + T) of the store, p = pos[bh] (int32, device) or pos_value where
+ * pos is NULL.  A block whose first token is written gets the scale
+ * max(largest finite |x| / 448 or 127, 2^-100); one that holds earlier tokens
+ * keeps its scale, or takes the least power-of-two multiple of it that holds the
+ * new tokens, and its earlier codes are rounded to that.  (An earlier scale that
+ * is no positive finite number counts as none, and the earlier codes stay.)
+ * Codes are the nearest to x * (1 / scale), ties to even; infinities saturate;
+ * NaN is stored as NaN in e4m3 and as 0 in int8.  Tokens behind p + T keep their
+ * codes, though not the values of those in the last written block.  A row of
+ * `pos` whose tokens do not all fit into [0, cap) is left as it is.
+ */
+int fathom_rows8_write(const void *K, const void *V, int dtype, int64_t k_row_stride, int64_t k_tok_stride,
+                       int64_t v_row_stride, int64_t v_tok_stride, const int32_t *pos, int64_t pos_value, int64_t BH,
+                       int64_t T, int64_t D, int64_t cap, int code_dtype, void *k8, void *v8, float *k_scale,
+                       float *v_scale, void *stream);
+
+/*
+ * Values of R tokens per row, K, V [BH, R, D] of dtype (16-byte aligned): token
+ * idx[bh, r] (int64, device) where idx is given, else pos[bh] + r (int32,
+ * device), or pos_value + r where pos is NULL too.  Tokens outside [0, cap) give
+ * zero rows.
+ */
+int fathom_rows8_read(const void *k8, const void *v8, const float *k_scale, const float *v_scale, int code_dtype, int64_t BH,
+                      int64_t cap, int64_t D, const int64_t *idx, const int32_t *pos, int64_t pos_value, int64_t R,
+                      int dtype, void *K, void *V, void *stream);
+
+/*
+ * Attention of one token per row over the store: with len = lens[bh] (int32,
+ * device, taken as within [0, cap]) or n where lens is NULL, over tokens
+ * [max(0, len - window), len) (window 0: all),
+ *   z_t = softcap * tanh(u_t / softcap) + slopes[bh, g] * (t - (len - 1)),
+ *   u_t = scale * q[bh, g] . K_t;   out[bh, g] = softmax(z) . V
+ * without the cap for softcap = 0 and without the bias for slopes = NULL.  q
+ * [BH, G, D] of q_dtype (FATHOM_DT_F32/F16/BF16, 16-byte aligned), out
+ * [BH, G, D] float32.  A row without tokens gives zeros.
+ * workspace: fathom_rows8_attention_workspace_bytes(BH, G, D, positions) bytes,
+ * positions = the smaller of the longest length the host knows (n, or cap where
+ * lens is given) and, if not 0, the window.
+ */
+size_t fathom_rows8_attention_workspace_bytes(int64_t BH, int64_t G, int64_t D, int64_t positions);
+int fathom_rows8_attention(const void *q, int q_dtype, const void *k8, const void *v8, const float *k_scale,
+                           const float *v_scale, int code_dtype, int64_t BH, int64_t G, int64_t D, int64_t cap,
+                           const int32_t *lens, int64_t n, int64_t window, float scale, float softcap,
+                           const float *slopes, float *out, void *workspace, size_t workspace_bytes, void *stream);
+
+/*
+ * The same attention over listed tokens, t = idx[bh, g, j] for j < k (int64,
+ * device; a token listed twice counts twice).  Tokens outside [0, len) take no
+ * part (fathom_gather_attention's zero rows score 0 instead).
+ * workspace: fathom_rows8_gather_attention_workspace_bytes(BH, G, D, k) bytes.
+ */
+size_t fathom_rows8_gather_attention_workspace_bytes(int64_t BH, int64_t G, int64_t D, int64_t k);
+int fathom_rows8_gather_attention(const void *q, int q_dtype, const int64_t *idx, const void *k8, const void *v8,
+                                  const float *k_scale, const float *v_scale, int code_dtype, int64_t BH, int64_t G,
+                                  int64_t k, int64_t D, int64_t cap, const int32_t *lens, int64_t n, float scale,
+                                  float softcap, const float *slopes, float *out, void *workspace,
+                                  size_t workspace_bytes, void *stream);
 
 /*
  * One chunk of the chunked copy/scan pipeline (scripts/B_e2e_offload_v2.py:

@@ -14,7 +14,9 @@ namespace rows8 {
 namespace {
 
 constexpr int kWaves = 4;  // of a workgroup
-constexpr int kTile = 32;  // positions of a wave at a time
+constexpr int kTile = 32;  // listed positions of a wave at a time
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLowest = -3.0e38f;  // below every score: the running maximum of no token
 
 struct AttnArgs {
   const void *q;
@@ -38,21 +40,21 @@ __device__ __forceinline__ float load_q(const void *q, int dt, int64_t i) {
                                : load_elem<FATHOM_DT_BF16>(q, i);
 }
 
-// Adds (m1, l1, o1) to the running (m, l, o) of a softmax.
+// Adds (m1, l1, o1) to the running (m, l, o) of a softmax (maxima in log2 units).
 template <int N>
 __device__ __forceinline__ void join(float &m, float &l, float (&o)[N], float m1, float l1, const float (&o1)[N]) {
   const float M = fmaxf(m, m1);
-  const float f = m == -INFINITY ? 0.0f : expf(m - M), f1 = m1 == -INFINITY ? 0.0f : expf(m1 - M);
+  const float f = __builtin_amdgcn_exp2f(m - M), f1 = __builtin_amdgcn_exp2f(m1 - M);
   l = l * f + l1 * f1;
 #pragma unroll
   for (int e = 0; e < N; ++e) o[e] = o[e] * f + o1[e] * f1;
   m = M;
 }
 
-// One workgroup per (split, query head, row); its waves take tiles of 32
-// positions in turn.  16 channels of a row per lane.
-template <int D, bool I8, bool LIST>
-__global__ __launch_bounds__(kWaves *kWave) void attn_kernel(AttnArgs a) {
+// Attention over listed tokens: one workgroup per (split, query head, row); its
+// waves take tiles of 32 positions in turn.  16 channels of a row per lane.
+template <int D, bool I8>
+__global__ __launch_bounds__(kWaves *kWave) void list_kernel(AttnArgs a) {
   constexpr int kLanes = D / 16;         // lanes of a row
   constexpr int kRows = kWave / kLanes;  // rows of a load
   constexpr int kLoads = kTile / kRows;
@@ -61,13 +63,12 @@ __global__ __launch_bounds__(kWaves *kWave) void attn_kernel(AttnArgs a) {
   const int64_t s = blockIdx.x, g = blockIdx.y, bh = blockIdx.z;
   const int d0 = 16 * (lane % kLanes), rg = lane / kLanes;
   const int64_t len = row_length(a.lens, a.n, a.cap, bh);
-  const int64_t lo = !LIST && a.window > 0 && len > a.window ? len - a.window : 0;
-  const int64_t count = LIST ? a.k : len - lo;
-  const float slope = a.slopes ? a.slopes[bh * a.G + g] : 0.0f;
+  const int64_t count = a.k;
+  const float slope = a.slopes ? a.slopes[bh * a.G + g] * kLog2e : 0.0f;
   float q[16];
 #pragma unroll
   for (int e = 0; e < 16; ++e) q[e] = load_q(a.q, a.q_dtype, (bh * a.G + g) * D + d0 + e);
-  float m = -INFINITY, l = 0.0f, o[16];
+  float m = kLowest, l = 0.0f, o[16];
 #pragma unroll
   for (int e = 0; e < 16; ++e) o[e] = 0.0f;
   for (int64_t t0 = (s * kWaves + wave) * kTile; t0 < count; t0 += a.nsplit * kWaves * kTile) {
@@ -78,7 +79,7 @@ __global__ __launch_bounds__(kWaves *kWave) void attn_kernel(AttnArgs a) {
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
       const int64_t j = t0 + i * kRows + rg;
-      tok[i] = j >= count ? -1 : LIST ? a.idx[(bh * a.G + g) * a.k + j] : lo + j;
+      tok[i] = j >= count ? -1 : a.idx[(bh * a.G + g) * a.k + j];
       in[i] = tok[i] >= 0 && tok[i] < len;
       kc[i] = vc[i] = make_uint4(0u, 0u, 0u, 0u);
       ks[i] = vs[i] = 0.0f;
@@ -106,17 +107,18 @@ __global__ __launch_bounds__(kWaves *kWave) void attn_kernel(AttnArgs a) {
       for (int x = 1; x < kLanes; x <<= 1) dot += __shfl_xor(dot, x);
       float u = dot * (ks[i] * a.scale);
       if (a.softcap > 0.0f) u = a.softcap * tanhf(u / a.softcap);
+      u *= kLog2e;
       z[i] = in[i] ? fmaf(slope, (float)(tok[i] - (len - 1)), u) : -INFINITY;
       mt = fmaxf(mt, z[i]);
     }
-    const float f = m == -INFINITY ? 0.0f : expf(m - mt);
+    const float f = __builtin_amdgcn_exp2f(m - mt);
     l *= f;
 #pragma unroll
     for (int e = 0; e < 16; ++e) o[e] *= f;
     m = mt;
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
-      const float p = z[i] == -INFINITY ? 0.0f : expf(z[i] - m);
+      const float p = __builtin_amdgcn_exp2f(z[i] - m);
       l += p;
       const float pv = p * vs[i];
       const uint32_t w[4] = {vc[i].x, vc[i].y, vc[i].z, vc[i].w};
@@ -166,12 +168,354 @@ __global__ __launch_bounds__(kWaves *kWave) void attn_kernel(AttnArgs a) {
   }
 }
 
+// Sum or maximum over the four lanes l, l ^ 16, l ^ 32, l ^ 48 (v_permlane32_swap
+// and v_permlane16_swap give each lane its partner's value).
+template <bool MAX>
+__device__ __forceinline__ float across_groups(float v) {
+  auto op = [](float x, float y) { return MAX ? fmaxf(x, y) : x + y; };
+  const uint32_t x = __float_as_uint(v);
+  const auto p32 = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+  v = op(__uint_as_float(p32[0]), __uint_as_float(p32[1]));
+  const uint32_t y = __float_as_uint(v);
+  const auto p16 = __builtin_amdgcn_permlane16_swap(y, y, false, false);
+  return op(__uint_as_float(p16[0]), __uint_as_float(p16[1]));
+}
+
+template <int N>
+struct VPiece {
+  typedef uint32_t type;
+};
+template <>
+struct VPiece<8> {
+  typedef unsigned int type __attribute__((ext_vector_type(2)));
+};
+__device__ __forceinline__ uint32_t dword_of(uint32_t v, int) { return v; }
+__device__ __forceinline__ uint32_t dword_of(VPiece<8>::type v, int d) { return v[d]; }
+
+// Block b of a row's codes through a buffer descriptor that holds its tokens
+// before `end`: loads behind that give zeros.
+struct RowsOf {
+  __amdgpu_buffer_rsrc_t rsrc;
+  __device__ __forceinline__ RowsOf(const uint8_t *codes, int64_t row0, int64_t b, int64_t end, int D) {
+    const int64_t left = end - b * kBlk;
+    const int tokens = left < 0 ? 0 : left < kBlk ? (int)left : kBlk;
+    rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(codes) + (row0 + (tokens ? b * kBlk : 0)) * D, 0, tokens * D,
+                                             0x00027000);
+  }
+  typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
+  typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+  __device__ __forceinline__ u32x4 load16(int off) const {
+    return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, off, 0, 0));
+  }
+  __device__ __forceinline__ void load(int off, u32x2 &v) const {
+    v = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rsrc, off, 0, 0));
+  }
+  __device__ __forceinline__ void load(int off, uint32_t &v) const { v = __builtin_amdgcn_raw_buffer_load_b32(rsrc, off, 0, 0); }
+};
+
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+
+
+// Bytes 0, 1 (HI: 2, 3) of a dword of codes as two f16 values (exact: e4m3 and
+// int8 both fit f16).  int8 codes come with their sign bit flipped (flip_sign),
+// as c + 128 in 0 .. 255: under the exponent byte 0x64 that is the f16 number
+// 1024 + (c + 128).
+template <bool I8>
+__device__ __forceinline__ uint32_t flip_sign(uint32_t w) {
+  return I8 ? w ^ 0x80808080u : w;
+}
+template <bool I8, bool HI>
+__device__ __forceinline__ f16x2 pair16(uint32_t w) {
+  if constexpr (I8) {
+    const uint32_t h = __builtin_amdgcn_perm(0x64646464u, w, HI ? 0x04030402u : 0x04010400u);
+    const f16x2 b = {(_Float16)-1152.0f, (_Float16)-1152.0f};
+    return __builtin_bit_cast(f16x2, h) + b;
+  } else {
+    return __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)w, 1.0f, HI));
+  }
+}
+__device__ __forceinline__ f16x8 join8(f16x2 a, f16x2 b, f16x2 c, f16x2 d) {
+  return f16x8{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
+}
+
+// v + the value of the lane 8 columns away in the same row of 16 lanes (row_ror:8).
+__device__ __forceinline__ float add_other_half(float v) {
+  return v + __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x128, 0xF, 0xF, false));
+}
+
+// Attention over every token of [lo, len): flash decoding on the matrix cores.
+//
+// A workgroup takes one split of a row for a group of 8 NG query heads; its waves
+// take the split's 64-token blocks in turn.  Per block (v_mfma_f32_16x16x32_f16,
+// lane l = column l & 15, group l >> 4):
+//   S^T = K q^T: A holds 16 tokens' codes as f16 (exact), straight from the
+//     16-byte pieces of the rows (the channel order inside the contraction is
+//     free, so it is the order that the pieces arrive in); B holds the queries,
+//     column c < 8 the f16 part of head c's q 2^sigma, column c + 8 the f16 of what
+//     that leaves: 22 bits of q, at no cost, as 8 heads fill half of the 16 columns.
+//     One row rotation adds the halves.
+//   softmax: a lane holds 16 scores of its head, tokens 16 i + 4 (l >> 4) + j; the
+//     running maximum m (in log2 units) is raised only in the blocks where some
+//     score passes it.
+//   O^T += V^T p^T: D^T's column layout of the scores is B's layout of the weights
+//     once the contraction's token order is (tile, j), so the weights never leave their lane.
+//     Columns c < 8 hold the f16 of w = p s_V 2^(14 - E), columns c + 8 the f16 of
+//     the rest (22 bits of p); E is the running largest exponent of s_V, so w < 2^15.
+//     A holds V's codes, transposed inside the lane: it reads 8 (D = 64: 4) channels of 8
+//     tokens and pairs two tokens' bytes with one v_perm.
+// Rows are read through buffer descriptors that end at the row's length: what lies
+// behind it reads as zeros.
+//
+// Bound: HBM, 2 D bytes per token; the next block's K rows are requested once
+// the scores are formed, its V rows once the products are.
+template <int D, bool I8, int NG, bool EXTRA>
+__global__ __launch_bounds__(kWaves *kWave, NG == 1 ? 2 : 1) void dense_kernel(AttnArgs a) {
+  constexpr int kHalves = D / 64;  // 16-byte pieces of a row per lane
+  constexpr int kSteps = D / 32;   // matrix instructions along the channels
+  constexpr int kCh = D / 16;      // channels of V per lane
+  __shared__ float wm[kWaves][8 * NG], wl[kWaves][8 * NG], wo[kWaves][8 * NG][D];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane & 15, grp = lane >> 4;
+  const int64_t split = blockIdx.x, g0 = (int64_t)blockIdx.y * 8 * NG, bh = blockIdx.z;
+  const int64_t len = row_length(a.lens, a.n, a.cap, bh);
+  const int64_t lo = a.window > 0 && len > a.window ? len - a.window : 0;
+  // the split's blocks
+  const int64_t blk0 = lo / kBlk, nb = cdiv(len, (int64_t)kBlk) - blk0, per = cdiv(nb, a.nsplit);
+  const int64_t first = blk0 + split * per, last = first + per < blk0 + nb ? first + per : blk0 + nb;
+
+  f16x8 qf[NG][kSteps];
+  float fac[NG], slope[NG];  // per lane: its head's factor of a score, its bias per token
+#pragma unroll
+  for (int n = 0; n < NG; ++n) {
+    const int64_t g = g0 + 8 * n + (col & 7);
+    const bool has = g < a.G;
+    const int64_t row = (bh * a.G + (has ? g : a.G - 1)) * D;
+    float q[kSteps][8], mx = 0.0f;
+#pragma unroll
+    for (int h = 0; h < kSteps; ++h)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        // step h = (piece, half): channels 64 (h / 2) + 16 grp + 8 (h & 1) + e
+        q[h][e] = load_q(a.q, a.q_dtype, row + 64 * (h / 2) + 16 * grp + 8 * (h & 1) + e);
+        mx = fmaxf(mx, fabsf(q[h][e]));
+      }
+    mx = across_groups<true>(mx);
+    int sigma = 0;  // the largest |q| of the head in [2^13, 2^14)
+    if (mx > 0.0f && mx < INFINITY) {
+      frexpf(mx, &sigma);
+      sigma = 14 - sigma;
+    }
+#pragma unroll
+    for (int h = 0; h < kSteps; ++h)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float x = ldexpf(q[h][e], sigma);
+        const _Float16 hi = (_Float16)x;
+        qf[n][h][e] = col < 8 ? hi : (_Float16)(x - (float)hi);
+      }
+    fac[n] = ldexpf(EXTRA && a.softcap > 0.0f ? a.scale / a.softcap : a.scale * kLog2e, -sigma);
+    slope[n] = EXTRA && a.slopes && has ? a.slopes[bh * a.G + g] * kLog2e : 0.0f;
+  }
+  const float keep = col < 8 ? 0.0f : -1.0f;  // columns 8 .. 15 hold what the f16 weights leave
+
+  f32x4 o[NG][kCh];
+  float m[NG], l[NG];
+#pragma unroll
+  for (int n = 0; n < NG; ++n) {
+    m[n] = kLowest;
+    l[n] = 0.0f;
+#pragma unroll
+    for (int e = 0; e < kCh; ++e) o[n][e] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+  int E = -1000;
+
+  u32x4 kr[4][kHalves];
+  typedef typename VPiece<kCh>::type vpiece;
+  vpiece vr[4][4];
+  const int koff = col * D + 16 * grp, voff = 4 * grp * D + kCh * col;
+  auto load_k = [&](int64_t b) {
+    const RowsOf r(a.k8, bh * a.cap, b, b < last ? len : 0, D);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int h = 0; h < kHalves; ++h) kr[i][h] = r.load16(koff + 16 * i * D + 64 * h);
+  };
+  auto load_v = [&](int64_t b) {
+    const RowsOf r(a.v8, bh * a.cap, b, b < last ? len : 0, D);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) r.load(voff + (16 * i + j) * D, vr[i][j]);
+  };
+  load_k(first + wave);
+  load_v(first + wave);
+  for (int64_t b = first + wave; b < last; b += kWaves) {
+    const float ks = a.ks[bh * a.nblk + b], vs = a.vs[bh * a.nblk + b];
+    f32x4 s[NG][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+#pragma unroll
+      for (int n = 0; n < NG; ++n) s[n][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int h = 0; h < kSteps; ++h) {
+        const uint32_t w0 = flip_sign<I8>(kr[i][h / 2][2 * (h & 1)]), w1 = flip_sign<I8>(kr[i][h / 2][2 * (h & 1) + 1]);
+        const f16x8 k = join8(pair16<I8, false>(w0), pair16<I8, true>(w0), pair16<I8, false>(w1), pair16<I8, true>(w1));
+#pragma unroll
+        for (int n = 0; n < NG; ++n) s[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qf[n][h], s[n][i], 0, 0, 0);
+      }
+    }
+    load_k(b + kWaves);
+    // ---- scores, in log2 units; tokens outside [lo, len) have none
+    const int t0 = (int)(b * kBlk);
+    const bool edge = (int64_t)t0 < lo || (int64_t)t0 + kBlk > len;
+#pragma unroll
+    for (int n = 0; n < NG; ++n) {
+      const float f = fac[n] * ks;
+      float mx = kLowest;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float z = add_other_half(s[n][i][j]) * f;
+          if constexpr (EXTRA) {
+            if (a.softcap > 0.0f) z = a.softcap * kLog2e * tanhf(z);
+            z = fmaf(slope[n], (float)(t0 + 16 * i + 4 * grp + j - (int)(len - 1)), z);
+          }
+          if (edge) {
+            const int64_t t = t0 + 16 * i + 4 * grp + j;
+            z = t >= lo && t < len ? z : -INFINITY;
+          }
+          s[n][i][j] = z;
+          mx = fmaxf(mx, z);
+        }
+      if (__any(mx > m[n])) {
+        const float M = fmaxf(m[n], across_groups<true>(mx));
+        const float down = __builtin_amdgcn_exp2f(m[n] - M);
+        m[n] = M;
+        l[n] *= down;
+#pragma unroll
+        for (int e = 0; e < kCh; ++e) o[n][e] *= down;
+      }
+    }
+    const int ev = (int)((__float_as_uint(vs) >> 23) & 0xFF) - 127;
+    if (ev > E) {  // uniform: a larger scale of V than any before
+      const float down = ldexpf(1.0f, E - ev);
+      E = ev;
+#pragma unroll
+      for (int n = 0; n < NG; ++n)
+#pragma unroll
+        for (int e = 0; e < kCh; ++e) o[n][e] *= down;
+    }
+    const float wv = ldexpf(vs, 14 - E);
+    if (edge) {  // a token outside has no value either (its codes may be NaN)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (t0 + 16 * i + 4 * grp + j < lo) vr[i][j] = vpiece{};
+    }
+    // ---- weights and products, 32 tokens at a time
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      f16x8 p[NG];
+#pragma unroll
+      for (int n = 0; n < NG; ++n) {
+        f16x2 pp[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {  // tokens (tile 2 c + x / 2, j = 2 (x & 1), + 1)
+          const float p0 = __builtin_amdgcn_exp2f(s[n][2 * c + x / 2][2 * (x & 1)] - m[n]);
+          const float p1 = __builtin_amdgcn_exp2f(s[n][2 * c + x / 2][2 * (x & 1) + 1] - m[n]);
+          l[n] += p0 + p1;
+          const float w0 = p0 * wv, w1 = p1 * wv;
+          const f16x2 hi = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(w0, w1));
+          pp[x] = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(fmaf((float)hi.x, keep, w0), fmaf((float)hi.y, keep, w1)));
+        }
+        p[n] = join8(pp[0], pp[1], pp[2], pp[3]);
+      }
+#pragma unroll
+      for (int d = 0; d < kCh / 4; ++d) {  // dword d of the lane's channels
+        uint32_t w[2][4];
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) w[x][j] = flip_sign<I8>(dword_of(vr[2 * c + x][j], d));
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {  // channels 4 d + 2 y, + 1
+          uint32_t ab[2][2];
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+              ab[x][j] = __builtin_amdgcn_perm(w[x][2 * j + 1], w[x][2 * j], y ? 0x07030602u : 0x05010400u);
+          const f16x8 v0 = join8(pair16<I8, false>(ab[0][0]), pair16<I8, false>(ab[0][1]), pair16<I8, false>(ab[1][0]),
+                                 pair16<I8, false>(ab[1][1]));
+          const f16x8 v1 = join8(pair16<I8, true>(ab[0][0]), pair16<I8, true>(ab[0][1]), pair16<I8, true>(ab[1][0]),
+                                 pair16<I8, true>(ab[1][1]));
+#pragma unroll
+          for (int n = 0; n < NG; ++n) {
+            o[n][4 * d + 2 * y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, p[n], o[n][4 * d + 2 * y], 0, 0, 0);
+            o[n][4 * d + 2 * y + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, p[n], o[n][4 * d + 2 * y + 1], 0, 0, 0);
+          }
+        }
+      }
+    }
+    load_v(b + kWaves);
+  }
+  // ---- the workgroup's waves
+  const float up = E > -1000 ? ldexpf(1.0f, E - 14) : 0.0f;
+#pragma unroll
+  for (int n = 0; n < NG; ++n) {
+    const float L = across_groups<false>(l[n]);
+    if (lane < 8) {
+      wm[wave][8 * n + lane] = m[n];
+      wl[wave][8 * n + lane] = L;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int e = 0; e < kCh; ++e) {
+        const float v = add_other_half(o[n][e][j]) * up;
+        if (col < 8) wo[wave][8 * n + col][(4 * grp + j) * kCh + e] = v;
+      }
+  }
+  __syncthreads();
+  for (int x = tid; x < 8 * NG * D; x += kWaves * kWave) {
+    const int h = x / D, d = x % D;
+    if (g0 + h >= a.G) break;
+    float M = wm[0][h];
+#pragma unroll
+    for (int v = 1; v < kWaves; ++v) M = fmaxf(M, wm[v][h]);
+    float L = 0.0f, O = 0.0f;
+#pragma unroll
+    for (int v = 0; v < kWaves; ++v) {
+      const float e = __builtin_amdgcn_exp2f(wm[v][h] - M);
+      L = fmaf(wl[v][h], e, L);
+      O = fmaf(wo[v][h][d], e, O);
+    }
+    const int64_t r = bh * a.G + g0 + h;
+    if (a.nsplit == 1) {
+      a.out[r * D + d] = L == 0.0f ? 0.0f : O / L;
+    } else {
+      float *pb = a.part + (r * a.nsplit + split) * (D + 2);
+      pb[2 + d] = O;
+      if (d == 0) {
+        pb[0] = M;
+        pb[1] = L;
+      }
+    }
+  }
+}
+
 // Joins the splits of a query head, in their order.
 template <int D>
 __global__ __launch_bounds__(D) void merge_kernel(const float *__restrict__ part, int64_t nsplit, float *__restrict__ out) {
   const int64_t r = blockIdx.x;
   const int d = threadIdx.x;
-  float m = -INFINITY, l = 0.0f, o[1] = {0.0f};
+  float m = kLowest, l = 0.0f, o[1] = {0.0f};
   for (int64_t s = 0; s < nsplit; ++s) {
     const float *pb = part + (r * nsplit + s) * (D + 2);
     const float o1[1] = {pb[2 + d]};
@@ -180,36 +524,62 @@ __global__ __launch_bounds__(D) void merge_kernel(const float *__restrict__ part
   out[r * D + d] = l == 0.0f ? 0.0f : o[0] / l;
 }
 
-// Splits of a head's positions: enough workgroups for the chip, at least one tile each.
-int64_t splits(int64_t heads, int64_t positions) {
+// Splits of a head's listed positions: enough workgroups for the chip, at least one tile each.
+int64_t list_splits(int64_t heads, int64_t positions) {
   const int64_t most = cdiv(positions, (int64_t)kWaves * kTile), want = cdiv((int64_t)2048, heads);
   const int64_t s = most < want ? most : want;
   return s < 1 ? 1 : s;
 }
 
-size_t workspace(int64_t BH, int64_t G, int64_t D, int64_t positions) {
-  if (BH < 1 || G < 1 || D < 1 || positions < 0) return 0;
-  const int64_t ns = splits(BH * G, positions);
-  return ns == 1 ? 0 : (size_t)(BH * G * ns * (D + 2)) * sizeof(float);
+// Head groups of a row and their size in eights: a workgroup holds up to 16 heads.
+int64_t head_groups(int64_t G) { return cdiv(G, (int64_t)16); }
+
+// Splits of a row's tokens: two workgroups per CU, at least one block per wave.
+int64_t dense_splits(int64_t BH, int64_t G, int64_t positions) {
+  const int64_t most = cdiv(cdiv(positions, (int64_t)kBlk) + 1, (int64_t)kWaves), want = cdiv((int64_t)512, BH * head_groups(G));
+  return most < want ? most : want;
 }
 
-template <bool LIST>
-int run(const char *what, AttnArgs a, int64_t BH, int64_t D, bool i8, int64_t positions, size_t workspace_bytes,
-        hipStream_t st) {
-  const size_t need = workspace(BH, a.G, D, positions);
-  if (need && (!a.part || workspace_bytes < need))
-    return fail(FATHOM_ERR_WORKSPACE, "%s: workspace %zu bytes, need %zu", what, workspace_bytes, need);
-  a.nsplit = splits(BH * a.G, positions);
-  const dim3 grid((unsigned)a.nsplit, (unsigned)a.G, (unsigned)BH);
-  if (D == 128 && i8) attn_kernel<128, true, LIST><<<grid, kWaves * kWave, 0, st>>>(a);
-  else if (D == 128) attn_kernel<128, false, LIST><<<grid, kWaves * kWave, 0, st>>>(a);
-  else if (i8) attn_kernel<64, true, LIST><<<grid, kWaves * kWave, 0, st>>>(a);
-  else attn_kernel<64, false, LIST><<<grid, kWaves * kWave, 0, st>>>(a);
-  const int rc = launch_status(what);
-  if (rc || a.nsplit == 1) return rc;
+size_t part_bytes(int64_t BH, int64_t G, int64_t D, int64_t nsplit) {
+  return nsplit <= 1 ? 0 : (size_t)(BH * G * nsplit * (D + 2)) * sizeof(float);
+}
+
+int merge(const AttnArgs &a, int64_t BH, int64_t D, hipStream_t st) {
   if (D == 128) merge_kernel<128><<<(unsigned)(BH * a.G), 128, 0, st>>>(a.part, a.nsplit, a.out);
   else merge_kernel<64><<<(unsigned)(BH * a.G), 64, 0, st>>>(a.part, a.nsplit, a.out);
   return launch_status("rows8 merge_kernel");
+}
+
+int run_list(AttnArgs a, int64_t BH, int64_t D, bool i8, hipStream_t st) {
+  const dim3 grid((unsigned)a.nsplit, (unsigned)a.G, (unsigned)BH);
+  if (D == 128 && i8) list_kernel<128, true><<<grid, kWaves * kWave, 0, st>>>(a);
+  else if (D == 128) list_kernel<128, false><<<grid, kWaves * kWave, 0, st>>>(a);
+  else if (i8) list_kernel<64, true><<<grid, kWaves * kWave, 0, st>>>(a);
+  else list_kernel<64, false><<<grid, kWaves * kWave, 0, st>>>(a);
+  const int rc = launch_status("rows8 list_kernel");
+  return rc || a.nsplit == 1 ? rc : merge(a, BH, D, st);
+}
+
+template <int D, bool I8, int NG>
+void launch_dense(const AttnArgs &a, int64_t BH, hipStream_t st) {
+  const dim3 grid((unsigned)a.nsplit, (unsigned)head_groups(a.G), (unsigned)BH);
+  if (a.softcap > 0.0f || a.slopes) dense_kernel<D, I8, NG, true><<<grid, kWaves * kWave, 0, st>>>(a);
+  else dense_kernel<D, I8, NG, false><<<grid, kWaves * kWave, 0, st>>>(a);
+}
+
+template <int D, bool I8>
+void launch_dense(const AttnArgs &a, int64_t BH, hipStream_t st) {
+  if (a.G > 8) launch_dense<D, I8, 2>(a, BH, st);
+  else launch_dense<D, I8, 1>(a, BH, st);
+}
+
+int run_dense(AttnArgs a, int64_t BH, int64_t D, bool i8, hipStream_t st) {
+  if (D == 128 && i8) launch_dense<128, true>(a, BH, st);
+  else if (D == 128) launch_dense<128, false>(a, BH, st);
+  else if (i8) launch_dense<64, true>(a, BH, st);
+  else launch_dense<64, false>(a, BH, st);
+  const int rc = launch_status("rows8 dense_kernel");
+  return rc || a.nsplit == 1 ? rc : merge(a, BH, D, st);
 }
 
 int check_query(const char *what, const void *q, int q_dtype, int64_t BH, int64_t G, int64_t D, int64_t cap, const int32_t *lens,
@@ -239,7 +609,8 @@ using namespace fathom;
 using namespace fathom::rows8;
 
 extern "C" size_t fathom_rows8_attention_workspace_bytes(int64_t BH, int64_t G, int64_t D, int64_t positions) {
-  return workspace(BH, G, D, positions);
+  if (BH < 1 || G < 1 || D < 1 || positions < 1) return 0;
+  return part_bytes(BH, G, D, dense_splits(BH, G, positions));
 }
 
 extern "C" int fathom_rows8_attention(const void *q, int q_dtype, const void *k8, const void *v8, const float *k_scale,
@@ -253,12 +624,16 @@ extern "C" int fathom_rows8_attention(const void *q, int q_dtype, const void *k8
   if (window < 0) return fail(FATHOM_ERR_INVALID, "rows8_attention: window %lld", (long long)window);
   AttnArgs a{q, q_dtype, (const uint8_t *)k8, (const uint8_t *)v8, k_scale, v_scale, G, cap, cdiv(cap, kBlk), lens, n, window,
              nullptr, 0, scale, softcap, slopes, out, (float *)workspace, 1};
-  return run<false>("rows8_attention", a, BH, D, code_dtype == FATHOM_DT_I8, dense_positions(lens, n, cap, window),
-                    workspace_bytes, (hipStream_t)stream);
+  a.nsplit = dense_splits(BH, G, dense_positions(lens, n, cap, window));
+  const size_t need = part_bytes(BH, G, D, a.nsplit);
+  if (need && (!workspace || workspace_bytes < need))
+    return fail(FATHOM_ERR_WORKSPACE, "rows8_attention: workspace %zu bytes, need %zu", workspace_bytes, need);
+  return run_dense(a, BH, D, code_dtype == FATHOM_DT_I8, (hipStream_t)stream);
 }
 
 extern "C" size_t fathom_rows8_gather_attention_workspace_bytes(int64_t BH, int64_t G, int64_t D, int64_t k) {
-  return workspace(BH, G, D, k);
+  if (BH < 1 || G < 1 || D < 1 || k < 1) return 0;
+  return part_bytes(BH, G, D, list_splits(BH * G, k));
 }
 
 extern "C" int fathom_rows8_gather_attention(const void *q, int q_dtype, const int64_t *idx, const void *k8, const void *v8,
@@ -273,5 +648,9 @@ extern "C" int fathom_rows8_gather_attention(const void *q, int q_dtype, const i
   if (k > 0 && !idx) return fail(FATHOM_ERR_INVALID, "rows8_gather_attention: null index pointer");
   AttnArgs a{q, q_dtype, (const uint8_t *)k8, (const uint8_t *)v8, k_scale, v_scale, G, cap, cdiv(cap, kBlk), lens, n, 0,
              idx, k, scale, softcap, slopes, out, (float *)workspace, 1};
-  return run<true>("rows8_gather_attention", a, BH, D, code_dtype == FATHOM_DT_I8, k, workspace_bytes, (hipStream_t)stream);
+  a.nsplit = list_splits(BH * G, k);
+  const size_t need = part_bytes(BH, G, D, a.nsplit);
+  if (need && (!workspace || workspace_bytes < need))
+    return fail(FATHOM_ERR_WORKSPACE, "rows8_gather_attention: workspace %zu bytes, need %zu", workspace_bytes, need);
+  return run_list(a, BH, D, code_dtype == FATHOM_DT_I8, (hipStream_t)stream);
 }

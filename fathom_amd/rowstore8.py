@@ -16,7 +16,7 @@ asynchronously on the device's current stream.
 import torch
 
 from . import _lib
-from .bitplane import BLK, D, _KDT, _need_gpu, _ptr, _stream
+from .bitplane import BLK, D, _KDT, _need_gpu
 
 __all__ = ["RowStore8"]
 
@@ -43,22 +43,24 @@ class RowStore8:
     keeps nothing else, and methods write into them."""
 
     def __init__(self, k8, v8, k_scale, v_scale):
-        _need_gpu(k8, v8, k_scale, v_scale)
-        if k8.dim() != 3 or k8.dtype not in _CODES or k8.shape[2] not in (64, 128):
-            raise ValueError(f"codes must be float8_e4m3fn or int8 [BH, cap, 64 or 128], got {k8.dtype} {tuple(k8.shape)}")
-        self.BH, self.cap, self.d = k8.shape
-        if v8.shape != k8.shape or v8.dtype != k8.dtype:
-            raise ValueError(f"v8 {v8.dtype} {tuple(v8.shape)} must be like k8 {k8.dtype} {tuple(k8.shape)}")
-        nblk = -(-self.cap // BLK)
+        shape, dev = k8.shape, k8.device
+        _need_gpu(k8)
+        if len(shape) != 3 or k8.dtype not in _CODES or shape[2] not in (64, 128):
+            raise ValueError(f"codes must be float8_e4m3fn or int8 [BH, cap, 64 or 128], got {k8.dtype} {tuple(shape)}")
+        self.BH, self.cap, self.d = shape
+        if v8.shape != shape or v8.dtype != k8.dtype:
+            raise ValueError(f"v8 {v8.dtype} {tuple(v8.shape)} must be like k8 {k8.dtype} {tuple(shape)}")
+        scales = (self.BH, -(-self.cap // BLK))
         for s in (k_scale, v_scale):
-            if s.dtype != torch.float32 or s.shape != (self.BH, nblk):
-                raise ValueError(f"scales must be float32 [{self.BH}, {nblk}], got {s.dtype} {tuple(s.shape)}")
+            if s.dtype != torch.float32 or s.shape != scales:
+                raise ValueError(f"scales must be float32 {list(scales)}, got {s.dtype} {tuple(s.shape)}")
         for t in (k8, v8, k_scale, v_scale):
-            if not t.is_contiguous() or t.device != k8.device:
+            if t.device != dev or not t.is_contiguous():
                 raise ValueError("the store's tensors must be contiguous and on one device")
         self.k8, self.v8, self.k_scale, self.v_scale = k8, v8, k_scale, v_scale
-        self.device = k8.device
+        self.device = dev
         self._code = _CODES[k8.dtype]
+        self._sizes = {}
 
     @classmethod
     def empty(cls, BH, cap, dtype=torch.float8_e4m3fn, d=D, device=None):
@@ -69,50 +71,73 @@ class RowStore8:
         return cls(k8, v8, ks, vs)
 
     # ------------------------------------------------------------------ arguments
+    # A call of a few tokens is as long as its host side, so arguments go to the
+    # library as plain ints and are checked without building objects.
     def _call(self, name, *args):
         """The entry point on the store's device and its current stream."""
-        if torch.cuda.current_device() == self.device.index:
-            _lib.call(name, *args, _stream(self.device))
+        dev = self.device.index
+        fn = getattr(_lib.lib(), name)
+        stream = torch._C._cuda_getCurrentRawStream(dev)
+        if torch._C._cuda_getDevice() == dev:
+            rc = fn(*args, stream)
         else:
-            with torch.cuda.device(self.device):
-                _lib.call(name, *args, _stream(self.device))
+            with torch.cuda.device(dev):
+                rc = fn(*args, stream)
+        if rc:
+            _lib.check(rc, name)
 
-    def _tensors(self):
-        return _ptr(self.k8), _ptr(self.v8), _ptr(self.k_scale), _ptr(self.v_scale)
+    def _store(self):
+        return self.k8.data_ptr(), self.v8.data_ptr(), self.k_scale.data_ptr(), self.v_scale.data_ptr()
 
-    def _here(self, *tensors):
-        _need_gpu(*tensors)
-        for t in tensors:
-            if t.device != self.device:
-                raise ValueError(f"a tensor on {t.device}, the store is on {self.device}")
+    def _elsewhere(self, t):
+        _need_gpu(t)
+        raise ValueError(f"a tensor on {t.device}, the store is on {self.device}")
 
     def _per_row(self, v, what):
-        """A per-row argument as (int32 tensor or None, int)."""
-        if not torch.is_tensor(v):
-            return None, int(v)
-        self._here(v)
+        """A per-row argument as (int32 tensor or None, its address, int)."""
+        if not isinstance(v, torch.Tensor):
+            return None, None, int(v)
+        if v.device != self.device:
+            self._elsewhere(v)
         if v.shape != (self.BH,) or v.dtype.is_floating_point or v.dtype == torch.bool:
             raise ValueError(f"{what} must be an int or integers [{self.BH}], got {v.dtype} {tuple(v.shape)}")
         if v.dtype == torch.int64:  # places beyond int32 stay beyond every store
             v = v.clamp(-(1 << 31), (1 << 31) - 1)
-        return v.to(torch.int32).contiguous(), 0
+        v = v.to(torch.int32).contiguous()
+        return v, v.data_ptr(), 0
 
     def _query(self, q, scale, softcap, slopes):
-        self._here(q)
-        if q.dim() != 3 or q.shape[0] != self.BH or q.shape[2] != self.d or q.shape[1] < 1:
-            raise ValueError(f"q {tuple(q.shape)} must be [{self.BH}, G, {self.d}]")
+        """q as the kernels read it, with its address; the scale, cap and slopes of a call."""
+        if q.device != self.device:
+            self._elsewhere(q)
+        shape = q.shape
+        if len(shape) != 3 or shape[0] != self.BH or shape[2] != self.d or shape[1] < 1:
+            raise ValueError(f"q {tuple(shape)} must be [{self.BH}, G, {self.d}]")
         q = (q if q.dtype in _KDT else q.float()).contiguous()
-        q = q.clone() if q.data_ptr() % 16 else q
+        at = q.data_ptr()
+        if at % 16:
+            q = q.clone()
+            at = q.data_ptr()
         softcap = 0.0 if softcap is None else float(softcap)
         if not softcap >= 0.0:
             raise ValueError(f"softcap {softcap} must be positive (None or 0: no cap)")
         if slopes is not None:
-            self._here(slopes)
-            slopes = slopes.float().expand(q.shape[:2]).contiguous()
-        return q, float(self.d) ** -0.5 if scale is None else float(scale), softcap, slopes
+            if slopes.device != self.device:
+                self._elsewhere(slopes)
+            slopes = slopes.float().expand(shape[:2]).contiguous()
+        return q, at, self.d ** -0.5 if scale is None else float(scale), softcap, slopes
 
-    def _workspace(self, nbytes):
-        return torch.empty(nbytes, dtype=torch.uint8, device=self.device) if nbytes else None
+    def _workspace(self, query, G, positions):
+        """The call's workspace (or None), its address and size, for at least `positions`: sizes grow with them, so one query
+        serves up to the next power of two."""
+        key = query, G, positions.bit_length()
+        nbytes = self._sizes.get(key)
+        if nbytes is None:
+            nbytes = self._sizes[key] = getattr(_lib.lib(), query)(self.BH, G, self.d, 1 << positions.bit_length())
+        if not nbytes:
+            return None, None, 0
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+        return ws, ws.data_ptr(), nbytes
 
     # ------------------------------------------------------------------ writing and reading
     def write(self, K, V, pos=0):
@@ -126,36 +151,44 @@ class RowStore8:
         With a tensor `pos`, rows whose tokens do not all fit into the store (a negative
         pos among them) are left as they are; an int pos that does not fit raises.  K
         and V may be views with any strides (their rows dense)."""
-        self._here(K, V)
+        for t in (K, V):
+            if t.device != self.device:
+                self._elsewhere(t)
         if K.dim() != 3 or K.shape != V.shape or K.shape[0] != self.BH or K.shape[2] != self.d or K.dtype != V.dtype:
             raise ValueError(f"K {K.dtype} {tuple(K.shape)} and V {V.dtype} {tuple(V.shape)} must be alike, "
                              f"[{self.BH}, T, {self.d}]")
-        rows, at = self._per_row(pos, "pos")
+        rows, rows_at, at = self._per_row(pos, "pos")
         K, V = _aligned(K), _aligned(V)
-        self._call("fathom_rows8_write", _ptr(K), _ptr(V), _KDT[K.dtype], K.stride(0), K.stride(1), V.stride(0), V.stride(1),
-                   _ptr(rows), at, self.BH, K.shape[1], self.d, self.cap, self._code, *self._tensors())
+        (kr, kt, _), (vr, vt, _) = K.stride(), V.stride()
+        self._call("fathom_rows8_write", K.data_ptr(), V.data_ptr(), _KDT[K.dtype], kr, kt, vr, vt, rows_at, at, self.BH,
+                   K.shape[1], self.d, self.cap, self._code, *self._store())
 
-    def _read(self, idx, rows, at, R, dtype):
+    def _read(self, idx_at, rows_at, at, R, dtype):
         if dtype not in _KDT:
             raise ValueError(f"dtype {dtype} unsupported (float32, float16, bfloat16)")
-        K, V = (torch.empty(self.BH, R, self.d, dtype=dtype, device=self.device) for _ in "kv")
-        self._call("fathom_rows8_read", *self._tensors(), self._code, self.BH, self.cap, self.d, _ptr(idx), _ptr(rows), at, R,
-                   _KDT[dtype], _ptr(K), _ptr(V))
+        if R < 0:
+            raise ValueError(f"{R} tokens")
+        K = torch.empty(self.BH, R, self.d, dtype=dtype, device=self.device)
+        V = torch.empty_like(K)
+        self._call("fathom_rows8_read", *self._store(), self._code, self.BH, self.cap, self.d, idx_at, rows_at, at, R,
+                   _KDT[dtype], K.data_ptr(), V.data_ptr())
         return K, V
 
     def read(self, pos, T, dtype=torch.bfloat16):
         """The values of tokens pos .. pos + T - 1 of each row, K, V [BH, T, d];
         tokens outside the store are zeros."""
-        rows, at = self._per_row(pos, "pos")
-        return self._read(None, rows, at, int(T), dtype)
+        rows, rows_at, at = self._per_row(pos, "pos")
+        return self._read(None, rows_at, at, int(T), dtype)
 
     def gather_rows(self, idx, dtype=torch.bfloat16):
         """The values of the listed tokens idx [BH, R], K, V [BH, R, d]; tokens outside
         the store give zero rows, as offload.gather_rows does."""
-        self._here(idx)
+        if idx.device != self.device:
+            self._elsewhere(idx)
         if idx.dim() != 2 or idx.shape[0] != self.BH:
             raise ValueError(f"idx {tuple(idx.shape)} must be [{self.BH}, R]")
-        return self._read(idx.to(torch.int64).contiguous(), None, 0, idx.shape[1], dtype)
+        idx = idx.to(torch.int64).contiguous()
+        return self._read(idx.data_ptr(), None, 0, idx.shape[1], dtype)
 
     # ------------------------------------------------------------------ attention
     def attention(self, q, length, window=0, scale=None, softcap=None, slopes=None):
@@ -166,16 +199,16 @@ class RowStore8:
                 then biased by slopes[bh, g] (t - (length - 1)) if slopes are given
         (slopes [BH, G], or [G]; scale defaults to d ** -0.5).  A tensor length is taken
         as within [0, cap].  A row without tokens gives zeros."""
-        q, scale, softcap, slopes = self._query(q, scale, softcap, slopes)
-        lens, n = self._per_row(length, "length")
+        q, q_at, scale, softcap, slopes = self._query(q, scale, softcap, slopes)
+        lens, lens_at, n = self._per_row(length, "length")
         G, window = q.shape[1], int(window)
-        positions = self.cap if lens is not None else n
-        positions = min(positions, window) if window > 0 else positions
-        nbytes = _lib.lib().fathom_rows8_attention_workspace_bytes(self.BH, G, self.d, positions)
-        ws = self._workspace(nbytes)
-        out = torch.empty(self.BH, G, self.d, dtype=torch.float32, device=self.device)
-        self._call("fathom_rows8_attention", _ptr(q), _KDT[q.dtype], *self._tensors(), self._code, self.BH, G, self.d,
-                   self.cap, _ptr(lens), n, window, scale, softcap, _ptr(slopes), _ptr(out), _ptr(ws), nbytes)
+        positions = n if lens is None else self.cap
+        positions = max(min(positions, window) if window > 0 else positions, 0)
+        ws, ws_at, nbytes = self._workspace("fathom_rows8_attention_workspace_bytes", G, positions)
+        out = torch.empty(q.shape, dtype=torch.float32, device=self.device)
+        self._call("fathom_rows8_attention", q_at, _KDT[q.dtype], *self._store(), self._code, self.BH, G, self.d, self.cap,
+                   lens_at, n, window, scale, softcap, None if slopes is None else slopes.data_ptr(), out.data_ptr(), ws_at,
+                   nbytes)
         return out
 
     def gather_attention(self, q, idx, length=None, scale=None, softcap=None, slopes=None):
@@ -184,17 +217,18 @@ class RowStore8:
         twice.  Tokens outside [0, length) (length defaults to cap) take no part, so a
         selection may be padded with -1 (offload.gather_attention's zero rows score 0
         instead)."""
-        q, scale, softcap, slopes = self._query(q, scale, softcap, slopes)
-        self._here(idx)
+        q, q_at, scale, softcap, slopes = self._query(q, scale, softcap, slopes)
+        if idx.device != self.device:
+            self._elsewhere(idx)
         G = q.shape[1]
         if idx.dim() != 3 or idx.shape[:2] != q.shape[:2]:
             raise ValueError(f"idx {tuple(idx.shape)} must be [{self.BH}, {G}, k]")
         idx = idx.to(torch.int64).contiguous()
         k = idx.shape[2]
-        lens, n = self._per_row(self.cap if length is None else length, "length")
-        nbytes = _lib.lib().fathom_rows8_gather_attention_workspace_bytes(self.BH, G, self.d, k)
-        ws = self._workspace(nbytes)
-        out = torch.empty(self.BH, G, self.d, dtype=torch.float32, device=self.device)
-        self._call("fathom_rows8_gather_attention", _ptr(q), _KDT[q.dtype], _ptr(idx), *self._tensors(), self._code, self.BH,
-                   G, k, self.d, self.cap, _ptr(lens), n, scale, softcap, _ptr(slopes), _ptr(out), _ptr(ws), nbytes)
+        lens, lens_at, n = self._per_row(self.cap if length is None else length, "length")
+        ws, ws_at, nbytes = self._workspace("fathom_rows8_gather_attention_workspace_bytes", G, k)
+        out = torch.empty(q.shape, dtype=torch.float32, device=self.device)
+        self._call("fathom_rows8_gather_attention", q_at, _KDT[q.dtype], idx.data_ptr(), *self._store(), self._code, self.BH, G,
+                   k, self.d, self.cap, lens_at, n, scale, softcap, None if slopes is None else slopes.data_ptr(),
+                   out.data_ptr(), ws_at, nbytes)
         return out

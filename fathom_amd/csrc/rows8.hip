@@ -21,6 +21,7 @@ namespace rows8 {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kReadPieces = 4;
 
 struct WriteArgs {
   const void *x[2];
@@ -134,33 +135,63 @@ struct ReadArgs {
   int64_t pos_value, R, cap, nblk;
 };
 
-// Four values of a row per thread: row r of the output is token idx[bh, r], or
-// pos + r; tokens outside the store give zeros.
+// Row r of the output is token idx[bh, r], or pos + r; tokens outside the store give
+// zeros.  A thread writes kReadPieces pieces of 16 bytes, kThreads pieces apart, with all of
+// their codes requested first.
+//
+// Bound: HBM (D codes in, 2 D or 4 D bytes out per token).
 template <int D, int DT, bool I8>
 __global__ __launch_bounds__(kThreads) void read_kernel(ReadArgs a) {
-  const int64_t bh = blockIdx.y;
+  constexpr int kElem = DT == FATHOM_DT_F32 ? 4 : 8;  // values of a piece
+  constexpr int kRows = kReadPieces * kThreads * kElem / D;
+  const int64_t bh = blockIdx.y, r0 = (int64_t)blockIdx.x * kRows;
   const int kv = blockIdx.z;
-  const int64_t e0 = ((int64_t)blockIdx.x * kThreads + threadIdx.x) * 4;
-  const int64_t r = e0 / D;
-  const int d = (int)(e0 % D);
-  if (r >= a.R) return;
-  const int64_t tok = a.idx ? a.idx[bh * a.R + r] : (a.pos ? (int64_t)a.pos[bh] : a.pos_value) + r;
-  float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-  if (tok >= 0 && tok < a.cap) {
-    decode4<I8>(*reinterpret_cast<const uint32_t *>(a.codes[kv] + (bh * a.cap + tok) * D + d), v);
-    const float s = a.scale[kv][bh * a.nblk + tok / kBlk];
+  const int64_t p = a.pos ? (int64_t)a.pos[bh] : a.pos_value;
+  const uint8_t *codes = a.codes[kv] + bh * a.cap * D;
+  const float *scale = a.scale[kv] + bh * a.nblk;
+  uint32_t w[kReadPieces][kElem / 4];
+  float s[kReadPieces];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] *= s;
+  for (int i = 0; i < kReadPieces; ++i) {
+    const int e = (i * kThreads + (int)threadIdx.x) * kElem;
+    const int64_t r = r0 + e / D;
+    int64_t tok = -1;
+    if (r < a.R) tok = a.idx ? a.idx[bh * a.R + r] : p + r;
+    s[i] = 0.0f;
+#pragma unroll
+    for (int x = 0; x < kElem / 4; ++x) w[i][x] = 0u;
+    if (tok >= 0 && tok < a.cap) {
+      const uint8_t *c = codes + tok * D + e % D;
+      if constexpr (kElem == 8) {
+        const uint2 v = *reinterpret_cast<const uint2 *>(c);
+        w[i][0] = v.x;
+        w[i][1] = v.y;
+      } else {
+        w[i][0] = *reinterpret_cast<const uint32_t *>(c);
+      }
+      s[i] = scale[(uint64_t)tok / kBlk];
+    }
   }
-  const int64_t o = (bh * a.R + r) * D + d;
-  if constexpr (DT == FATHOM_DT_F32) {
-    *reinterpret_cast<float4 *>(static_cast<float *>(a.out[kv]) + o) = make_float4(v[0], v[1], v[2], v[3]);
-  } else {
-    uint16_t h[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) h[e] = DT == FATHOM_DT_BF16 ? float_to_bf16_bits(v[e]) : float_to_f16_bits(v[e]);
-    *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(a.out[kv]) + o) =
-        make_uint2(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16);
+  for (int i = 0; i < kReadPieces; ++i) {
+    const int e = (i * kThreads + (int)threadIdx.x) * kElem;
+    const int64_t r = r0 + e / D;
+    if (r >= a.R) continue;
+    float v[kElem];
+#pragma unroll
+    for (int x = 0; x < kElem / 4; ++x) {
+      float c[4];
+      decode4<I8>(w[i][x], c);
+#pragma unroll
+      for (int y = 0; y < 4; ++y) v[4 * x + y] = c[y] * s[i];
+    }
+    const int64_t o = (bh * a.R + r0) * D + e;
+    if constexpr (DT == FATHOM_DT_F32) {
+      *reinterpret_cast<float4 *>(static_cast<float *>(a.out[kv]) + o) = make_float4(v[0], v[1], v[2], v[3]);
+    } else {
+      *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(a.out[kv]) + o) =
+          make_uint4(pack2<DT>(v[0], v[1]), pack2<DT>(v[2], v[3]), pack2<DT>(v[4], v[5]), pack2<DT>(v[6], v[7]));
+    }
   }
 }
 
@@ -172,7 +203,7 @@ void launch_write(const WriteArgs &a, int64_t BH, hipStream_t st) {
 
 template <int D, int DT, bool I8>
 void launch_read(const ReadArgs &a, int64_t BH, hipStream_t st) {
-  read_kernel<D, DT, I8><<<dim3((unsigned)cdiv(a.R * D, 4 * kThreads), (unsigned)BH, 2), kThreads, 0, st>>>(a);
+  read_kernel<D, DT, I8><<<dim3((unsigned)cdiv(a.R, (int64_t)kReadPieces * kThreads * (DT == FATHOM_DT_F32 ? 4 : 8) / D), (unsigned)BH, 2), kThreads, 0, st>>>(a);
 }
 
 #define FATHOM_ROWS8_DISPATCH(fn, ...)                                         \

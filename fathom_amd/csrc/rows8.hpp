@@ -74,6 +74,17 @@ __device__ __forceinline__ void unpack2(uint32_t w, float &a, float &b) {
   }
 }
 
+// Two floats as 16-bit elements of a dword, rounded to nearest even.
+template <int DT>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (DT == FATHOM_DT_BF16) {
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, bf16x2{(__bf16)a, (__bf16)b});  // one v_cvt_pk_bf16_f32
+  } else {
+    return float_to_f16_bits(a) | (uint32_t)float_to_f16_bits(b) << 16;
+  }
+}
+
 // The length of row bh: the array's value, kept inside the store, or n.
 __device__ __forceinline__ int64_t row_length(const int32_t *lens, int64_t n, int64_t cap, int64_t bh) {
   if (!lens) return n;

@@ -13,8 +13,12 @@ namespace fathom {
 namespace rows8 {
 namespace {
 
-constexpr int kWaves = 4;  // of a workgroup
+constexpr int kWaves = 4;       // of a workgroup of list_kernel
+constexpr int kDenseWaves = 4;  // of a workgroup of dense_kernel
 constexpr int kTile = 32;  // listed positions of a wave at a time
+constexpr int kMergeThreads = 256;
+constexpr int kDenseGroups = 2048 / kDenseWaves;  // workgroups of a dense call: eight waves per CU
+constexpr int kMaxSplits = 512;  // of a query head
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLowest = -3.0e38f;  // below every score: the running maximum of no token
 
@@ -30,14 +34,28 @@ struct AttnArgs {
   int64_t k;
   float scale, softcap;
   const float *slopes;
-  float *out, *part;
-  int64_t nsplit;
+  float *out;
+  float2 *ml;   // [slots, G] a split's (m, l): slot bh nsplit + split, or where[bh].x + split
+  float *part;  // [slots, G, D] its weighted rows
+  int2 *where;  // [BH] a row's first slot and its splits, where lengths are on the device; else null
+  int64_t nsplit, BH, groups;
 };
 
-__device__ __forceinline__ float load_q(const void *q, int dt, int64_t i) {
-  return dt == FATHOM_DT_F32   ? load_elem<FATHOM_DT_F32>(q, i)
-         : dt == FATHOM_DT_F16 ? load_elem<FATHOM_DT_F16>(q, i)
-                               : load_elem<FATHOM_DT_BF16>(q, i);
+// Eight consecutive elements of q from i (a multiple of eight).
+__device__ __forceinline__ void load8_q(const void *q, int dt, int64_t i, float (&v)[8]) {
+  if (dt == FATHOM_DT_F32) {
+    const float4 *p = reinterpret_cast<const float4 *>(static_cast<const float *>(q) + i);
+    const float4 x = p[0], y = p[1];
+    v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w, v[4] = y.x, v[5] = y.y, v[6] = y.z, v[7] = y.w;
+  } else {
+    const uint4 x = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(q) + i);
+    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (dt == FATHOM_DT_BF16) unpack2<FATHOM_DT_BF16>(w[e], v[2 * e], v[2 * e + 1]);
+      else unpack2<FATHOM_DT_F16>(w[e], v[2 * e], v[2 * e + 1]);
+    }
+  }
 }
 
 // Adds (m1, l1, o1) to the running (m, l, o) of a softmax (maxima in log2 units).
@@ -65,9 +83,9 @@ __global__ __launch_bounds__(kWaves *kWave) void list_kernel(AttnArgs a) {
   const int64_t len = row_length(a.lens, a.n, a.cap, bh);
   const int64_t count = a.k;
   const float slope = a.slopes ? a.slopes[bh * a.G + g] * kLog2e : 0.0f;
-  float q[16];
+  float q[2][8];
 #pragma unroll
-  for (int e = 0; e < 16; ++e) q[e] = load_q(a.q, a.q_dtype, (bh * a.G + g) * D + d0 + e);
+  for (int h = 0; h < 2; ++h) load8_q(a.q, a.q_dtype, (bh * a.G + g) * D + d0 + 8 * h, q[h]);
   float m = kLowest, l = 0.0f, o[16];
 #pragma unroll
   for (int e = 0; e < 16; ++e) o[e] = 0.0f;
@@ -101,7 +119,7 @@ __global__ __launch_bounds__(kWaves *kWave) void list_kernel(AttnArgs a) {
         float c[4];
         decode4<I8>(w[e], c);
 #pragma unroll
-        for (int f = 0; f < 4; ++f) dot = fmaf(q[4 * e + f], c[f], dot);
+        for (int f = 0; f < 4; ++f) dot = fmaf(q[e / 2][4 * (e & 1) + f], c[f], dot);
       }
 #pragma unroll
       for (int x = 1; x < kLanes; x <<= 1) dot += __shfl_xor(dot, x);
@@ -158,12 +176,9 @@ __global__ __launch_bounds__(kWaves *kWave) void list_kernel(AttnArgs a) {
     if (a.nsplit == 1) {
       a.out[r * D + tid] = L == 0.0f ? 0.0f : O[0] / L;
     } else {
-      float *pb = a.part + (r * a.nsplit + s) * (D + 2);
-      pb[2 + tid] = O[0];
-      if (tid == 0) {
-        pb[0] = M;
-        pb[1] = L;
-      }
+      const int64_t at = (bh * a.nsplit + s) * a.G + g;
+      a.part[at * D + tid] = O[0];
+      if (tid == 0) a.ml[at] = make_float2(M, L);
     }
   }
 }
@@ -247,6 +262,55 @@ __device__ __forceinline__ float add_other_half(float v) {
   return v + __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x128, 0xF, 0xF, false));
 }
 
+// The blocks of a row that a call takes.
+__device__ __forceinline__ void row_blocks(const AttnArgs &a, int64_t bh, int64_t &lo, int64_t &len, int64_t &blk0, int &nb) {
+  len = row_length(a.lens, a.n, a.cap, bh);
+  lo = a.window > 0 && len > a.window ? len - a.window : 0;
+  blk0 = lo / kBlk;
+  nb = (int)(cdiv(len, (int64_t)kBlk) - blk0);
+}
+
+// The part of a workgroup: row, split of the row, the row's splits, blocks per split.
+struct Part {
+  int64_t bh;
+  int split, active, per;
+};
+// Rows of their own lengths (on the device): every workgroup takes `per` blocks, so
+// that the longest row does not hold the call up.  Each wave sums the rows'
+// blocks (a lane per row), which gives `per`, and finds its workgroup's row in the prefix sums
+// of ceil(blocks / per).  Those are at most kDenseGroups / groups + BH, the grid.
+__device__ __forceinline__ Part find_part(const AttnArgs &a, int w) {
+  const int lane = threadIdx.x & 63;
+  auto blocks = [&](int64_t r) {
+    int64_t lo, len, blk0;
+    int nb = 0;
+    if (r < a.BH) row_blocks(a, r, lo, len, blk0, nb);
+    return nb;
+  };
+  int64_t total = 0;
+  for (int64_t r0 = 0; r0 < a.BH; r0 += kWave) total += wave_sum_i(blocks(r0 + lane));
+  const int groups = kDenseGroups / (int)a.groups > 0 ? kDenseGroups / (int)a.groups : 1;
+  const int even = __builtin_amdgcn_readfirstlane((int)((total + groups - 1) / groups));
+  Part p{a.BH, 0, 0, even > kDenseWaves ? even : kDenseWaves};
+  uint32_t before = 0;
+  for (int64_t r0 = 0; r0 < a.BH; r0 += kWave) {
+    // a row without tokens takes a workgroup too: it writes the row's zeros
+    const int nb = blocks(r0 + lane);
+    const uint32_t act = r0 + lane >= a.BH ? 0u : nb <= p.per ? 1u : (uint32_t)((nb + p.per - 1) / p.per);
+    const uint32_t upto = before + wave_incl_scan_u32(act);
+    const uint64_t past = __ballot(upto > (uint32_t)w);
+    if (past) {
+      const int at = __builtin_ctzll(past);
+      p.bh = r0 + at;
+      p.active = __builtin_amdgcn_readlane((int)act, at);
+      p.split = w - (__builtin_amdgcn_readlane((int)upto, at) - p.active);
+      return p;
+    }
+    before = __builtin_amdgcn_readlane((int)upto, 63);
+  }
+  return p;  // bh = BH: the call needs no such workgroup
+}
+
 // Attention over every token of [lo, len): flash decoding on the matrix cores.
 //
 // A workgroup takes one split of a row for a group of 8 NG query heads; its waves
@@ -273,20 +337,50 @@ __device__ __forceinline__ float add_other_half(float v) {
 // Bound: HBM, 2 D bytes per token; the next block's K rows are requested once
 // the scores are formed, its V rows once the products are.
 template <int D, bool I8, int NG, bool EXTRA>
-__global__ __launch_bounds__(kWaves *kWave, NG == 1 ? 2 : 1) void dense_kernel(AttnArgs a) {
+__global__ __launch_bounds__(kDenseWaves *kWave, NG == 1 ? 2 : 1) void dense_kernel(AttnArgs a) {
   constexpr int kHalves = D / 64;  // 16-byte pieces of a row per lane
   constexpr int kSteps = D / 32;   // matrix instructions along the channels
   constexpr int kCh = D / 16;      // channels of V per lane
-  __shared__ float wm[kWaves][8 * NG], wl[kWaves][8 * NG], wo[kWaves][8 * NG][D];
+  __shared__ float wm[kDenseWaves][8 * NG], wl[kDenseWaves][8 * NG], wo[kDenseWaves][8 * NG][D];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, grp = lane >> 4;
-  const int64_t split = blockIdx.x, g0 = (int64_t)blockIdx.y * 8 * NG, bh = blockIdx.z;
-  const int64_t len = row_length(a.lens, a.n, a.cap, bh);
-  const int64_t lo = a.window > 0 && len > a.window ? len - a.window : 0;
-  // the split's blocks
-  const int64_t blk0 = lo / kBlk, nb = cdiv(len, (int64_t)kBlk) - blk0, per = cdiv(nb, a.nsplit);
-  const int64_t first = blk0 + split * per, last = first + per < blk0 + nb ? first + per : blk0 + nb;
+  const int64_t g0 = (int64_t)blockIdx.y * 8 * NG;
+  Part part{(int64_t)blockIdx.z, (int)blockIdx.x, (int)a.nsplit, 0};
+  int64_t slot = (int64_t)blockIdx.z * a.nsplit + blockIdx.x;  // of the partial results
+  if (a.where) {
+    part = find_part(a, (int)blockIdx.x);
+    if (part.bh >= a.BH) return;
+    slot = blockIdx.x;
+    if (part.split == 0 && blockIdx.y == 0 && tid == 0) a.where[part.bh] = make_int2((int)blockIdx.x, part.active);
+  }
+  const int64_t bh = part.bh;
+  int64_t lo, len, blk0;
+  int nb;
+  row_blocks(a, bh, lo, len, blk0, nb);
+  if (!a.where) part.per = (nb + part.active - 1) / part.active;
+  const int64_t first = blk0 + (int64_t)part.split * part.per;
+  const int64_t last = part.split + 1 < part.active ? first + part.per : blk0 + nb;
 
+  u32x4 kr[4][kHalves];
+  typedef typename VPiece<kCh>::type vpiece;
+  vpiece vr[4][4];
+  const int koff = col * D + 16 * grp, voff = 4 * grp * D + kCh * col;
+  auto load_k = [&](int64_t b) {
+    const RowsOf r(a.k8, bh * a.cap, b, b < last ? len : 0, D);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int h = 0; h < kHalves; ++h) kr[i][h] = r.load16(koff + 16 * i * D + 64 * h);
+  };
+  auto load_v = [&](int64_t b) {
+    const RowsOf r(a.v8, bh * a.cap, b, b < last ? len : 0, D);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) r.load(voff + (16 * i + j) * D, vr[i][j]);
+  };
+  load_k(first + wave);
+  load_v(first + wave);
   f16x8 qf[NG][kSteps];
   float fac[NG], slope[NG];  // per lane: its head's factor of a score, its bias per token
 #pragma unroll
@@ -296,13 +390,12 @@ __global__ __launch_bounds__(kWaves *kWave, NG == 1 ? 2 : 1) void dense_kernel(A
     const int64_t row = (bh * a.G + (has ? g : a.G - 1)) * D;
     float q[kSteps][8], mx = 0.0f;
 #pragma unroll
-    for (int h = 0; h < kSteps; ++h)
+    for (int h = 0; h < kSteps; ++h) {
+      // step h = (piece, half): channels 64 (h / 2) + 16 grp + 8 (h & 1) + e
+      load8_q(a.q, a.q_dtype, row + 64 * (h / 2) + 16 * grp + 8 * (h & 1), q[h]);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        // step h = (piece, half): channels 64 (h / 2) + 16 grp + 8 (h & 1) + e
-        q[h][e] = load_q(a.q, a.q_dtype, row + 64 * (h / 2) + 16 * grp + 8 * (h & 1) + e);
-        mx = fmaxf(mx, fabsf(q[h][e]));
-      }
+      for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(q[h][e]));
+    }
     mx = across_groups<true>(mx);
     int sigma = 0;  // the largest |q| of the head in [2^13, 2^14)
     if (mx > 0.0f && mx < INFINITY) {
@@ -333,27 +426,7 @@ __global__ __launch_bounds__(kWaves *kWave, NG == 1 ? 2 : 1) void dense_kernel(A
   }
   int E = -1000;
 
-  u32x4 kr[4][kHalves];
-  typedef typename VPiece<kCh>::type vpiece;
-  vpiece vr[4][4];
-  const int koff = col * D + 16 * grp, voff = 4 * grp * D + kCh * col;
-  auto load_k = [&](int64_t b) {
-    const RowsOf r(a.k8, bh * a.cap, b, b < last ? len : 0, D);
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int h = 0; h < kHalves; ++h) kr[i][h] = r.load16(koff + 16 * i * D + 64 * h);
-  };
-  auto load_v = [&](int64_t b) {
-    const RowsOf r(a.v8, bh * a.cap, b, b < last ? len : 0, D);
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) r.load(voff + (16 * i + j) * D, vr[i][j]);
-  };
-  load_k(first + wave);
-  load_v(first + wave);
-  for (int64_t b = first + wave; b < last; b += kWaves) {
+  for (int64_t b = first + wave; b < last; b += kDenseWaves) {
     const float ks = a.ks[bh * a.nblk + b], vs = a.vs[bh * a.nblk + b];
     f32x4 s[NG][4];
 #pragma unroll
@@ -368,7 +441,7 @@ __global__ __launch_bounds__(kWaves *kWave, NG == 1 ? 2 : 1) void dense_kernel(A
         for (int n = 0; n < NG; ++n) s[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qf[n][h], s[n][i], 0, 0, 0);
       }
     }
-    load_k(b + kWaves);
+    load_k(b + kDenseWaves);
     // ---- scores, in log2 units; tokens outside [lo, len) have none
     const int t0 = (int)(b * kBlk);
     const bool edge = (int64_t)t0 < lo || (int64_t)t0 + kBlk > len;
@@ -463,7 +536,7 @@ __global__ __launch_bounds__(kWaves *kWave, NG == 1 ? 2 : 1) void dense_kernel(A
         }
       }
     }
-    load_v(b + kWaves);
+    load_v(b + kDenseWaves);
   }
   // ---- the workgroup's waves
   const float up = E > -1000 ? ldexpf(1.0f, E - 14) : 0.0f;
@@ -483,50 +556,106 @@ __global__ __launch_bounds__(kWaves *kWave, NG == 1 ? 2 : 1) void dense_kernel(A
       }
   }
   __syncthreads();
-  for (int x = tid; x < 8 * NG * D; x += kWaves * kWave) {
+  for (int x = tid; x < 8 * NG * D; x += kDenseWaves * kWave) {
     const int h = x / D, d = x % D;
     if (g0 + h >= a.G) break;
     float M = wm[0][h];
 #pragma unroll
-    for (int v = 1; v < kWaves; ++v) M = fmaxf(M, wm[v][h]);
+    for (int v = 1; v < kDenseWaves; ++v) M = fmaxf(M, wm[v][h]);
     float L = 0.0f, O = 0.0f;
 #pragma unroll
-    for (int v = 0; v < kWaves; ++v) {
+    for (int v = 0; v < kDenseWaves; ++v) {
       const float e = __builtin_amdgcn_exp2f(wm[v][h] - M);
       L = fmaf(wl[v][h], e, L);
       O = fmaf(wo[v][h][d], e, O);
     }
     const int64_t r = bh * a.G + g0 + h;
-    if (a.nsplit == 1) {
+    if (part.active <= 1) {
       a.out[r * D + d] = L == 0.0f ? 0.0f : O / L;
     } else {
-      float *pb = a.part + (r * a.nsplit + split) * (D + 2);
-      pb[2 + d] = O;
-      if (d == 0) {
-        pb[0] = M;
-        pb[1] = L;
-      }
+      const int64_t at = slot * a.G + g0 + h;
+      a.part[at * D + d] = O;
+      if (d == 0) a.ml[at] = make_float2(M, L);
     }
   }
 }
 
-// Joins the splits of a query head, in their order.
+// Joins the splits of a query head: their factors first, then the weighted rows,
+// 16 bytes per thread and every split of a thread in flight, summed in a fixed order.
 template <int D>
-__global__ __launch_bounds__(D) void merge_kernel(const float *__restrict__ part, int64_t nsplit, float *__restrict__ out) {
+__global__ __launch_bounds__(kMergeThreads) void merge_kernel(AttnArgs a) {
+  constexpr int kLanes = D / 4, kGroups = kMergeThreads / kLanes;
+  __shared__ float fac[kMaxSplits], red[2][kMergeThreads / kWave];
+  __shared__ float4 acc[kGroups][kLanes];
   const int64_t r = blockIdx.x;
-  const int d = threadIdx.x;
-  float m = kLowest, l = 0.0f, o[1] = {0.0f};
-  for (int64_t s = 0; s < nsplit; ++s) {
-    const float *pb = part + (r * nsplit + s) * (D + 2);
-    const float o1[1] = {pb[2 + d]};
-    join<1>(m, l, o, pb[0], pb[1], o1);
+  const int tid = threadIdx.x;
+  const int64_t bh = r / a.G;
+  const int2 w = a.where ? a.where[bh] : make_int2((int)(bh * a.nsplit), (int)a.nsplit);
+  const int ns = w.y;
+  if (ns <= 1) return;  // written already
+  const int64_t at = (int64_t)w.x * a.G + r % a.G;  // split s at + s G
+  float2 x[kMaxSplits / kMergeThreads];
+  float m = kLowest;
+#pragma unroll
+  for (int i = 0; i < kMaxSplits / kMergeThreads; ++i) {
+    const int s = i * kMergeThreads + tid;
+    x[i] = s < ns ? a.ml[at + s * a.G] : make_float2(kLowest, 0.0f);
+    m = fmaxf(m, x[i].x);
   }
-  out[r * D + d] = l == 0.0f ? 0.0f : o[0] / l;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+  if ((tid & 63) == 0) red[0][tid >> 6] = m;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kMergeThreads / kWave; ++w) m = fmaxf(m, red[0][w]);
+  float l = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kMaxSplits / kMergeThreads; ++i) {
+    const float f = __builtin_amdgcn_exp2f(x[i].x - m);
+    fac[i * kMergeThreads + tid] = f;
+    l = fmaf(x[i].y, f, l);
+  }
+  l = wave_sum_f(l);
+  if ((tid & 63) == 0) red[1][tid >> 6] = l;
+  __syncthreads();
+  l = 0.0f;
+#pragma unroll
+  for (int w = 0; w < kMergeThreads / kWave; ++w) l += red[1][w];
+  const int lane = tid % kLanes, grp = tid / kLanes;
+  const float4 *p = reinterpret_cast<const float4 *>(a.part) + at * kLanes + lane;
+  float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  for (int s0 = grp; s0 < ns; s0 += 8 * kGroups) {
+    float4 v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int s = s0 + i * kGroups;
+      v[i] = p[(s < ns ? s : s0) * a.G * kLanes];
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int s = s0 + i * kGroups;
+      const float f = s < ns ? fac[s] : 0.0f;
+      o.x = fmaf(v[i].x, f, o.x);
+      o.y = fmaf(v[i].y, f, o.y);
+      o.z = fmaf(v[i].z, f, o.z);
+      o.w = fmaf(v[i].w, f, o.w);
+    }
+  }
+  acc[grp][lane] = o;
+  __syncthreads();
+  if (tid < D) {
+    float v = 0.0f;
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) v += reinterpret_cast<const float *>(acc[g])[tid];
+    a.out[r * D + tid] = l == 0.0f ? 0.0f : v / l;
+  }
 }
 
 // Splits of a head's listed positions: enough workgroups for the chip, at least one tile each.
 int64_t list_splits(int64_t heads, int64_t positions) {
-  const int64_t most = cdiv(positions, (int64_t)kWaves * kTile), want = cdiv((int64_t)2048, heads);
+  const int64_t most = cdiv(positions, (int64_t)kWaves * kTile);
+  int64_t want = cdiv((int64_t)2048, heads);
+  if (want > kMaxSplits) want = kMaxSplits;
   const int64_t s = most < want ? most : want;
   return s < 1 ? 1 : s;
 }
@@ -534,19 +663,38 @@ int64_t list_splits(int64_t heads, int64_t positions) {
 // Head groups of a row and their size in eights: a workgroup holds up to 16 heads.
 int64_t head_groups(int64_t G) { return cdiv(G, (int64_t)16); }
 
-// Splits of a row's tokens: two workgroups per CU, at least one block per wave.
-int64_t dense_splits(int64_t BH, int64_t G, int64_t positions) {
-  const int64_t most = cdiv(cdiv(positions, (int64_t)kBlk) + 1, (int64_t)kWaves), want = cdiv((int64_t)512, BH * head_groups(G));
+// Splits of a row of up to nb blocks in a call of `rows` rows (head groups counted):
+// kDenseGroups workgroups in all, at least one block per wave.
+int64_t dense_splits(int64_t rows, int64_t nb) {
+  const int64_t want = cdiv((int64_t)kDenseGroups, rows), most = cdiv(nb, (int64_t)kDenseWaves);
   return most < want ? most : want;
 }
 
-size_t part_bytes(int64_t BH, int64_t G, int64_t D, int64_t nsplit) {
-  return nsplit <= 1 ? 0 : (size_t)(BH * G * nsplit * (D + 2)) * sizeof(float);
+// Slots of partial results of a dense call whose longest row has up to nb blocks
+// (with lengths on the device, the bound of find_part); 0: every row fits one
+// workgroup.  Neither falls as nb grows.
+int64_t dense_slots(int64_t BH, int64_t G, int64_t nb, bool lens) {
+  const int64_t ns = dense_splits(BH * head_groups(G), nb);
+  if (ns <= 1) return 0;
+  const int64_t all = kDenseGroups / head_groups(G) + BH, most = BH * cdiv(nb, (int64_t)kDenseWaves);
+  return !lens ? BH * ns : all < most ? all : most;
+}
+
+// Bytes of `slots` partial results: rows, (m, l), the rows' slots.
+size_t part_bytes(int64_t BH, int64_t G, int64_t D, int64_t slots) {
+  return slots < 1 ? 0 : (size_t)(slots * G * (D + 2) + 2 * BH) * sizeof(float);
+}
+
+void place(AttnArgs &a, void *workspace, int64_t D, int64_t slots, bool lens) {
+  if (slots < 1) return;
+  a.part = static_cast<float *>(workspace);
+  a.ml = reinterpret_cast<float2 *>(a.part + slots * a.G * D);
+  if (lens) a.where = reinterpret_cast<int2 *>(a.ml + slots * a.G);
 }
 
 int merge(const AttnArgs &a, int64_t BH, int64_t D, hipStream_t st) {
-  if (D == 128) merge_kernel<128><<<(unsigned)(BH * a.G), 128, 0, st>>>(a.part, a.nsplit, a.out);
-  else merge_kernel<64><<<(unsigned)(BH * a.G), 64, 0, st>>>(a.part, a.nsplit, a.out);
+  if (D == 128) merge_kernel<128><<<(unsigned)(BH * a.G), kMergeThreads, 0, st>>>(a);
+  else merge_kernel<64><<<(unsigned)(BH * a.G), kMergeThreads, 0, st>>>(a);
   return launch_status("rows8 merge_kernel");
 }
 
@@ -562,9 +710,9 @@ int run_list(AttnArgs a, int64_t BH, int64_t D, bool i8, hipStream_t st) {
 
 template <int D, bool I8, int NG>
 void launch_dense(const AttnArgs &a, int64_t BH, hipStream_t st) {
-  const dim3 grid((unsigned)a.nsplit, (unsigned)head_groups(a.G), (unsigned)BH);
-  if (a.softcap > 0.0f || a.slopes) dense_kernel<D, I8, NG, true><<<grid, kWaves * kWave, 0, st>>>(a);
-  else dense_kernel<D, I8, NG, false><<<grid, kWaves * kWave, 0, st>>>(a);
+  const dim3 grid((unsigned)a.nsplit, (unsigned)head_groups(a.G), a.where ? 1u : (unsigned)BH);
+  if (a.softcap > 0.0f || a.slopes) dense_kernel<D, I8, NG, true><<<grid, kDenseWaves * kWave, 0, st>>>(a);
+  else dense_kernel<D, I8, NG, false><<<grid, kDenseWaves * kWave, 0, st>>>(a);
 }
 
 template <int D, bool I8>
@@ -610,7 +758,9 @@ using namespace fathom::rows8;
 
 extern "C" size_t fathom_rows8_attention_workspace_bytes(int64_t BH, int64_t G, int64_t D, int64_t positions) {
   if (BH < 1 || G < 1 || D < 1 || positions < 1) return 0;
-  return part_bytes(BH, G, D, dense_splits(BH, G, positions));
+  const int64_t nb = cdiv(positions, (int64_t)kBlk) + 1;  // a window may begin inside a block
+  const int64_t one = dense_slots(BH, G, nb, false), own = dense_slots(BH, G, nb, true);
+  return part_bytes(BH, G, D, one > own ? one : own);
 }
 
 extern "C" int fathom_rows8_attention(const void *q, int q_dtype, const void *k8, const void *v8, const float *k_scale,
@@ -623,17 +773,26 @@ extern "C" int fathom_rows8_attention(const void *q, int q_dtype, const void *k8
   if (rc) return rc;
   if (window < 0) return fail(FATHOM_ERR_INVALID, "rows8_attention: window %lld", (long long)window);
   AttnArgs a{q, q_dtype, (const uint8_t *)k8, (const uint8_t *)v8, k_scale, v_scale, G, cap, cdiv(cap, kBlk), lens, n, window,
-             nullptr, 0, scale, softcap, slopes, out, (float *)workspace, 1};
-  a.nsplit = dense_splits(BH, G, dense_positions(lens, n, cap, window));
-  const size_t need = part_bytes(BH, G, D, a.nsplit);
+             nullptr, 0, scale, softcap, slopes, out, nullptr, nullptr, nullptr, 1, BH, 1};
+  const int64_t most = dense_positions(lens, n, cap, window);
+  const int64_t nb = lens ? cdiv(most, (int64_t)kBlk) + (window > 0) : cdiv(n, (int64_t)kBlk) - (n - most) / kBlk;
+  const int64_t slots = dense_slots(BH, G, nb, lens != nullptr);
+  a.BH = BH;
+  a.groups = head_groups(G);
+  a.nsplit = slots < 1 ? 1 : lens ? slots : cdiv(nb, cdiv(nb, slots / BH));  // as many as shares of that size fill
+  const size_t need = part_bytes(BH, G, D, slots);
   if (need && (!workspace || workspace_bytes < need))
     return fail(FATHOM_ERR_WORKSPACE, "rows8_attention: workspace %zu bytes, need %zu", workspace_bytes, need);
+  if (need && reinterpret_cast<uintptr_t>(workspace) & 15)
+    return fail(FATHOM_ERR_INVALID, "rows8_attention: the workspace must be 16-byte aligned");
+  place(a, workspace, D, slots, lens != nullptr);
   return run_dense(a, BH, D, code_dtype == FATHOM_DT_I8, (hipStream_t)stream);
 }
 
 extern "C" size_t fathom_rows8_gather_attention_workspace_bytes(int64_t BH, int64_t G, int64_t D, int64_t k) {
   if (BH < 1 || G < 1 || D < 1 || k < 1) return 0;
-  return part_bytes(BH, G, D, list_splits(BH * G, k));
+  const int64_t ns = list_splits(BH * G, k);
+  return part_bytes(BH, G, D, ns > 1 ? BH * ns : 0);
 }
 
 extern "C" int fathom_rows8_gather_attention(const void *q, int q_dtype, const int64_t *idx, const void *k8, const void *v8,
@@ -647,10 +806,14 @@ extern "C" int fathom_rows8_gather_attention(const void *q, int q_dtype, const i
   if (k < 0 || G * k > 0x7FFFFFFF) return fail(FATHOM_ERR_INVALID, "rows8_gather_attention: G=%lld k=%lld", (long long)G, (long long)k);
   if (k > 0 && !idx) return fail(FATHOM_ERR_INVALID, "rows8_gather_attention: null index pointer");
   AttnArgs a{q, q_dtype, (const uint8_t *)k8, (const uint8_t *)v8, k_scale, v_scale, G, cap, cdiv(cap, kBlk), lens, n, 0,
-             idx, k, scale, softcap, slopes, out, (float *)workspace, 1};
+             idx, k, scale, softcap, slopes, out, nullptr, nullptr, nullptr, 1, BH, 1};
   a.nsplit = list_splits(BH * G, k);
-  const size_t need = part_bytes(BH, G, D, a.nsplit);
+  const int64_t slots = a.nsplit > 1 ? BH * a.nsplit : 0;
+  const size_t need = part_bytes(BH, G, D, slots);
   if (need && (!workspace || workspace_bytes < need))
     return fail(FATHOM_ERR_WORKSPACE, "rows8_gather_attention: workspace %zu bytes, need %zu", workspace_bytes, need);
+  if (need && reinterpret_cast<uintptr_t>(workspace) & 15)
+    return fail(FATHOM_ERR_INVALID, "rows8_gather_attention: the workspace must be 16-byte aligned");
+  place(a, workspace, D, slots, false);
   return run_list(a, BH, D, code_dtype == FATHOM_DT_I8, (hipStream_t)stream);
 }

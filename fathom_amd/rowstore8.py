@@ -20,6 +20,9 @@ from .bitplane import BLK, D, _KDT, _need_gpu
 
 __all__ = ["RowStore8"]
 
+_raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
+_F32, _I32, _I64 = torch.float32, torch.int32, torch.int64
+_SIZES = {}  # workspace bytes by query and shape
 _CODES = {torch.float8_e4m3fn: _lib.DT_E4M3, torch.int8: _lib.DT_I8}
 
 
@@ -28,10 +31,11 @@ def _aligned(x):
     rows, and every row at a multiple of 16 bytes (a copy is made of others)."""
     if x.dtype not in _KDT:
         x = x.float()
-    size = x.element_size()
-    if x.stride(2) != 1 or x.data_ptr() % 16 or x.stride(0) * size % 16 or x.stride(1) * size % 16:
+    size = 4 if x.dtype == _F32 else 2
+    sr, st, sd = x.stride()
+    if sd != 1 or (x.data_ptr() | sr * size | st * size) & 15:
         x = x.contiguous()
-        x = x.clone() if x.data_ptr() % 16 else x
+        x = x.clone() if x.data_ptr() & 15 else x
     return x
 
 
@@ -44,23 +48,23 @@ class RowStore8:
 
     def __init__(self, k8, v8, k_scale, v_scale):
         shape, dev = k8.shape, k8.device
-        _need_gpu(k8)
+        if dev.type != "cuda":
+            _need_gpu(k8)
         if len(shape) != 3 or k8.dtype not in _CODES or shape[2] not in (64, 128):
             raise ValueError(f"codes must be float8_e4m3fn or int8 [BH, cap, 64 or 128], got {k8.dtype} {tuple(shape)}")
         self.BH, self.cap, self.d = shape
         if v8.shape != shape or v8.dtype != k8.dtype:
             raise ValueError(f"v8 {v8.dtype} {tuple(v8.shape)} must be like k8 {k8.dtype} {tuple(shape)}")
         scales = (self.BH, -(-self.cap // BLK))
-        for s in (k_scale, v_scale):
-            if s.dtype != torch.float32 or s.shape != scales:
-                raise ValueError(f"scales must be float32 {list(scales)}, got {s.dtype} {tuple(s.shape)}")
-        for t in (k8, v8, k_scale, v_scale):
-            if t.device != dev or not t.is_contiguous():
-                raise ValueError("the store's tensors must be contiguous and on one device")
+        if k_scale.shape != scales or v_scale.shape != scales or k_scale.dtype != _F32 or v_scale.dtype != _F32:
+            raise ValueError(f"scales must be float32 {list(scales)}, got {k_scale.dtype} {tuple(k_scale.shape)} and "
+                             f"{v_scale.dtype} {tuple(v_scale.shape)}")
+        if not (v8.device == k_scale.device == v_scale.device == dev and k8.is_contiguous() and v8.is_contiguous()
+                and k_scale.is_contiguous() and v_scale.is_contiguous()):
+            raise ValueError("the store's tensors must be contiguous and on one device")
         self.k8, self.v8, self.k_scale, self.v_scale = k8, v8, k_scale, v_scale
         self.device = dev
         self._code = _CODES[k8.dtype]
-        self._sizes = {}
 
     @classmethod
     def empty(cls, BH, cap, dtype=torch.float8_e4m3fn, d=D, device=None):
@@ -77,12 +81,11 @@ class RowStore8:
         """The entry point on the store's device and its current stream."""
         dev = self.device.index
         fn = getattr(_lib.lib(), name)
-        stream = torch._C._cuda_getCurrentRawStream(dev)
-        if torch._C._cuda_getDevice() == dev:
-            rc = fn(*args, stream)
+        if _current_device() == dev:
+            rc = fn(*args, _raw_stream(dev))
         else:
             with torch.cuda.device(dev):
-                rc = fn(*args, stream)
+                rc = fn(*args, _raw_stream(dev))
         if rc:
             _lib.check(rc, name)
 
@@ -101,9 +104,10 @@ class RowStore8:
             self._elsewhere(v)
         if v.shape != (self.BH,) or v.dtype.is_floating_point or v.dtype == torch.bool:
             raise ValueError(f"{what} must be an int or integers [{self.BH}], got {v.dtype} {tuple(v.shape)}")
-        if v.dtype == torch.int64:  # places beyond int32 stay beyond every store
+        if v.dtype == _I64:  # places beyond int32 stay beyond every store
             v = v.clamp(-(1 << 31), (1 << 31) - 1)
-        v = v.to(torch.int32).contiguous()
+        if v.dtype != _I32 or not v.is_contiguous():
+            v = v.to(_I32).contiguous()
         return v, v.data_ptr(), 0
 
     def _query(self, q, scale, softcap, slopes):
@@ -113,7 +117,8 @@ class RowStore8:
         shape = q.shape
         if len(shape) != 3 or shape[0] != self.BH or shape[2] != self.d or shape[1] < 1:
             raise ValueError(f"q {tuple(shape)} must be [{self.BH}, G, {self.d}]")
-        q = (q if q.dtype in _KDT else q.float()).contiguous()
+        if q.dtype not in _KDT or not q.is_contiguous():
+            q = (q if q.dtype in _KDT else q.float()).contiguous()
         at = q.data_ptr()
         if at % 16:
             q = q.clone()
@@ -124,16 +129,17 @@ class RowStore8:
         if slopes is not None:
             if slopes.device != self.device:
                 self._elsewhere(slopes)
-            slopes = slopes.float().expand(shape[:2]).contiguous()
+            if slopes.dtype != _F32 or slopes.shape != shape[:2] or not slopes.is_contiguous():
+                slopes = slopes.float().expand(shape[:2]).contiguous()
         return q, at, self.d ** -0.5 if scale is None else float(scale), softcap, slopes
 
     def _workspace(self, query, G, positions):
         """The call's workspace (or None), its address and size, for at least `positions`: sizes grow with them, so one query
         serves up to the next power of two."""
-        key = query, G, positions.bit_length()
-        nbytes = self._sizes.get(key)
+        key = query, self.BH, G, self.d, positions.bit_length()
+        nbytes = _SIZES.get(key)
         if nbytes is None:
-            nbytes = self._sizes[key] = getattr(_lib.lib(), query)(self.BH, G, self.d, 1 << positions.bit_length())
+            nbytes = _SIZES[key] = getattr(_lib.lib(), query)(self.BH, G, self.d, 1 << positions.bit_length())
         if not nbytes:
             return None, None, 0
         ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
@@ -168,7 +174,7 @@ class RowStore8:
             raise ValueError(f"dtype {dtype} unsupported (float32, float16, bfloat16)")
         if R < 0:
             raise ValueError(f"{R} tokens")
-        K = torch.empty(self.BH, R, self.d, dtype=dtype, device=self.device)
+        K = torch.empty((self.BH, R, self.d), dtype=dtype, device=self.device)
         V = torch.empty_like(K)
         self._call("fathom_rows8_read", *self._store(), self._code, self.BH, self.cap, self.d, idx_at, rows_at, at, R,
                    _KDT[dtype], K.data_ptr(), V.data_ptr())
@@ -187,7 +193,8 @@ class RowStore8:
             self._elsewhere(idx)
         if idx.dim() != 2 or idx.shape[0] != self.BH:
             raise ValueError(f"idx {tuple(idx.shape)} must be [{self.BH}, R]")
-        idx = idx.to(torch.int64).contiguous()
+        if idx.dtype != _I64 or not idx.is_contiguous():
+            idx = idx.to(_I64).contiguous()
         return self._read(idx.data_ptr(), None, 0, idx.shape[1], dtype)
 
     # ------------------------------------------------------------------ attention
@@ -205,7 +212,7 @@ class RowStore8:
         positions = n if lens is None else self.cap
         positions = max(min(positions, window) if window > 0 else positions, 0)
         ws, ws_at, nbytes = self._workspace("fathom_rows8_attention_workspace_bytes", G, positions)
-        out = torch.empty(q.shape, dtype=torch.float32, device=self.device)
+        out = torch.empty_like(q, dtype=_F32)
         self._call("fathom_rows8_attention", q_at, _KDT[q.dtype], *self._store(), self._code, self.BH, G, self.d, self.cap,
                    lens_at, n, window, scale, softcap, None if slopes is None else slopes.data_ptr(), out.data_ptr(), ws_at,
                    nbytes)
@@ -221,13 +228,15 @@ class RowStore8:
         if idx.device != self.device:
             self._elsewhere(idx)
         G = q.shape[1]
-        if idx.dim() != 3 or idx.shape[:2] != q.shape[:2]:
+        shape = idx.shape
+        if len(shape) != 3 or shape[0] != self.BH or shape[1] != G:
             raise ValueError(f"idx {tuple(idx.shape)} must be [{self.BH}, {G}, k]")
-        idx = idx.to(torch.int64).contiguous()
-        k = idx.shape[2]
+        if idx.dtype != _I64 or not idx.is_contiguous():
+            idx = idx.to(_I64).contiguous()
+        k = shape[2]
         lens, lens_at, n = self._per_row(self.cap if length is None else length, "length")
         ws, ws_at, nbytes = self._workspace("fathom_rows8_gather_attention_workspace_bytes", G, k)
-        out = torch.empty(q.shape, dtype=torch.float32, device=self.device)
+        out = torch.empty_like(q, dtype=_F32)
         self._call("fathom_rows8_gather_attention", q_at, _KDT[q.dtype], idx.data_ptr(), *self._store(), self._code, self.BH, G,
                    k, self.d, self.cap, lens_at, n, scale, softcap, None if slopes is None else slopes.data_ptr(),
                    out.data_ptr(), ws_at, nbytes)

@@ -13,7 +13,6 @@ namespace fathom {
 namespace rows8 {
 namespace {
 
-constexpr int kWaves = 4;       // of a workgroup of list_kernel
 constexpr int kDenseWaves = 4;  // of a workgroup of dense_kernel
 constexpr int kTile = 32;  // listed positions of a wave at a time
 constexpr int kMergeThreads = 256;
@@ -58,131 +57,6 @@ __device__ __forceinline__ void load8_q(const void *q, int dt, int64_t i, float 
   }
 }
 
-// Adds (m1, l1, o1) to the running (m, l, o) of a softmax (maxima in log2 units).
-template <int N>
-__device__ __forceinline__ void join(float &m, float &l, float (&o)[N], float m1, float l1, const float (&o1)[N]) {
-  const float M = fmaxf(m, m1);
-  const float f = __builtin_amdgcn_exp2f(m - M), f1 = __builtin_amdgcn_exp2f(m1 - M);
-  l = l * f + l1 * f1;
-#pragma unroll
-  for (int e = 0; e < N; ++e) o[e] = o[e] * f + o1[e] * f1;
-  m = M;
-}
-
-// Attention over listed tokens: one workgroup per (split, query head, row); its
-// waves take tiles of 32 positions in turn.  16 channels of a row per lane.
-template <int D, bool I8>
-__global__ __launch_bounds__(kWaves *kWave) void list_kernel(AttnArgs a) {
-  constexpr int kLanes = D / 16;         // lanes of a row
-  constexpr int kRows = kWave / kLanes;  // rows of a load
-  constexpr int kLoads = kTile / kRows;
-  __shared__ float wm[kWaves], wl[kWaves], wo[kWaves][D];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int64_t s = blockIdx.x, g = blockIdx.y, bh = blockIdx.z;
-  const int d0 = 16 * (lane % kLanes), rg = lane / kLanes;
-  const int64_t len = row_length(a.lens, a.n, a.cap, bh);
-  const int64_t count = a.k;
-  const float slope = a.slopes ? a.slopes[bh * a.G + g] * kLog2e : 0.0f;
-  float q[2][8];
-#pragma unroll
-  for (int h = 0; h < 2; ++h) load8_q(a.q, a.q_dtype, (bh * a.G + g) * D + d0 + 8 * h, q[h]);
-  float m = kLowest, l = 0.0f, o[16];
-#pragma unroll
-  for (int e = 0; e < 16; ++e) o[e] = 0.0f;
-  for (int64_t t0 = (s * kWaves + wave) * kTile; t0 < count; t0 += a.nsplit * kWaves * kTile) {
-    int64_t tok[kLoads];
-    bool in[kLoads];
-    uint4 kc[kLoads], vc[kLoads];
-    float ks[kLoads], vs[kLoads], z[kLoads];
-#pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      const int64_t j = t0 + i * kRows + rg;
-      tok[i] = j >= count ? -1 : a.idx[(bh * a.G + g) * a.k + j];
-      in[i] = tok[i] >= 0 && tok[i] < len;
-      kc[i] = vc[i] = make_uint4(0u, 0u, 0u, 0u);
-      ks[i] = vs[i] = 0.0f;
-      if (in[i]) {
-        const int64_t at = (bh * a.cap + tok[i]) * D + d0, b = bh * a.nblk + tok[i] / kBlk;
-        kc[i] = *reinterpret_cast<const uint4 *>(a.k8 + at);
-        vc[i] = *reinterpret_cast<const uint4 *>(a.v8 + at);
-        ks[i] = a.ks[b];
-        vs[i] = a.vs[b];
-      }
-    }
-    float mt = m;
-#pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      const uint32_t w[4] = {kc[i].x, kc[i].y, kc[i].z, kc[i].w};
-      float dot = 0.0f;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        float c[4];
-        decode4<I8>(w[e], c);
-#pragma unroll
-        for (int f = 0; f < 4; ++f) dot = fmaf(q[e / 2][4 * (e & 1) + f], c[f], dot);
-      }
-#pragma unroll
-      for (int x = 1; x < kLanes; x <<= 1) dot += __shfl_xor(dot, x);
-      float u = dot * (ks[i] * a.scale);
-      if (a.softcap > 0.0f) u = a.softcap * tanhf(u / a.softcap);
-      u *= kLog2e;
-      z[i] = in[i] ? fmaf(slope, (float)(tok[i] - (len - 1)), u) : -INFINITY;
-      mt = fmaxf(mt, z[i]);
-    }
-    const float f = __builtin_amdgcn_exp2f(m - mt);
-    l *= f;
-#pragma unroll
-    for (int e = 0; e < 16; ++e) o[e] *= f;
-    m = mt;
-#pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      const float p = __builtin_amdgcn_exp2f(z[i] - m);
-      l += p;
-      const float pv = p * vs[i];
-      const uint32_t w[4] = {vc[i].x, vc[i].y, vc[i].z, vc[i].w};
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        float c[4];
-        decode4<I8>(w[e], c);
-#pragma unroll
-        for (int x = 0; x < 4; ++x) o[4 * e + x] = fmaf(pv, c[x], o[4 * e + x]);
-      }
-    }
-  }
-  // the wave's row groups, then the workgroup's waves
-#pragma unroll
-  for (int x = kLanes; x < kWave; x <<= 1) {
-    float o1[16];
-#pragma unroll
-    for (int e = 0; e < 16; ++e) o1[e] = __shfl_xor(o[e], x);
-    const float m1 = __shfl_xor(m, x), l1 = __shfl_xor(l, x);
-    join<16>(m, l, o, m1, l1, o1);
-  }
-  if (rg == 0)
-#pragma unroll
-    for (int e = 0; e < 16; ++e) wo[wave][d0 + e] = o[e];
-  if (lane == 0) {
-    wm[wave] = m;
-    wl[wave] = l;
-  }
-  __syncthreads();
-  if (tid < D) {
-    float M = wm[0], L = wl[0], O[1] = {wo[0][tid]};
-    for (int v = 1; v < kWaves; ++v) {
-      const float o1[1] = {wo[v][tid]};
-      join<1>(M, L, O, wm[v], wl[v], o1);
-    }
-    const int64_t r = bh * a.G + g;
-    if (a.nsplit == 1) {
-      a.out[r * D + tid] = L == 0.0f ? 0.0f : O[0] / L;
-    } else {
-      const int64_t at = (bh * a.nsplit + s) * a.G + g;
-      a.part[at * D + tid] = O[0];
-      if (tid == 0) a.ml[at] = make_float2(M, L);
-    }
-  }
-}
-
 // Sum or maximum over the four lanes l, l ^ 16, l ^ 32, l ^ 48 (v_permlane32_swap
 // and v_permlane16_swap give each lane its partner's value).
 template <bool MAX>
@@ -194,6 +68,179 @@ __device__ __forceinline__ float across_groups(float v) {
   const uint32_t y = __float_as_uint(v);
   const auto p16 = __builtin_amdgcn_permlane16_swap(y, y, false, false);
   return op(__uint_as_float(p16[0]), __uint_as_float(p16[1]));
+}
+
+
+// v of another lane of the same row of 16, by a DPP control.
+template <int CTRL>
+__device__ __forceinline__ float dpp(float v) {
+  return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), CTRL, 0xF, 0xF, false));
+}
+constexpr int kXor1 = 0xB1, kXor2 = 0x4E;           // quad_perm [1,0,3,2], [2,3,0,1]
+constexpr int kHalfMirror = 0x141;                  // row_half_mirror: lane 7 - l of a half row
+constexpr int kRor4 = 0x124, kXor8 = 0x128;         // row_ror:4 and :8
+
+// Sum over the LANES lanes (4 or 8) that hold one row; row_half_mirror pairs quads
+// whose lanes already agree.
+template <int LANES>
+__device__ __forceinline__ float sum_row(float v) {
+  v += dpp<kXor1>(v);
+  v += dpp<kXor2>(v);
+  if constexpr (LANES == 8) v += dpp<kHalfMirror>(v);
+  return v;
+}
+// Sum or maximum over the wave's groups of LANES lanes, lane by lane; first inside a row of 16.
+template <int LANES, bool MAX>
+__device__ __forceinline__ float over_row16(float v) {
+  if constexpr (LANES == 4) v = MAX ? fmaxf(v, dpp<kRor4>(v)) : v + dpp<kRor4>(v);
+  return MAX ? fmaxf(v, dpp<kXor8>(v)) : v + dpp<kXor8>(v);
+}
+template <int LANES, bool MAX>
+__device__ __forceinline__ float over_rows(float v) {
+  return across_groups<MAX>(over_row16<LANES, MAX>(v));
+}
+
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+__device__ const u32x4 kNoRow[8] = {};  // the row of a token that takes no part
+
+// Attention over listed tokens: one workgroup of NW waves per (split, query head,
+// row); its waves take tiles of 32 positions in turn.  A row is 16 channels in
+// each of D / 16 lanes, and those lanes keep a softmax of their own (maximum, sum,
+// weighted rows) over the positions they see, so that nothing crosses lanes inside
+// the loop but the score's sum.  All pieces of a tile, K's first, are requested before the
+// first score.  The groups of lanes are joined at the end by row swaps that add two
+// channels at once (16 channels over 64 lanes: 12 swaps and 4 or 8 rotations), the waves in
+// LDS.
+//
+// Bound: latency (index, then row, then the joins): 512 positions of 32 x 4 heads move
+// 17.5 MB.
+template <int D, bool I8, int NW>
+__global__ __launch_bounds__(NW *kWave) void list_kernel(AttnArgs a) {
+  constexpr int kLanes = D / 16;         // lanes of a row
+  constexpr int kRows = kWave / kLanes;  // rows of a load
+  constexpr int kLoads = kTile / kRows;
+  __shared__ float wm[NW], wl[NW], wo[NW][D];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int64_t s = blockIdx.x, g = blockIdx.y, bh = blockIdx.z;
+  const int d0 = 16 * (lane % kLanes), rg = lane / kLanes;
+  const int64_t len = row_length(a.lens, a.n, a.cap, bh);
+  const float slope = a.slopes ? a.slopes[bh * a.G + g] * kLog2e : 0.0f;
+  const int64_t *idx = a.idx + (bh * a.G + g) * a.k;
+  const uint8_t *kb = a.k8 + bh * a.cap * D + d0, *vb = a.v8 + bh * a.cap * D + d0;
+  const float *ksb = a.ks + bh * a.nblk, *vsb = a.vs + bh * a.nblk;
+  const uint8_t *none = reinterpret_cast<const uint8_t *>(kNoRow);
+  float q[2][8];
+  float m = kLowest, l = 0.0f, o[16];
+#pragma unroll
+  for (int e = 0; e < 16; ++e) o[e] = 0.0f;
+  bool first = true;
+  for (int64_t t0 = (s * NW + wave) * kTile; t0 < a.k; t0 += a.nsplit * NW * kTile) {
+    int64_t tok[kLoads];
+    bool in[kLoads];
+    u32x4 kc[kLoads], vc[kLoads];
+    float ks[kLoads], vs[kLoads], z[kLoads];
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int64_t j = t0 + i * kRows + rg;
+      tok[i] = idx[j < a.k ? j : a.k - 1];
+      in[i] = j < a.k && tok[i] >= 0 && tok[i] < len;
+    }
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      kc[i] = *reinterpret_cast<const u32x4 *>(in[i] ? kb + tok[i] * D : none);
+      ks[i] = ksb[in[i] ? (uint64_t)tok[i] / kBlk : 0];
+    }
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      vc[i] = *reinterpret_cast<const u32x4 *>(in[i] ? vb + tok[i] * D : none);
+      vs[i] = vsb[in[i] ? (uint64_t)tok[i] / kBlk : 0];
+    }
+    if (first) {
+      first = false;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) load8_q(a.q, a.q_dtype, (bh * a.G + g) * D + d0 + 8 * h, q[h]);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    float mt = m;
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      float dot = 0.0f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float c[4];
+        decode4<I8>(kc[i][e], c);
+#pragma unroll
+        for (int f = 0; f < 4; ++f) dot = fmaf(q[e / 2][4 * (e & 1) + f], c[f], dot);
+      }
+      float u = sum_row<kLanes>(dot) * (ks[i] * a.scale);
+      if (a.softcap > 0.0f) u = a.softcap * tanhf(u / a.softcap);
+      u = fmaf(slope, (float)(tok[i] - (len - 1)), u * kLog2e);
+      z[i] = in[i] ? u : -INFINITY;
+      mt = fmaxf(mt, z[i]);
+    }
+    const float f = __builtin_amdgcn_exp2f(m - mt);
+    l *= f;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[e] *= f;
+    m = mt;
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const float p = __builtin_amdgcn_exp2f(z[i] - m);
+      l += p;
+      const float pv = in[i] ? p * vs[i] : 0.0f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float c[4];
+        decode4<I8>(vc[i][e], c);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) o[4 * e + x] = fmaf(pv, c[x], o[4 * e + x]);
+      }
+    }
+  }
+  // ---- the wave's groups against its maximum
+  const float M = over_rows<kLanes, true>(m);
+  const float f = __builtin_amdgcn_exp2f(m - M);
+  l = over_rows<kLanes, false>(l * f);
+  float r[4];
+  {
+    float h[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {  // lanes 0 .. 31: channel e, lanes 32 .. 63: channel e + 8
+      const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(o[e] * f), __float_as_uint(o[e + 8] * f), false, false);
+      h[e] = __uint_as_float(x[0]) + __uint_as_float(x[1]);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {  // odd rows of 16 lanes: channel e + 4
+      const auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(h[e]), __float_as_uint(h[e + 4]), false, false);
+      r[e] = over_row16<kLanes, false>(__uint_as_float(x[0]) + __uint_as_float(x[1]));
+    }
+  }
+  if ((lane & 15) < kLanes)
+    *reinterpret_cast<float4 *>(&wo[wave][d0 + 8 * (lane >> 5) + 4 * (lane >> 4 & 1)]) = make_float4(r[0], r[1], r[2], r[3]);
+  if (lane == 0) {
+    wm[wave] = M;
+    wl[wave] = l;
+  }
+  __syncthreads();
+  if (tid < D) {
+    float mx = wm[0];
+#pragma unroll
+    for (int v = 1; v < NW; ++v) mx = fmaxf(mx, wm[v]);
+    float L = 0.0f, O = 0.0f;
+#pragma unroll
+    for (int v = 0; v < NW; ++v) {
+      const float e = __builtin_amdgcn_exp2f(wm[v] - mx);
+      L = fmaf(wl[v], e, L);
+      O = fmaf(wo[v][tid], e, O);
+    }
+    if (a.nsplit == 1) {
+      a.out[(bh * a.G + g) * D + tid] = L == 0.0f ? 0.0f : O / L;
+    } else {
+      const int64_t at = (bh * a.nsplit + s) * a.G + g;
+      a.part[at * D + tid] = O;
+      if (tid == 0) a.ml[at] = make_float2(mx, L);
+    }
+  }
 }
 
 template <int N>
@@ -218,7 +265,6 @@ struct RowsOf {
                                              0x00027000);
   }
   typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
-  typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
   __device__ __forceinline__ u32x4 load16(int off) const {
     return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, off, 0, 0));
   }
@@ -231,8 +277,6 @@ struct RowsOf {
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
-typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 
 
 // Bytes 0, 1 (HI: 2, 3) of a dword of codes as two f16 values (exact: e4m3 and
@@ -278,7 +322,7 @@ struct Part {
 // Rows of their own lengths (on the device): every workgroup takes `per` blocks, so
 // that the longest row does not hold the call up.  Each wave sums the rows'
 // blocks (a lane per row), which gives `per`, and finds its workgroup's row in the prefix sums
-// of ceil(blocks / per).  Those are at most kDenseGroups / groups + BH, the grid.
+// of ceil(blocks / per).  Those are at most kDenseGroups / head groups + BH, the grid.
 __device__ __forceinline__ Part find_part(const AttnArgs &a, int w) {
   const int lane = threadIdx.x & 63;
   auto blocks = [&](int64_t r) {
@@ -289,7 +333,9 @@ __device__ __forceinline__ Part find_part(const AttnArgs &a, int w) {
   };
   int64_t total = 0;
   for (int64_t r0 = 0; r0 < a.BH; r0 += kWave) total += wave_sum_i(blocks(r0 + lane));
-  const int groups = kDenseGroups / (int)a.groups > 0 ? kDenseGroups / (int)a.groups : 1;
+  // a row's last workgroup may have less to do: with BH of them, the call's workgroups are
+  // at most kDenseGroups, all at work at once
+  const int fit = kDenseGroups / (int)a.groups, groups = fit > 2 * a.BH ? fit - (int)a.BH : fit / 2 > 0 ? fit / 2 : 1;
   const int even = __builtin_amdgcn_readfirstlane((int)((total + groups - 1) / groups));
   Part p{a.BH, 0, 0, even > kDenseWaves ? even : kDenseWaves};
   uint32_t before = 0;
@@ -651,10 +697,19 @@ __global__ __launch_bounds__(kMergeThreads) void merge_kernel(AttnArgs a) {
   }
 }
 
-// Splits of a head's listed positions: enough workgroups for the chip, at least one tile each.
-int64_t list_splits(int64_t heads, int64_t positions) {
-  const int64_t most = cdiv(positions, (int64_t)kWaves * kTile);
-  int64_t want = cdiv((int64_t)2048, heads);
+// Waves of list_kernel's workgroups, by the same rule as gather_attention's: 16 (512
+// positions) for heads of 129 to 512, which then need no join of splits, and
+// for longer ones where that still gives about a workgroup to every other CU; else 4.
+int list_waves(int64_t heads, int64_t k) {
+  constexpr int64_t kOne = 16 * kTile;
+  if (k <= kOne) return k > 4 * kTile ? 16 : 4;
+  return heads * cdiv(k, kOne) >= 96 ? 16 : 4;
+}
+// Splits of a head's listed positions: a tile per wave, as long as the chip has room for more workgroups.
+int64_t list_splits(int64_t heads, int64_t k) {
+  const int waves = list_waves(heads, k);
+  const int64_t most = cdiv(k, (int64_t)waves * kTile);
+  int64_t want = cdiv((int64_t)8192 / waves, heads);
   if (want > kMaxSplits) want = kMaxSplits;
   const int64_t s = most < want ? most : want;
   return s < 1 ? 1 : s;
@@ -698,12 +753,18 @@ int merge(const AttnArgs &a, int64_t BH, int64_t D, hipStream_t st) {
   return launch_status("rows8 merge_kernel");
 }
 
-int run_list(AttnArgs a, int64_t BH, int64_t D, bool i8, hipStream_t st) {
+template <int D, bool I8>
+void launch_list(const AttnArgs &a, int64_t BH, hipStream_t st) {
   const dim3 grid((unsigned)a.nsplit, (unsigned)a.G, (unsigned)BH);
-  if (D == 128 && i8) list_kernel<128, true><<<grid, kWaves * kWave, 0, st>>>(a);
-  else if (D == 128) list_kernel<128, false><<<grid, kWaves * kWave, 0, st>>>(a);
-  else if (i8) list_kernel<64, true><<<grid, kWaves * kWave, 0, st>>>(a);
-  else list_kernel<64, false><<<grid, kWaves * kWave, 0, st>>>(a);
+  if (list_waves(BH * a.G, a.k) == 16) list_kernel<D, I8, 16><<<grid, 16 * kWave, 0, st>>>(a);
+  else list_kernel<D, I8, 4><<<grid, 4 * kWave, 0, st>>>(a);
+}
+
+int run_list(AttnArgs a, int64_t BH, int64_t D, bool i8, hipStream_t st) {
+  if (D == 128 && i8) launch_list<128, true>(a, BH, st);
+  else if (D == 128) launch_list<128, false>(a, BH, st);
+  else if (i8) launch_list<64, true>(a, BH, st);
+  else launch_list<64, false>(a, BH, st);
   const int rc = launch_status("rows8 list_kernel");
   return rc || a.nsplit == 1 ? rc : merge(a, BH, D, st);
 }
@@ -791,7 +852,11 @@ extern "C" int fathom_rows8_attention(const void *q, int q_dtype, const void *k8
 
 extern "C" size_t fathom_rows8_gather_attention_workspace_bytes(int64_t BH, int64_t G, int64_t D, int64_t k) {
   if (BH < 1 || G < 1 || D < 1 || k < 1) return 0;
-  const int64_t ns = list_splits(BH * G, k);
+  if (k <= 16 * kTile) return 0;
+  // of the narrower workgroups, so that it never falls as k grows
+  int64_t ns = cdiv(k, (int64_t)4 * kTile);
+  if (ns > cdiv((int64_t)2048, BH * G)) ns = cdiv((int64_t)2048, BH * G);
+  if (ns > kMaxSplits) ns = kMaxSplits;
   return part_bytes(BH, G, D, ns > 1 ? BH * ns : 0);
 }
 

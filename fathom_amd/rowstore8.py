@@ -136,10 +136,13 @@ class RowStore8:
     def _workspace(self, query, G, positions):
         """The call's workspace (or None), its address and size, for at least `positions`: sizes grow with them, so one query
         serves up to the next power of two."""
-        key = query, self.BH, G, self.d, positions.bit_length()
+        if positions < 1:
+            return None, None, 0
+        bits = (positions - 1).bit_length()
+        key = query, self.BH, G, self.d, bits
         nbytes = _SIZES.get(key)
         if nbytes is None:
-            nbytes = _SIZES[key] = getattr(_lib.lib(), query)(self.BH, G, self.d, 1 << positions.bit_length())
+            nbytes = _SIZES[key] = getattr(_lib.lib(), query)(self.BH, G, self.d, 1 << bits)
         if not nbytes:
             return None, None, 0
         ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device)

@@ -13,10 +13,9 @@ namespace fathom {
 namespace rows8 {
 namespace {
 
-constexpr int kDenseWaves = 4;  // of a workgroup of dense_kernel
 constexpr int kTile = 32;  // listed positions of a wave at a time
 constexpr int kMergeThreads = 256;
-constexpr int kDenseGroups = 2048 / kDenseWaves;  // workgroups of a dense call: eight waves per CU
+constexpr int kDenseTotal = 2048;  // waves of a dense call: eight per CU, all at work at once
 constexpr int kMaxSplits = 512;  // of a query head
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLowest = -3.0e38f;  // below every score: the running maximum of no token
@@ -322,7 +321,8 @@ struct Part {
 // Rows of their own lengths (on the device): every workgroup takes `per` blocks, so
 // that the longest row does not hold the call up.  Each wave sums the rows'
 // blocks (a lane per row), which gives `per`, and finds its workgroup's row in the prefix sums
-// of ceil(blocks / per).  Those are at most kDenseGroups / head groups + BH, the grid.
+// of ceil(blocks / per).  Those are at most kDenseTotal / NW / head groups + BH, the grid.
+template <int NW>
 __device__ __forceinline__ Part find_part(const AttnArgs &a, int w) {
   const int lane = threadIdx.x & 63;
   auto blocks = [&](int64_t r) {
@@ -334,10 +334,10 @@ __device__ __forceinline__ Part find_part(const AttnArgs &a, int w) {
   int64_t total = 0;
   for (int64_t r0 = 0; r0 < a.BH; r0 += kWave) total += wave_sum_i(blocks(r0 + lane));
   // a row's last workgroup may have less to do: with BH of them, the call's workgroups are
-  // at most kDenseGroups, all at work at once
-  const int fit = kDenseGroups / (int)a.groups, groups = fit > 2 * a.BH ? fit - (int)a.BH : fit / 2 > 0 ? fit / 2 : 1;
+  // at most kDenseTotal / NW, all at work at once
+  const int fit = kDenseTotal / NW / (int)a.groups, groups = fit > 2 * a.BH ? fit - (int)a.BH : fit / 2 > 0 ? fit / 2 : 1;
   const int even = __builtin_amdgcn_readfirstlane((int)((total + groups - 1) / groups));
-  Part p{a.BH, 0, 0, even > kDenseWaves ? even : kDenseWaves};
+  Part p{a.BH, 0, 0, even > NW ? even : NW};
   uint32_t before = 0;
   for (int64_t r0 = 0; r0 < a.BH; r0 += kWave) {
     // a row without tokens takes a workgroup too: it writes the row's zeros
@@ -382,19 +382,19 @@ __device__ __forceinline__ Part find_part(const AttnArgs &a, int w) {
 //
 // Bound: HBM, 2 D bytes per token; the next block's K rows are requested once
 // the scores are formed, its V rows once the products are.
-template <int D, bool I8, int NG, bool EXTRA>
-__global__ __launch_bounds__(kDenseWaves *kWave, NG == 1 ? 2 : 1) void dense_kernel(AttnArgs a) {
+template <int D, bool I8, int NG, bool EXTRA, int NW>
+__global__ __launch_bounds__(NW *kWave, 2) void dense_kernel(AttnArgs a) {
   constexpr int kHalves = D / 64;  // 16-byte pieces of a row per lane
   constexpr int kSteps = D / 32;   // matrix instructions along the channels
   constexpr int kCh = D / 16;      // channels of V per lane
-  __shared__ float wm[kDenseWaves][8 * NG], wl[kDenseWaves][8 * NG], wo[kDenseWaves][8 * NG][D];
+  __shared__ float wm[NW][8 * NG], wl[NW][8 * NG], wo[NW][8 * NG][D + 4];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, grp = lane >> 4;
   const int64_t g0 = (int64_t)blockIdx.y * 8 * NG;
   Part part{(int64_t)blockIdx.z, (int)blockIdx.x, (int)a.nsplit, 0};
   int64_t slot = (int64_t)blockIdx.z * a.nsplit + blockIdx.x;  // of the partial results
   if (a.where) {
-    part = find_part(a, (int)blockIdx.x);
+    part = find_part<NW>(a, (int)blockIdx.x);
     if (part.bh >= a.BH) return;
     slot = blockIdx.x;
     if (part.split == 0 && blockIdx.y == 0 && tid == 0) a.where[part.bh] = make_int2((int)blockIdx.x, part.active);
@@ -407,6 +407,15 @@ __global__ __launch_bounds__(kDenseWaves *kWave, NG == 1 ? 2 : 1) void dense_ker
   const int64_t first = blk0 + (int64_t)part.split * part.per;
   const int64_t last = part.split + 1 < part.active ? first + part.per : blk0 + nb;
 
+  // the queries are requested first and made ready while the first block's rows come
+  float q[NG][kSteps][8];
+#pragma unroll
+  for (int n = 0; n < NG; ++n) {
+    const int64_t g = g0 + 8 * n + (col & 7), row = (bh * a.G + (g < a.G ? g : a.G - 1)) * D;
+#pragma unroll
+    for (int h = 0; h < kSteps; ++h)  // step h = (piece, half): channels 64 (h / 2) + 16 grp + 8 (h & 1) + e
+      load8_q(a.q, a.q_dtype, row + 64 * (h / 2) + 16 * grp + 8 * (h & 1), q[n][h]);
+  }
   u32x4 kr[4][kHalves];
   typedef typename VPiece<kCh>::type vpiece;
   vpiece vr[4][4];
@@ -432,16 +441,11 @@ __global__ __launch_bounds__(kDenseWaves *kWave, NG == 1 ? 2 : 1) void dense_ker
 #pragma unroll
   for (int n = 0; n < NG; ++n) {
     const int64_t g = g0 + 8 * n + (col & 7);
-    const bool has = g < a.G;
-    const int64_t row = (bh * a.G + (has ? g : a.G - 1)) * D;
-    float q[kSteps][8], mx = 0.0f;
+    float mx = 0.0f;
 #pragma unroll
-    for (int h = 0; h < kSteps; ++h) {
-      // step h = (piece, half): channels 64 (h / 2) + 16 grp + 8 (h & 1) + e
-      load8_q(a.q, a.q_dtype, row + 64 * (h / 2) + 16 * grp + 8 * (h & 1), q[h]);
+    for (int h = 0; h < kSteps; ++h)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(q[h][e]));
-    }
+      for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(q[n][h][e]));
     mx = across_groups<true>(mx);
     int sigma = 0;  // the largest |q| of the head in [2^13, 2^14)
     if (mx > 0.0f && mx < INFINITY) {
@@ -452,12 +456,12 @@ __global__ __launch_bounds__(kDenseWaves *kWave, NG == 1 ? 2 : 1) void dense_ker
     for (int h = 0; h < kSteps; ++h)
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float x = ldexpf(q[h][e], sigma);
+        const float x = ldexpf(q[n][h][e], sigma);
         const _Float16 hi = (_Float16)x;
         qf[n][h][e] = col < 8 ? hi : (_Float16)(x - (float)hi);
       }
     fac[n] = ldexpf(EXTRA && a.softcap > 0.0f ? a.scale / a.softcap : a.scale * kLog2e, -sigma);
-    slope[n] = EXTRA && a.slopes && has ? a.slopes[bh * a.G + g] * kLog2e : 0.0f;
+    slope[n] = EXTRA && a.slopes && g < a.G ? a.slopes[bh * a.G + g] * kLog2e : 0.0f;
   }
   const float keep = col < 8 ? 0.0f : -1.0f;  // columns 8 .. 15 hold what the f16 weights leave
 
@@ -472,7 +476,7 @@ __global__ __launch_bounds__(kDenseWaves *kWave, NG == 1 ? 2 : 1) void dense_ker
   }
   int E = -1000;
 
-  for (int64_t b = first + wave; b < last; b += kDenseWaves) {
+  for (int64_t b = first + wave; b < last; b += NW) {
     const float ks = a.ks[bh * a.nblk + b], vs = a.vs[bh * a.nblk + b];
     f32x4 s[NG][4];
 #pragma unroll
@@ -487,7 +491,7 @@ __global__ __launch_bounds__(kDenseWaves *kWave, NG == 1 ? 2 : 1) void dense_ker
         for (int n = 0; n < NG; ++n) s[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qf[n][h], s[n][i], 0, 0, 0);
       }
     }
-    load_k(b + kDenseWaves);
+    load_k(b + NW);
     // ---- scores, in log2 units; tokens outside [lo, len) have none
     const int t0 = (int)(b * kBlk);
     const bool edge = (int64_t)t0 < lo || (int64_t)t0 + kBlk > len;
@@ -582,7 +586,7 @@ __global__ __launch_bounds__(kDenseWaves *kWave, NG == 1 ? 2 : 1) void dense_ker
         }
       }
     }
-    load_v(b + kDenseWaves);
+    load_v(b + NW);
   }
   // ---- the workgroup's waves
   const float up = E > -1000 ? ldexpf(1.0f, E - 14) : 0.0f;
@@ -596,21 +600,25 @@ __global__ __launch_bounds__(kDenseWaves *kWave, NG == 1 ? 2 : 1) void dense_ker
 #pragma unroll
     for (int j = 0; j < 4; ++j)
 #pragma unroll
-      for (int e = 0; e < kCh; ++e) {
-        const float v = add_other_half(o[n][e][j]) * up;
-        if (col < 8) wo[wave][8 * n + col][(4 * grp + j) * kCh + e] = v;
+      for (int e = 0; e < kCh; e += 4) {
+        float4 v;
+        v.x = add_other_half(o[n][e][j]) * up;
+        v.y = add_other_half(o[n][e + 1][j]) * up;
+        v.z = add_other_half(o[n][e + 2][j]) * up;
+        v.w = add_other_half(o[n][e + 3][j]) * up;
+        if (col < 8) *reinterpret_cast<float4 *>(&wo[wave][8 * n + col][(4 * grp + j) * kCh + e]) = v;
       }
   }
   __syncthreads();
-  for (int x = tid; x < 8 * NG * D; x += kDenseWaves * kWave) {
+  for (int x = tid; x < 8 * NG * D; x += NW * kWave) {
     const int h = x / D, d = x % D;
     if (g0 + h >= a.G) break;
     float M = wm[0][h];
 #pragma unroll
-    for (int v = 1; v < kDenseWaves; ++v) M = fmaxf(M, wm[v][h]);
+    for (int v = 1; v < NW; ++v) M = fmaxf(M, wm[v][h]);
     float L = 0.0f, O = 0.0f;
 #pragma unroll
-    for (int v = 0; v < kDenseWaves; ++v) {
+    for (int v = 0; v < NW; ++v) {
       const float e = __builtin_amdgcn_exp2f(wm[v][h] - M);
       L = fmaf(wl[v][h], e, L);
       O = fmaf(wo[v][h][d], e, O);
@@ -626,24 +634,33 @@ __global__ __launch_bounds__(kDenseWaves *kWave, NG == 1 ? 2 : 1) void dense_ker
   }
 }
 
-// Joins the splits of a query head: their factors first, then the weighted rows,
-// 16 bytes per thread and every split of a thread in flight, summed in a fixed order.
+// Joins the splits of a query head, 32 channels per workgroup: a thread takes 16 bytes
+// of every 32nd split, requested before the splits' factors are known; sums run in a fixed order.
 template <int D>
 __global__ __launch_bounds__(kMergeThreads) void merge_kernel(AttnArgs a) {
-  constexpr int kLanes = D / 4, kGroups = kMergeThreads / kLanes;
+  constexpr int kLanes = 8, kGroups = kMergeThreads / kLanes, kBatch = 4;
+  constexpr int kOwn = kMaxSplits / kMergeThreads;  // splits whose factor a thread computes
   __shared__ float fac[kMaxSplits], red[2][kMergeThreads / kWave];
   __shared__ float4 acc[kGroups][kLanes];
   const int64_t r = blockIdx.x;
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, lane = tid % kLanes, grp = tid / kLanes;
   const int64_t bh = r / a.G;
   const int2 w = a.where ? a.where[bh] : make_int2((int)(bh * a.nsplit), (int)a.nsplit);
   const int ns = w.y;
   if (ns <= 1) return;  // written already
   const int64_t at = (int64_t)w.x * a.G + r % a.G;  // split s at + s G
-  float2 x[kMaxSplits / kMergeThreads];
+  const float4 *p = reinterpret_cast<const float4 *>(a.part + at * D + 32 * blockIdx.y) + lane;
+  const int64_t step = a.G * (D / 4);
+  float4 v[kBatch];
+#pragma unroll
+  for (int i = 0; i < kBatch; ++i) {
+    const int s = grp + i * kGroups;
+    v[i] = p[(s < ns ? s : 0) * step];
+  }
+  float2 x[kOwn];
   float m = kLowest;
 #pragma unroll
-  for (int i = 0; i < kMaxSplits / kMergeThreads; ++i) {
+  for (int i = 0; i < kOwn; ++i) {
     const int s = i * kMergeThreads + tid;
     x[i] = s < ns ? a.ml[at + s * a.G] : make_float2(kLowest, 0.0f);
     m = fmaxf(m, x[i].x);
@@ -653,10 +670,10 @@ __global__ __launch_bounds__(kMergeThreads) void merge_kernel(AttnArgs a) {
   if ((tid & 63) == 0) red[0][tid >> 6] = m;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kMergeThreads / kWave; ++w) m = fmaxf(m, red[0][w]);
+  for (int k = 0; k < kMergeThreads / kWave; ++k) m = fmaxf(m, red[0][k]);
   float l = 0.0f;
 #pragma unroll
-  for (int i = 0; i < kMaxSplits / kMergeThreads; ++i) {
+  for (int i = 0; i < kOwn; ++i) {
     const float f = __builtin_amdgcn_exp2f(x[i].x - m);
     fac[i * kMergeThreads + tid] = f;
     l = fmaf(x[i].y, f, l);
@@ -664,23 +681,20 @@ __global__ __launch_bounds__(kMergeThreads) void merge_kernel(AttnArgs a) {
   l = wave_sum_f(l);
   if ((tid & 63) == 0) red[1][tid >> 6] = l;
   __syncthreads();
-  l = 0.0f;
-#pragma unroll
-  for (int w = 0; w < kMergeThreads / kWave; ++w) l += red[1][w];
-  const int lane = tid % kLanes, grp = tid / kLanes;
-  const float4 *p = reinterpret_cast<const float4 *>(a.part) + at * kLanes + lane;
   float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  for (int s0 = grp; s0 < ns; s0 += 8 * kGroups) {
-    float4 v[8];
+  for (int s0 = grp; s0 < ns; s0 += kBatch * kGroups) {
+    if (s0 != grp) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int s = s0 + i * kGroups;
-      v[i] = p[(s < ns ? s : s0) * a.G * kLanes];
+      for (int i = 0; i < kBatch; ++i) {
+        const int s = s0 + i * kGroups;
+        v[i] = p[(s < ns ? s : 0) * step];
+      }
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < kBatch; ++i) {
       const int s = s0 + i * kGroups;
-      const float f = s < ns ? fac[s] : 0.0f;
+      if (s >= ns) break;
+      const float f = fac[s];
       o.x = fmaf(v[i].x, f, o.x);
       o.y = fmaf(v[i].y, f, o.y);
       o.z = fmaf(v[i].z, f, o.z);
@@ -689,11 +703,14 @@ __global__ __launch_bounds__(kMergeThreads) void merge_kernel(AttnArgs a) {
   }
   acc[grp][lane] = o;
   __syncthreads();
-  if (tid < D) {
-    float v = 0.0f;
+  if (tid < 32) {
+    float u = 0.0f;
 #pragma unroll
-    for (int g = 0; g < kGroups; ++g) v += reinterpret_cast<const float *>(acc[g])[tid];
-    a.out[r * D + tid] = l == 0.0f ? 0.0f : v / l;
+    for (int g = 0; g < kGroups; ++g) u += reinterpret_cast<const float *>(acc[g])[tid];
+    l = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kMergeThreads / kWave; ++k) l += red[1][k];
+    a.out[r * D + 32 * blockIdx.y + tid] = l == 0.0f ? 0.0f : u / l;
   }
 }
 
@@ -718,20 +735,38 @@ int64_t list_splits(int64_t heads, int64_t k) {
 // Head groups of a row and their size in eights: a workgroup holds up to 16 heads.
 int64_t head_groups(int64_t G) { return cdiv(G, (int64_t)16); }
 
-// Splits of a row of up to nb blocks in a call of `rows` rows (head groups counted):
-// kDenseGroups workgroups in all, at least one block per wave.
-int64_t dense_splits(int64_t rows, int64_t nb) {
-  const int64_t want = cdiv((int64_t)kDenseGroups, rows), most = cdiv(nb, (int64_t)kDenseWaves);
+// Blocks of a row that one workgroup of eight waves takes: two per wave, and one
+// more as a window of that length may begin inside a block.
+constexpr int64_t kOneGroup = 17;
+
+// Waves of dense_kernel's workgroups, for rows of up to nb blocks in a call of `rows`
+// rows (head groups counted).  Eight where a row then needs no split (up to two blocks per wave: one launch for
+// two), and where a wave takes a few blocks, as fewer splits are joined; four where it takes less than one (a
+// wave alone on its SIMD is done sooner) and where it takes many.
+//   us in a graph, 4 waves; 8: 1 x 4096 tokens 9.6; 11.3, 8 x 8192 12.0; 12.9, 32 x 4096 14.8; 14.5, 1 x 262144
+//   21.3; 19.5, 8 x 131072 55.2; 54.3, 8 x 1048576 366; 372.
+// Lengths on the device are not known here; rows of 16 ragged lengths up to 50021 take 24.8; 22.8.
+int dense_waves(int64_t rows, int64_t nb, bool lens) {
+  if (nb <= 4) return 4;
+  if (nb <= kOneGroup || lens) return 8;
+  return rows * nb > kDenseTotal && rows * nb <= 32 * kDenseTotal ? 8 : 4;
+}
+
+// Splits of such a row: kDenseTotal waves in all, at least one block per wave.
+int64_t dense_splits(int64_t rows, int64_t nb, int waves) {
+  if (nb <= kOneGroup && waves == 8) return 1;
+  const int64_t want = cdiv((int64_t)kDenseTotal / waves, rows), most = cdiv(nb, (int64_t)waves);
   return most < want ? most : want;
 }
 
-// Slots of partial results of a dense call whose longest row has up to nb blocks
-// (with lengths on the device, the bound of find_part); 0: every row fits one
-// workgroup.  Neither falls as nb grows.
+// Slots of partial results of a dense call; 0: every row fits one workgroup.  With
+// lengths on the device: the bound of find_part.
 int64_t dense_slots(int64_t BH, int64_t G, int64_t nb, bool lens) {
-  const int64_t ns = dense_splits(BH * head_groups(G), nb);
+  const int64_t groups = head_groups(G);
+  const int waves = dense_waves(BH * groups, nb, lens);
+  const int64_t ns = dense_splits(BH * groups, nb, waves);
   if (ns <= 1) return 0;
-  const int64_t all = kDenseGroups / head_groups(G) + BH, most = BH * cdiv(nb, (int64_t)kDenseWaves);
+  const int64_t all = kDenseTotal / waves / groups + BH, most = BH * cdiv(nb, (int64_t)waves);
   return !lens ? BH * ns : all < most ? all : most;
 }
 
@@ -748,8 +783,8 @@ void place(AttnArgs &a, void *workspace, int64_t D, int64_t slots, bool lens) {
 }
 
 int merge(const AttnArgs &a, int64_t BH, int64_t D, hipStream_t st) {
-  if (D == 128) merge_kernel<128><<<(unsigned)(BH * a.G), kMergeThreads, 0, st>>>(a);
-  else merge_kernel<64><<<(unsigned)(BH * a.G), kMergeThreads, 0, st>>>(a);
+  if (D == 128) merge_kernel<128><<<dim3((unsigned)(BH * a.G), 4), kMergeThreads, 0, st>>>(a);
+  else merge_kernel<64><<<dim3((unsigned)(BH * a.G), 2), kMergeThreads, 0, st>>>(a);
   return launch_status("rows8 merge_kernel");
 }
 
@@ -769,24 +804,26 @@ int run_list(AttnArgs a, int64_t BH, int64_t D, bool i8, hipStream_t st) {
   return rc || a.nsplit == 1 ? rc : merge(a, BH, D, st);
 }
 
-template <int D, bool I8, int NG>
+template <int D, bool I8, int NG, int NW>
 void launch_dense(const AttnArgs &a, int64_t BH, hipStream_t st) {
   const dim3 grid((unsigned)a.nsplit, (unsigned)head_groups(a.G), a.where ? 1u : (unsigned)BH);
-  if (a.softcap > 0.0f || a.slopes) dense_kernel<D, I8, NG, true><<<grid, kDenseWaves * kWave, 0, st>>>(a);
-  else dense_kernel<D, I8, NG, false><<<grid, kDenseWaves * kWave, 0, st>>>(a);
+  if (a.softcap > 0.0f || a.slopes) dense_kernel<D, I8, NG, true, NW><<<grid, NW * kWave, 0, st>>>(a);
+  else dense_kernel<D, I8, NG, false, NW><<<grid, NW * kWave, 0, st>>>(a);
 }
 
 template <int D, bool I8>
-void launch_dense(const AttnArgs &a, int64_t BH, hipStream_t st) {
-  if (a.G > 8) launch_dense<D, I8, 2>(a, BH, st);
-  else launch_dense<D, I8, 1>(a, BH, st);
+void launch_dense(const AttnArgs &a, int64_t BH, int waves, hipStream_t st) {
+  if (a.G > 8 && waves == 8) launch_dense<D, I8, 2, 8>(a, BH, st);
+  else if (a.G > 8) launch_dense<D, I8, 2, 4>(a, BH, st);
+  else if (waves == 8) launch_dense<D, I8, 1, 8>(a, BH, st);
+  else launch_dense<D, I8, 1, 4>(a, BH, st);
 }
 
-int run_dense(AttnArgs a, int64_t BH, int64_t D, bool i8, hipStream_t st) {
-  if (D == 128 && i8) launch_dense<128, true>(a, BH, st);
-  else if (D == 128) launch_dense<128, false>(a, BH, st);
-  else if (i8) launch_dense<64, true>(a, BH, st);
-  else launch_dense<64, false>(a, BH, st);
+int run_dense(AttnArgs a, int64_t BH, int64_t D, bool i8, int waves, hipStream_t st) {
+  if (D == 128 && i8) launch_dense<128, true>(a, BH, waves, st);
+  else if (D == 128) launch_dense<128, false>(a, BH, waves, st);
+  else if (i8) launch_dense<64, true>(a, BH, waves, st);
+  else launch_dense<64, false>(a, BH, waves, st);
   const int rc = launch_status("rows8 dense_kernel");
   return rc || a.nsplit == 1 ? rc : merge(a, BH, D, st);
 }
@@ -819,9 +856,14 @@ using namespace fathom::rows8;
 
 extern "C" size_t fathom_rows8_attention_workspace_bytes(int64_t BH, int64_t G, int64_t D, int64_t positions) {
   if (BH < 1 || G < 1 || D < 1 || positions < 1) return 0;
-  const int64_t nb = cdiv(positions, (int64_t)kBlk) + 1;  // a window may begin inside a block
-  const int64_t one = dense_slots(BH, G, nb, false), own = dense_slots(BH, G, nb, true);
-  return part_bytes(BH, G, D, one > own ? one : own);
+  // the most slots of any choice of waves, for one length or lengths on the device: does not fall as positions grow
+  const int64_t nb = cdiv(positions, (int64_t)kBlk) + 1, groups = head_groups(G);  // a window may begin inside a block
+  if (nb <= kOneGroup) return 0;
+  const int64_t blocks = cdiv(nb, (int64_t)4), share = cdiv((int64_t)kDenseTotal / 4, BH * groups);
+  int64_t slots = BH * (blocks < share ? blocks : share);
+  const int64_t own = kDenseTotal / 8 / groups + BH, most = BH * cdiv(nb, (int64_t)8);
+  if (slots < (own < most ? own : most)) slots = own < most ? own : most;
+  return part_bytes(BH, G, D, slots);
 }
 
 extern "C" int fathom_rows8_attention(const void *q, int q_dtype, const void *k8, const void *v8, const float *k_scale,
@@ -847,7 +889,7 @@ extern "C" int fathom_rows8_attention(const void *q, int q_dtype, const void *k8
   if (need && reinterpret_cast<uintptr_t>(workspace) & 15)
     return fail(FATHOM_ERR_INVALID, "rows8_attention: the workspace must be 16-byte aligned");
   place(a, workspace, D, slots, lens != nullptr);
-  return run_dense(a, BH, D, code_dtype == FATHOM_DT_I8, (hipStream_t)stream);
+  return run_dense(a, BH, D, code_dtype == FATHOM_DT_I8, dense_waves(BH * a.groups, nb, lens != nullptr), (hipStream_t)stream);
 }
 
 extern "C" size_t fathom_rows8_gather_attention_workspace_bytes(int64_t BH, int64_t G, int64_t D, int64_t k) {

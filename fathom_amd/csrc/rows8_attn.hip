@@ -254,7 +254,11 @@ __device__ __forceinline__ uint32_t dword_of(uint32_t v, int) { return v; }
 __device__ __forceinline__ uint32_t dword_of(VPiece<8>::type v, int d) { return v[d]; }
 
 // Block b of a row's codes through a buffer descriptor that holds its tokens
-// before `end`: loads behind that give zeros.
+// before `end`: loads behind that give zeros.  They are streams (the nt bit): a
+// step reads a row once, and other layers' rows come before its next step.  us with, without, rows
+// that come from HBM: 8 x 1048576 tokens 345, 380; 32 x 32768 52, 57; 16 x 18432 21.6, 22.4 (while they fit the
+// 256 MB cache and nothing else runs: 21.2, 19.9).
+constexpr int kStream = 2;
 struct RowsOf {
   __amdgpu_buffer_rsrc_t rsrc;
   __device__ __forceinline__ RowsOf(const uint8_t *codes, int64_t row0, int64_t b, int64_t end, int D) {
@@ -265,12 +269,12 @@ struct RowsOf {
   }
   typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
   __device__ __forceinline__ u32x4 load16(int off) const {
-    return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, off, 0, 0));
+    return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, off, 0, kStream));
   }
   __device__ __forceinline__ void load(int off, u32x2 &v) const {
-    v = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rsrc, off, 0, 0));
+    v = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rsrc, off, 0, kStream));
   }
-  __device__ __forceinline__ void load(int off, uint32_t &v) const { v = __builtin_amdgcn_raw_buffer_load_b32(rsrc, off, 0, 0); }
+  __device__ __forceinline__ void load(int off, uint32_t &v) const { v = __builtin_amdgcn_raw_buffer_load_b32(rsrc, off, 0, kStream); }
 };
 
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));

@@ -56,6 +56,24 @@ __device__ __forceinline__ void load8_q(const void *q, int dt, int64_t i, float 
   }
 }
 
+// tanh to about a step of float32: below 1/2 u + u^3 P(u^2), P the least-squares fit of
+// degree 4 to (tanh u - u) / u^3; from there (1 - t) / (1 + t), t = e^(-2 |u|), the quotient
+// by the reciprocal and one correction.
+__device__ __forceinline__ float tanh_near(float u) {
+  const float x = fabsf(u), w = u * u;
+  float p = -0.006947011f;
+  p = fmaf(p, w, 0.021472726f);
+  p = fmaf(p, w, -0.05393379f);
+  p = fmaf(p, w, 0.13333227f);
+  p = fmaf(p, w, -0.3333333f);
+  const float near = fmaf(u * w, p, u);
+  const float t = __builtin_amdgcn_exp2f(x * (-2.0f * kLog2e));
+  const float n = 1.0f - t, d = 1.0f + t, r = __builtin_amdgcn_rcpf(d);
+  float far = n * r;
+  far = fmaf(fmaf(-far, d, n), r, far);
+  return x < 0.5f ? near : copysignf(far, u);
+}
+
 // Sum or maximum over the four lanes l, l ^ 16, l ^ 32, l ^ 48 (v_permlane32_swap
 // and v_permlane16_swap give each lane its partner's value).
 template <bool MAX>
@@ -73,7 +91,7 @@ __device__ __forceinline__ float across_groups(float v) {
 // v of another lane of the same row of 16, by a DPP control.
 template <int CTRL>
 __device__ __forceinline__ float dpp(float v) {
-  return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), CTRL, 0xF, 0xF, false));
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xF, 0xF, true));  // folds into its use
 }
 constexpr int kXor1 = 0xB1, kXor2 = 0x4E;           // quad_perm [1,0,3,2], [2,3,0,1]
 constexpr int kHalfMirror = 0x141;                  // row_half_mirror: lane 7 - l of a half row
@@ -172,8 +190,8 @@ __global__ __launch_bounds__(NW *kWave) void list_kernel(AttnArgs a) {
         for (int f = 0; f < 4; ++f) dot = fmaf(q[e / 2][4 * (e & 1) + f], c[f], dot);
       }
       float u = sum_row<kLanes>(dot) * (ks[i] * a.scale);
-      if (a.softcap > 0.0f) u = a.softcap * tanhf(u / a.softcap);
-      u = fmaf(slope, (float)(tok[i] - (len - 1)), u * kLog2e);
+      if (a.softcap > 0.0f) u = a.softcap * tanh_near(u / a.softcap);
+      u = fmaf(slope, (float)(int)(tok[i] - (len - 1)), u * kLog2e);
       z[i] = in[i] ? u : -INFINITY;
       mt = fmaxf(mt, z[i]);
     }
@@ -304,9 +322,16 @@ __device__ __forceinline__ f16x8 join8(f16x2 a, f16x2 b, f16x2 c, f16x2 d) {
   return f16x8{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
 }
 
+// Two floats as f16 (keep = 0), or as the f16 of what those leave (keep = -1): to nearest both times.
+__device__ __forceinline__ f16x2 split16(float x, float y, float keep) {
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  const f16x2 hi = __builtin_convertvector(f32x2{x, y}, f16x2);
+  return __builtin_convertvector(f32x2{fmaf((float)hi.x, keep, x), fmaf((float)hi.y, keep, y)}, f16x2);
+}
+
 // v + the value of the lane 8 columns away in the same row of 16 lanes (row_ror:8).
 __device__ __forceinline__ float add_other_half(float v) {
-  return v + __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x128, 0xF, 0xF, false));
+  return v + dpp<kXor8>(v);
 }
 
 // The blocks of a row that a call takes.
@@ -440,6 +465,7 @@ __global__ __launch_bounds__(NW *kWave, 2) void dense_kernel(AttnArgs a) {
   };
   load_k(first + wave);
   load_v(first + wave);
+  const float keep = col < 8 ? 0.0f : -1.0f;  // columns 8 .. 15 hold what the f16 of columns 0 .. 7 leave
   f16x8 qf[NG][kSteps];
   float fac[NG], slope[NG];  // per lane: its head's factor of a score, its bias per token
 #pragma unroll
@@ -457,17 +483,18 @@ __global__ __launch_bounds__(NW *kWave, 2) void dense_kernel(AttnArgs a) {
       sigma = 14 - sigma;
     }
 #pragma unroll
-    for (int h = 0; h < kSteps; ++h)
+    for (int h = 0; h < kSteps; ++h) {
+      f16x2 part[4];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float x = ldexpf(q[n][h][e], sigma);
-        const _Float16 hi = (_Float16)x;
-        qf[n][h][e] = col < 8 ? hi : (_Float16)(x - (float)hi);
+      for (int e = 0; e < 4; ++e) {
+        const float x = ldexpf(q[n][h][2 * e], sigma), y = ldexpf(q[n][h][2 * e + 1], sigma);
+        part[e] = split16(x, y, keep);
       }
+      qf[n][h] = join8(part[0], part[1], part[2], part[3]);
+    }
     fac[n] = ldexpf(EXTRA && a.softcap > 0.0f ? a.scale / a.softcap : a.scale * kLog2e, -sigma);
     slope[n] = EXTRA && a.slopes && g < a.G ? a.slopes[bh * a.G + g] * kLog2e : 0.0f;
   }
-  const float keep = col < 8 ? 0.0f : -1.0f;  // columns 8 .. 15 hold what the f16 weights leave
 
   f32x4 o[NG][kCh];
   float m[NG], l[NG];
@@ -480,8 +507,16 @@ __global__ __launch_bounds__(NW *kWave, 2) void dense_kernel(AttnArgs a) {
   }
   int E = -1000;
 
+  // the scales come through the scalar cache, a block ahead too
+  typedef const __attribute__((address_space(4))) float *scalar_ptr;
+  const scalar_ptr ksp = (scalar_ptr)(a.ks + bh * a.nblk), vsp = (scalar_ptr)(a.vs + bh * a.nblk);
+  float ks_next = 0.0f, vs_next = 0.0f;
+  if (first + wave < last) {
+    ks_next = ksp[first + wave];
+    vs_next = vsp[first + wave];
+  }
   for (int64_t b = first + wave; b < last; b += NW) {
-    const float ks = a.ks[bh * a.nblk + b], vs = a.vs[bh * a.nblk + b];
+    const float ks = ks_next, vs = vs_next;
     f32x4 s[NG][4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -496,29 +531,49 @@ __global__ __launch_bounds__(NW *kWave, 2) void dense_kernel(AttnArgs a) {
       }
     }
     load_k(b + NW);
+    if (b + NW < last) {
+      ks_next = ksp[b + NW];
+      vs_next = vsp[b + NW];
+    }
     // ---- scores, in log2 units; tokens outside [lo, len) have none
-    const int t0 = (int)(b * kBlk);
+    const int t0 = (int)(b * kBlk), in_block = t0 + 4 * grp;
     const bool edge = (int64_t)t0 < lo || (int64_t)t0 + kBlk > len;
 #pragma unroll
     for (int n = 0; n < NG; ++n) {
       const float f = fac[n] * ks;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[n][i][j] = add_other_half(s[n][i][j]) * f;
+      if constexpr (EXTRA) {
+        if (a.softcap > 0.0f) {
+          const float c = a.softcap * kLog2e;
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s[n][i][j] = c * tanh_near(s[n][i][j]);
+        }
+        const float back = (float)(in_block - (int)(len - 1));
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) s[n][i][j] = fmaf(slope[n], back + (float)(16 * i + j), s[n][i][j]);
+      }
+      if (edge) {
+        asm volatile("");  // a branch, not selects in every block
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int t = in_block + 16 * i + j;
+            s[n][i][j] = t >= (int)lo && t < (int)len ? s[n][i][j] : -INFINITY;
+          }
+      }
       float mx = kLowest;
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          float z = add_other_half(s[n][i][j]) * f;
-          if constexpr (EXTRA) {
-            if (a.softcap > 0.0f) z = a.softcap * kLog2e * tanhf(z);
-            z = fmaf(slope[n], (float)(t0 + 16 * i + 4 * grp + j - (int)(len - 1)), z);
-          }
-          if (edge) {
-            const int64_t t = t0 + 16 * i + 4 * grp + j;
-            z = t >= lo && t < len ? z : -INFINITY;
-          }
-          s[n][i][j] = z;
-          mx = fmaxf(mx, z);
-        }
+        for (int j = 0; j < 4; ++j) mx = fmaxf(mx, s[n][i][j]);
       if (__any(mx > m[n])) {
         const float M = fmaxf(m[n], across_groups<true>(mx));
         const float down = __builtin_amdgcn_exp2f(m[n] - M);
@@ -543,7 +598,7 @@ __global__ __launch_bounds__(NW *kWave, 2) void dense_kernel(AttnArgs a) {
       for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          if (t0 + 16 * i + 4 * grp + j < lo) vr[i][j] = vpiece{};
+          if (in_block + 16 * i + j < (int)lo) vr[i][j] = vpiece{};
     }
     // ---- weights and products, 32 tokens at a time
 #pragma unroll
@@ -557,9 +612,7 @@ __global__ __launch_bounds__(NW *kWave, 2) void dense_kernel(AttnArgs a) {
           const float p0 = __builtin_amdgcn_exp2f(s[n][2 * c + x / 2][2 * (x & 1)] - m[n]);
           const float p1 = __builtin_amdgcn_exp2f(s[n][2 * c + x / 2][2 * (x & 1) + 1] - m[n]);
           l[n] += p0 + p1;
-          const float w0 = p0 * wv, w1 = p1 * wv;
-          const f16x2 hi = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(w0, w1));
-          pp[x] = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(fmaf((float)hi.x, keep, w0), fmaf((float)hi.y, keep, w1)));
+          pp[x] = split16(p0 * wv, p1 * wv, keep);
         }
         p[n] = join8(pp[0], pp[1], pp[2], pp[3]);
       }

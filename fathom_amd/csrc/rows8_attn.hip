@@ -492,7 +492,7 @@ __global__ __launch_bounds__(NW *kWave, 2) void dense_kernel(AttnArgs a) {
       }
       qf[n][h] = join8(part[0], part[1], part[2], part[3]);
     }
-    fac[n] = ldexpf(EXTRA && a.softcap > 0.0f ? a.scale / a.softcap : a.scale * kLog2e, -sigma);
+    fac[n] = ldexpf(EXTRA && a.softcap > 0.0f ? fminf(fmaxf(a.scale / a.softcap, -3.0e38f), 3.0e38f) : a.scale * kLog2e, -sigma);
     slope[n] = EXTRA && a.slopes && g < a.G ? a.slopes[bh * a.G + g] * kLog2e : 0.0f;
   }
 
@@ -885,16 +885,14 @@ int run_dense(AttnArgs a, int64_t BH, int64_t D, bool i8, int waves, hipStream_t
   return rc || a.nsplit == 1 ? rc : merge(a, BH, D, st);
 }
 
-int check_query(const char *what, const void *q, int q_dtype, int64_t BH, int64_t G, int64_t D, int64_t cap, const int32_t *lens,
-                int64_t n, float softcap, const float *out) {
+int check_query(const char *what, const void *q, int q_dtype, int64_t G, int64_t cap, const int32_t *lens, int64_t n,
+                float softcap, const float *out) {
   if (!q || !out) return fail(FATHOM_ERR_INVALID, "%s: null pointer", what);
   if (q_dtype < FATHOM_DT_F32 || q_dtype > FATHOM_DT_BF16) return fail(FATHOM_ERR_INVALID, "%s: q_dtype %d", what, q_dtype);
   if (G < 1 || G > 65535) return fail(FATHOM_ERR_INVALID, "%s: G=%lld", what, (long long)G);
   if (!lens && (n < 0 || n > cap)) return fail(FATHOM_ERR_INVALID, "%s: length %lld outside [0, cap=%lld]", what, (long long)n, (long long)cap);
-  if (!(softcap >= 0.0f)) return fail(FATHOM_ERR_INVALID, "%s: softcap must be 0 (none) or positive", what);
+  if (!(softcap >= 0.0f && softcap < INFINITY)) return fail(FATHOM_ERR_INVALID, "%s: softcap must be 0 (none) or positive and finite", what);
   if (reinterpret_cast<uintptr_t>(q) & 15) return fail(FATHOM_ERR_INVALID, "%s: q must be 16-byte aligned", what);
-  (void)BH;
-  (void)D;
   return FATHOM_OK;
 }
 
@@ -929,7 +927,7 @@ extern "C" int fathom_rows8_attention(const void *q, int q_dtype, const void *k8
                                       const float *slopes, float *out, void *workspace, size_t workspace_bytes,
                                       void *stream) {
   int rc = check_store("rows8_attention", k8, v8, k_scale, v_scale, code_dtype, BH, cap, D);
-  if (!rc) rc = check_query("rows8_attention", q, q_dtype, BH, G, D, cap, lens, n, softcap, out);
+  if (!rc) rc = check_query("rows8_attention", q, q_dtype, G, cap, lens, n, softcap, out);
   if (rc) return rc;
   if (window < 0) return fail(FATHOM_ERR_INVALID, "rows8_attention: window %lld", (long long)window);
   AttnArgs a{q, q_dtype, (const uint8_t *)k8, (const uint8_t *)v8, k_scale, v_scale, G, cap, cdiv(cap, kBlk), lens, n, window,
@@ -965,7 +963,7 @@ extern "C" int fathom_rows8_gather_attention(const void *q, int q_dtype, const i
                                              float scale, float softcap, const float *slopes, float *out, void *workspace,
                                              size_t workspace_bytes, void *stream) {
   int rc = check_store("rows8_gather_attention", k8, v8, k_scale, v_scale, code_dtype, BH, cap, D);
-  if (!rc) rc = check_query("rows8_gather_attention", q, q_dtype, BH, G, D, cap, lens, n, softcap, out);
+  if (!rc) rc = check_query("rows8_gather_attention", q, q_dtype, G, cap, lens, n, softcap, out);
   if (rc) return rc;
   if (k < 0 || G * k > 0x7FFFFFFF) return fail(FATHOM_ERR_INVALID, "rows8_gather_attention: G=%lld k=%lld", (long long)G, (long long)k);
   if (k > 0 && !idx) return fail(FATHOM_ERR_INVALID, "rows8_gather_attention: null index pointer");

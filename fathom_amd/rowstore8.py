@@ -13,6 +13,8 @@ RowStore8 keeps, per row and for K and V apart, codes [BH, cap, d]
 lengths (also in captured graphs, where they change between replays).  Calls run
 asynchronously on the device's current stream.
 """
+import math
+
 import torch
 
 from . import _lib
@@ -124,8 +126,8 @@ class RowStore8:
             q = q.clone()
             at = q.data_ptr()
         softcap = 0.0 if softcap is None else float(softcap)
-        if not softcap >= 0.0:
-            raise ValueError(f"softcap {softcap} must be positive (None or 0: no cap)")
+        if not 0.0 <= softcap < math.inf:
+            raise ValueError(f"softcap {softcap} must be positive and finite (None or 0: no cap)")
         if slopes is not None:
             if slopes.device != self.device:
                 self._elsewhere(slopes)

@@ -483,3 +483,105 @@ def test_offsets_past_32_bits():
                                       float(np.float32(D ** -0.5)))
             _close(out, b, g, want, bound)
             _close(sel, b, g, want, bound)
+
+
+# ----------------------------------------------------------------------------- how rows are shared out
+@pytest.mark.parametrize("BH, cap", [(70, 3000), (200, 1500), (300, 1200), (600, 1200)])
+@pytest.mark.parametrize("G", [2, 20])
+def test_attention_many_rows(BH, cap, G):
+    """More rows than one wave has lanes, and more than the workgroups of a call; rows without tokens among them."""
+    rng = np.random.default_rng(BH)
+    lens = rng.integers(0, cap + 1, BH)
+    lens[[0, BH // 2, BH - 1]] = [0, cap, 0]
+    lens[rng.integers(0, BH, 5)] = 1
+    st, K, V = _filled(BH, cap, 64, "int8", lens)
+    q = _q(BH, G, 64, 7)
+    got = st.attention(q.to(DEV), torch.from_numpy(lens.astype(np.int32)).to(DEV))
+    some = sorted({0, 1, 63, BH - 1, BH // 2, *rng.integers(0, BH, 12).tolist()})
+    for b in some:
+        for g in (0, G - 1):
+            want, bound = R.attention(q[b, g].double().numpy(), K[b], V[b], np.arange(lens[b]), lens[b],
+                                      float(np.float32(64 ** -0.5)))
+            _close(got, b, g, want, bound)
+    listed = torch.arange(cap).expand(BH, G, cap).contiguous().to(DEV)
+    every = st.gather_attention(q.to(DEV), listed, torch.from_numpy(lens.astype(np.int32)).to(DEV))
+    assert (got - every).abs().max() <= 2e-5 * every.abs().max()
+
+
+@pytest.mark.parametrize("BH, G, D", [(1, 1, 128), (3, 5, 64), (2, 33, 128)])
+def test_attention_every_share(BH, G, D):
+    """Lengths and windows across every way of sharing a row out: one length, one length as a tensor, and the list of the
+    same tokens agree."""
+    cap = 40000
+    st, _, _ = _filled(BH, cap, D, "e4m3", [cap] * BH, spread=0.3)
+    q = _q(BH, G, D, 3).to(DEV)
+    ns = [1, 60, 64, 65, 200, 256, 257, 320, 500, 512, 513, 1023, 1024, 1025, 1087, 1088, 1089, 1100, 2047, 2049, 4095, 4160, 8191,
+          8200, 16383, 16385, 20000, 32767, 39999, 40000]
+    for i, n in enumerate(ns):
+        for window in (0, ns[(i * 7) % len(ns)]):
+            lo = max(0, n - window) if window else 0
+            a = st.attention(q, n, window=window)
+            b = st.attention(q, torch.full((BH,), n, dtype=torch.int32, device=DEV), window=window)
+            c = st.gather_attention(q, torch.arange(lo, n, device=DEV).expand(BH, G, n - lo))
+            size = c.abs().max()
+            assert (a - c).abs().max() <= 2e-5 * size and (b - c).abs().max() <= 2e-5 * size, (n, window)
+
+
+@pytest.mark.parametrize("window", [1, 64, 1000, 1090, 4096, 19999])
+def test_attention_long_windows(window):
+    lens = [20011, 7, 15000, 0, 4097]
+    st, K, V = _filled(5, 20020, 64, "int8", lens)
+    slopes = torch.rand(5, 3, generator=torch.Generator().manual_seed(4)) * 0.01
+    _check(st, K, V, _q(5, 3, 64, 6), lens, torch.tensor(lens, dtype=torch.int32, device=DEV), window, 20.0, slopes)
+
+
+def test_captured_long_rows_replayed():
+    """Rows shared out by lengths on the device, in a graph whose lengths grow between replays."""
+    BH, cap, G, D = 3, 30000, 4, 128
+    st, _, _ = _filled(BH, cap, D, "e4m3", [cap] * BH, spread=0.3)
+    q, length = torch.zeros(BH, G, D, device=DEV), torch.tensor([100, 0, 29000], dtype=torch.int32, device=DEV)
+    q.normal_()
+    st.attention(q, length)
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for _ in range(2):  # two graphs of the same store, replayed in turn and together
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append((st.attention(q, length), st.attention(q, length, window=5000)))
+        graphs.append(graph)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for i in range(6):
+        q.normal_()
+        want = st.attention(q, length), st.attention(q, length, window=5000)
+        torch.cuda.synchronize()
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        for pair in outs:
+            assert all(torch.equal(a, b) for a, b in zip(pair, want))
+        length.copy_((length * 2 + 77) % (cap + 1))
+
+
+def test_query_layouts():
+    """Queries with any strides and addresses, of other types, and slopes per head."""
+    st, K, V = _filled(2, 500, 64, "int8", [500, 500])
+    wide = torch.randn(2, 3, 200, generator=torch.Generator().manual_seed(5)).to(DEV)
+    slopes = torch.tensor([0.1, 0.2, 0.05], device=DEV)
+    idx = torch.arange(500, device=DEV).expand(2, 3, 500)
+    for q in (wide[..., 3:67], wide[..., :64].transpose(0, 1).contiguous().transpose(0, 1), wide[..., :64].double()):
+        same = q.float().contiguous()
+        every = slopes.expand(2, 3).contiguous()
+        assert torch.equal(st.attention(q, 500, slopes=slopes), st.attention(same, 500, slopes=every))
+        assert torch.equal(st.gather_attention(q, idx.int(), 500, slopes=slopes.double()),
+                           st.gather_attention(same, idx.contiguous(), 500, slopes=every))
+
+
+def test_same_result_twice():
+    st, _, _ = _filled(4, 9000, 128, "e4m3", [9000, 1, 5000, 8999])
+    q = _q(4, 9, 128, 2).to(DEV)
+    lens = torch.tensor([9000, 1, 5000, 8999], dtype=torch.int32, device=DEV)
+    idx = torch.randint(0, 9000, (4, 9, 700), generator=torch.Generator().manual_seed(2)).to(DEV)
+    for call in (lambda: st.attention(q, lens), lambda: st.attention(q, 8000), lambda: st.gather_attention(q, idx, lens)):
+        first = call().view(torch.int32)  # bits: rows past their written tokens hold NaN
+        assert all(torch.equal(first, call().view(torch.int32)) for _ in range(5))

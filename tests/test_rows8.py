@@ -106,6 +106,7 @@ def _attn_args(**kw):
     (dict(G=65536), b"G=", _lib.ERR_INVALID), (dict(n=100001), b"length", _lib.ERR_INVALID),
     (dict(n=-1), b"length", _lib.ERR_INVALID), (dict(window=-1), b"window", _lib.ERR_INVALID),
     (dict(softcap=-1.0), b"softcap", _lib.ERR_INVALID), (dict(softcap=float("nan")), b"softcap", _lib.ERR_INVALID),
+    (dict(softcap=float("inf")), b"softcap", _lib.ERR_INVALID),
     (dict(q=(1 << 20) + 4), b"aligned", _lib.ERR_INVALID), (dict(D=32), b"D=32", _lib.ERR_INVALID),
     (dict(), b"workspace", _lib.ERR_WORKSPACE)])
 def test_attention_refusals(bad, text, status):
@@ -133,3 +134,14 @@ def test_workspace_queries():
     assert L.fathom_rows8_attention_workspace_bytes(1, 1, 128, 0) == 0
     assert L.fathom_rows8_attention_workspace_bytes(8, 4, 128, 1 << 20) > 0
     assert L.fathom_rows8_gather_attention_workspace_bytes(1, 1, 128, 1) == 0
+
+
+@pytest.mark.parametrize("G", [1, 8, 9, 40])
+@pytest.mark.parametrize("BH", [1, 7, 64, 300, 5000])
+def test_workspace_sizes_do_not_fall_as_positions_grow(BH, G):
+    """Callers ask for the next power of two and keep the answer."""
+    L = _lib.lib()
+    at = sorted({n + d for n in [1 << i for i in range(27)] + [300, 1088, 1089, 5000] for d in (-1, 0, 1) if n + d > 0})
+    for query in (L.fathom_rows8_attention_workspace_bytes, L.fathom_rows8_gather_attention_workspace_bytes):
+        sizes = [query(BH, G, 128, n) for n in at]
+        assert sizes == sorted(sizes) and all(b % 4 == 0 for b in sizes)

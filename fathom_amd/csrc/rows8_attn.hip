@@ -56,6 +56,15 @@ __device__ __forceinline__ void load8_q(const void *q, int dt, int64_t i, float 
   }
 }
 
+// The factor that the queries take before the product, (scale log2 e, or scale /
+// softcap), as a fraction in [1/2, 1) that multiplies q and a power of two for the
+// scale of K: a rounding there would shift all scores of a block alike, in q they average out.
+__device__ __forceinline__ float query_factor(const AttnArgs &a, int &e) {
+  const float c = a.softcap > 0.0f ? fminf(fmaxf(a.scale / a.softcap, -3.0e38f), 3.0e38f) : a.scale * kLog2e;
+  e = 0;
+  return c == 0.0f || !(fabsf(c) < INFINITY) ? c : frexpf(c, &e);
+}
+
 // tanh to about a step of float32: below 1/2 u + u^3 P(u^2), P the least-squares fit of
 // degree 4 to (tanh u - u) / u^3; from there (1 - t) / (1 + t), t = e^(-2 |u|), the quotient
 // by the reciprocal and one correction.
@@ -150,12 +159,14 @@ __global__ __launch_bounds__(NW *kWave) void list_kernel(AttnArgs a) {
   float m = kLowest, l = 0.0f, o[16];
 #pragma unroll
   for (int e = 0; e < 16; ++e) o[e] = 0.0f;
+  int ce;
+  const float cm = query_factor(a, ce);
   bool first = true;
   for (int64_t t0 = (s * NW + wave) * kTile; t0 < a.k; t0 += a.nsplit * NW * kTile) {
     int64_t tok[kLoads];
     bool in[kLoads];
     u32x4 kc[kLoads], vc[kLoads];
-    float ks[kLoads], vs[kLoads], z[kLoads];
+    float ks[kLoads], vs[kLoads], x[kLoads], y[kLoads], bias[kLoads];
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
       const int64_t j = t0 + i * kRows + rg;
@@ -178,6 +189,12 @@ __global__ __launch_bounds__(NW *kWave) void list_kernel(AttnArgs a) {
       for (int h = 0; h < 2; ++h) load8_q(a.q, a.q_dtype, (bh * a.G + g) * D + d0 + 8 * h, q[h]);
     }
     __builtin_amdgcn_sched_barrier(0);
+    if (t0 < (s + 1) * NW * kTile) {  // the wave's first tile
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) q[h][e] *= cm;
+    }
     float mt = m;
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
@@ -189,11 +206,16 @@ __global__ __launch_bounds__(NW *kWave) void list_kernel(AttnArgs a) {
 #pragma unroll
         for (int f = 0; f < 4; ++f) dot = fmaf(q[e / 2][4 * (e & 1) + f], c[f], dot);
       }
-      float u = sum_row<kLanes>(dot) * (ks[i] * a.scale);
-      if (a.softcap > 0.0f) u = a.softcap * tanh_near(u / a.softcap);
-      u = fmaf(slope, (float)(int)(tok[i] - (len - 1)), u * kLog2e);
-      z[i] = in[i] ? u : -INFINITY;
-      mt = fmaxf(mt, z[i]);
+      // z = x y + bias: the product is rounded only once it is relative to the maximum
+      x[i] = sum_row<kLanes>(dot);
+      y[i] = ldexpf(ks[i], ce);
+      if (a.softcap > 0.0f) {
+        x[i] = tanh_near(x[i] * y[i]);
+        y[i] = a.softcap * kLog2e;
+      }
+      bias[i] = slope * (float)(int)(tok[i] - (len - 1));
+      const float z = fmaf(x[i], y[i], bias[i]);
+      mt = fmaxf(mt, in[i] ? z : kLowest);
     }
     const float f = __builtin_amdgcn_exp2f(m - mt);
     l *= f;
@@ -202,7 +224,7 @@ __global__ __launch_bounds__(NW *kWave) void list_kernel(AttnArgs a) {
     m = mt;
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
-      const float p = __builtin_amdgcn_exp2f(z[i] - m);
+      const float p = in[i] ? __builtin_amdgcn_exp2f(fmaf(x[i], y[i], bias[i] - m)) : 0.0f;
       l += p;
       const float pv = in[i] ? p * vs[i] : 0.0f;
 #pragma unroll
@@ -210,7 +232,7 @@ __global__ __launch_bounds__(NW *kWave) void list_kernel(AttnArgs a) {
         float c[4];
         decode4<I8>(vc[i][e], c);
 #pragma unroll
-        for (int x = 0; x < 4; ++x) o[4 * e + x] = fmaf(pv, c[x], o[4 * e + x]);
+        for (int f = 0; f < 4; ++f) o[4 * e + f] = fmaf(pv, c[f], o[4 * e + f]);
       }
     }
   }
@@ -467,7 +489,9 @@ __global__ __launch_bounds__(NW *kWave, 2) void dense_kernel(AttnArgs a) {
   load_v(first + wave);
   const float keep = col < 8 ? 0.0f : -1.0f;  // columns 8 .. 15 hold what the f16 of columns 0 .. 7 leave
   f16x8 qf[NG][kSteps];
-  float fac[NG], slope[NG];  // per lane: its head's factor of a score, its bias per token
+  int ce, ex[NG];   // per lane: the exponent that its head's scores take
+  float slope[NG];  // its bias per token
+  const float cm = query_factor(a, ce);
 #pragma unroll
   for (int n = 0; n < NG; ++n) {
     const int64_t g = g0 + 8 * n + (col & 7);
@@ -488,11 +512,11 @@ __global__ __launch_bounds__(NW *kWave, 2) void dense_kernel(AttnArgs a) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float x = ldexpf(q[n][h][2 * e], sigma), y = ldexpf(q[n][h][2 * e + 1], sigma);
-        part[e] = split16(x, y, keep);
+        part[e] = split16(x * cm, y * cm, keep);
       }
       qf[n][h] = join8(part[0], part[1], part[2], part[3]);
     }
-    fac[n] = ldexpf(EXTRA && a.softcap > 0.0f ? fminf(fmaxf(a.scale / a.softcap, -3.0e38f), 3.0e38f) : a.scale * kLog2e, -sigma);
+    ex[n] = ce - sigma;
     slope[n] = EXTRA && a.slopes && g < a.G ? a.slopes[bh * a.G + g] * kLog2e : 0.0f;
   }
 
@@ -538,26 +562,35 @@ __global__ __launch_bounds__(NW *kWave, 2) void dense_kernel(AttnArgs a) {
     // ---- scores, in log2 units; tokens outside [lo, len) have none
     const int t0 = (int)(b * kBlk), in_block = t0 + 4 * grp;
     const bool edge = (int64_t)t0 < lo || (int64_t)t0 + kBlk > len;
+    float fz[NG];
 #pragma unroll
     for (int n = 0; n < NG; ++n) {
-      const float f = fac[n] * ks;
+      // z = s f; not rounded itself, but relative to the maximum
+      float f = ldexpf(fabsf(ks), ex[n]);
+      f = f == f ? fmaxf(f, 1.2e-38f) : f;  // never 0: a score of -inf has to stay one
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) s[n][i][j] = add_other_half(s[n][i][j]) * f;
+        for (int j = 0; j < 4; ++j) s[n][i][j] = add_other_half(s[n][i][j]);
+      if (ks < 0.0f) {  // not written by this store's writer
+        asm volatile("");
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[n][i] = -s[n][i];
+      }
       if constexpr (EXTRA) {
         if (a.softcap > 0.0f) {
-          const float c = a.softcap * kLog2e;
 #pragma unroll
           for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) s[n][i][j] = c * tanh_near(s[n][i][j]);
+            for (int j = 0; j < 4; ++j) s[n][i][j] = tanh_near(s[n][i][j] * f);
+          f = a.softcap * kLog2e;
         }
         const float back = (float)(in_block - (int)(len - 1));
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) s[n][i][j] = fmaf(slope[n], back + (float)(16 * i + j), s[n][i][j]);
+          for (int j = 0; j < 4; ++j) s[n][i][j] = fmaf(s[n][i][j], f, slope[n] * (back + (float)(16 * i + j)));
+        f = 1.0f;
       }
       if (edge) {
         asm volatile("");  // a branch, not selects in every block
@@ -569,11 +602,13 @@ __global__ __launch_bounds__(NW *kWave, 2) void dense_kernel(AttnArgs a) {
             s[n][i][j] = t >= (int)lo && t < (int)len ? s[n][i][j] : -INFINITY;
           }
       }
-      float mx = kLowest;
+      float mx = -INFINITY;
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) mx = fmaxf(mx, s[n][i][j]);
+      mx *= f;
+      fz[n] = f;
       if (__any(mx > m[n])) {
         const float M = fmaxf(m[n], across_groups<true>(mx));
         const float down = __builtin_amdgcn_exp2f(m[n] - M);
@@ -607,13 +642,15 @@ __global__ __launch_bounds__(NW *kWave, 2) void dense_kernel(AttnArgs a) {
 #pragma unroll
       for (int n = 0; n < NG; ++n) {
         f16x2 pp[4];
+        float ps[4];  // added together first: alone, most weights would be lost beside a large sum
 #pragma unroll
         for (int x = 0; x < 4; ++x) {  // tokens (tile 2 c + x / 2, j = 2 (x & 1), + 1)
-          const float p0 = __builtin_amdgcn_exp2f(s[n][2 * c + x / 2][2 * (x & 1)] - m[n]);
-          const float p1 = __builtin_amdgcn_exp2f(s[n][2 * c + x / 2][2 * (x & 1) + 1] - m[n]);
-          l[n] += p0 + p1;
+          const float p0 = __builtin_amdgcn_exp2f(fmaf(s[n][2 * c + x / 2][2 * (x & 1)], fz[n], -m[n]));
+          const float p1 = __builtin_amdgcn_exp2f(fmaf(s[n][2 * c + x / 2][2 * (x & 1) + 1], fz[n], -m[n]));
+          ps[x] = p0 + p1;
           pp[x] = split16(p0 * wv, p1 * wv, keep);
         }
+        l[n] += (ps[0] + ps[1]) + (ps[2] + ps[3]);
         p[n] = join8(pp[0], pp[1], pp[2], pp[3]);
       }
 #pragma unroll

@@ -68,19 +68,22 @@ __device__ __forceinline__ float query_factor(const AttnArgs &a, int &e) {
 // tanh to about a step of float32: below 1/2 u + u^3 P(u^2), P the least-squares fit of
 // degree 4 to (tanh u - u) / u^3; from there (1 - t) / (1 + t), t = e^(-2 |u|), the quotient
 // by the reciprocal and one correction.
-__device__ __forceinline__ float tanh_near(float u) {
-  const float x = fabsf(u), w = u * u;
+__device__ __forceinline__ float tanh_small(float u) {
+  const float w = u * u;
   float p = -0.006947011f;
   p = fmaf(p, w, 0.021472726f);
   p = fmaf(p, w, -0.05393379f);
   p = fmaf(p, w, 0.13333227f);
   p = fmaf(p, w, -0.3333333f);
-  const float near = fmaf(u * w, p, u);
+  return fmaf(u * w, p, u);
+}
+__device__ __forceinline__ float tanh_any(float u) {
+  const float x = fabsf(u);
   const float t = __builtin_amdgcn_exp2f(x * (-2.0f * kLog2e));
   const float n = 1.0f - t, d = 1.0f + t, r = __builtin_amdgcn_rcpf(d);
   float far = n * r;
   far = fmaf(fmaf(-far, d, n), r, far);
-  return x < 0.5f ? near : copysignf(far, u);
+  return x < 0.5f ? tanh_small(u) : copysignf(far, u);
 }
 
 // Sum or maximum over the four lanes l, l ^ 16, l ^ 32, l ^ 48 (v_permlane32_swap
@@ -210,7 +213,7 @@ __global__ __launch_bounds__(NW *kWave) void list_kernel(AttnArgs a) {
       x[i] = sum_row<kLanes>(dot);
       y[i] = ldexpf(ks[i], ce);
       if (a.softcap > 0.0f) {
-        x[i] = tanh_near(x[i] * y[i]);
+        x[i] = tanh_any(x[i] * y[i]);
         y[i] = a.softcap * kLog2e;
       }
       bias[i] = slope * (float)(int)(tok[i] - (len - 1));
@@ -373,34 +376,37 @@ struct Part {
 // that the longest row does not hold the call up.  Each wave sums the rows'
 // blocks (a lane per row), which gives `per`, and finds its workgroup's row in the prefix sums
 // of ceil(blocks / per).  Those are at most kDenseTotal / NW / head groups + BH, the grid.
+// (32 bits hold the sums: 2^31 blocks of D = 64 are 17 TB.)
 template <int NW>
-__device__ __forceinline__ Part find_part(const AttnArgs &a, int w) {
-  const int lane = threadIdx.x & 63;
-  auto blocks = [&](int64_t r) {
+__device__ __forceinline__ Part find_part(const AttnArgs &a, uint32_t w) {
+  const int lane = threadIdx.x & 63, BH = (int)a.BH;
+  auto blocks = [&](int r) {
     int64_t lo, len, blk0;
     int nb = 0;
-    if (r < a.BH) row_blocks(a, r, lo, len, blk0, nb);
-    return nb;
+    if (r < BH) row_blocks(a, r, lo, len, blk0, nb);
+    return (uint32_t)nb;
   };
-  int64_t total = 0;
-  for (int64_t r0 = 0; r0 < a.BH; r0 += kWave) total += wave_sum_i(blocks(r0 + lane));
+  const uint32_t own = blocks(lane);  // rows 0 .. 63, most often all
+  uint32_t total = __builtin_amdgcn_readlane(wave_incl_scan_u32(own), 63);
+  for (int r0 = kWave; r0 < BH; r0 += kWave) total += __builtin_amdgcn_readlane(wave_incl_scan_u32(blocks(r0 + lane)), 63);
   // a row's last workgroup may have less to do: with BH of them, the call's workgroups are
   // at most kDenseTotal / NW, all at work at once
-  const int fit = kDenseTotal / NW / (int)a.groups, groups = fit > 2 * a.BH ? fit - (int)a.BH : fit / 2 > 0 ? fit / 2 : 1;
-  const int even = __builtin_amdgcn_readfirstlane((int)((total + groups - 1) / groups));
-  Part p{a.BH, 0, 0, even > NW ? even : NW};
+  const int fit = kDenseTotal / NW / (int)a.groups;
+  const uint32_t groups = fit > 2 * BH ? fit - BH : fit / 2 > 0 ? fit / 2 : 1;
+  const uint32_t even = (total + groups - 1) / groups, per = even > (uint32_t)NW ? even : (uint32_t)NW;
+  Part p{a.BH, 0, 0, (int)per};
   uint32_t before = 0;
-  for (int64_t r0 = 0; r0 < a.BH; r0 += kWave) {
+  for (int r0 = 0; r0 < BH; r0 += kWave) {
     // a row without tokens takes a workgroup too: it writes the row's zeros
-    const int nb = blocks(r0 + lane);
-    const uint32_t act = r0 + lane >= a.BH ? 0u : nb <= p.per ? 1u : (uint32_t)((nb + p.per - 1) / p.per);
+    const uint32_t nb = r0 ? blocks(r0 + lane) : own;
+    const uint32_t act = r0 + lane >= BH ? 0u : nb <= per ? 1u : (nb + per - 1) / per;
     const uint32_t upto = before + wave_incl_scan_u32(act);
-    const uint64_t past = __ballot(upto > (uint32_t)w);
+    const uint64_t past = __ballot(upto > w);
     if (past) {
       const int at = __builtin_ctzll(past);
       p.bh = r0 + at;
       p.active = __builtin_amdgcn_readlane((int)act, at);
-      p.split = w - (__builtin_amdgcn_readlane((int)upto, at) - p.active);
+      p.split = (int)(w - (__builtin_amdgcn_readlane((int)upto, at) - p.active));
       return p;
     }
     before = __builtin_amdgcn_readlane((int)upto, 63);
@@ -445,7 +451,7 @@ __global__ __launch_bounds__(NW *kWave, 2) void dense_kernel(AttnArgs a) {
   Part part{(int64_t)blockIdx.z, (int)blockIdx.x, (int)a.nsplit, 0};
   int64_t slot = (int64_t)blockIdx.z * a.nsplit + blockIdx.x;  // of the partial results
   if (a.where) {
-    part = find_part<NW>(a, (int)blockIdx.x);
+    part = find_part<NW>(a, blockIdx.x);
     if (part.bh >= a.BH) return;
     slot = blockIdx.x;
     if (part.split == 0 && blockIdx.y == 0 && tid == 0) a.where[part.bh] = make_int2((int)blockIdx.x, part.active);
@@ -579,10 +585,25 @@ __global__ __launch_bounds__(NW *kWave, 2) void dense_kernel(AttnArgs a) {
       }
       if constexpr (EXTRA) {
         if (a.softcap > 0.0f) {
+          float big = 0.0f;
 #pragma unroll
           for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) s[n][i][j] = tanh_near(s[n][i][j] * f);
+            for (int j = 0; j < 4; ++j) {
+              s[n][i][j] *= f;
+              big = fmaxf(big, fabsf(s[n][i][j]));
+            }
+          if (__any(big >= 0.5f)) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) s[n][i][j] = tanh_any(s[n][i][j]);
+          } else {  // most blocks: scores well below the cap
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) s[n][i][j] = tanh_small(s[n][i][j]);
+          }
           f = a.softcap * kLog2e;
         }
         const float back = (float)(in_block - (int)(len - 1));
@@ -842,8 +863,8 @@ constexpr int64_t kOneGroup = 17;
 // Lengths on the device are not known here; rows of 16 ragged lengths up to 50021 take 24.8; 22.8.
 int dense_waves(int64_t rows, int64_t nb, bool lens) {
   if (nb <= 4) return 4;
-  if (nb <= kOneGroup || lens) return 8;
-  return rows * nb > kDenseTotal && rows * nb <= 32 * kDenseTotal ? 8 : 4;
+  if (nb <= kOneGroup) return 8;
+  return rows * nb > kDenseTotal && (lens || rows * nb <= 32 * kDenseTotal) ? 8 : 4;
 }
 
 // Splits of such a row: kDenseTotal waves in all, at least one block per wave.
@@ -948,13 +969,12 @@ using namespace fathom::rows8;
 
 extern "C" size_t fathom_rows8_attention_workspace_bytes(int64_t BH, int64_t G, int64_t D, int64_t positions) {
   if (BH < 1 || G < 1 || D < 1 || positions < 1) return 0;
-  // the most slots of any choice of waves, for one length or lengths on the device: does not fall as positions grow
+  // the most slots of either choice of waves, for one length or lengths on the device: does not fall as positions grow
   const int64_t nb = cdiv(positions, (int64_t)kBlk) + 1, groups = head_groups(G);  // a window may begin inside a block
   if (nb <= kOneGroup) return 0;
   const int64_t blocks = cdiv(nb, (int64_t)4), share = cdiv((int64_t)kDenseTotal / 4, BH * groups);
-  int64_t slots = BH * (blocks < share ? blocks : share);
-  const int64_t own = kDenseTotal / 8 / groups + BH, most = BH * cdiv(nb, (int64_t)8);
-  if (slots < (own < most ? own : most)) slots = own < most ? own : most;
+  const int64_t own = kDenseTotal / 4 / groups + BH, one = BH * (blocks < share ? blocks : share);
+  const int64_t many = own < BH * blocks ? own : BH * blocks, slots = one > many ? one : many;
   return part_bytes(BH, G, D, slots);
 }
 

@@ -15,6 +15,7 @@ namespace {
 
 constexpr int kTile = 32;  // listed positions of a wave at a time
 constexpr int kMergeThreads = 256;
+constexpr int kDenseWaves = 4;     // of a workgroup that takes a split of a row
 constexpr int kDenseTotal = 2048;  // waves of a dense call: eight per CU, all at work at once
 constexpr int kMaxSplits = 512;  // of a query head
 constexpr float kLog2e = 1.44269504088896340736f;
@@ -375,9 +376,8 @@ struct Part {
 // Rows of their own lengths (on the device): every workgroup takes `per` blocks, so
 // that the longest row does not hold the call up.  Each wave sums the rows'
 // blocks (a lane per row), which gives `per`, and finds its workgroup's row in the prefix sums
-// of ceil(blocks / per).  Those are at most kDenseTotal / NW / head groups + BH, the grid.
+// of ceil(blocks / per).  Those are at most kDenseTotal / kDenseWaves / head groups + BH, the grid.
 // (32 bits hold the sums: 2^31 blocks of D = 64 are 17 TB.)
-template <int NW>
 __device__ __forceinline__ Part find_part(const AttnArgs &a, uint32_t w) {
   const int lane = threadIdx.x & 63, BH = (int)a.BH;
   auto blocks = [&](int r) {
@@ -390,10 +390,10 @@ __device__ __forceinline__ Part find_part(const AttnArgs &a, uint32_t w) {
   uint32_t total = __builtin_amdgcn_readlane(wave_incl_scan_u32(own), 63);
   for (int r0 = kWave; r0 < BH; r0 += kWave) total += __builtin_amdgcn_readlane(wave_incl_scan_u32(blocks(r0 + lane)), 63);
   // a row's last workgroup may have less to do: with BH of them, the call's workgroups are
-  // at most kDenseTotal / NW, all at work at once
-  const int fit = kDenseTotal / NW / (int)a.groups;
+  // at most kDenseTotal / kDenseWaves, all at work at once
+  const int fit = kDenseTotal / kDenseWaves / (int)a.groups;
   const uint32_t groups = fit > 2 * BH ? fit - BH : fit / 2 > 0 ? fit / 2 : 1;
-  const uint32_t even = (total + groups - 1) / groups, per = even > (uint32_t)NW ? even : (uint32_t)NW;
+  const uint32_t even = (total + groups - 1) / groups, per = even > (uint32_t)kDenseWaves ? even : (uint32_t)kDenseWaves;
   Part p{a.BH, 0, 0, (int)per};
   uint32_t before = 0;
   for (int r0 = 0; r0 < BH; r0 += kWave) {
@@ -450,8 +450,8 @@ __global__ __launch_bounds__(NW *kWave, 2) void dense_kernel(AttnArgs a) {
   const int64_t g0 = (int64_t)blockIdx.y * 8 * NG;
   Part part{(int64_t)blockIdx.z, (int)blockIdx.x, (int)a.nsplit, 0};
   int64_t slot = (int64_t)blockIdx.z * a.nsplit + blockIdx.x;  // of the partial results
-  if (a.where) {
-    part = find_part<NW>(a, blockIdx.x);
+  if (NW == kDenseWaves && a.where) {
+    part = find_part(a, blockIdx.x);
     if (part.bh >= a.BH) return;
     slot = blockIdx.x;
     if (part.split == 0 && blockIdx.y == 0 && tid == 0) a.where[part.bh] = make_int2((int)blockIdx.x, part.active);
@@ -854,34 +854,27 @@ int64_t head_groups(int64_t G) { return cdiv(G, (int64_t)16); }
 // more as a window of that length may begin inside a block.
 constexpr int64_t kOneGroup = 17;
 
-// Waves of dense_kernel's workgroups, for rows of up to nb blocks in a call of `rows`
-// rows (head groups counted).  Eight where a row then needs no split (up to two blocks per wave: one launch for
-// two), and where a wave takes a few blocks, as fewer splits are joined; four where it takes less than one (a
-// wave alone on its SIMD is done sooner) and where it takes many.
-//   us in a graph, 4 waves; 8: 1 x 4096 tokens 9.6; 11.3, 8 x 8192 12.0; 12.9, 32 x 4096 14.8; 14.5, 1 x 262144
-//   21.3; 19.5, 8 x 131072 55.2; 54.3, 8 x 1048576 366; 372.
-// Lengths on the device are not known here; rows of 16 ragged lengths up to 50021 take 24.8; 22.8.
-int dense_waves(int64_t rows, int64_t nb, bool lens) {
-  if (nb <= 4) return 4;
-  if (nb <= kOneGroup) return 8;
-  return rows * nb > kDenseTotal && (lens || rows * nb <= 32 * kDenseTotal) ? 8 : 4;
-}
+// Whether rows of up to nb blocks go to workgroups of eight waves, one per row: one launch for two (the join)
+// and no workspace, two blocks per wave at most.  A call of 1 x 1000 tokens takes 10.0 us from Python and 11.2 in a
+// graph, with splits of four waves 14.5 and 8.4: the host's part of a call counts more often.  Rows of up to four
+// blocks need no split of four waves either, and split rows are no faster in eight (32 x 4096 tokens 14.6 us
+// both ways, 8 x 8192 11.1 with four; 13.8, 8 x 1048576 326; 331).
+bool one_group(int64_t nb) { return nb > kDenseWaves && nb <= kOneGroup; }
 
-// Splits of such a row: kDenseTotal waves in all, at least one block per wave.
-int64_t dense_splits(int64_t rows, int64_t nb, int waves) {
-  if (nb <= kOneGroup && waves == 8) return 1;
-  const int64_t want = cdiv((int64_t)kDenseTotal / waves, rows), most = cdiv(nb, (int64_t)waves);
+// Splits of a row of up to nb blocks in a call of `rows` rows (head groups counted):
+// kDenseTotal waves in all, at least one block per wave.
+int64_t dense_splits(int64_t rows, int64_t nb) {
+  if (nb <= kOneGroup) return 1;
+  const int64_t want = cdiv((int64_t)kDenseTotal / kDenseWaves, rows), most = cdiv(nb, (int64_t)kDenseWaves);
   return most < want ? most : want;
 }
 
 // Slots of partial results of a dense call; 0: every row fits one workgroup.  With
-// lengths on the device: the bound of find_part.
+// lengths on the device: the bound of find_part.  Neither falls as nb grows.
 int64_t dense_slots(int64_t BH, int64_t G, int64_t nb, bool lens) {
-  const int64_t groups = head_groups(G);
-  const int waves = dense_waves(BH * groups, nb, lens);
-  const int64_t ns = dense_splits(BH * groups, nb, waves);
+  const int64_t groups = head_groups(G), ns = dense_splits(BH * groups, nb);
   if (ns <= 1) return 0;
-  const int64_t all = kDenseTotal / waves / groups + BH, most = BH * cdiv(nb, (int64_t)waves);
+  const int64_t all = kDenseTotal / kDenseWaves / groups + BH, most = BH * cdiv(nb, (int64_t)kDenseWaves);
   return !lens ? BH * ns : all < most ? all : most;
 }
 
@@ -927,18 +920,18 @@ void launch_dense(const AttnArgs &a, int64_t BH, hipStream_t st) {
 }
 
 template <int D, bool I8>
-void launch_dense(const AttnArgs &a, int64_t BH, int waves, hipStream_t st) {
-  if (a.G > 8 && waves == 8) launch_dense<D, I8, 2, 8>(a, BH, st);
-  else if (a.G > 8) launch_dense<D, I8, 2, 4>(a, BH, st);
-  else if (waves == 8) launch_dense<D, I8, 1, 8>(a, BH, st);
-  else launch_dense<D, I8, 1, 4>(a, BH, st);
+void launch_dense(const AttnArgs &a, int64_t BH, bool one, hipStream_t st) {
+  if (a.G > 8 && one) launch_dense<D, I8, 2, 8>(a, BH, st);
+  else if (a.G > 8) launch_dense<D, I8, 2, kDenseWaves>(a, BH, st);
+  else if (one) launch_dense<D, I8, 1, 8>(a, BH, st);
+  else launch_dense<D, I8, 1, kDenseWaves>(a, BH, st);
 }
 
-int run_dense(AttnArgs a, int64_t BH, int64_t D, bool i8, int waves, hipStream_t st) {
-  if (D == 128 && i8) launch_dense<128, true>(a, BH, waves, st);
-  else if (D == 128) launch_dense<128, false>(a, BH, waves, st);
-  else if (i8) launch_dense<64, true>(a, BH, waves, st);
-  else launch_dense<64, false>(a, BH, waves, st);
+int run_dense(AttnArgs a, int64_t BH, int64_t D, bool i8, bool one, hipStream_t st) {
+  if (D == 128 && i8) launch_dense<128, true>(a, BH, one, st);
+  else if (D == 128) launch_dense<128, false>(a, BH, one, st);
+  else if (i8) launch_dense<64, true>(a, BH, one, st);
+  else launch_dense<64, false>(a, BH, one, st);
   const int rc = launch_status("rows8 dense_kernel");
   return rc || a.nsplit == 1 ? rc : merge(a, BH, D, st);
 }
@@ -969,12 +962,8 @@ using namespace fathom::rows8;
 
 extern "C" size_t fathom_rows8_attention_workspace_bytes(int64_t BH, int64_t G, int64_t D, int64_t positions) {
   if (BH < 1 || G < 1 || D < 1 || positions < 1) return 0;
-  // the most slots of either choice of waves, for one length or lengths on the device: does not fall as positions grow
-  const int64_t nb = cdiv(positions, (int64_t)kBlk) + 1, groups = head_groups(G);  // a window may begin inside a block
-  if (nb <= kOneGroup) return 0;
-  const int64_t blocks = cdiv(nb, (int64_t)4), share = cdiv((int64_t)kDenseTotal / 4, BH * groups);
-  const int64_t own = kDenseTotal / 4 / groups + BH, one = BH * (blocks < share ? blocks : share);
-  const int64_t many = own < BH * blocks ? own : BH * blocks, slots = one > many ? one : many;
+  const int64_t nb = cdiv(positions, (int64_t)kBlk) + 1;  // a window may begin inside a block
+  const int64_t one = dense_slots(BH, G, nb, false), own = dense_slots(BH, G, nb, true), slots = one > own ? one : own;
   return part_bytes(BH, G, D, slots);
 }
 
@@ -1001,7 +990,7 @@ extern "C" int fathom_rows8_attention(const void *q, int q_dtype, const void *k8
   if (need && reinterpret_cast<uintptr_t>(workspace) & 15)
     return fail(FATHOM_ERR_INVALID, "rows8_attention: the workspace must be 16-byte aligned");
   place(a, workspace, D, slots, lens != nullptr);
-  return run_dense(a, BH, D, code_dtype == FATHOM_DT_I8, dense_waves(BH * a.groups, nb, lens != nullptr), (hipStream_t)stream);
+  return run_dense(a, BH, D, code_dtype == FATHOM_DT_I8, one_group(nb), (hipStream_t)stream);
 }
 
 extern "C" size_t fathom_rows8_gather_attention_workspace_bytes(int64_t BH, int64_t G, int64_t D, int64_t k) {

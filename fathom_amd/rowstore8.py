@@ -104,11 +104,12 @@ class RowStore8:
             return None, None, int(v)
         if v.device != self.device:
             self._elsewhere(v)
-        if v.shape != (self.BH,) or v.dtype.is_floating_point or v.dtype == torch.bool:
-            raise ValueError(f"{what} must be an int or integers [{self.BH}], got {v.dtype} {tuple(v.shape)}")
-        if v.dtype == _I64:  # places beyond int32 stay beyond every store
-            v = v.clamp(-(1 << 31), (1 << 31) - 1)
-        if v.dtype != _I32 or not v.is_contiguous():
+        dtype = v.dtype
+        if v.shape != (self.BH,) or (dtype != _I32 and (dtype.is_floating_point or dtype.is_complex or dtype == torch.bool)):
+            raise ValueError(f"{what} must be an int or integers [{self.BH}], got {dtype} {tuple(v.shape)}")
+        if dtype != _I32 or not v.is_contiguous():
+            if dtype == _I64:  # places beyond int32 stay beyond every store
+                v = v.clamp(-(1 << 31), (1 << 31) - 1)
             v = v.to(_I32).contiguous()
         return v, v.data_ptr(), 0
 
@@ -147,7 +148,7 @@ class RowStore8:
             nbytes = _SIZES[key] = getattr(_lib.lib(), query)(self.BH, G, self.d, 1 << bits)
         if not nbytes:
             return None, None, 0
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+        ws = torch.empty((nbytes,), dtype=torch.uint8, device=self.device)
         return ws, ws.data_ptr(), nbytes
 
     # ------------------------------------------------------------------ writing and reading

@@ -2,6 +2,7 @@
 
 ``fathom_amd.bitplane`` is the drop-in for the reference module
 kernels/bitplane.py; ``fathom_amd.offload`` holds the host-resident store
-helpers and the top-k row gather.  All compute runs in libfathom_hip.so.
+helpers and the top-k row gather; ``fathom_amd.rowstore8`` holds K/V rows in 8
+bits and the attention over them.  All compute runs in libfathom_hip.so.
 """
 __version__ = "0.1.0"

@@ -142,8 +142,9 @@ __device__ const u32x4 kNoRow[8] = {};  // the row of a token that takes no part
 // channels at once (16 channels over 64 lanes: 12 swaps and 4 or 8 rotations), the waves in
 // LDS.
 //
-// Bound: latency (index, then row, then the joins): 512 positions of 32 x 4 heads move
-// 17.5 MB.
+// Bound: latency (index, then row, then the joins).  32 x 4 heads of 512 positions (17.6 MB of rows):
+// 7.2 us, of 8 x 7 of 2048 (30.5 MB) 9.9 and the join's 4.0.  With shuffles for the joins and
+// four waves per workgroup throughout: 11.5 with its join, and 14.5.
 template <int D, bool I8, int NW>
 __global__ __launch_bounds__(NW *kWave) void list_kernel(AttnArgs a) {
   constexpr int kLanes = D / 16;         // lanes of a row
@@ -414,7 +415,7 @@ __device__ __forceinline__ Part find_part(const AttnArgs &a, uint32_t w) {
   return p;  // bh = BH: the call needs no such workgroup
 }
 
-// Attention over every token of [lo, len): flash decoding on the matrix cores.
+// Attention over every token of [lo, len), in splits, on the matrix cores.
 //
 // A workgroup takes one split of a row for a group of 8 NG query heads; its waves
 // take the split's 64-token blocks in turn.  Per block (v_mfma_f32_16x16x32_f16,
@@ -422,14 +423,14 @@ __device__ __forceinline__ Part find_part(const AttnArgs &a, uint32_t w) {
 //   S^T = K q^T: A holds 16 tokens' codes as f16 (exact), straight from the
 //     16-byte pieces of the rows (the channel order inside the contraction is
 //     free, so it is the order that the pieces arrive in); B holds the queries,
-//     column c < 8 the f16 part of head c's q 2^sigma, column c + 8 the f16 of what
-//     that leaves: 22 bits of q, at no cost, as 8 heads fill half of the 16 columns.
-//     One row rotation adds the halves.
+//     column c < 8 the f16 of head c's q 2^sigma (times query_factor), column c + 8 the
+//     f16 of what that leaves: 22 bits of q, at no cost, as 8 heads fill half of
+//     the 16 columns.  One row rotation adds the halves.
 //   softmax: a lane holds 16 scores of its head, tokens 16 i + 4 (l >> 4) + j; the
 //     running maximum m (in log2 units) is raised only in the blocks where some
-//     score passes it.
-//   O^T += V^T p^T: D^T's column layout of the scores is B's layout of the weights
-//     once the contraction's token order is (tile, j), so the weights never leave their lane.
+//     score passes it.  A weight is 2^(S f - m) with one rounding, f = s_K times a power of two.
+//   O^T += V^T p^T: the layout that the scores come in is the one that B takes the
+//     weights in once the contraction's token order is (tile, j): they never leave their lane.
 //     Columns c < 8 hold the f16 of w = p s_V 2^(14 - E), columns c + 8 the f16 of
 //     the rest (22 bits of p); E is the running largest exponent of s_V, so w < 2^15.
 //     A holds V's codes, transposed inside the lane: it reads 8 (D = 64: 4) channels of 8
@@ -437,8 +438,12 @@ __device__ __forceinline__ Part find_part(const AttnArgs &a, uint32_t w) {
 // Rows are read through buffer descriptors that end at the row's length: what lies
 // behind it reads as zeros.
 //
-// Bound: HBM, 2 D bytes per token; the next block's K rows are requested once
-// the scores are formed, its V rows once the products are.
+// Bound: HBM, 2 D bytes per token.  The next block's K rows are requested once the
+// scores are formed, its V rows once the products are, so that a wave has 8 to 16 KB on the way all the
+// time.  A block takes 342 VALU instructions and 32 matrix ones (D = 128, NG = 1), a third of the
+// time that its rows take.  8 x 1048576 tokens of 4 heads (2.15 GB) 303 us, 7.1 TB/s; 32 x
+// 32768 (0.27 GB) 46 us with the join of the splits; one dot product per lane group and no matrix
+// cores: 917 and 127 us.  Short rows are bound by latency: the launch, the rows' way from HBM, one block's arithmetic.
 template <int D, bool I8, int NG, bool EXTRA, int NW>
 __global__ __launch_bounds__(NW *kWave, 2) void dense_kernel(AttnArgs a) {
   constexpr int kHalves = D / 64;  // 16-byte pieces of a row per lane
@@ -751,6 +756,7 @@ __global__ __launch_bounds__(NW *kWave, 2) void dense_kernel(AttnArgs a) {
 
 // Joins the splits of a query head, 32 channels per workgroup: a thread takes 16 bytes
 // of every 32nd split, requested before the splits' factors are known; sums run in a fixed order.
+// Bound: latency, 2.5 to 4.6 us (one thread per channel and splits in a row: 26 us for 64 splits).
 template <int D>
 __global__ __launch_bounds__(kMergeThreads) void merge_kernel(AttnArgs a) {
   constexpr int kLanes = 8, kGroups = kMergeThreads / kLanes, kBatch = 4;

@@ -24,21 +24,24 @@ __all__ = ["RowStore8"]
 
 _raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
 _F32, _I32, _I64 = torch.float32, torch.int32, torch.int64
+_FAR = 1 << 62  # ctypes would wrap what is longer
 _SIZES = {}  # workspace bytes by query and shape
 _CODES = {torch.float8_e4m3fn: _lib.DT_E4M3, torch.int8: _lib.DT_I8}
 
 
-def _aligned(x):
-    """Rows [BH, T, d] of a float type as the kernels read them: any strides, but dense
-    rows, and every row at a multiple of 16 bytes (a copy is made of others)."""
+def _rows(x):
+    """Rows [BH, T, d] of a float type as the kernels read them, with their strides: any,
+    but dense rows, each at a multiple of 16 bytes (a copy is made of others)."""
     if x.dtype not in _KDT:
         x = x.float()
     size = 4 if x.dtype == _F32 else 2
+    BH, T, _ = x.shape
     sr, st, sd = x.stride()
+    sr, st = sr if BH > 1 else 0, st if T > 1 else 0  # the stride of a single row says nothing
     if sd != 1 or (x.data_ptr() | sr * size | st * size) & 15:
-        x = x.contiguous()
-        x = x.clone() if x.data_ptr() & 15 else x
-    return x
+        x = torch.empty(x.shape, dtype=x.dtype, device=x.device).copy_(x)
+        sr, st, _ = x.stride()
+    return x, sr, st
 
 
 class RowStore8:
@@ -101,7 +104,10 @@ class RowStore8:
     def _per_row(self, v, what):
         """A per-row argument as (int32 tensor or None, its address, int)."""
         if not isinstance(v, torch.Tensor):
-            return None, None, int(v)
+            v = int(v)
+            if not -_FAR < v < _FAR:
+                raise ValueError(f"{what} {v}")
+            return None, None, v
         if v.device != self.device:
             self._elsewhere(v)
         dtype = v.dtype
@@ -170,8 +176,8 @@ class RowStore8:
             raise ValueError(f"K {K.dtype} {tuple(K.shape)} and V {V.dtype} {tuple(V.shape)} must be alike, "
                              f"[{self.BH}, T, {self.d}]")
         rows, rows_at, at = self._per_row(pos, "pos")
-        K, V = _aligned(K), _aligned(V)
-        (kr, kt, _), (vr, vt, _) = K.stride(), V.stride()
+        K, kr, kt = _rows(K)
+        V, vr, vt = _rows(V)
         self._call("fathom_rows8_write", K.data_ptr(), V.data_ptr(), _KDT[K.dtype], kr, kt, vr, vt, rows_at, at, self.BH,
                    K.shape[1], self.d, self.cap, self._code, *self._store())
 
@@ -214,7 +220,7 @@ class RowStore8:
         as within [0, cap].  A row without tokens gives zeros."""
         q, q_at, scale, softcap, slopes = self._query(q, scale, softcap, slopes)
         lens, lens_at, n = self._per_row(length, "length")
-        G, window = q.shape[1], int(window)
+        G, window = q.shape[1], min(int(window), _FAR)
         positions = n if lens is None else self.cap
         positions = max(min(positions, window) if window > 0 else positions, 0)
         ws, ws_at, nbytes = self._workspace("fathom_rows8_attention_workspace_bytes", G, positions)

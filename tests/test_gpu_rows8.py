@@ -156,6 +156,12 @@ def test_write_strided_views():
     st.write(every, K[0][:1].expand(H, T, D), 0)
     R.write(o, _f32(K[0].cpu()), _f32(K[0][:1].expand(H, T, D).cpu()), 0, "int8")
     _same(st, o, "int8")
+    one = qkv.view(-1)[4:4 + 203 * 3].view(1, 3, 203)  # a single row and token, with strides that are no multiple of 16 bytes
+    st1, o1 = _empty(1, 100, D, "int8")
+    for x in (one[:, 1:2, 4:68], one[:, :1, 20:84], one[:, ::2, 4:68]):
+        st1.write(x, x, 9)
+        R.write(o1, _f32(x.cpu()), _f32(x.cpu()), 9, "int8")
+        _same(st1, o1, "int8")
     st.write(K[0].double(), V[0].double(), 0)  # other types go through float32
     R.write(o, _f32(K[0].cpu()), _f32(V[0].cpu()), 0, "int8")
     _same(st, o, "int8")
@@ -352,7 +358,8 @@ def test_refusals():
     st = RowStore8.empty(2, 100, torch.int8, 64, DEV)
     K = torch.zeros(2, 10, 64, device=DEV)
     q, idx = torch.zeros(2, 3, 64, device=DEV), torch.zeros(2, 3, 5, dtype=torch.int64, device=DEV)
-    for bad in (lambda: st.write(K, K, 91), lambda: st.write(K, K, -1), lambda: st.write(K, K[:, :5]), lambda: st.write(K, K.half()),
+    for bad in (lambda: st.write(K, K, 2 ** 64), lambda: st.attention(q, 2 ** 64 + 5), lambda: st.read(2 ** 64, 5),
+                lambda: st.write(K, K, 91), lambda: st.write(K, K, -1), lambda: st.write(K, K[:, :5]), lambda: st.write(K, K.half()),
                 lambda: st.write(K[:1], K[:1]), lambda: st.write(K[..., :32], K[..., :32]), lambda: st.write(K.cpu(), K),
                 lambda: st.write(K, K, torch.zeros(3, dtype=torch.int32, device=DEV)),
                 lambda: st.write(K, K, torch.zeros(2, device=DEV)), lambda: st.read(0, 5, torch.int32), lambda: st.read(0, -1),
@@ -506,6 +513,26 @@ def test_attention_many_rows(BH, cap, G):
     listed = torch.arange(cap).expand(BH, G, cap).contiguous().to(DEV)
     every = st.gather_attention(q.to(DEV), listed, torch.from_numpy(lens.astype(np.int32)).to(DEV))
     assert (got - every).abs().max() <= 2e-5 * every.abs().max()
+
+
+@pytest.mark.parametrize("BH, G", [(520, 2), (65, 9)])
+def test_one_long_row_among_many(BH, G):
+    """A batch of short rows with a few long ones: every row equals the call on that row alone."""
+    cap, D = 9000, 64
+    st = RowStore8.empty(BH, cap, torch.float8_e4m3fn, D, DEV)
+    gen = torch.Generator(device=DEV).manual_seed(BH)
+    for t in (st.k8, st.v8):
+        t.view(torch.uint8).random_(0, 96, generator=gen).bitwise_xor_((torch.rand(t.shape, generator=gen, device=DEV) < 0.5) * 128)
+    for t in (st.k_scale, st.v_scale):
+        t.uniform_(0.1, 1.0, generator=gen)
+    lens = torch.randint(0, 200, (BH,), generator=gen, device=DEV, dtype=torch.int32)
+    lens[[3, BH // 2, BH - 1]] = torch.tensor([9000, 8001, 4000], dtype=torch.int32, device=DEV)
+    q = torch.randn(BH, G, D, generator=gen, device=DEV)
+    got = st.attention(q, lens)
+    for b in (0, 1, 2, 3, 4, 63, 64, BH // 2, BH - 2, BH - 1):
+        alone = RowStore8(st.k8[b:b + 1], st.v8[b:b + 1], st.k_scale[b:b + 1], st.v_scale[b:b + 1])
+        want = alone.attention(q[b:b + 1], int(lens[b]))
+        assert (got[b] - want[0]).abs().max() <= 2e-5 * want.abs().max(), b
 
 
 @pytest.mark.parametrize("BH, G, D", [(1, 1, 128), (3, 5, 64), (2, 33, 128)])

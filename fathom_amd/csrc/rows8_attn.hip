@@ -375,44 +375,81 @@ struct Part {
   int split, active, per;
 };
 // Rows of their own lengths (on the device): every workgroup takes `per` blocks, so
-// that the longest row does not hold the call up.  Each wave sums the rows'
-// blocks (a lane per row), which gives `per`, and finds its workgroup's row in the prefix sums
-// of ceil(blocks / per).  Those are at most kDenseTotal / kDenseWaves / head groups + BH, the grid.
-// (32 bits hold the sums: 2^31 blocks of D = 64 are 17 TB.)
+// that the longest row does not hold the call up.  Each workgroup sums the rows'
+// blocks, which gives `per`, and finds its row in the prefix sums of ceil(blocks /
+// per).  Those are at most kDenseTotal / kDenseWaves / head groups + BH, the grid.  (32
+// bits hold the sums: 2^31 blocks of D = 64 are 17 TB.)
+__device__ __forceinline__ uint32_t blocks_of(const AttnArgs &a, int r) {
+  int64_t lo, len, blk0;
+  int nb = 0;
+  if (r < (int)a.BH) row_blocks(a, r, lo, len, blk0, nb);
+  return (uint32_t)nb;
+}
+// Blocks per workgroup.  A row's last workgroup may have less to do: with few rows the
+// share leaves room for those, so that all of the call's workgroups are at work at once.
+__device__ __forceinline__ uint32_t share_of(const AttnArgs &a, uint32_t total) {
+  const int BH = (int)a.BH, fit = kDenseTotal / kDenseWaves / (int)a.groups;
+  const uint32_t groups = fit > 2 * BH ? fit - BH : fit > 0 ? fit : 1, even = (total + groups - 1) / groups;
+  return even > (uint32_t)kDenseWaves ? even : (uint32_t)kDenseWaves;
+}
+// Workgroups of row r of nb blocks; a row without tokens takes one too: it writes the row's zeros.
+__device__ __forceinline__ uint32_t groups_of(const AttnArgs &a, int r, uint32_t nb, uint32_t per) {
+  return r >= (int)a.BH ? 0u : nb <= per ? 1u : (nb + per - 1) / per;
+}
+
+// Up to 64 rows: a lane per row, each wave for itself.
 __device__ __forceinline__ Part find_part(const AttnArgs &a, uint32_t w) {
-  const int lane = threadIdx.x & 63, BH = (int)a.BH;
-  auto blocks = [&](int r) {
-    int64_t lo, len, blk0;
-    int nb = 0;
-    if (r < BH) row_blocks(a, r, lo, len, blk0, nb);
-    return (uint32_t)nb;
-  };
-  const uint32_t own = blocks(lane);  // rows 0 .. 63, most often all
-  uint32_t total = __builtin_amdgcn_readlane(wave_incl_scan_u32(own), 63);
-  for (int r0 = kWave; r0 < BH; r0 += kWave) total += __builtin_amdgcn_readlane(wave_incl_scan_u32(blocks(r0 + lane)), 63);
-  // a row's last workgroup may have less to do: with BH of them, the call's workgroups are
-  // at most kDenseTotal / kDenseWaves, all at work at once
-  const int fit = kDenseTotal / kDenseWaves / (int)a.groups;
-  const uint32_t groups = fit > 2 * BH ? fit - BH : fit / 2 > 0 ? fit / 2 : 1;
-  const uint32_t even = (total + groups - 1) / groups, per = even > (uint32_t)kDenseWaves ? even : (uint32_t)kDenseWaves;
-  Part p{a.BH, 0, 0, (int)per};
-  uint32_t before = 0;
-  for (int r0 = 0; r0 < BH; r0 += kWave) {
-    // a row without tokens takes a workgroup too: it writes the row's zeros
-    const uint32_t nb = r0 ? blocks(r0 + lane) : own;
-    const uint32_t act = r0 + lane >= BH ? 0u : nb <= per ? 1u : (nb + per - 1) / per;
-    const uint32_t upto = before + wave_incl_scan_u32(act);
-    const uint64_t past = __ballot(upto > w);
-    if (past) {
-      const int at = __builtin_ctzll(past);
-      p.bh = r0 + at;
-      p.active = __builtin_amdgcn_readlane((int)act, at);
-      p.split = (int)(w - (__builtin_amdgcn_readlane((int)upto, at) - p.active));
-      return p;
+  const int lane = threadIdx.x & 63;
+  const uint32_t nb = blocks_of(a, lane), per = share_of(a, __builtin_amdgcn_readlane(wave_incl_scan_u32(nb), 63));
+  const uint32_t act = groups_of(a, lane, nb, per), upto = wave_incl_scan_u32(act);
+  const uint64_t past = __ballot(upto > w);
+  if (!past) return Part{a.BH, 0, 0, 0};  // the call needs no such workgroup
+  const int at = __builtin_ctzll(past);
+  const int active = __builtin_amdgcn_readlane((int)act, at);
+  return Part{at, (int)w - (__builtin_amdgcn_readlane((int)upto, at) - active), active, (int)per};
+}
+
+// More rows: a thread takes BH / 256 of them in a row.  (512 rows, eight of them of 20032
+// tokens, the others of 700: 38 us, against 268 with a workgroup for every row; all of 2048 tokens 48.9, 44.8.)
+struct FindShared {
+  uint32_t wave[2][kDenseWaves];
+  int part[4];
+};
+__device__ __forceinline__ Part find_part_wide(const AttnArgs &a, uint32_t w, FindShared &sh) {
+  constexpr int kThreads = kDenseWaves * kWave;
+  const int tid = threadIdx.x, wave = tid >> 6;
+  const int c = ((int)a.BH + kThreads - 1) / kThreads, r0 = tid * c;
+  uint32_t sum = 0;
+  for (int i = 0; i < c; ++i) sum += blocks_of(a, r0 + i);
+  sum = wave_incl_scan_u32(sum);
+  if ((tid & 63) == 63) sh.wave[0][wave] = sum;
+  if (tid == 0) sh.part[0] = (int)a.BH;
+  __syncthreads();
+  uint32_t total = 0;
+#pragma unroll
+  for (int v = 0; v < kDenseWaves; ++v) total += sh.wave[0][v];
+  const uint32_t per = share_of(a, total);
+  uint32_t mine = 0;
+  for (int i = 0; i < c; ++i) mine += groups_of(a, r0 + i, blocks_of(a, r0 + i), per);
+  uint32_t upto = wave_incl_scan_u32(mine);
+  if ((tid & 63) == 63) sh.wave[1][wave] = upto;
+  __syncthreads();
+  for (int v = 0; v < wave; ++v) upto += sh.wave[1][v];
+  uint32_t at = upto - mine;
+  if (w >= at && w < upto)
+    for (int i = 0; i < c; ++i) {
+      const uint32_t act = groups_of(a, r0 + i, blocks_of(a, r0 + i), per);
+      if (w < at + act) {
+        sh.part[0] = r0 + i;
+        sh.part[1] = (int)(w - at);
+        sh.part[2] = (int)act;
+        break;
+      }
+      at += act;
     }
-    before = __builtin_amdgcn_readlane((int)upto, 63);
-  }
-  return p;  // bh = BH: the call needs no such workgroup
+  __syncthreads();
+  return Part{__builtin_amdgcn_readfirstlane(sh.part[0]), __builtin_amdgcn_readfirstlane(sh.part[1]),
+              __builtin_amdgcn_readfirstlane(sh.part[2]), __builtin_amdgcn_readfirstlane((int)per)};
 }
 
 // Attention over every token of [lo, len), in splits, on the matrix cores.
@@ -455,8 +492,13 @@ __global__ __launch_bounds__(NW *kWave, 2) void dense_kernel(AttnArgs a) {
   const int64_t g0 = (int64_t)blockIdx.y * 8 * NG;
   Part part{(int64_t)blockIdx.z, (int)blockIdx.x, (int)a.nsplit, 0};
   int64_t slot = (int64_t)blockIdx.z * a.nsplit + blockIdx.x;  // of the partial results
-  if (NW == kDenseWaves && a.where) {
-    part = find_part(a, blockIdx.x);
+  if (NW == kDenseWaves && a.where) {  // uniform over the workgroup
+    if (a.BH <= kWave) {
+      part = find_part(a, blockIdx.x);
+    } else {
+      __shared__ FindShared find;
+      part = find_part_wide(a, blockIdx.x, find);
+    }
     if (part.bh >= a.BH) return;
     slot = blockIdx.x;
     if (part.split == 0 && blockIdx.y == 0 && tid == 0) a.where[part.bh] = make_int2((int)blockIdx.x, part.active);
@@ -847,7 +889,7 @@ int list_waves(int64_t heads, int64_t k) {
 int64_t list_splits(int64_t heads, int64_t k) {
   const int waves = list_waves(heads, k);
   const int64_t most = cdiv(k, (int64_t)waves * kTile);
-  int64_t want = cdiv((int64_t)8192 / waves, heads);
+  int64_t want = (int64_t)8192 / waves / heads;
   if (want > kMaxSplits) want = kMaxSplits;
   const int64_t s = most < want ? most : want;
   return s < 1 ? 1 : s;
@@ -868,20 +910,28 @@ constexpr int64_t kOneGroup = 17;
 bool one_group(int64_t nb) { return nb > kDenseWaves && nb <= kOneGroup; }
 
 // Splits of a row of up to nb blocks in a call of `rows` rows (head groups counted):
-// kDenseTotal waves in all, at least one block per wave.
+// at least one block per wave, and no more than kDenseTotal waves in all, as
+// workgroups that have to wait for a place cost their whole prologue: 24 rows of 32768
+// tokens take 39.3 us in 21 splits, 47.8 in 22.  Two splits all the same where one
+// would leave more than a quarter of the places empty: 300 rows of 4096 tokens 67.7 us, in one split 73.0.
 int64_t dense_splits(int64_t rows, int64_t nb) {
   if (nb <= kOneGroup) return 1;
-  const int64_t want = cdiv((int64_t)kDenseTotal / kDenseWaves, rows), most = cdiv(nb, (int64_t)kDenseWaves);
-  return most < want ? most : want;
+  constexpr int64_t kPlaces = kDenseTotal / kDenseWaves;
+  const int64_t most = cdiv(nb, (int64_t)kDenseWaves);
+  int64_t room = kPlaces / rows;
+  if (room == 1 && rows < kPlaces * 3 / 4) room = 2;
+  const int64_t ns = most < room ? most : room;
+  return ns < 1 ? 1 : ns;
 }
 
 // Slots of partial results of a dense call; 0: every row fits one workgroup.  With
 // lengths on the device: the bound of find_part.  Neither falls as nb grows.
 int64_t dense_slots(int64_t BH, int64_t G, int64_t nb, bool lens) {
+  if (nb <= kOneGroup) return 0;
   const int64_t groups = head_groups(G), ns = dense_splits(BH * groups, nb);
-  if (ns <= 1) return 0;
+  if (!lens) return ns > 1 ? BH * ns : 0;
   const int64_t all = kDenseTotal / kDenseWaves / groups + BH, most = BH * cdiv(nb, (int64_t)kDenseWaves);
-  return !lens ? BH * ns : all < most ? all : most;
+  return all < most ? all : most;
 }
 
 // Bytes of `slots` partial results: rows, (m, l), the rows' slots.

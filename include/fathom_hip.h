@@ -393,12 +393,14 @@ int fathom_rows8_read(const void *k8, const void *v8, const float *k_scale, cons
  * [max(0, len - window), len) (window 0: all),
  *   z_t = softcap * tanh(u_t / softcap) + slopes[bh, g] * (t - (len - 1)),
  *   u_t = scale * q[bh, g] . K_t;   out[bh, g] = softmax(z) . V
- * without the cap for softcap = 0 and without the bias for slopes = NULL.  q
- * [BH, G, D] of q_dtype (FATHOM_DT_F32/F16/BF16, 16-byte aligned), out
- * [BH, G, D] float32.  A row without tokens gives zeros.
- * workspace: fathom_rows8_attention_workspace_bytes(BH, G, D, positions) bytes,
- * positions = the smaller of the longest length the host knows (n, or cap where
- * lens is given) and, if not 0, the window.
+ * without the cap for softcap = 0 (else positive and finite) and without the bias
+ * for slopes = NULL.  q [BH, G, D] of q_dtype (FATHOM_DT_F32/F16/BF16, 16-byte
+ * aligned), out [BH, G, D] float32.  A row without tokens gives zeros; what lies
+ * behind a row's length is not used.
+ * workspace (16-byte aligned): fathom_rows8_attention_workspace_bytes(BH, G, D,
+ * positions) bytes, positions = the smaller of the longest length the host knows
+ * (n, or cap where lens is given) and, if not 0, the window.  The query never falls
+ * as positions grow.  0 bytes: workspace may be NULL.
  */
 size_t fathom_rows8_attention_workspace_bytes(int64_t BH, int64_t G, int64_t D, int64_t positions);
 int fathom_rows8_attention(const void *q, int q_dtype, const void *k8, const void *v8, const float *k_scale,
@@ -410,7 +412,8 @@ int fathom_rows8_attention(const void *q, int q_dtype, const void *k8, const voi
  * The same attention over listed tokens, t = idx[bh, g, j] for j < k (int64,
  * device; a token listed twice counts twice).  Tokens outside [0, len) take no
  * part (fathom_gather_attention's zero rows score 0 instead).
- * workspace: fathom_rows8_gather_attention_workspace_bytes(BH, G, D, k) bytes.
+ * workspace: fathom_rows8_gather_attention_workspace_bytes(BH, G, D, k) bytes, as
+ * above; the query never falls as k grows.
  */
 size_t fathom_rows8_gather_attention_workspace_bytes(int64_t BH, int64_t G, int64_t D, int64_t k);
 int fathom_rows8_gather_attention(const void *q, int q_dtype, const int64_t *idx, const void *k8, const void *v8,

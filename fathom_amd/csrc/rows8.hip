@@ -211,7 +211,8 @@ void launch_write(const WriteArgs &a, int64_t BH, hipStream_t st) {
 
 template <int D, int DT, bool I8>
 void launch_read(const ReadArgs &a, int64_t BH, hipStream_t st) {
-  read_kernel<D, DT, I8><<<dim3((unsigned)cdiv(a.R, (int64_t)kReadPieces * kThreads * (DT == FATHOM_DT_F32 ? 4 : 8) / D), (unsigned)BH, 2), kThreads, 0, st>>>(a);
+  constexpr int64_t kRows = kReadPieces * kThreads * (DT == FATHOM_DT_F32 ? 4 : 8) / D;
+  read_kernel<D, DT, I8><<<dim3((unsigned)cdiv(a.R, kRows), (unsigned)BH, 2), kThreads, 0, st>>>(a);
 }
 
 #define FATHOM_ROWS8_DISPATCH(fn, ...)                                         \

@@ -885,14 +885,18 @@ int list_waves(int64_t heads, int64_t k) {
   if (k <= kOne) return k > 4 * kTile ? 16 : 4;
   return heads * cdiv(k, kOne) >= 96 ? 16 : 4;
 }
-// Splits of a head's listed positions: a tile per wave, as long as the chip has room for more workgroups.
+// Splits of a head's listed positions: a tile per wave, as long as the chip has room
+// for all workgroups at once (kListTotal waves, 16 per CU).  With twice as many:
+// 32 x 4 heads of 2048 positions 21.1 us, 17.4 so; 64 x 4 of 1024 21.2, 13.6; 32 x 8 of 4096 50.7, 45.2.
+constexpr int64_t kListTotal = 4096;
+int64_t list_room(int64_t heads, int waves) {
+  const int64_t room = kListTotal / waves / heads;
+  return room < 1 ? 1 : room < kMaxSplits ? room : kMaxSplits;
+}
 int64_t list_splits(int64_t heads, int64_t k) {
   const int waves = list_waves(heads, k);
-  const int64_t most = cdiv(k, (int64_t)waves * kTile);
-  int64_t want = (int64_t)8192 / waves / heads;
-  if (want > kMaxSplits) want = kMaxSplits;
-  const int64_t s = most < want ? most : want;
-  return s < 1 ? 1 : s;
+  const int64_t most = cdiv(k, (int64_t)waves * kTile), room = list_room(heads, waves);
+  return most < 1 ? 1 : most < room ? most : room;
 }
 
 // Head groups of a row and their size in eights: a workgroup holds up to 16 heads.
@@ -1054,8 +1058,7 @@ extern "C" size_t fathom_rows8_gather_attention_workspace_bytes(int64_t BH, int6
   if (k <= 16 * kTile) return 0;
   // of the narrower workgroups, so that it never falls as k grows
   int64_t ns = cdiv(k, (int64_t)4 * kTile);
-  if (ns > cdiv((int64_t)2048, BH * G)) ns = cdiv((int64_t)2048, BH * G);
-  if (ns > kMaxSplits) ns = kMaxSplits;
+  if (ns > list_room(BH * G, 4)) ns = list_room(BH * G, 4);
   return part_bytes(BH, G, D, ns > 1 ? BH * ns : 0);
 }
 

@@ -100,7 +100,6 @@ __device__ __forceinline__ float across_groups(float v) {
   return op(__uint_as_float(p16[0]), __uint_as_float(p16[1]));
 }
 
-
 // v of another lane of the same row of 16, by a DPP control.
 template <int CTRL>
 __device__ __forceinline__ float dpp(float v) {
@@ -188,13 +187,14 @@ __global__ __launch_bounds__(NW *kWave) void list_kernel(AttnArgs a) {
       vc[i] = *reinterpret_cast<const u32x4 *>(in[i] ? vb + tok[i] * D : none);
       vs[i] = vsb[in[i] ? (uint64_t)tok[i] / kBlk : 0];
     }
+    // the queries are requested with the first tile, behind its rows
     if (first) {
-      first = false;
 #pragma unroll
       for (int h = 0; h < 2; ++h) load8_q(a.q, a.q_dtype, (bh * a.G + g) * D + d0 + 8 * h, q[h]);
     }
     __builtin_amdgcn_sched_barrier(0);
-    if (t0 < (s + 1) * NW * kTile) {  // the wave's first tile
+    if (first) {
+      first = false;
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll

@@ -341,6 +341,22 @@ def test_extreme_scores_and_values(code):
             _check(st, Kv, Vv, (q * size), [n], n, scale=scale, idx=torch.arange(n).expand(1, 2, n))
 
 
+@pytest.mark.parametrize("code", ["e4m3", "int8"])
+def test_negative_scales(code):
+    """A negative score scale, and stores from elsewhere whose block scales have signs, or are 0."""
+    st, K, V = _filled(2, 400, 64, code, [400, 390])
+    for t, vals in ((st.k_scale, K), (st.v_scale, V)):
+        t[:, 1::3] *= -1
+        t[:, 4] = 0
+        vals[:, np.arange(400) // BLK % 3 == 1] *= -1
+        vals[:, 256:320] = 0
+    q = _q(2, 3, 64, 4)
+    idx = torch.randint(0, 390, (2, 3, 100), generator=torch.Generator().manual_seed(4))
+    for scale, softcap in ((None, None), (-0.2, None), (-0.2, 4.0), (0.0, None)):
+        _check(st, K, V, q, [390, 390], 390, softcap=softcap, scale=scale)
+        _check(st, K, V, q, [390, 390], 390, softcap=softcap, scale=scale, idx=idx)
+
+
 def test_nan_in_a_row_reaches_its_heads_only():
     st, K, V = _filled(2, 300, 128, "e4m3", [300, 300])
     st.v8.view(torch.uint8)[0, 150, 7] = 0x7F

@@ -108,7 +108,7 @@ def _attn_args(**kw):
     (dict(softcap=-1.0), b"softcap", _lib.ERR_INVALID), (dict(softcap=float("nan")), b"softcap", _lib.ERR_INVALID),
     (dict(softcap=float("inf")), b"softcap", _lib.ERR_INVALID),
     (dict(q=(1 << 20) + 4), b"aligned", _lib.ERR_INVALID), (dict(D=32), b"D=32", _lib.ERR_INVALID),
-    (dict(), b"workspace", _lib.ERR_WORKSPACE)])
+    (dict(ws=(1 << 28) + 8, wsb=1 << 34), b"aligned", _lib.ERR_INVALID), (dict(), b"workspace", _lib.ERR_WORKSPACE)])
 def test_attention_refusals(bad, text, status):
     L = _lib.lib()
     assert L.fathom_rows8_attention(*_attn_args(**bad)) == status
@@ -117,7 +117,8 @@ def test_attention_refusals(bad, text, status):
 
 @pytest.mark.parametrize("bad, text, status", [
     (dict(idx=None), b"null", _lib.ERR_INVALID), (dict(k=-1), b"k=-1", _lib.ERR_INVALID),
-    (dict(k=1 << 30), b"k=", _lib.ERR_INVALID), (dict(k=1 << 20), b"workspace", _lib.ERR_WORKSPACE)])
+    (dict(k=1 << 30), b"k=", _lib.ERR_INVALID), (dict(k=1 << 20), b"workspace", _lib.ERR_WORKSPACE),
+    (dict(k=1 << 20, ws=(1 << 28) + 4, wsb=1 << 34), b"aligned", _lib.ERR_INVALID)])
 def test_gather_attention_refusals(bad, text, status):
     a = dict(q=1 << 20, q_dtype=_lib.DT_F32, idx=1 << 27, k8=1 << 22, v8=1 << 23, ks=1 << 24, vs=1 << 25, code=_lib.DT_I8, BH=2,
              G=4, k=512, D=128, cap=1000, lens=None, n=1000, scale=0.1, softcap=0.0, slopes=None, out=1 << 26, ws=None, wsb=0,

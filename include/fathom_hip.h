@@ -355,7 +355,8 @@ int fathom_gather_attention(const float *q, const int64_t *idx, int64_t BH, int6
  * reference.  Per (batch, KV head) row, for K and V apart: codes k8, v8
  * [BH, cap, D] of one byte (code_dtype FATHOM_DT_E4M3 or FATHOM_DT_I8) and
  * scales k_scale, v_scale [BH, ceil(cap / 64)] float32, one per 64-token block;
- * value = code * scale.  D = 64 or 128; codes 16-byte aligned; BH <= 65535.
+ * value = code * scale.  D = 64 or 128; codes 16-byte aligned; BH and G <= 65535;
+ * cap < 2^31 - 64.
  */
 
 /*

@@ -20,6 +20,10 @@ constexpr int kDenseTotal = 2048;  // waves of a dense call: eight per CU, all a
 constexpr int kMaxSplits = 512;  // of a query head
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLowest = -3.0e38f;  // below every score: the running maximum of no token
+// A weight is 2^(x y - m), m the largest rounded x y: below kLarge with one rounding (a fused multiply-add), which leaves the
+// maximum's own rounding in the weights, all alike, at most 2^(1/16) here.  Past it that would be 2 and more, up to
+// infinity or 0, so there the product is rounded first and the largest weight is 1.
+constexpr float kLarge = 1048576.0f;  // 2^20
 
 struct AttnArgs {
   const void *q;
@@ -170,7 +174,7 @@ __global__ __launch_bounds__(NW *kWave) void list_kernel(AttnArgs a) {
     int64_t tok[kLoads];
     bool in[kLoads];
     u32x4 kc[kLoads], vc[kLoads];
-    float ks[kLoads], vs[kLoads], x[kLoads], y[kLoads], bias[kLoads];
+    float ks[kLoads], vs[kLoads], x[kLoads], y[kLoads], bias[kLoads], z[kLoads];
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
       const int64_t j = t0 + i * kRows + rg;
@@ -211,7 +215,7 @@ __global__ __launch_bounds__(NW *kWave) void list_kernel(AttnArgs a) {
 #pragma unroll
         for (int f = 0; f < 4; ++f) dot = fmaf(q[e / 2][4 * (e & 1) + f], c[f], dot);
       }
-      // z = x y + bias: the product is rounded only once it is relative to the maximum
+      // z = x y + bias: below kLarge the product is rounded only once it is relative to the maximum
       x[i] = sum_row<kLanes>(dot);
       y[i] = ldexpf(ks[i], ce);
       if (a.softcap > 0.0f) {
@@ -219,8 +223,8 @@ __global__ __launch_bounds__(NW *kWave) void list_kernel(AttnArgs a) {
         y[i] = a.softcap * kLog2e;
       }
       bias[i] = slope * (float)(int)(tok[i] - (len - 1));
-      const float z = fmaf(x[i], y[i], bias[i]);
-      mt = fmaxf(mt, in[i] ? z : kLowest);
+      z[i] = fmaf(x[i], y[i], bias[i]);
+      mt = fmaxf(mt, in[i] ? z[i] : kLowest);
     }
     const float f = __builtin_amdgcn_exp2f(m - mt);
     l *= f;
@@ -229,7 +233,8 @@ __global__ __launch_bounds__(NW *kWave) void list_kernel(AttnArgs a) {
     m = mt;
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
-      const float p = in[i] ? __builtin_amdgcn_exp2f(fmaf(x[i], y[i], bias[i] - m)) : 0.0f;
+      const float d = fabsf(m) < kLarge ? fmaf(x[i], y[i], bias[i] - m) : z[i] - m;
+      const float p = in[i] ? __builtin_amdgcn_exp2f(d) : 0.0f;
       l += p;
       const float pv = in[i] ? p * vs[i] : 0.0f;
 #pragma unroll
@@ -465,7 +470,7 @@ __device__ __forceinline__ Part find_part_wide(const AttnArgs &a, uint32_t w, Fi
 //     the 16 columns.  One row rotation adds the halves.
 //   softmax: a lane holds 16 scores of its head, tokens 16 i + 4 (l >> 4) + j; the
 //     running maximum m (in log2 units) is raised only in the blocks where some
-//     score passes it.  A weight is 2^(S f - m) with one rounding, f = s_K times a power of two.
+//     score passes it.  A weight is 2^(S f - m) with one rounding (see kLarge), f = s_K times a power of two.
 //   O^T += V^T p^T: the layout that the scores come in is the one that B takes the
 //     weights in once the contraction's token order is (tile, j): they never leave their lane.
 //     Columns c < 8 hold the f16 of w = p s_V 2^(14 - E), columns c + 8 the f16 of
@@ -618,7 +623,7 @@ __global__ __launch_bounds__(NW *kWave, 2) void dense_kernel(AttnArgs a) {
     float fz[NG];
 #pragma unroll
     for (int n = 0; n < NG; ++n) {
-      // z = s f; not rounded itself, but relative to the maximum
+      // z = s f; below kLarge not rounded itself, but relative to the maximum
       float f = ldexpf(fabsf(ks), ex[n]);
       f = f == f ? fmaxf(f, 1.2e-38f) : f;  // never 0: a score of -inf has to stay one
 #pragma unroll
@@ -676,6 +681,14 @@ __global__ __launch_bounds__(NW *kWave, 2) void dense_kernel(AttnArgs a) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) mx = fmaxf(mx, s[n][i][j]);
       mx *= f;
+      if constexpr (!EXTRA) {
+        if (__any(fabsf(mx) >= kLarge && fabsf(mx) < INFINITY)) {
+          asm volatile("");  // a branch, not products in every block
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[n][i] *= f;
+          f = 1.0f;
+        }
+      }
       fz[n] = f;
       if (__any(mx > m[n])) {
         const float M = fmaxf(m[n], across_groups<true>(mx));

@@ -24,6 +24,8 @@ constexpr float kLowest = -3.0e38f;  // below every score: the running maximum o
 // maximum's own rounding in the weights, all alike, at most 2^(1/16) here.  Past it that would be 2 and more, up to
 // infinity or 0, so there the product is rounded first and the largest weight is 1.
 constexpr float kLarge = 1048576.0f;  // 2^20
+constexpr float kNoValue = -1000.0f;  // log2 of the largest weight times scale before any
+constexpr float kLeast = -112.0f;     // a block counts there with that weight at least: 2^14 s_V / (weight s_V) is finite
 
 struct AttnArgs {
   const void *q;
@@ -474,7 +476,10 @@ __device__ __forceinline__ Part find_part_wide(const AttnArgs &a, uint32_t w, Fi
 //   O^T += V^T p^T: the layout that the scores come in is the one that B takes the
 //     weights in once the contraction's token order is (tile, j): they never leave their lane.
 //     Columns c < 8 hold the f16 of w = p s_V 2^(14 - E), columns c + 8 the f16 of
-//     the rest (22 bits of p); E is the running largest exponent of s_V, so w < 2^15.
+//     the rest: 22 bits of p, down to 2^-38 of the largest p s_V.  E = ceil(R), R the running
+//     largest log2(p s_V) of a head, taken block by block as the block's largest score and
+//     the exponent of its scale, and relative to m (it falls as m rises).  So w < 2^15, and a block of
+//     large values without weight takes no bits from the others.
 //     A holds V's codes, transposed inside the lane: it reads 8 (D = 64: 4) channels of 8
 //     tokens and pairs two tokens' bytes with one v_perm.
 // Rows are read through buffer descriptors that end at the row's length: what lies
@@ -579,15 +584,15 @@ __global__ __launch_bounds__(NW *kWave, 2) void dense_kernel(AttnArgs a) {
   }
 
   f32x4 o[NG][kCh];
-  float m[NG], l[NG];
+  float m[NG], l[NG], R[NG];
 #pragma unroll
   for (int n = 0; n < NG; ++n) {
     m[n] = kLowest;
     l[n] = 0.0f;
+    R[n] = kNoValue;
 #pragma unroll
     for (int e = 0; e < kCh; ++e) o[n][e] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   }
-  int E = -1000;
 
   // the scales come through the scalar cache, a block ahead too
   typedef const __attribute__((address_space(4))) float *scalar_ptr;
@@ -620,6 +625,7 @@ __global__ __launch_bounds__(NW *kWave, 2) void dense_kernel(AttnArgs a) {
     // ---- scores, in log2 units; tokens outside [lo, len) have none
     const int t0 = (int)(b * kBlk), in_block = t0 + 4 * grp;
     const bool edge = (int64_t)t0 < lo || (int64_t)t0 + kBlk > len;
+    const int ev = (int)((__float_as_uint(vs) >> 23) & 0xFF) - 127;
     float fz[NG];
 #pragma unroll
     for (int n = 0; n < NG; ++n) {
@@ -690,25 +696,24 @@ __global__ __launch_bounds__(NW *kWave, 2) void dense_kernel(AttnArgs a) {
         }
       }
       fz[n] = f;
-      if (__any(mx > m[n])) {
-        const float M = fmaxf(m[n], across_groups<true>(mx));
-        const float down = __builtin_amdgcn_exp2f(m[n] - M);
+      float by = 1.0f;
+      const float was = R[n];
+      if (__any(fmaxf(mx - m[n], kLeast) > fminf(0.0f, was - (float)ev))) {  // a larger score, or weight times scale
+        mx = across_groups<true>(mx);
+        const float M = fmaxf(m[n], mx), down = __builtin_amdgcn_exp2f(m[n] - M);
+        R[n] = fmaxf(was + (m[n] - M), (float)ev + fmaxf(mx - M, kLeast));
         m[n] = M;
         l[n] *= down;
+        by = ldexpf(down, (int)ceilf(was) - (int)ceilf(R[n]));
+      }
+      if (__any(by != 1.0f)) {  // apart from the branch above, which would take more registers (8 x 65536, 12 heads: 45 us for 35)
 #pragma unroll
-        for (int e = 0; e < kCh; ++e) o[n][e] *= down;
+        for (int e = 0; e < kCh; ++e) o[n][e] *= by;
       }
     }
-    const int ev = (int)((__float_as_uint(vs) >> 23) & 0xFF) - 127;
-    if (ev > E) {  // uniform: a larger scale of V than any before
-      const float down = ldexpf(1.0f, E - ev);
-      E = ev;
+    float wv[NG];
 #pragma unroll
-      for (int n = 0; n < NG; ++n)
-#pragma unroll
-        for (int e = 0; e < kCh; ++e) o[n][e] *= down;
-    }
-    const float wv = ldexpf(vs, 14 - E);
+    for (int n = 0; n < NG; ++n) wv[n] = ldexpf(vs, 14 - (int)ceilf(R[n]));
     if (edge) {  // a token outside has no value either (its codes may be NaN)
 #pragma unroll
       for (int i = 0; i < 4; ++i)
@@ -729,7 +734,7 @@ __global__ __launch_bounds__(NW *kWave, 2) void dense_kernel(AttnArgs a) {
           const float p0 = __builtin_amdgcn_exp2f(fmaf(s[n][2 * c + x / 2][2 * (x & 1)], fz[n], -m[n]));
           const float p1 = __builtin_amdgcn_exp2f(fmaf(s[n][2 * c + x / 2][2 * (x & 1) + 1], fz[n], -m[n]));
           ps[x] = p0 + p1;
-          pp[x] = split16(p0 * wv, p1 * wv, keep);
+          pp[x] = split16(p0 * wv[n], p1 * wv[n], keep);
         }
         l[n] += (ps[0] + ps[1]) + (ps[2] + ps[3]);
         p[n] = join8(pp[0], pp[1], pp[2], pp[3]);
@@ -764,10 +769,10 @@ __global__ __launch_bounds__(NW *kWave, 2) void dense_kernel(AttnArgs a) {
     load_v(b + NW);
   }
   // ---- the workgroup's waves
-  const float up = E > -1000 ? ldexpf(1.0f, E - 14) : 0.0f;
 #pragma unroll
   for (int n = 0; n < NG; ++n) {
     const float L = across_groups<false>(l[n]);
+    const int up = (int)ceilf(R[n]) - 14;
     if (lane < 8) {
       wm[wave][8 * n + lane] = m[n];
       wl[wave][8 * n + lane] = L;
@@ -777,10 +782,10 @@ __global__ __launch_bounds__(NW *kWave, 2) void dense_kernel(AttnArgs a) {
 #pragma unroll
       for (int e = 0; e < kCh; e += 4) {
         float4 v;
-        v.x = add_other_half(o[n][e][j]) * up;
-        v.y = add_other_half(o[n][e + 1][j]) * up;
-        v.z = add_other_half(o[n][e + 2][j]) * up;
-        v.w = add_other_half(o[n][e + 3][j]) * up;
+        v.x = ldexpf(add_other_half(o[n][e][j]), up);
+        v.y = ldexpf(add_other_half(o[n][e + 1][j]), up);
+        v.z = ldexpf(add_other_half(o[n][e + 2][j]), up);
+        v.w = ldexpf(add_other_half(o[n][e + 3][j]), up);
         if (col < 8) *reinterpret_cast<float4 *>(&wo[wave][8 * n + col][(4 * grp + j) * kCh + e]) = v;
       }
   }

@@ -102,7 +102,9 @@ def attention(q, K, V, toks, length, scale, softcap=0.0, slope=None):
     most U relative to the sum of their sizes (A), the scale, cap and bias a few more U of the
     score's size; a score's error enters its weight e^z, once above and once below the
     fraction.  Sums over tokens run in chains of at most an eighth of them plus the
-    joins; a weight held as two f16 parts is off by 2^-22 of itself or 2^-38."""
+    joins; a weight w held as two f16 parts is off by 2^-22 of itself, or by 2^-38 of the
+    largest w s of a token (s: its block's scale of V) times the format's largest code, which is at most
+    twice the largest |V| of the block."""
     D = q.shape[0]
     if len(toks) == 0:
         return np.zeros(D), np.zeros(D)
@@ -118,4 +120,5 @@ def attention(q, K, V, toks, length, scale, softcap=0.0, slope=None):
     weight = w @ np.abs(v)
     dz = (D + 24) * U * a + 8 * U * (np.abs(z).max() + np.abs(bias).max())
     rel = 2 * dz + (len(toks) / 8 + 64) * U + 2.0 ** -20
-    return w @ v, rel * weight + len(toks) * 2.0 ** -37 * np.abs(v).max(0)
+    blocks = np.nan_to_num(np.abs(np.pad(V, ((0, -len(V) % BLK), (0, 0))))).reshape(-1, BLK * D).max(1)
+    return w @ v, rel * weight + len(toks) * 2.0 ** -37 * (w * blocks[np.asarray(toks) // BLK]).max()

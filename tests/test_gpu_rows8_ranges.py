@@ -83,3 +83,42 @@ def test_scores_that_differ_by_little_beside_their_size():
     for got in _both(st, q.to(DEV), n, scale=1.0):
         got = got[0].double().cpu().numpy()
         assert (got >= least - slack).all() and (got <= most + slack).all()
+
+
+# ----------------------------------------------------------------------------- scales of V far apart
+@pytest.mark.parametrize("code", ["e4m3", "int8"])
+@pytest.mark.parametrize("D, G", [(64, 3), (128, 3), (64, 12), (128, 12)])
+@pytest.mark.parametrize("power", [20, 40, 60])
+def test_large_values_without_weight(code, D, G, power):
+    """Blocks of large values whose tokens have next to no weight, before, behind and among those that have it: the others'
+    values keep their bits."""
+    for n, where in ((500, "first"), (500, "last"), (1000, "first"), (1000, "every fifth"), (4000, "first"), (4000, "last")):
+        rng = np.random.default_rng(power)
+        K, V = rng.standard_normal((1, n, D)), rng.standard_normal((1, n, D))
+        blk = np.arange(n) // BLK
+        big = blk == 0 if where == "first" else blk == blk[-1] if where == "last" else blk % 5 == 0
+        V[0, big] *= 2.0 ** power
+        q = _q(1, G, D, 5)
+        far = -(power * np.log(2.0) + 30.0) * D ** 0.5  # the large values' weights: e^-30 beside their size
+        K[0, :, 0] = np.where(big, far / 8, 0.0)
+        q[..., 0] = 8.0
+        st, Kv, Vv = _rows(K, V, code)
+        _check(st, Kv, Vv, q, [n], n)
+        _check(st, Kv, Vv, q, [n], torch.tensor([n], dtype=torch.int32, device=DEV))
+        _check(st, Kv, Vv, q, [n], n, softcap=1e4, slopes=torch.full((1, G), 1e-3))
+
+
+@pytest.mark.parametrize("code", ["e4m3", "int8"])
+@pytest.mark.parametrize("falls", [True, False])
+def test_values_and_weights_over_many_decades(code, falls):
+    """Scales of V and weights that rise and fall together or against each other, over more than the float32 range."""
+    n, D = 1500, 64
+    rng = np.random.default_rng(2)
+    t = np.linspace(1.0, 0.0, n) if falls else np.linspace(0.0, 1.0, n)
+    for values, weights in ((60, 0), (60, 40), (60, -40), (-60, 200), (60, -200)):
+        K, V = np.zeros((1, n, D)), rng.standard_normal((1, n, D)) * np.exp(values * t)[:, None]
+        K[0, :, 0] = weights * t
+        q = torch.zeros(1, 2, D)
+        q[0, :, 0] = 1.0
+        st, Kv, Vv = _rows(K, V, code)
+        _check(st, Kv, Vv, q, [n], n, scale=1.0)

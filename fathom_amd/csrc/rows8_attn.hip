@@ -363,6 +363,14 @@ __device__ __forceinline__ f16x2 split16(float x, float y, float keep) {
   return __builtin_convertvector(f32x2{fmaf((float)hi.x, keep, x), fmaf((float)hi.y, keep, y)}, f16x2);
 }
 
+// Of a query channel x (the head's largest in [2^12, 2^14)): whether two f16 may hold fewer than 19 bits
+// of it, and what they leave of such a one, times 2^38 (at most 2^13: they end at 2^-24).
+__device__ __forceinline__ bool small_channel(float x) { return fabsf(x) < 0x1p-6f && x != 0.0f; }
+__device__ __forceinline__ float rest_of(float x) {
+  const float left = x - (float)(_Float16)x;
+  return small_channel(x) ? ldexpf(left - (float)(_Float16)left, 38) : 0.0f;
+}
+
 // v + the value of the lane 8 columns away in the same row of 16 lanes (row_ror:8).
 __device__ __forceinline__ float add_other_half(float v) {
   return v + dpp<kXor8>(v);
@@ -469,7 +477,10 @@ __device__ __forceinline__ Part find_part_wide(const AttnArgs &a, uint32_t w, Fi
 //     free, so it is the order that the pieces arrive in); B holds the queries,
 //     column c < 8 the f16 of head c's q 2^sigma (times query_factor), column c + 8 the
 //     f16 of what that leaves: 22 bits of q, at no cost, as 8 heads fill half of
-//     the 16 columns.  One row rotation adds the halves.
+//     the 16 columns.  One row rotation adds the halves.  Channels far below their head's
+//     largest would have fewer: where a group has one below 2^-18 (1 % of normal queries), what is
+//     left of those takes a second product, times 2^38, before the first (8 x 1048576 tokens 310 us for
+//     305).  So 19 bits and more down to 2^-56 of the largest channel, and none below 2^-76.
 //   softmax: a lane holds 16 scores of its head, tokens 16 i + 4 (l >> 4) + j; the
 //     running maximum m (in log2 units) is raised only in the blocks where some
 //     score passes it.  A weight is 2^(S f - m) with one rounding (see kLarge), f = s_K times a power of two.
@@ -552,6 +563,8 @@ __global__ __launch_bounds__(NW *kWave, 2) void dense_kernel(AttnArgs a) {
   load_v(first + wave);
   const float keep = col < 8 ? 0.0f : -1.0f;  // columns 8 .. 15 hold what the f16 of columns 0 .. 7 leave
   f16x8 qf[NG][kSteps];
+  __shared__ f16x8 rest[NG][kSteps][kWave];  // what qf leaves of small channels, 2^38
+  bool far = false;  // some channel is that small
   int ce, ex[NG];   // per lane: the exponent that its head's scores take
   float slope[NG];  // its bias per token
   const float cm = query_factor(a, ce);
@@ -559,11 +572,17 @@ __global__ __launch_bounds__(NW *kWave, 2) void dense_kernel(AttnArgs a) {
   for (int n = 0; n < NG; ++n) {
     const int64_t g = g0 + 8 * n + (col & 7);
     float mx = 0.0f;
+    uint32_t mn = 0xFFFFFFFFu;  // the bits of the smallest |q| but 0, doubled, less 1
 #pragma unroll
     for (int h = 0; h < kSteps; ++h)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fabsf(q[n][h][e]));
+      for (int e = 0; e < 8; ++e) {
+        mx = fmaxf(mx, fabsf(q[n][h][e]));
+        const uint32_t v = 2u * __float_as_uint(q[n][h][e]) - 1u;
+        mn = v < mn ? v : mn;
+      }
     mx = across_groups<true>(mx);
+    far |= mn < 2u * (__float_as_uint(mx) - (18u << 23));  // below mx 2^-18; wraps for mx < 2^-108, where all count as such
     int sigma = 0;  // the largest |q| of the head in [2^13, 2^14)
     if (mx > 0.0f && mx < INFINITY) {
       frexpf(mx, &sigma);
@@ -574,13 +593,44 @@ __global__ __launch_bounds__(NW *kWave, 2) void dense_kernel(AttnArgs a) {
       f16x2 part[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float x = ldexpf(q[n][h][2 * e], sigma), y = ldexpf(q[n][h][2 * e + 1], sigma);
-        part[e] = split16(x * cm, y * cm, keep);
+        const float x = ldexpf(q[n][h][2 * e], sigma) * cm, y = ldexpf(q[n][h][2 * e + 1], sigma) * cm;
+        part[e] = split16(x, y, keep);
+        q[n][h][2 * e] = x;
+        q[n][h][2 * e + 1] = y;
       }
       qf[n][h] = join8(part[0], part[1], part[2], part[3]);
     }
     ex[n] = ce - sigma;
     slope[n] = EXTRA && a.slopes && g < a.G ? a.slopes[bh * a.G + g] * kLog2e : 0.0f;
+  }
+
+  far = __any(far);  // uniform over the workgroup: its waves hold the same queries
+  // Two groups of eight heads keep them in LDS: in registers, D = 128 with cap and bias spills (8 x 65536 tokens, 12 heads
+  // 47 us; 40).
+  constexpr bool kQueryLds = NG > 1;
+  __shared__ f16x8 qs[kQueryLds ? NG : 1][kSteps][kWave];
+  if constexpr (kQueryLds) {
+    if (wave == 0) {
+#pragma unroll
+      for (int n = 0; n < NG; ++n)
+#pragma unroll
+        for (int h = 0; h < kSteps; ++h) qs[n][h][lane] = qf[n][h];
+    }
+    __syncthreads();
+  }
+  if (__builtin_expect(far, 0)) {
+    if (wave == 0) {
+#pragma unroll
+      for (int n = 0; n < NG; ++n)
+#pragma unroll
+        for (int h = 0; h < kSteps; ++h) {
+          f16x2 part[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) part[e] = split16(rest_of(q[n][h][2 * e]), rest_of(q[n][h][2 * e + 1]), keep);
+          rest[n][h][lane] = join8(part[0], part[1], part[2], part[3]);
+        }
+    }
+    __syncthreads();
   }
 
   f32x4 o[NG][kCh];
@@ -606,17 +656,41 @@ __global__ __launch_bounds__(NW *kWave, 2) void dense_kernel(AttnArgs a) {
     const float ks = ks_next, vs = vs_next;
     f32x4 s[NG][4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int n = 0; n < NG; ++n) s[n][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    auto keys = [&](int i, int h) {
+      const uint32_t w0 = flip_sign<I8>(kr[i][h / 2][2 * (h & 1)]), w1 = flip_sign<I8>(kr[i][h / 2][2 * (h & 1) + 1]);
+      return join8(pair16<I8, false>(w0), pair16<I8, true>(w0), pair16<I8, false>(w1), pair16<I8, true>(w1));
+    };
+    if (__builtin_expect(far, 0)) {
 #pragma unroll
-      for (int h = 0; h < kSteps; ++h) {
-        const uint32_t w0 = flip_sign<I8>(kr[i][h / 2][2 * (h & 1)]), w1 = flip_sign<I8>(kr[i][h / 2][2 * (h & 1) + 1]);
-        const f16x8 k = join8(pair16<I8, false>(w0), pair16<I8, true>(w0), pair16<I8, false>(w1), pair16<I8, true>(w1));
+      for (int i = 0; i < 4; ++i) {
 #pragma unroll
-        for (int n = 0; n < NG; ++n) s[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qf[n][h], s[n][i], 0, 0, 0);
+        for (int h = 0; h < kSteps; ++h) {
+          const f16x8 k = keys(i, h);
+#pragma unroll
+          for (int n = 0; n < NG; ++n) s[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, rest[n][h][lane], s[n][i], 0, 0, 0);
+        }
+#pragma unroll
+        for (int n = 0; n < NG; ++n) s[n][i] *= 0x1p-38f;
       }
     }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)  // the operands are made anew: kept, they would take 64 registers
+#pragma unroll
+      for (int h = 0; h < kHalves; ++h) asm volatile("" : "+v"(kr[i][h]));
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int h = 0; h < kSteps; ++h) {
+        const f16x8 k = keys(i, h);
+#pragma unroll
+        for (int n = 0; n < NG; ++n) {
+          const f16x8 query = kQueryLds ? qs[n][h][lane] : qf[n][h];
+          s[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, query, s[n][i], 0, 0, 0);
+        }
+      }
     load_k(b + NW);
     if (b + NW < last) {
       ks_next = ksp[b + NW];

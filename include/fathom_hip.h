@@ -397,7 +397,10 @@ int fathom_rows8_read(const void *k8, const void *v8, const float *k_scale, cons
  * without the cap for softcap = 0 (else positive and finite) and without the bias
  * for slopes = NULL.  q [BH, G, D] of q_dtype (FATHOM_DT_F32/F16/BF16, 16-byte
  * aligned), out [BH, G, D] float32.  A row without tokens gives zeros; what lies
- * behind a row's length is not used.
+ * behind a row's length is not used.  Products, scores and sums are float32.  Of
+ * q's channels 19 bits and more take part down to 2^-56 of their head's largest,
+ * and none below 2^-76; of a weight 22 bits, down to 2^-38 of the largest weight
+ * times scale of V.
  * workspace (16-byte aligned): fathom_rows8_attention_workspace_bytes(BH, G, D,
  * positions) bytes, positions = the smaller of the longest length the host knows
  * (n, or cap where lens is given) and, if not 0, the window.  The query never falls

@@ -122,3 +122,24 @@ def test_values_and_weights_over_many_decades(code, falls):
         q[0, :, 0] = 1.0
         st, Kv, Vv = _rows(K, V, code)
         _check(st, Kv, Vv, q, [n], n, scale=1.0)
+
+
+# ----------------------------------------------------------------------------- queries
+@pytest.mark.parametrize("code", ["e4m3", "int8"])
+@pytest.mark.parametrize("D, G", [(64, 3), (128, 3), (64, 12), (128, 12)])
+@pytest.mark.parametrize("power", [12, 20, 30, 45])
+def test_queries_with_a_large_channel(code, D, G, power):
+    """A query channel far above the others whose keys are zero: the scores come from the others."""
+    for n in (100, 1500):
+        rng = np.random.default_rng(power)
+        K, V = rng.standard_normal((1, n, D)), rng.standard_normal((1, n, D))
+        K[..., [5, 40]] = 0.0
+        st, Kv, Vv = _rows(K, V, code)
+        q = _q(1, G, D, power) * 2.0
+        q[..., 5] = 2.0 ** power
+        q[0, 1, 40] = -(2.0 ** power)
+        _check(st, Kv, Vv, q, [n], n)
+        _check(st, Kv, Vv, q, [n], n, softcap=20.0, slopes=torch.full((1, G), 0.01))
+        _check(st, Kv, Vv, q, [n], n, idx=torch.arange(n).expand(1, G, n))
+    q[0, 0] = 0.0
+    _check(st, Kv, Vv, q, [n], n)

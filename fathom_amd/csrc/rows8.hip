@@ -249,9 +249,9 @@ extern "C" int fathom_rows8_write(const void *K, const void *V, int dtype, int64
   if (rc) return rc;
   if (dtype < FATHOM_DT_F32 || dtype > FATHOM_DT_BF16) return fail(FATHOM_ERR_INVALID, "rows8_write: dtype %d", dtype);
   if (T < 0 || T > cap) return fail(FATHOM_ERR_INVALID, "rows8_write: T=%lld outside [0, cap=%lld]", (long long)T, (long long)cap);
-  if (!pos && (pos_value < 0 || pos_value + T > cap))
-    return fail(FATHOM_ERR_INVALID, "rows8_write: tokens [%lld, %lld) outside [0, cap=%lld)", (long long)pos_value,
-                (long long)(pos_value + T), (long long)cap);
+  if (!pos && (pos_value < 0 || pos_value > cap - T))  // in this form, as a sum could wrap
+    return fail(FATHOM_ERR_INVALID, "rows8_write: %lld tokens from %lld outside [0, cap=%lld)", (long long)T,
+                (long long)pos_value, (long long)cap);
   if (T == 0) return FATHOM_OK;
   if (!K || !V) return fail(FATHOM_ERR_INVALID, "rows8_write: null pointer");
   const int64_t size = dtype == FATHOM_DT_F32 ? 4 : 2;

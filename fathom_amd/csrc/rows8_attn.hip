@@ -1162,7 +1162,7 @@ extern "C" int fathom_rows8_gather_attention(const void *q, int q_dtype, const i
   int rc = check_store("rows8_gather_attention", k8, v8, k_scale, v_scale, code_dtype, BH, cap, D);
   if (!rc) rc = check_query("rows8_gather_attention", q, q_dtype, G, cap, lens, n, softcap, out);
   if (rc) return rc;
-  if (k < 0 || G * k > 0x7FFFFFFF) return fail(FATHOM_ERR_INVALID, "rows8_gather_attention: G=%lld k=%lld", (long long)G, (long long)k);
+  if (k < 0 || k > 0x7FFFFFFF / G) return fail(FATHOM_ERR_INVALID, "rows8_gather_attention: G=%lld k=%lld", (long long)G, (long long)k);
   if (k > 0 && !idx) return fail(FATHOM_ERR_INVALID, "rows8_gather_attention: null index pointer");
   AttnArgs a{q, q_dtype, (const uint8_t *)k8, (const uint8_t *)v8, k_scale, v_scale, G, cap, cdiv(cap, kBlk), lens, n, 0,
              idx, k, scale, softcap, slopes, out, nullptr, nullptr, nullptr, 1, BH, 1};

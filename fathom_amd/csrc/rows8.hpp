@@ -92,6 +92,9 @@ __device__ __forceinline__ int64_t row_length(const int32_t *lens, int64_t n, in
   return v < 0 ? 0 : v < cap ? v : cap;
 }
 
+constexpr int64_t kMaxRows = 65535;           // of BH, and of heads G
+constexpr int64_t kMaxCap = 0x7FFFFFFF - 64;  // tokens of a row
+
 // Host checks common to the entry points: the store's shape, formats and alignment.
 inline int check_store(const char *what, const void *k8, const void *v8, const float *ks, const float *vs, int code_dtype,
                        int64_t BH, int64_t cap, int64_t D) {
@@ -99,8 +102,8 @@ inline int check_store(const char *what, const void *k8, const void *v8, const f
   if (code_dtype != FATHOM_DT_E4M3 && code_dtype != FATHOM_DT_I8)
     return fail(FATHOM_ERR_INVALID, "%s: code_dtype %d is neither e4m3 nor int8", what, code_dtype);
   if (D != 64 && D != 128) return fail(FATHOM_ERR_INVALID, "%s: D=%lld, the store holds rows of 64 or 128", what, (long long)D);
-  if (BH < 1 || BH > 65535) return fail(FATHOM_ERR_INVALID, "%s: BH=%lld outside [1, 65535]", what, (long long)BH);
-  if (cap < 1 || cap > 0x7FFFFFFF - 64) return fail(FATHOM_ERR_INVALID, "%s: cap=%lld", what, (long long)cap);
+  if (BH < 1 || BH > kMaxRows) return fail(FATHOM_ERR_INVALID, "%s: BH=%lld outside [1, 65535]", what, (long long)BH);
+  if (cap < 1 || cap > kMaxCap) return fail(FATHOM_ERR_INVALID, "%s: cap=%lld", what, (long long)cap);
   if ((reinterpret_cast<uintptr_t>(k8) | reinterpret_cast<uintptr_t>(v8)) & 15)
     return fail(FATHOM_ERR_INVALID, "%s: the codes must be 16-byte aligned", what);
   if ((reinterpret_cast<uintptr_t>(ks) | reinterpret_cast<uintptr_t>(vs)) & 3)

@@ -1092,11 +1092,16 @@ int check_query(const char *what, const void *q, int q_dtype, int64_t G, int64_t
                 float softcap, const float *out) {
   if (!q || !out) return fail(FATHOM_ERR_INVALID, "%s: null pointer", what);
   if (q_dtype < FATHOM_DT_F32 || q_dtype > FATHOM_DT_BF16) return fail(FATHOM_ERR_INVALID, "%s: q_dtype %d", what, q_dtype);
-  if (G < 1 || G > 65535) return fail(FATHOM_ERR_INVALID, "%s: G=%lld", what, (long long)G);
+  if (G < 1 || G > kMaxRows) return fail(FATHOM_ERR_INVALID, "%s: G=%lld", what, (long long)G);
   if (!lens && (n < 0 || n > cap)) return fail(FATHOM_ERR_INVALID, "%s: length %lld outside [0, cap=%lld]", what, (long long)n, (long long)cap);
   if (!(softcap >= 0.0f && softcap < INFINITY)) return fail(FATHOM_ERR_INVALID, "%s: softcap must be 0 (none) or positive and finite", what);
   if (reinterpret_cast<uintptr_t>(q) & 15) return fail(FATHOM_ERR_INVALID, "%s: q must be 16-byte aligned", what);
   return FATHOM_OK;
+}
+
+// Whether the calls take this shape: the queries answer 0 for others, as their products could wrap.
+bool shape_taken(int64_t BH, int64_t G, int64_t D) {
+  return BH >= 1 && BH <= kMaxRows && G >= 1 && G <= kMaxRows && (D == 64 || D == 128);
 }
 
 // An upper bound of a row's positions that the host knows.
@@ -1113,7 +1118,8 @@ using namespace fathom;
 using namespace fathom::rows8;
 
 extern "C" size_t fathom_rows8_attention_workspace_bytes(int64_t BH, int64_t G, int64_t D, int64_t positions) {
-  if (BH < 1 || G < 1 || D < 1 || positions < 1) return 0;
+  if (!shape_taken(BH, G, D) || positions < 1) return 0;
+  if (positions > kMaxCap) positions = kMaxCap;
   const int64_t nb = cdiv(positions, (int64_t)kBlk) + 1;  // a window may begin inside a block
   const int64_t one = dense_slots(BH, G, nb, false), own = dense_slots(BH, G, nb, true), slots = one > own ? one : own;
   return part_bytes(BH, G, D, slots);
@@ -1146,8 +1152,8 @@ extern "C" int fathom_rows8_attention(const void *q, int q_dtype, const void *k8
 }
 
 extern "C" size_t fathom_rows8_gather_attention_workspace_bytes(int64_t BH, int64_t G, int64_t D, int64_t k) {
-  if (BH < 1 || G < 1 || D < 1 || k < 1) return 0;
-  if (k <= 16 * kTile) return 0;
+  if (!shape_taken(BH, G, D) || k <= 16 * kTile) return 0;
+  if (k > 0x7FFFFFFF / G) k = 0x7FFFFFFF / G;
   // of the narrower workgroups, so that it never falls as k grows
   int64_t ns = cdiv(k, (int64_t)4 * kTile);
   if (ns > list_room(BH * G, 4)) ns = list_room(BH * G, 4);

@@ -404,7 +404,8 @@ int fathom_rows8_read(const void *k8, const void *v8, const float *k_scale, cons
  * workspace (16-byte aligned): fathom_rows8_attention_workspace_bytes(BH, G, D,
  * positions) bytes, positions = the smaller of the longest length the host knows
  * (n, or cap where lens is given) and, if not 0, the window.  The query never falls
- * as positions grow.  0 bytes: workspace may be NULL.
+ * as positions grow; it is 0 for shapes that the call refuses.  0 bytes: workspace
+ * may be NULL.
  */
 size_t fathom_rows8_attention_workspace_bytes(int64_t BH, int64_t G, int64_t D, int64_t positions);
 int fathom_rows8_attention(const void *q, int q_dtype, const void *k8, const void *v8, const float *k_scale,

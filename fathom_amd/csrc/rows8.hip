@@ -276,6 +276,8 @@ extern "C" int fathom_rows8_read(const void *k8, const void *v8, const float *k_
   if (!K || !V) return fail(FATHOM_ERR_INVALID, "rows8_read: null pointer");
   if ((reinterpret_cast<uintptr_t>(K) | reinterpret_cast<uintptr_t>(V)) & 15)
     return fail(FATHOM_ERR_INVALID, "rows8_read: the outputs must be 16-byte aligned");
+  // wholly outside the store from there on: the kernel's sums do not wrap
+  pos_value = pos_value > cap ? cap : pos_value < -R ? -R : pos_value;
   const ReadArgs a{{(const uint8_t *)k8, (const uint8_t *)v8}, {k_scale, v_scale}, {K, V}, pos, idx, pos_value, R, cap,
                    cdiv(cap, kBlk)};
   const int dt = dtype;

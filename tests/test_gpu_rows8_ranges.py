@@ -143,3 +143,19 @@ def test_queries_with_a_large_channel(code, D, G, power):
         _check(st, Kv, Vv, q, [n], n, idx=torch.arange(n).expand(1, G, n))
     q[0, 0] = 0.0
     _check(st, Kv, Vv, q, [n], n)
+
+
+# ----------------------------------------------------------------------------- arguments
+def test_read_far_behind_the_store():
+    """Places at the ends of 64 bits are outside the store: zero rows, from the C call too."""
+    st, _, _ = _filled(2, 100, 64, "int8", [100, 100])
+    K, V = torch.ones(2, 2, 7, 64, device=DEV)
+    for at in (2 ** 63 - 1, 2 ** 63 - 4, -(2 ** 63), -(2 ** 63) + 5, 100, -7):
+        K.fill_(1.0)
+        V.fill_(1.0)
+        _lib.call("fathom_rows8_read", st.k8.data_ptr(), st.v8.data_ptr(), st.k_scale.data_ptr(), st.v_scale.data_ptr(),
+                  _lib.DT_I8, 2, 100, 64, None, None, at, 7, _lib.DT_F32, K.data_ptr(), V.data_ptr(),
+                  torch.cuda.current_stream().cuda_stream)
+        assert not K.any() and not V.any(), at
+    full = st.read(0, 100, torch.float32)[0]
+    assert torch.equal(st.read(-3, 7, torch.float32)[0][:, 3:], full[:, :4])

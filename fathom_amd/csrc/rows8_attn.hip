@@ -897,14 +897,13 @@ __global__ __launch_bounds__(kMergeThreads) void merge_kernel(AttnArgs a) {
   constexpr int kOwn = kMaxSplits / kMergeThreads;  // splits whose factor a thread computes
   __shared__ float fac[kMaxSplits], red[2][kMergeThreads / kWave];
   __shared__ float4 acc[kGroups][kLanes];
-  const int64_t r = blockIdx.x;
+  const int64_t bh = blockIdx.y, r = bh * a.G + blockIdx.x;
   const int tid = threadIdx.x, lane = tid % kLanes, grp = tid / kLanes;
-  const int64_t bh = r / a.G;
   const int2 w = a.where ? a.where[bh] : make_int2((int)(bh * a.nsplit), (int)a.nsplit);
   const int ns = w.y;
   if (ns <= 1) return;  // written already
-  const int64_t at = (int64_t)w.x * a.G + r % a.G;  // split s at + s G
-  const float4 *p = reinterpret_cast<const float4 *>(a.part + at * D + 32 * blockIdx.y) + lane;
+  const int64_t at = (int64_t)w.x * a.G + blockIdx.x;  // split s at + s G
+  const float4 *p = reinterpret_cast<const float4 *>(a.part + at * D + 32 * blockIdx.z) + lane;
   const int64_t step = a.G * (D / 4);
   float4 v[kBatch];
 #pragma unroll
@@ -965,7 +964,7 @@ __global__ __launch_bounds__(kMergeThreads) void merge_kernel(AttnArgs a) {
     l = 0.0f;
 #pragma unroll
     for (int k = 0; k < kMergeThreads / kWave; ++k) l += red[1][k];
-    a.out[r * D + 32 * blockIdx.y + tid] = l == 0.0f ? 0.0f : u / l;
+    a.out[r * D + 32 * blockIdx.z + tid] = l == 0.0f ? 0.0f : u / l;
   }
 }
 
@@ -1043,8 +1042,9 @@ void place(AttnArgs &a, void *workspace, int64_t D, int64_t slots, bool lens) {
 }
 
 int merge(const AttnArgs &a, int64_t BH, int64_t D, hipStream_t st) {
-  if (D == 128) merge_kernel<128><<<dim3((unsigned)(BH * a.G), 4), kMergeThreads, 0, st>>>(a);
-  else merge_kernel<64><<<dim3((unsigned)(BH * a.G), 2), kMergeThreads, 0, st>>>(a);
+  const dim3 grid((unsigned)a.G, (unsigned)BH, (unsigned)D / 32);  // an axis of BH G workgroups could pass 2^32 threads
+  if (D == 128) merge_kernel<128><<<grid, kMergeThreads, 0, st>>>(a);
+  else merge_kernel<64><<<grid, kMergeThreads, 0, st>>>(a);
   return launch_status("rows8 merge_kernel");
 }
 

@@ -159,3 +159,24 @@ def test_read_far_behind_the_store():
         assert not K.any() and not V.any(), at
     full = st.read(0, 100, torch.float32)[0]
     assert torch.equal(st.read(-3, 7, torch.float32)[0][:, 3:], full[:, :4])
+
+
+def test_more_heads_than_one_axis_of_a_grid_takes():
+    """BH G past 2^24, at lengths of their own: splits and their join."""
+    BH, G, D, cap = 65535, 257, 64, 1100
+    st = RowStore8.empty(BH, cap, torch.int8, D, DEV)
+    st.v8[:, :3] = (torch.arange(3 * D, device=DEV) - 96).to(torch.int8).view(3, D)
+    st.v_scale.fill_(0.5)
+    rows = [0, 1, 300, 40000, BH - 1]
+    lens = torch.zeros(BH, dtype=torch.int32, device=DEV)
+    for i, b in enumerate(rows):
+        lens[b] = i % 3 + 1
+    lens[300] = cap
+    q = torch.zeros(BH, G, D, dtype=torch.float16, device=DEV)  # every score 0: means of V
+    got = st.attention(q, lens)
+    for b in rows:
+        n = int(lens[b])
+        want = st.v8[b, :n].double().mul(0.5).mean(0)
+        assert (got[b].double() - want).abs().max() <= 2.0 ** -20 * want.abs().max(), b
+    got[rows] = 0
+    assert not got.any()

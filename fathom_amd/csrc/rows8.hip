@@ -25,6 +25,7 @@ typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kThreads = 256;
 constexpr int kReadPieces = 4;
+constexpr int64_t kMaxWrite = (1 << 30) - 128;  // tokens of a write: its grid stays below 2^32 threads
 
 struct WriteArgs {
   const void *x[2];
@@ -249,6 +250,7 @@ extern "C" int fathom_rows8_write(const void *K, const void *V, int dtype, int64
   if (rc) return rc;
   if (dtype < FATHOM_DT_F32 || dtype > FATHOM_DT_BF16) return fail(FATHOM_ERR_INVALID, "rows8_write: dtype %d", dtype);
   if (T < 0 || T > cap) return fail(FATHOM_ERR_INVALID, "rows8_write: T=%lld outside [0, cap=%lld]", (long long)T, (long long)cap);
+  if (T > kMaxWrite) return fail(FATHOM_ERR_INVALID, "rows8_write: T=%lld, at most %lld at a time", (long long)T, (long long)kMaxWrite);
   if (!pos && (pos_value < 0 || pos_value > cap - T))  // in this form, as a sum could wrap
     return fail(FATHOM_ERR_INVALID, "rows8_write: %lld tokens from %lld outside [0, cap=%lld)", (long long)T,
                 (long long)pos_value, (long long)cap);

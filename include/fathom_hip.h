@@ -371,7 +371,8 @@ int fathom_gather_attention(const float *q, const int64_t *idx, int64_t BH, int6
  * Codes are the nearest to x * (1 / scale), ties to even; infinities saturate;
  * NaN is stored as NaN in e4m3 and as 0 in int8.  Tokens behind p + T keep their
  * codes, though not the values of those in the last written block.  A row of
- * `pos` whose tokens do not all fit into [0, cap) is left as it is.
+ * `pos` whose tokens do not all fit into [0, cap) is left as it is.  At most
+ * 2^30 - 128 tokens at a time.
  */
 int fathom_rows8_write(const void *K, const void *V, int dtype, int64_t k_row_stride, int64_t k_tok_stride,
                        int64_t v_row_stride, int64_t v_tok_stride, const int32_t *pos, int64_t pos_value, int64_t BH,

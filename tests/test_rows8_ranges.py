@@ -48,3 +48,10 @@ def test_workspace_queries_do_not_divide_by_zero():
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     run = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
     assert run.returncode == 0 and run.stdout.strip() == "[0, 0]", (run.returncode, run.stderr[-500:])
+
+
+@pytest.mark.parametrize("T", [2 ** 30 - 127, 2 ** 30, 2 ** 31 - 65])
+def test_writes_longer_than_a_grid_are_refused(T):
+    L = _lib.lib()
+    assert L.fathom_rows8_write(*_write_args(T=T, cap=2 ** 31 - 65)) == _lib.ERR_INVALID
+    assert f"T={T}".encode() in L.fathom_last_error()

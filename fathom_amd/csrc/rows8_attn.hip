@@ -221,6 +221,7 @@ __global__ __launch_bounds__(NW *kWave) void list_kernel(AttnArgs a) {
       x[i] = sum_row<kLanes>(dot);
       y[i] = ldexpf(ks[i], ce);
       if (a.softcap > 0.0f) {
+        y[i] = y[i] == y[i] ? __builtin_amdgcn_fmed3f(y[i], -3.0e38f, 3.0e38f) : y[i];  // finite: a score of 0 has to stay one
         x[i] = tanh_any(x[i] * y[i]);
         y[i] = a.softcap * kLog2e;
       }
@@ -705,7 +706,8 @@ __global__ __launch_bounds__(NW *kWave, 2) void dense_kernel(AttnArgs a) {
     for (int n = 0; n < NG; ++n) {
       // z = s f; below kLarge not rounded itself, but relative to the maximum
       float f = ldexpf(fabsf(ks), ex[n]);
-      f = f == f ? fmaxf(f, 1.2e-38f) : f;  // never 0: a score of -inf has to stay one
+      // never infinite: a score of 0 has to stay one; nor 0 without a cap: a score of -inf has to stay one too
+      f = f == f ? __builtin_amdgcn_fmed3f(f, EXTRA && a.softcap > 0.0f ? 0.0f : 1.2e-38f, 3.0e38f) : f;
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -1104,6 +1106,12 @@ bool shape_taken(int64_t BH, int64_t G, int64_t D) {
   return BH >= 1 && BH <= kMaxRows && G >= 1 && G <= kMaxRows && (D == 64 || D == 128);
 }
 
+// The cap as the kernels take it, in a range where scale / softcap and its products stay normal: below
+// 2^-64 every weight is 1 either way, and above 2^90 (0: none) scores below 2^78 do not notice a cap.
+float kernel_cap(float softcap) {
+  return softcap > 0x1p90f ? 0.0f : softcap > 0.0f && softcap < 0x1p-64f ? 0x1p-64f : softcap;
+}
+
 // An upper bound of a row's positions that the host knows.
 int64_t dense_positions(const int32_t *lens, int64_t n, int64_t cap, int64_t window) {
   const int64_t most = lens ? cap : n;
@@ -1135,7 +1143,7 @@ extern "C" int fathom_rows8_attention(const void *q, int q_dtype, const void *k8
   if (rc) return rc;
   if (window < 0) return fail(FATHOM_ERR_INVALID, "rows8_attention: window %lld", (long long)window);
   AttnArgs a{q, q_dtype, (const uint8_t *)k8, (const uint8_t *)v8, k_scale, v_scale, G, cap, cdiv(cap, kBlk), lens, n, window,
-             nullptr, 0, scale, softcap, slopes, out, nullptr, nullptr, nullptr, 1, BH, 1};
+             nullptr, 0, scale, kernel_cap(softcap), slopes, out, nullptr, nullptr, nullptr, 1, BH, 1};
   const int64_t most = dense_positions(lens, n, cap, window);
   const int64_t nb = lens ? cdiv(most, (int64_t)kBlk) + (window > 0) : cdiv(n, (int64_t)kBlk) - (n - most) / kBlk;
   const int64_t slots = dense_slots(BH, G, nb, lens != nullptr);
@@ -1171,7 +1179,7 @@ extern "C" int fathom_rows8_gather_attention(const void *q, int q_dtype, const i
   if (k < 0 || k > 0x7FFFFFFF / G) return fail(FATHOM_ERR_INVALID, "rows8_gather_attention: G=%lld k=%lld", (long long)G, (long long)k);
   if (k > 0 && !idx) return fail(FATHOM_ERR_INVALID, "rows8_gather_attention: null index pointer");
   AttnArgs a{q, q_dtype, (const uint8_t *)k8, (const uint8_t *)v8, k_scale, v_scale, G, cap, cdiv(cap, kBlk), lens, n, 0,
-             idx, k, scale, softcap, slopes, out, nullptr, nullptr, nullptr, 1, BH, 1};
+             idx, k, scale, kernel_cap(softcap), slopes, out, nullptr, nullptr, nullptr, 1, BH, 1};
   a.nsplit = list_splits(BH * G, k);
   const int64_t slots = a.nsplit > 1 ? BH * a.nsplit : 0;
   const size_t need = part_bytes(BH, G, D, slots);

@@ -135,6 +135,8 @@ class RowStore8:
         softcap = 0.0 if softcap is None else float(softcap)
         if not 0.0 <= softcap < math.inf:
             raise ValueError(f"softcap {softcap} must be positive and finite (None or 0: no cap)")
+        if softcap:  # float32 would make 0 or infinity of others
+            softcap = min(max(softcap, 1e-30), 1e30)
         if slopes is not None:
             if slopes.device != self.device:
                 self._elsewhere(slopes)

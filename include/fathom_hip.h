@@ -395,8 +395,8 @@ int fathom_rows8_read(const void *k8, const void *v8, const float *k_scale, cons
  * [max(0, len - window), len) (window 0: all),
  *   z_t = softcap * tanh(u_t / softcap) + slopes[bh, g] * (t - (len - 1)),
  *   u_t = scale * q[bh, g] . K_t;   out[bh, g] = softmax(z) . V
- * without the cap for softcap = 0 (else positive and finite) and without the bias
- * for slopes = NULL.  q [BH, G, D] of q_dtype (FATHOM_DT_F32/F16/BF16, 16-byte
+ * without the cap for softcap = 0 (else positive and finite; below 2^-64 it counts
+ * as that, above 2^90 as none) and without the bias for slopes = NULL.  q [BH, G, D] of q_dtype (FATHOM_DT_F32/F16/BF16, 16-byte
  * aligned), out [BH, G, D] float32.  A row without tokens gives zeros; what lies
  * behind a row's length is not used.  Products, scores and sums are float32.  Of
  * q's channels 19 bits and more take part down to 2^-56 of their head's largest,

@@ -180,3 +180,26 @@ def test_more_heads_than_one_axis_of_a_grid_takes():
         assert (got[b].double() - want).abs().max() <= 2.0 ** -20 * want.abs().max(), b
     got[rows] = 0
     assert not got.any()
+
+
+# ----------------------------------------------------------------------------- caps
+@pytest.mark.parametrize("code", ["e4m3", "int8"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("size", [1e-10, 1.0, 1e10])
+def test_extreme_caps(code, D, size):
+    """A cap far below the scores leaves every token the same weight; one far above them changes nothing."""
+    for softcap in (1e-300, 1e-50, 1e-38, 1e-20, 1e-4, 1e10, 1e20, 1e26, 1e28, 1e32, 1e38, 1e200):
+        if size > 1.0 and softcap > 1e4:
+            size = 30.0  # scores of 1e10 differ by more than a float32 bound can say
+        n = 300
+        st, K, V = _filled(1, n, D, code, [n])
+        K = K.copy()
+        st.k_scale[0, 2], K[0, 128:192] = 0.0, 0.0
+        st.k8.view(torch.uint8)[0, 70], K[0, 70] = 0, 0.0
+        q = _q(1, 2, D, 4) * size
+        for idx in (None, torch.arange(n).expand(1, 2, n)):
+            with np.errstate(over="ignore"):
+                got = _check(st, K, V, q, [n], n, softcap=softcap, idx=idx)
+            if softcap <= 1e-4:  # scores within the cap: weights within e^(2 cap) of each other
+                err = np.abs(got[0].double().cpu().numpy() - V[0].mean(0))
+                assert (err <= (2.1 * softcap + (n / 8 + 64) * R.U + 2.0 ** -20) * np.abs(V[0]).mean(0)).all()

@@ -222,7 +222,7 @@ class RowStore8:
         as within [0, cap].  A row without tokens gives zeros."""
         q, q_at, scale, softcap, slopes = self._query(q, scale, softcap, slopes)
         lens, lens_at, n = self._per_row(length, "length")
-        G, window = q.shape[1], min(int(window), _FAR)
+        G, window = q.shape[1], max(min(int(window), _FAR), -1)  # the library refuses negative ones
         positions = n if lens is None else self.cap
         positions = max(min(positions, window) if window > 0 else positions, 0)
         ws, ws_at, nbytes = self._workspace("fathom_rows8_attention_workspace_bytes", G, positions)

@@ -146,6 +146,15 @@ def test_queries_with_a_large_channel(code, D, G, power):
 
 
 # ----------------------------------------------------------------------------- arguments
+def test_negative_windows_are_refused():
+    n, D = 300, 64
+    st, _, _ = _filled(1, n, D, "int8", [n])
+    q = _q(1, 2, D, 6).to(DEV)
+    for window in (-1, -(2 ** 63), -(2 ** 64), -(2 ** 64) + 5):  # the last two wrap to 0 and 5
+        with pytest.raises(ValueError):
+            st.attention(q, n, window=window)
+
+
 def test_read_far_behind_the_store():
     """Places at the ends of 64 bits are outside the store: zero rows, from the C call too."""
     st, _, _ = _filled(2, 100, 64, "int8", [100, 100])

@@ -24,6 +24,7 @@ __all__ = ["RowStore8"]
 
 _raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
 _F32, _I32, _I64 = torch.float32, torch.int32, torch.int64
+_SHORT = {_I32, torch.int16, torch.uint16, torch.int8, torch.uint8}
 _FAR = 1 << 62  # ctypes would wrap what is longer
 _SIZES = {}  # workspace bytes by query and shape
 _CODES = {torch.float8_e4m3fn: _lib.DT_E4M3, torch.int8: _lib.DT_I8}
@@ -114,8 +115,11 @@ class RowStore8:
         if v.shape != (self.BH,) or (dtype != _I32 and (dtype.is_floating_point or dtype.is_complex or dtype == torch.bool)):
             raise ValueError(f"{what} must be an int or integers [{self.BH}], got {dtype} {tuple(v.shape)}")
         if dtype != _I32 or not v.is_contiguous():
-            if dtype == _I64:  # places beyond int32 stay beyond every store
-                v = v.clamp(-(1 << 31), (1 << 31) - 1)
+            if dtype not in _SHORT:  # places beyond int32 stay beyond every store
+                if dtype == torch.uint64:
+                    v = v.view(_I64)
+                    v = v.masked_fill(v < 0, _FAR)
+                v = v.to(_I64).clamp(-(1 << 31), (1 << 31) - 1)
             v = v.to(_I32).contiguous()
         return v, v.data_ptr(), 0
 

@@ -155,6 +155,16 @@ def test_negative_windows_are_refused():
             st.attention(q, n, window=window)
 
 
+def test_lengths_of_every_integer_type():
+    n, D = 300, 64
+    st, K, V = _filled(3, n, D, "int8", [n] * 3)
+    q = _q(3, 2, D, 6)
+    for dtype, lens in ((torch.uint64, [5, 2 ** 63, 2 ** 32]), (torch.uint32, [5, 2 ** 32 - 1, 2 ** 31]),
+                        (torch.int64, [5, 2 ** 62, 2 ** 32]), (torch.uint16, [5, 65535, 300]), (torch.int16, [-1, 299, 0]),
+                        (torch.uint8, [5, 255, 100]), (torch.int8, [127, -128, 1])):
+        _check(st, K, V, q, lens, torch.tensor(lens, dtype=dtype, device=DEV))
+
+
 def test_read_far_behind_the_store():
     """Places at the ends of 64 bits are outside the store: zero rows, from the C call too."""
     st, _, _ = _filled(2, 100, 64, "int8", [100, 100])

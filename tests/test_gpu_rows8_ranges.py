@@ -222,3 +222,19 @@ def test_extreme_caps(code, D, size):
             if softcap <= 1e-4:  # scores within the cap: weights within e^(2 cap) of each other
                 err = np.abs(got[0].double().cpu().numpy() - V[0].mean(0))
                 assert (err <= (2.1 * softcap + (n / 8 + 64) * R.U + 2.0 ** -20) * np.abs(V[0]).mean(0)).all()
+
+
+# ----------------------------------------------------------------------------- cap and bias with many heads
+@pytest.mark.parametrize("code", ["e4m3", "int8"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("G", [9, 12, 16, 17, 25])
+def test_cap_and_bias_of_many_heads(code, D, G):
+    """More than eight heads, with slopes of their own: rows of one workgroup and split ones, of one length and of their
+    own, with and without a window."""
+    slopes = torch.exp2(-torch.linspace(2.0, 9.0, 2 * G)).view(2, G).flip(1)
+    q = _q(2, G, D, G) * torch.linspace(0.5, 4.0, G)[None, :, None]
+    for cap, lens, window in ((700, [650, 333], 0), (2500, [2490, 1300], 0), (2500, [2490, 70], 1500), (130, [100, 1], 0)):
+        st, K, V = _filled(2, cap, D, code, lens)
+        for softcap, bias in ((5.0, None), (None, slopes), (30.0, slopes)):
+            _check(st, K, V, q, lens, torch.tensor(lens, dtype=torch.int32, device=DEV), window, softcap, bias)
+            _check(st, K, V, q, [min(lens)] * 2, min(lens), window, softcap, bias)

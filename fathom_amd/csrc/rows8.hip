@@ -4,11 +4,12 @@
 // a = the largest finite |x| among the block's new tokens and kMax the format's
 // largest code,
 //   need = max(fl(a / kMax), 2^-100)
-//   s'   = need               if the block holds no earlier token, or s is no
-//                             positive finite number
-//        = s 2^j, the least j >= 0 with s 2^j >= need, otherwise
+//   s'   = need               if the block holds no earlier token, or s is 0 or
+//                             not finite
+//        = s 2^j, the least j >= 0 with |s| 2^j >= need, otherwise
 //   code = RN(fl(x fl(1 / s')))        of the new tokens
-//        = RN(code 2^-j)               of the block's earlier ones
+//        = RN(code 2^-j)               of the block's earlier ones (0 where s is 0, as their
+//                                      values are; as they are where it is not finite)
 // (fl: one float32 rounding; RN: nearest code, ties to even).  Scales grow by
 // powers of two because a block that grows token by token is rounded anew each
 // time: an e4m3 code then only changes its exponent (its value is rounded again
@@ -93,15 +94,21 @@ __global__ __launch_bounds__(kThreads) void write_kernel(WriteArgs a) {
   amax = fmaxf(fmaxf(wave_max[0], wave_max[1]), fmaxf(wave_max[2], wave_max[3]));
   const float need = fmaxf(amax / code_max<I8>(), kMinScale);
   const int earlier = (int)(p > t0 ? p - t0 : 0);  // tokens that the block holds already
-  float s = need;
-  int by = 0;
-  if (earlier && was > 0.0f && was < INFINITY) {
-    if (was < need) {
-      int e0, e1;
-      const float m0 = frexpf(was, &e0), m1 = frexpf(need, &e1);
-      by = e1 - e0 + (m1 > m0 ? 1 : 0);
+  const float size = fabsf(was);
+  float s = need, f = 1.0f;  // f: what the earlier codes are multiplied by
+  if (earlier && size < INFINITY) {
+    if (size == 0.0f) {
+      f = 0.0f;
+    } else {
+      int by = 0;
+      if (size < need) {
+        int e0, e1;
+        const float m0 = frexpf(size, &e0), m1 = frexpf(need, &e1);
+        by = e1 - e0 + (m1 > m0 ? 1 : 0);
+      }
+      s = ldexpf(was, by);
+      f = ldexpf(1.0f, -by);
     }
-    s = ldexpf(was, by);
   }
   const float inv = 1.0f / s;
   uint8_t *dst = a.codes[kv] + (bh * a.cap + t0) * D;
@@ -119,8 +126,7 @@ __global__ __launch_bounds__(kThreads) void write_kernel(WriteArgs a) {
     if constexpr (kElem == 8) __builtin_nontemporal_store(u32x2{w[0], w[1]}, reinterpret_cast<u32x2 *>(dst + r * D + 8 * piece));
     else __builtin_nontemporal_store(w[0], reinterpret_cast<uint32_t *>(dst + r * D + 4 * piece));
   }
-  if (by) {
-    const float f = ldexpf(1.0f, -by);
+  if (f != 1.0f) {
     for (int o = 4 * tid; o < earlier * D; o += 4 * kThreads) {
       uint32_t *c = reinterpret_cast<uint32_t *>(dst + o);
       float y[4];

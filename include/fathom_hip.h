@@ -365,9 +365,10 @@ int fathom_gather_attention(const float *q, const int64_t *idx, int64_t BH, int6
  * tokens [p, p + T) of the store, p = pos[bh] (int32, device) or pos_value where
  * pos is NULL.  A block whose first token is written gets the scale
  * max(largest finite |x| / 448 or 127, 2^-100); one that holds earlier tokens
- * keeps its scale, or takes the least power-of-two multiple of it that holds the
- * new tokens, and its earlier codes are rounded to that.  (An earlier scale that
- * is no positive finite number counts as none, and the earlier codes stay.)
+ * keeps its scale (and its sign), or takes the least power-of-two multiple of it
+ * that holds the new tokens, and its earlier codes are rounded to that.  (A
+ * scale of 0 counts as none and its earlier codes become 0, as their values are;
+ * one that is not finite counts as none and its codes stay.)
  * Codes are the nearest to x * (1 / scale), ties to even; infinities saturate;
  * NaN is stored as NaN in e4m3 and as 0 in int8.  Tokens behind p + T keep their
  * codes, though not the values of those in the last written block.  A row of

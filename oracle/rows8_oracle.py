@@ -71,10 +71,13 @@ def write_row(codes, scale, x, p, code):
             need = np.maximum((a.max() if a.size else np.float32(0)) / np.float32(qmax(code)), MIN_SCALE)
         was = scale[b]
         s = need
-        if p > b * BLK and was > 0 and np.isfinite(was):
-            s, j = grown(was, need)
-            if j:
-                old = decode(codes[b * BLK:p], code).astype(np.float32) * np.float32(2.0 ** -j)
+        if p > b * BLK and np.isfinite(was):
+            j = None  # earlier values are 0
+            if was:
+                s, j = grown(abs(was), need)
+                s = np.copysign(s, was)
+            if j != 0:
+                old = decode(codes[b * BLK:p], code).astype(np.float32) * np.float32(2.0 ** -j if j else 0.0)
                 codes[b * BLK:p] = encode(old, code)
         with np.errstate(over="ignore", invalid="ignore"):
             codes[lo:hi] = encode(new * (np.float32(1.0) / s), code)

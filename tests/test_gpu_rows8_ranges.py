@@ -7,7 +7,7 @@ import torch
 from fathom_amd import _lib
 from fathom_amd.rowstore8 import RowStore8
 from oracle import rows8_oracle as R
-from test_gpu_rows8 import BLK, DEV, _check, _close, _f32, _filled, _from_numpy, _q, _rand
+from test_gpu_rows8 import BLK, DEV, _check, _close, _f32, _filled, _from_numpy, _q, _rand, _same
 
 pytestmark = pytest.mark.gpu
 
@@ -238,3 +238,26 @@ def test_cap_and_bias_of_many_heads(code, D, G):
         for softcap, bias in ((5.0, None), (None, slopes), (30.0, slopes)):
             _check(st, K, V, q, lens, torch.tensor(lens, dtype=torch.int32, device=DEV), window, softcap, bias)
             _check(st, K, V, q, [min(lens)] * 2, min(lens), window, softcap, bias)
+
+
+# ----------------------------------------------------------------------------- writes
+@pytest.mark.parametrize("code", ["e4m3", "int8"])
+def test_write_into_blocks_of_signed_and_zero_scales(code):
+    """Stores from elsewhere: a block keeps its scale's sign, and values of a scale of 0 stay 0."""
+    D, n = 64, 40
+    rng = np.random.default_rng(3)
+    o = {x: rng.integers(0, 127, (4, 64, D), dtype=np.uint8) for x in ("k8", "v8")}
+    o["ks"] = np.array([[-0.02], [0.0], [-1e-4], [-0.0]], np.float32)
+    o["vs"] = np.array([[0.0], [-0.5], [0.01], [-3.0]], np.float32)
+    st = _from_numpy(o, code)
+    before = st.read(0, n, torch.float32)
+    K, V = _rand((4, 3, D), 8), _rand((4, 3, D), 9)
+    st.write(K.to(DEV), V.to(DEV), n)
+    R.write(o, _f32(K), _f32(V), n, code)
+    _same(st, o, code)
+    for got, was, new in zip(st.read(0, n + 3, torch.float32), before, (K, V)):
+        # half a step of a scale that grew, at most twice largest / 448 or 127 (e4m3: or of the value), or of the earlier one
+        new = new.to(DEV)
+        step = new.abs().amax((1, 2)) * (2.0 ** -4 if code == "e4m3" else 1.0 / 127) + was.abs().amax((1, 2)) * 2.0 ** -7
+        assert ((got[:, :n] - was).abs() <= step[:, None, None]).all()
+        assert ((got[:, n:] - new).abs() <= step[:, None, None]).all()

@@ -573,17 +573,16 @@ __global__ __launch_bounds__(NW *kWave, 2) void dense_kernel(AttnArgs a) {
   for (int n = 0; n < NG; ++n) {
     const int64_t g = g0 + 8 * n + (col & 7);
     float mx = 0.0f;
-    uint32_t mn = 0xFFFFFFFFu;  // the bits of the smallest |q| but 0, doubled, less 1
+    float mn = INFINITY;
 #pragma unroll
     for (int h = 0; h < kSteps; ++h)
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         mx = fmaxf(mx, fabsf(q[n][h][e]));
-        const uint32_t v = 2u * __float_as_uint(q[n][h][e]) - 1u;
-        mn = v < mn ? v : mn;
+        mn = fminf(mn, fabsf(q[n][h][e]));
       }
     mx = across_groups<true>(mx);
-    far |= mn < 2u * (__float_as_uint(mx) - (18u << 23));  // below mx 2^-18; wraps for mx < 2^-108, where all count as such
+    far |= mn < mx * 0x1p-18f || mx < 0x1p-100f;
     int sigma = 0;  // the largest |q| of the head in [2^13, 2^14)
     if (mx > 0.0f && mx < INFINITY) {
       frexpf(mx, &sigma);
@@ -606,6 +605,16 @@ __global__ __launch_bounds__(NW *kWave, 2) void dense_kernel(AttnArgs a) {
   }
 
   far = __any(far);  // uniform over the workgroup: its waves hold the same queries
+  if (far) {  // channels of 0 are no small ones
+    far = false;
+#pragma unroll
+    for (int n = 0; n < NG; ++n)
+#pragma unroll
+      for (int h = 0; h < kSteps; ++h)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) far |= small_channel(q[n][h][e]);
+    far = __any(far);
+  }
   // Two groups of eight heads keep them in LDS: in registers, D = 128 with cap and bias spills (8 x 65536 tokens, 12 heads
   // 47 us; 40).
   constexpr bool kQueryLds = NG > 1;
@@ -848,7 +857,7 @@ __global__ __launch_bounds__(NW *kWave, 2) void dense_kernel(AttnArgs a) {
 #pragma unroll
   for (int n = 0; n < NG; ++n) {
     const float L = across_groups<false>(l[n]);
-    const int up = (int)ceilf(R[n]) - 14;
+    const float up = ldexpf(1.0f, (int)ceilf(R[n]) - 14);
     if (lane < 8) {
       wm[wave][8 * n + lane] = m[n];
       wl[wave][8 * n + lane] = L;
@@ -858,10 +867,10 @@ __global__ __launch_bounds__(NW *kWave, 2) void dense_kernel(AttnArgs a) {
 #pragma unroll
       for (int e = 0; e < kCh; e += 4) {
         float4 v;
-        v.x = ldexpf(add_other_half(o[n][e][j]), up);
-        v.y = ldexpf(add_other_half(o[n][e + 1][j]), up);
-        v.z = ldexpf(add_other_half(o[n][e + 2][j]), up);
-        v.w = ldexpf(add_other_half(o[n][e + 3][j]), up);
+        v.x = add_other_half(o[n][e][j]) * up;
+        v.y = add_other_half(o[n][e + 1][j]) * up;
+        v.z = add_other_half(o[n][e + 2][j]) * up;
+        v.w = add_other_half(o[n][e + 3][j]) * up;
         if (col < 8) *reinterpret_cast<float4 *>(&wo[wave][8 * n + col][(4 * grp + j) * kCh + e]) = v;
       }
   }

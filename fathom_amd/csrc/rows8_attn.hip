@@ -221,7 +221,8 @@ __global__ __launch_bounds__(NW *kWave) void list_kernel(AttnArgs a) {
       x[i] = sum_row<kLanes>(dot);
       y[i] = ldexpf(ks[i], ce);
       if (a.softcap > 0.0f) {
-        y[i] = y[i] == y[i] ? __builtin_amdgcn_fmed3f(y[i], -3.0e38f, 3.0e38f) : y[i];  // finite: a score of 0 has to stay one
+        // finite for a finite scale: a score of 0 has to stay one
+        y[i] = fabsf(ks[i]) < INFINITY ? __builtin_amdgcn_fmed3f(y[i], -3.0e38f, 3.0e38f) : y[i];
         x[i] = tanh_any(x[i] * y[i]);
         y[i] = a.softcap * kLog2e;
       }
@@ -716,7 +717,8 @@ __global__ __launch_bounds__(NW *kWave, 2) void dense_kernel(AttnArgs a) {
       // z = s f; below kLarge not rounded itself, but relative to the maximum
       float f = ldexpf(fabsf(ks), ex[n]);
       // never infinite: a score of 0 has to stay one; nor 0 without a cap: a score of -inf has to stay one too
-      f = f == f ? __builtin_amdgcn_fmed3f(f, EXTRA && a.softcap > 0.0f ? 0.0f : 1.2e-38f, 3.0e38f) : f;
+      // (an infinite or NaN scale stays what it is)
+      f = fabsf(ks) < INFINITY ? __builtin_amdgcn_fmed3f(f, EXTRA && a.softcap > 0.0f ? 0.0f : 1.2e-38f, 3.0e38f) : f;
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll

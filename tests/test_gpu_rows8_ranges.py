@@ -261,3 +261,25 @@ def test_write_into_blocks_of_signed_and_zero_scales(code):
         step = new.abs().amax((1, 2)) * (2.0 ** -4 if code == "e4m3" else 1.0 / 127) + was.abs().amax((1, 2)) * 2.0 ** -7
         assert ((got[:, :n] - was).abs() <= step[:, None, None]).all()
         assert ((got[:, n:] - new).abs() <= step[:, None, None]).all()
+
+
+@pytest.mark.parametrize("code", ["e4m3", "int8"])
+@pytest.mark.parametrize("bad", [float("inf"), -float("inf"), float("nan")])
+def test_scales_that_are_not_finite(code, bad):
+    """A block of such a scale of K makes NaN of the heads of its row, of V the channels' values (NaN for a code of 0 or beside
+    other signs); rows that do not hold it are as before, and so is a call that ends before it."""
+    st, K, V = _filled(3, 300, 64, code, [300] * 3)
+    q = _q(3, 2, 64, 3)
+    st.k_scale[0, 2] = bad
+    st.v_scale[1, 2] = bad
+    for softcap in (None, 5.0):
+        for idx in (None, torch.arange(300).expand(3, 2, 300)):
+            got = (st.attention(q.to(DEV), 300, softcap=softcap) if idx is None
+                   else st.gather_attention(q.to(DEV), idx.to(DEV), 300, softcap=softcap))
+            assert not got[1].isfinite().any()
+            if softcap is None or bad != bad:
+                assert got[0].isnan().all()
+            want = [R.attention(q[2, g].double().numpy(), K[2], V[2], np.arange(300), 300, 64 ** -0.5, softcap or 0.0) for g in (0, 1)]
+            for g in (0, 1):
+                _close(got, 2, g, *want[g])
+    _check(st, K, V, q, [128] * 3, 128)

@@ -42,8 +42,9 @@ struct WriteArgs {
 // the registers.  Rows and codes pass the caches as streams (nontemporal): nothing
 // here reads them again.
 //
-// Bound: HBM.  8 x 131072 bf16 rows (805 MB in and out): 130 us, 6.2 TB/s (143 us without
-// the streams).
+// Bound: HBM.  8 x 131072 bf16 rows (805 MB in and out): 131 us back to back, 6.1 TB/s (143 us without
+// the streams); a launch by itself 142, the median of twelve.  float32 rows of D = 128 take 230
+// registers, which leaves two waves per SIMD: 8 x 65536 (671 MB) 253 us, 2.7 TB/s.
 template <int D, int DT, bool I8>
 __global__ __launch_bounds__(kThreads) void write_kernel(WriteArgs a) {
   constexpr int kElem = DT == FATHOM_DT_F32 ? 4 : 8;  // elements of a thread's 16-byte piece
@@ -153,7 +154,8 @@ struct ReadArgs {
 // their codes requested first.
 //
 // Bound: HBM (D codes in, 2 D or 4 D bytes out per token).  8 x 131072 rows to bf16: 132 us,
-// 6.1 TB/s, stores as streams (137 us without; one piece of four values per thread: 241 us).
+// 6.1 TB/s, stores as streams (137 us without; one piece of four values per thread: 241 us).  8 x 16384 listed
+// rows of 262144 tokens (104 MB): 17 us, 6.0 TB/s.
 template <int D, int DT, bool I8>
 __global__ __launch_bounds__(kThreads) void read_kernel(ReadArgs a) {
   constexpr int kElem = DT == FATHOM_DT_F32 ? 4 : 8;  // values of a piece

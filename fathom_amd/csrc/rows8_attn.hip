@@ -148,7 +148,7 @@ __device__ const u32x4 kNoRow[8] = {};  // the row of a token that takes no part
 // LDS.
 //
 // Bound: latency (index, then row, then the joins).  32 x 4 heads of 512 positions (17.6 MB of rows):
-// 7.2 us, of 8 x 7 of 2048 (30.5 MB) 9.9 and the join's 4.0.  With shuffles for the joins and
+// 7.3 us, of 8 x 7 of 2048 (30.5 MB) 10.0 and the join's 3.8.  With shuffles for the joins and
 // four waves per workgroup throughout: 11.5 with its join, and 14.5.
 template <int D, bool I8, int NW>
 __global__ __launch_bounds__(NW *kWave) void list_kernel(AttnArgs a) {
@@ -498,10 +498,11 @@ __device__ __forceinline__ Part find_part_wide(const AttnArgs &a, uint32_t w, Fi
 // Rows are read through buffer descriptors that end at the row's length: what lies
 // behind it reads as zeros.
 //
-// Bound: HBM, 2 D bytes per token.  The next block's K rows are requested once the
-// scores are formed, its V rows once the products are, so that a wave has 8 to 16 KB on the way all the
-// time.  A block takes 342 VALU instructions and 32 matrix ones (D = 128, NG = 1), a third of the
-// time that its rows take.  8 x 1048576 tokens of 4 heads (2.15 GB) 303 us, 7.1 TB/s; 32 x
+// Bound: HBM, 2 D bytes per token and group of 16 heads: more heads read the rows once for each (8 x 65536
+// tokens of 32 heads 46 to 53 us, 1.4 times the rows' bytes from HBM; of 12 heads 34, with cap and bias 39).
+// The next block's K rows are requested once the scores are formed, its V rows once the products are, so that a
+// wave has 8 to 16 KB on the way all the time.  A block takes 364 VALU instructions and 32 matrix ones (D = 128,
+// NG = 1), a third of the time that its rows take.  8 x 1048576 tokens of 4 heads (2.15 GB) 304 us, 7.1 TB/s; 32 x
 // 32768 (0.27 GB) 46 us with the join of the splits; one dot product per lane group and no matrix
 // cores: 917 and 127 us.  Short rows are bound by latency: the launch, the rows' way from HBM, one block's arithmetic.
 template <int D, bool I8, int NG, bool EXTRA, int NW>
@@ -793,7 +794,7 @@ __global__ __launch_bounds__(NW *kWave, 2) void dense_kernel(AttnArgs a) {
         l[n] *= down;
         by = ldexpf(down, (int)ceilf(was) - (int)ceilf(R[n]));
       }
-      if (__any(by != 1.0f)) {  // apart from the branch above, which would take more registers (8 x 65536, 12 heads: 45 us for 35)
+      if (__any(by != 1.0f)) {  // apart from the branch above, which would take more registers (8 x 65536, G = 12: 45 us for 35)
 #pragma unroll
         for (int e = 0; e < kCh; ++e) o[n][e] *= by;
       }
@@ -1007,12 +1008,13 @@ int64_t list_splits(int64_t heads, int64_t k) {
 int64_t head_groups(int64_t G) { return cdiv(G, (int64_t)16); }
 
 // Blocks of a row that one workgroup of eight waves takes: two per wave, and one
-// more as a window of that length may begin inside a block.
+// more as a window of 1024 tokens may begin inside a block (its wave takes three then).
 constexpr int64_t kOneGroup = 17;
 
 // Whether rows of up to nb blocks go to workgroups of eight waves, one per row: one launch for two (the join)
-// and no workspace, two blocks per wave at most.  A call of 1 x 1000 tokens takes 10.0 us from Python and 11.2 in a
-// graph, with splits of four waves 14.5 and 8.4: the host's part of a call counts more often.  Rows of up to four
+// and no workspace, two or three blocks per wave.  A call of 1 x 1000 tokens takes 10.3 us from Python and 11.4 in a
+// graph, with splits of four waves 14.5 and 8.4: the host's part of a call counts more often, though a graph of
+// such rows loses by it.  Rows of up to four
 // blocks need no split of four waves either, and split rows are no faster in eight (32 x 4096 tokens 14.6 us
 // both ways, 8 x 8192 11.1 with four; 13.8, 8 x 1048576 326; 331).
 bool one_group(int64_t nb) { return nb > kDenseWaves && nb <= kOneGroup; }

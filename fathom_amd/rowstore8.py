@@ -169,7 +169,7 @@ class RowStore8:
         prompt, a piece of one, or one step's token.
 
         A 64-token block's scale is its largest finite |x| / 448 (e4m3) or 127 (int8); a
-        block that holds earlier tokens keeps its scale, or takes the least
+        block that holds earlier tokens keeps its scale and its sign, or takes the least
         power-of-two multiple of it that holds the new tokens, to which its earlier
         codes are then rounded.  Tokens at pos + T and behind are no longer the row's.
         With a tensor `pos`, rows whose tokens do not all fit into the store (a negative
@@ -222,7 +222,8 @@ class RowStore8:
         softmax(z) . V in float32 [BH, G, d], with
           z_t = scale q . K_t, capped to softcap tanh(z_t / softcap) if softcap is given,
                 then biased by slopes[bh, g] (t - (length - 1)) if slopes are given
-        (slopes [BH, G], or [G]; scale defaults to d ** -0.5).  A tensor length is taken
+        (slopes [BH, G], or [G]; scale defaults to d ** -0.5; a cap below 2^-64 counts as
+        that, one above 2^90 as none).  A tensor length is taken
         as within [0, cap].  A row without tokens gives zeros."""
         q, q_at, scale, softcap, slopes = self._query(q, scale, softcap, slopes)
         lens, lens_at, n = self._per_row(length, "length")

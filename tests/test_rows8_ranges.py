@@ -31,8 +31,8 @@ def test_selections_do_not_wrap(G, k):
 def test_workspace_queries_at_the_ends():
     """Shapes that the calls refuse need no workspace; positions and k past every store need what the longest do."""
     L = _lib.lib()
-    for query, most in ((L.fathom_rows8_attention_workspace_bytes, 2 ** 31 - 65), (L.fathom_rows8_gather_attention_workspace_bytes,
-                                                                                 (2 ** 31 - 1) // 4)):
+    for query, most in ((L.fathom_rows8_attention_workspace_bytes, 2 ** 31 - 65),
+                        (L.fathom_rows8_gather_attention_workspace_bytes, (2 ** 31 - 1) // 4)):
         for BH, G, D in ((65536, 4, 128), (4, 65536, 128), (4, 4, 96), (2 ** 32, 4, 128), (4, 2 ** 62, 128), (4, 4, 2 ** 62)):
             assert query(BH, G, D, 100000) == 0
         assert query(4, 4, 128, most) > 0

@@ -61,13 +61,25 @@ PROTOTYPES = {
                                        ctypes.c_float, _vp, _vp, _vp, _sz, _vp]),
     "fathom_rows8_write": (_i32, [_vp, _vp, _i32, _i64, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _i64, _i64, _i32, _vp,
                                   _vp, _vp, _vp, _vp]),
+    "fathom_rows8_write_rotated": (_i32, [_vp, _vp, _vp, _i32, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _vp, _i64,
+                                          _vp, _i64, _vp, _vp, _i32, ctypes.c_float, _i64, _i64, _i64, _i64, _i64, _i32, _vp,
+                                          _vp, _vp, _vp, _vp, _vp, _vp]),
     "fathom_rows8_read": (_i32, [_vp, _vp, _vp, _vp, _i32, _i64, _i64, _i64, _vp, _vp, _i64, _i64, _i32, _vp, _vp, _vp]),
     "fathom_rows8_attention_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64]),
     "fathom_rows8_attention": (_i32, [_vp, _i32, _vp, _vp, _vp, _vp, _i32, _i64, _i64, _i64, _i64, _vp, _i64, _i64,
                                       ctypes.c_float, ctypes.c_float, _vp, _vp, _vp, _sz, _vp]),
+    "fathom_rows8_sink_attention": (_i32, [_vp, _i32, _vp, _vp, _vp, _vp, _i32, _i64, _i64, _i64, _i64, _vp, _i64, _i64, _i64,
+                                           ctypes.c_float, ctypes.c_float, _vp, _vp, _vp, _sz, _vp]),
     "fathom_rows8_gather_attention_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64]),
     "fathom_rows8_gather_attention": (_i32, [_vp, _i32, _vp, _vp, _vp, _vp, _vp, _i32, _i64, _i64, _i64, _i64, _i64, _vp,
                                              _i64, ctypes.c_float, ctypes.c_float, _vp, _vp, _vp, _sz, _vp]),
+    "fathom_rows8_chunk_attention_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64, _i64]),
+    "fathom_rows8_chunk_attention": (_i32, [_vp, _i32, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _i32, _i64, _i64, _i64, _i64, _i64,
+                                            _vp, _i64, _i64, _i64, ctypes.c_float, ctypes.c_float, _vp, _vp, _vp, _sz, _vp]),
+    "fathom_rows8_shared_attention_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64, _i64, _i64]),
+    "fathom_rows8_shared_attention": (_i32, [_vp, _i32, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i32,
+                                             _i64, _i64, _i64, _i64, _vp, _i64, ctypes.c_float, ctypes.c_float, _vp, _vp, _vp,
+                                             _sz, _vp]),
     "fathom_gather_runs": (_i32, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp]),
     "fathom_copy_index": (_i32, [_vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp]),
     "fathom_copy_index_range": (_i32, [_vp, _i64, _i64, _i64, _i64, _i64, _i64, _i32, _vp, _vp, _vp, _vp, _vp]),

@@ -95,23 +95,8 @@ __global__ __launch_bounds__(kThreads) void write_kernel(WriteArgs a) {
   amax = fmaxf(fmaxf(wave_max[0], wave_max[1]), fmaxf(wave_max[2], wave_max[3]));
   const float need = fmaxf(amax / code_max<I8>(), kMinScale);
   const int earlier = (int)(p > t0 ? p - t0 : 0);  // tokens that the block holds already
-  const float size = fabsf(was);
-  float s = need, f = 1.0f;  // f: what the earlier codes are multiplied by
-  if (earlier && size < INFINITY) {
-    if (size == 0.0f) {
-      f = 0.0f;
-    } else {
-      int by = 0;
-      if (size < need) {
-        int e0, e1;
-        const float m0 = frexpf(size, &e0), m1 = frexpf(need, &e1);
-        by = e1 - e0 + (m1 > m0 ? 1 : 0);
-      }
-      s = ldexpf(was, by);
-      f = ldexpf(1.0f, -by);
-    }
-  }
-  const float inv = 1.0f / s;
+  const BlockScale to = block_scale(was, need, earlier);
+  const float inv = 1.0f / to.s;
   uint8_t *dst = a.codes[kv] + (bh * a.cap + t0) * D;
 #pragma unroll
   for (int i = 0; i < kPasses; ++i) {
@@ -127,17 +112,8 @@ __global__ __launch_bounds__(kThreads) void write_kernel(WriteArgs a) {
     if constexpr (kElem == 8) __builtin_nontemporal_store(u32x2{w[0], w[1]}, reinterpret_cast<u32x2 *>(dst + r * D + 8 * piece));
     else __builtin_nontemporal_store(w[0], reinterpret_cast<uint32_t *>(dst + r * D + 4 * piece));
   }
-  if (f != 1.0f) {
-    for (int o = 4 * tid; o < earlier * D; o += 4 * kThreads) {
-      uint32_t *c = reinterpret_cast<uint32_t *>(dst + o);
-      float y[4];
-      decode4<I8>(*c, y);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) y[e] *= f;
-      *c = encode4<I8>(y);
-    }
-  }
-  if (tid == 0) *scale = s;
+  if (to.f != 1.0f) rescale_codes<I8>(dst, earlier * D, to.f, tid, kThreads);
+  if (tid == 0) *scale = to.s;
 }
 
 struct ReadArgs {

@@ -85,6 +85,43 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   }
 }
 
+// The scale s that a written block takes, and the factor f of its earlier codes: `was` its scale, `need` what its
+// new tokens need, `earlier` the tokens that it holds already.
+struct BlockScale {
+  float s, f;
+};
+__device__ __forceinline__ BlockScale block_scale(float was, float need, int earlier) {
+  const float size = fabsf(was);
+  BlockScale to{need, 1.0f};
+  if (earlier && size < INFINITY) {
+    if (size == 0.0f) {
+      to.f = 0.0f;
+    } else {
+      int by = 0;
+      if (size < need) {
+        int e0, e1;
+        const float m0 = frexpf(size, &e0), m1 = frexpf(need, &e1);
+        by = e1 - e0 + (m1 > m0 ? 1 : 0);
+      }
+      to.s = ldexpf(was, by);
+      to.f = ldexpf(1.0f, -by);
+    }
+  }
+  return to;
+}
+// `bytes` codes, times f, by a workgroup's threads.
+template <bool I8>
+__device__ __forceinline__ void rescale_codes(uint8_t *codes, int bytes, float f, int tid, int threads) {
+  for (int o = 4 * tid; o < bytes; o += 4 * threads) {
+    uint32_t *c = reinterpret_cast<uint32_t *>(codes + o);
+    float y[4];
+    decode4<I8>(*c, y);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] *= f;
+    *c = encode4<I8>(y);
+  }
+}
+
 // The length of row bh: the array's value, kept inside the store, or n.
 __device__ __forceinline__ int64_t row_length(const int32_t *lens, int64_t n, int64_t cap, int64_t bh) {
   if (!lens) return n;

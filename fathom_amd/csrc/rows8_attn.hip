@@ -5,9 +5,9 @@
 //   u_t = scale s_K(t) (q . cK_t)
 //   z_t = softcap tanh(u_t / softcap) (u_t without a cap) + slope_g (t - (len - 1))
 //   out = sum_t e^(z_t - m) s_V(t) cV_t / sum_t e^(z_t - m)
-// over the tokens t of [max(0, len - window), len), or the listed ones of [0, len).
+// over the tokens t of [max(0, len - window), len) and of [0, sinks), or the listed ones of [0, len).
 // Scores, maxima, sums and the weighted rows are float32.
-#include "rows8.hpp"
+#include "rows8_core.hpp"
 
 namespace fathom {
 namespace rows8 {
@@ -18,12 +18,6 @@ constexpr int kMergeThreads = 256;
 constexpr int kDenseWaves = 4;     // of a workgroup that takes a split of a row
 constexpr int kDenseTotal = 2048;  // waves of a dense call: eight per CU, all at work at once
 constexpr int kMaxSplits = 512;  // of a query head
-constexpr float kLog2e = 1.44269504088896340736f;
-constexpr float kLowest = -3.0e38f;  // below every score: the running maximum of no token
-// A weight is 2^(x y - m), m the largest rounded x y: below kLarge with one rounding (a fused multiply-add), which leaves the
-// maximum's own rounding in the weights, all alike, at most 2^(1/16) here.  Past it that would be 2 and more, up to
-// infinity or 0, so there the product is rounded first and the largest weight is 1.
-constexpr float kLarge = 1048576.0f;  // 2^20
 constexpr float kNoValue = -1000.0f;  // log2 of the largest weight times scale before any
 constexpr float kLeast = -112.0f;     // a block counts there with that weight at least: 2^14 s_V / (weight s_V) is finite
 
@@ -34,7 +28,7 @@ struct AttnArgs {
   const float *ks, *vs;
   int64_t G, cap, nblk;
   const int32_t *lens;
-  int64_t n, window;
+  int64_t n, window, sinks;
   const int64_t *idx;
   int64_t k;
   float scale, softcap;
@@ -44,24 +38,8 @@ struct AttnArgs {
   float *part;  // [slots, G, D] its weighted rows
   int2 *where;  // [BH] a row's first slot and its splits, where lengths are on the device; else null
   int64_t nsplit, BH, groups;
+  bool join;  // the caller joins the results with others: every row leaves partial ones
 };
-
-// Eight consecutive elements of q from i (a multiple of eight).
-__device__ __forceinline__ void load8_q(const void *q, int dt, int64_t i, float (&v)[8]) {
-  if (dt == FATHOM_DT_F32) {
-    const float4 *p = reinterpret_cast<const float4 *>(static_cast<const float *>(q) + i);
-    const float4 x = p[0], y = p[1];
-    v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w, v[4] = y.x, v[5] = y.y, v[6] = y.z, v[7] = y.w;
-  } else {
-    const uint4 x = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(q) + i);
-    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      if (dt == FATHOM_DT_BF16) unpack2<FATHOM_DT_BF16>(w[e], v[2 * e], v[2 * e + 1]);
-      else unpack2<FATHOM_DT_F16>(w[e], v[2 * e], v[2 * e + 1]);
-    }
-  }
-}
 
 // The factor that the queries take before the product, (scale log2 e, or scale /
 // softcap), as a fraction in [1/2, 1) that multiplies q and a power of two for the
@@ -71,49 +49,6 @@ __device__ __forceinline__ float query_factor(const AttnArgs &a, int &e) {
   e = 0;
   return c == 0.0f || !(fabsf(c) < INFINITY) ? c : frexpf(c, &e);
 }
-
-// tanh to about a step of float32: below 1/2 u + u^3 P(u^2), P the least-squares fit of
-// degree 4 to (tanh u - u) / u^3; from there (1 - t) / (1 + t), t = e^(-2 |u|), the quotient
-// by the reciprocal and one correction.
-__device__ __forceinline__ float tanh_small(float u) {
-  const float w = u * u;
-  float p = -0.006947011f;
-  p = fmaf(p, w, 0.021472726f);
-  p = fmaf(p, w, -0.05393379f);
-  p = fmaf(p, w, 0.13333227f);
-  p = fmaf(p, w, -0.3333333f);
-  return fmaf(u * w, p, u);
-}
-__device__ __forceinline__ float tanh_any(float u) {
-  const float x = fabsf(u);
-  const float t = __builtin_amdgcn_exp2f(x * (-2.0f * kLog2e));
-  const float n = 1.0f - t, d = 1.0f + t, r = __builtin_amdgcn_rcpf(d);
-  float far = n * r;
-  far = fmaf(fmaf(-far, d, n), r, far);
-  return x < 0.5f ? tanh_small(u) : copysignf(far, u);
-}
-
-// Sum or maximum over the four lanes l, l ^ 16, l ^ 32, l ^ 48 (v_permlane32_swap
-// and v_permlane16_swap give each lane its partner's value).
-template <bool MAX>
-__device__ __forceinline__ float across_groups(float v) {
-  auto op = [](float x, float y) { return MAX ? fmaxf(x, y) : x + y; };
-  const uint32_t x = __float_as_uint(v);
-  const auto p32 = __builtin_amdgcn_permlane32_swap(x, x, false, false);
-  v = op(__uint_as_float(p32[0]), __uint_as_float(p32[1]));
-  const uint32_t y = __float_as_uint(v);
-  const auto p16 = __builtin_amdgcn_permlane16_swap(y, y, false, false);
-  return op(__uint_as_float(p16[0]), __uint_as_float(p16[1]));
-}
-
-// v of another lane of the same row of 16, by a DPP control.
-template <int CTRL>
-__device__ __forceinline__ float dpp(float v) {
-  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xF, 0xF, true));  // folds into its use
-}
-constexpr int kXor1 = 0xB1, kXor2 = 0x4E;           // quad_perm [1,0,3,2], [2,3,0,1]
-constexpr int kHalfMirror = 0x141;                  // row_half_mirror: lane 7 - l of a half row
-constexpr int kRor4 = 0x124, kXor8 = 0x128;         // row_ror:4 and :8
 
 // Sum over the LANES lanes (4 or 8) that hold one row; row_half_mirror pairs quads
 // whose lanes already agree.
@@ -135,7 +70,6 @@ __device__ __forceinline__ float over_rows(float v) {
   return across_groups<MAX>(over_row16<LANES, MAX>(v));
 }
 
-typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 __device__ const u32x4 kNoRow[8] = {};  // the row of a token that takes no part
 
 // Attention over listed tokens: one workgroup of NW waves per (split, query head,
@@ -307,64 +241,6 @@ struct VPiece<8> {
 __device__ __forceinline__ uint32_t dword_of(uint32_t v, int) { return v; }
 __device__ __forceinline__ uint32_t dword_of(VPiece<8>::type v, int d) { return v[d]; }
 
-// Block b of a row's codes through a buffer descriptor that holds its tokens
-// before `end`: loads behind that give zeros.  They are streams (the nt bit): a
-// step reads a row once, and other layers' rows come before its next step.  us with, without, rows
-// that come from HBM: 8 x 1048576 tokens 345, 380; 32 x 32768 52, 57; 16 x 18432 21.6, 22.4 (while they fit the
-// 256 MB cache and nothing else runs: 21.2, 19.9).
-constexpr int kStream = 2;
-struct RowsOf {
-  __amdgpu_buffer_rsrc_t rsrc;
-  __device__ __forceinline__ RowsOf(const uint8_t *codes, int64_t row0, int64_t b, int64_t end, int D) {
-    const int64_t left = end - b * kBlk;
-    const int tokens = left < 0 ? 0 : left < kBlk ? (int)left : kBlk;
-    rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(codes) + (row0 + (tokens ? b * kBlk : 0)) * D, 0, tokens * D,
-                                             0x00027000);
-  }
-  typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
-  __device__ __forceinline__ u32x4 load16(int off) const {
-    return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, off, 0, kStream));
-  }
-  __device__ __forceinline__ void load(int off, u32x2 &v) const {
-    v = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rsrc, off, 0, kStream));
-  }
-  __device__ __forceinline__ void load(int off, uint32_t &v) const { v = __builtin_amdgcn_raw_buffer_load_b32(rsrc, off, 0, kStream); }
-};
-
-typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-
-
-// Bytes 0, 1 (HI: 2, 3) of a dword of codes as two f16 values (exact: e4m3 and
-// int8 both fit f16).  int8 codes come with their sign bit flipped (flip_sign),
-// as c + 128 in 0 .. 255: under the exponent byte 0x64 that is the f16 number
-// 1024 + (c + 128).
-template <bool I8>
-__device__ __forceinline__ uint32_t flip_sign(uint32_t w) {
-  return I8 ? w ^ 0x80808080u : w;
-}
-template <bool I8, bool HI>
-__device__ __forceinline__ f16x2 pair16(uint32_t w) {
-  if constexpr (I8) {
-    const uint32_t h = __builtin_amdgcn_perm(0x64646464u, w, HI ? 0x04030402u : 0x04010400u);
-    const f16x2 b = {(_Float16)-1152.0f, (_Float16)-1152.0f};
-    return __builtin_bit_cast(f16x2, h) + b;
-  } else {
-    return __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)w, 1.0f, HI));
-  }
-}
-__device__ __forceinline__ f16x8 join8(f16x2 a, f16x2 b, f16x2 c, f16x2 d) {
-  return f16x8{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
-}
-
-// Two floats as f16 (keep = 0), or as the f16 of what those leave (keep = -1): to nearest both times.
-__device__ __forceinline__ f16x2 split16(float x, float y, float keep) {
-  typedef float f32x2 __attribute__((ext_vector_type(2)));
-  const f16x2 hi = __builtin_convertvector(f32x2{x, y}, f16x2);
-  return __builtin_convertvector(f32x2{fmaf((float)hi.x, keep, x), fmaf((float)hi.y, keep, y)}, f16x2);
-}
-
 // Of a query channel x (the head's largest in [2^12, 2^14)): whether two f16 may hold fewer than 19 bits
 // of it, and what they leave of such a one, times 2^38 (at most 2^13: they end at 2^-24).
 __device__ __forceinline__ bool small_channel(float x) { return fabsf(x) < 0x1p-6f && x != 0.0f; }
@@ -378,12 +254,22 @@ __device__ __forceinline__ float add_other_half(float v) {
   return v + dpp<kXor8>(v);
 }
 
-// The blocks of a row that a call takes.
-__device__ __forceinline__ void row_blocks(const AttnArgs &a, int64_t bh, int64_t &lo, int64_t &len, int64_t &blk0, int &nb) {
-  len = row_length(a.lens, a.n, a.cap, bh);
-  lo = a.window > 0 && len > a.window ? len - a.window : 0;
-  blk0 = lo / kBlk;
-  nb = (int)(cdiv(len, (int64_t)kBlk) - blk0);
+// The blocks of a row that a call takes: the first `sink` ones and, `skip` blocks further, those of the window, nb in
+// all.  Tokens of them that take no part: [from, lo), and from len on.
+struct Span {
+  int len, lo, from, sink, skip, nb;
+  __device__ __forceinline__ int block(int i) const { return i < sink ? i : i + skip; }  // the i-th of them
+};
+__device__ __forceinline__ Span row_span(const AttnArgs &a, int64_t bh) {
+  Span s;
+  s.len = (int)row_length(a.lens, a.n, a.cap, bh);
+  s.lo = a.window > 0 && s.len > a.window ? s.len - (int)a.window : 0;
+  s.from = a.sinks < s.lo ? (int)a.sinks : s.lo;
+  const int first = s.lo / kBlk, sink = (s.from + kBlk - 1) / kBlk;
+  s.sink = sink < first ? sink : first;  // the last sinks may be in the window's first block
+  s.skip = first - s.sink;
+  s.nb = (s.len + kBlk - 1) / kBlk - s.skip;
+  return s;
 }
 
 // The part of a workgroup: row, split of the row, the row's splits, blocks per split.
@@ -397,10 +283,7 @@ struct Part {
 // per).  Those are at most kDenseTotal / kDenseWaves / head groups + BH, the grid.  (32
 // bits hold the sums: 2^31 blocks of D = 64 are 17 TB.)
 __device__ __forceinline__ uint32_t blocks_of(const AttnArgs &a, int r) {
-  int64_t lo, len, blk0;
-  int nb = 0;
-  if (r < (int)a.BH) row_blocks(a, r, lo, len, blk0, nb);
-  return (uint32_t)nb;
+  return r < (int)a.BH ? (uint32_t)row_span(a, r).nb : 0u;
 }
 // Blocks per workgroup.  A row's last workgroup may have less to do: with few rows the
 // share leaves room for those, so that all of the call's workgroups are at work at once.
@@ -528,12 +411,11 @@ __global__ __launch_bounds__(NW *kWave, 2) void dense_kernel(AttnArgs a) {
     if (part.split == 0 && blockIdx.y == 0 && tid == 0) a.where[part.bh] = make_int2((int)blockIdx.x, part.active);
   }
   const int64_t bh = part.bh;
-  int64_t lo, len, blk0;
-  int nb;
-  row_blocks(a, bh, lo, len, blk0, nb);
-  if (!a.where) part.per = (nb + part.active - 1) / part.active;
-  const int64_t first = blk0 + (int64_t)part.split * part.per;
-  const int64_t last = part.split + 1 < part.active ? first + part.per : blk0 + nb;
+  const Span span = row_span(a, bh);
+  const int lo = span.lo, len = span.len;
+  if (!a.where) part.per = (span.nb + part.active - 1) / part.active;
+  const int first = part.split * part.per;  // of the row's blocks in the order of span.block
+  const int last = part.split + 1 < part.active ? first + part.per : span.nb;
 
   // the queries are requested first and made ready while the first block's rows come
   float q[NG][kSteps][8];
@@ -548,15 +430,15 @@ __global__ __launch_bounds__(NW *kWave, 2) void dense_kernel(AttnArgs a) {
   typedef typename VPiece<kCh>::type vpiece;
   vpiece vr[4][4];
   const int koff = col * D + 16 * grp, voff = 4 * grp * D + kCh * col;
-  auto load_k = [&](int64_t b) {
-    const RowsOf r(a.k8, bh * a.cap, b, b < last ? len : 0, D);
+  auto load_k = [&](int b) {
+    const RowsOf r(a.k8, bh * a.cap, span.block(b), b < last ? len : 0, D);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int h = 0; h < kHalves; ++h) kr[i][h] = r.load16(koff + 16 * i * D + 64 * h);
   };
-  auto load_v = [&](int64_t b) {
-    const RowsOf r(a.v8, bh * a.cap, b, b < last ? len : 0, D);
+  auto load_v = [&](int b) {
+    const RowsOf r(a.v8, bh * a.cap, span.block(b), b < last ? len : 0, D);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -661,10 +543,10 @@ __global__ __launch_bounds__(NW *kWave, 2) void dense_kernel(AttnArgs a) {
   const scalar_ptr ksp = (scalar_ptr)(a.ks + bh * a.nblk), vsp = (scalar_ptr)(a.vs + bh * a.nblk);
   float ks_next = 0.0f, vs_next = 0.0f;
   if (first + wave < last) {
-    ks_next = ksp[first + wave];
-    vs_next = vsp[first + wave];
+    ks_next = ksp[span.block(first + wave)];
+    vs_next = vsp[span.block(first + wave)];
   }
-  for (int64_t b = first + wave; b < last; b += NW) {
+  for (int b = first + wave; b < last; b += NW) {
     const float ks = ks_next, vs = vs_next;
     f32x4 s[NG][4];
 #pragma unroll
@@ -705,12 +587,24 @@ __global__ __launch_bounds__(NW *kWave, 2) void dense_kernel(AttnArgs a) {
       }
     load_k(b + NW);
     if (b + NW < last) {
-      ks_next = ksp[b + NW];
-      vs_next = vsp[b + NW];
+      ks_next = ksp[span.block(b + NW)];
+      vs_next = vsp[span.block(b + NW)];
     }
-    // ---- scores, in log2 units; tokens outside [lo, len) have none
-    const int t0 = (int)(b * kBlk), in_block = t0 + 4 * grp;
-    const bool edge = (int64_t)t0 < lo || (int64_t)t0 + kBlk > len;
+    // ---- scores, in log2 units; tokens of [from, lo) and from len on have none
+    const int t0 = span.block(b) * kBlk, in_block = t0 + 4 * grp;
+    const bool edge = (t0 < lo && t0 + kBlk > span.from) || t0 + kBlk > len;
+    // Bit 4 i + j: a token that takes no part.  Made where it is used, and in a register of the lane: as masks for
+    // every token the compiler fills the scalar registers with it (70 spilled at two groups of heads).
+    auto left_out = [&]() {
+      uint32_t none = 0;
+#pragma unroll
+      for (int x = 0; x < 16; ++x) {
+        const int t = in_block + 16 * (x / 4) + x % 4;
+        none |= ((t >= span.from && t < lo) || t >= len ? 1u : 0u) << x;
+      }
+      asm volatile("" : "+v"(none));
+      return none;
+    };
     const int ev = (int)((__float_as_uint(vs) >> 23) & 0xFF) - 127;
     float fz[NG];
 #pragma unroll
@@ -752,7 +646,7 @@ __global__ __launch_bounds__(NW *kWave, 2) void dense_kernel(AttnArgs a) {
           }
           f = a.softcap * kLog2e;
         }
-        const float back = (float)(in_block - (int)(len - 1));
+        const float back = (float)(in_block - (len - 1));
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -760,14 +654,11 @@ __global__ __launch_bounds__(NW *kWave, 2) void dense_kernel(AttnArgs a) {
         f = 1.0f;
       }
       if (edge) {
-        asm volatile("");  // a branch, not selects in every block
+        const uint32_t none = left_out();
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int t = in_block + 16 * i + j;
-            s[n][i][j] = t >= (int)lo && t < (int)len ? s[n][i][j] : -INFINITY;
-          }
+          for (int j = 0; j < 4; ++j) s[n][i][j] = none >> (4 * i + j) & 1 ? -INFINITY : s[n][i][j];
       }
       float mx = -INFINITY;
 #pragma unroll
@@ -803,11 +694,12 @@ __global__ __launch_bounds__(NW *kWave, 2) void dense_kernel(AttnArgs a) {
 #pragma unroll
     for (int n = 0; n < NG; ++n) wv[n] = ldexpf(vs, 14 - (int)ceilf(R[n]));
     if (edge) {  // a token outside has no value either (its codes may be NaN)
+      const uint32_t none = left_out();
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          if (in_block + 16 * i + j < (int)lo) vr[i][j] = vpiece{};
+          if (none >> (4 * i + j) & 1) vr[i][j] = vpiece{};
     }
     // ---- weights and products, 32 tokens at a time
 #pragma unroll
@@ -892,7 +784,7 @@ __global__ __launch_bounds__(NW *kWave, 2) void dense_kernel(AttnArgs a) {
       O = fmaf(wo[v][h][d], e, O);
     }
     const int64_t r = bh * a.G + g0 + h;
-    if (part.active <= 1) {
+    if (part.active <= 1 && !a.join) {
       a.out[r * D + d] = L == 0.0f ? 0.0f : O / L;
     } else {
       const int64_t at = slot * a.G + g0 + h;
@@ -1100,38 +992,79 @@ int run_dense(AttnArgs a, int64_t BH, int64_t D, bool i8, bool one, hipStream_t 
   else if (i8) launch_dense<64, true>(a, BH, one, st);
   else launch_dense<64, false>(a, BH, one, st);
   const int rc = launch_status("rows8 dense_kernel");
-  return rc || a.nsplit == 1 ? rc : merge(a, BH, D, st);
+  return rc || a.nsplit == 1 || a.join ? rc : merge(a, BH, D, st);
 }
 
-int check_query(const char *what, const void *q, int q_dtype, int64_t G, int64_t cap, const int32_t *lens, int64_t n,
-                float softcap, const float *out) {
-  if (!q || !out) return fail(FATHOM_ERR_INVALID, "%s: null pointer", what);
-  if (q_dtype < FATHOM_DT_F32 || q_dtype > FATHOM_DT_BF16) return fail(FATHOM_ERR_INVALID, "%s: q_dtype %d", what, q_dtype);
-  if (G < 1 || G > kMaxRows) return fail(FATHOM_ERR_INVALID, "%s: G=%lld", what, (long long)G);
-  if (!lens && (n < 0 || n > cap)) return fail(FATHOM_ERR_INVALID, "%s: length %lld outside [0, cap=%lld]", what, (long long)n, (long long)cap);
-  if (!(softcap >= 0.0f && softcap < INFINITY)) return fail(FATHOM_ERR_INVALID, "%s: softcap must be 0 (none) or positive and finite", what);
-  if (reinterpret_cast<uintptr_t>(q) & 15) return fail(FATHOM_ERR_INVALID, "%s: q must be 16-byte aligned", what);
-  return FATHOM_OK;
+// Blocks of a row at most, from what the host knows: exact without lengths on the device.
+int64_t dense_blocks(const int32_t *lens, int64_t n, int64_t cap, int64_t window, int64_t sinks) {
+  const int64_t all = cdiv(lens ? cap : n, (int64_t)kBlk);
+  if (window <= 0 || window >= (lens ? cap : n)) return lens && window > 0 ? all + 1 : all;
+  if (lens) {
+    const int64_t nb = cdiv(window, (int64_t)kBlk) + 1, some = nb + cdiv(sinks < cap ? sinks : cap, (int64_t)kBlk);
+    return sinks > 0 && some > all ? all : some;
+  }
+  const int64_t lo = n - window, from = sinks < lo ? sinks : lo, first = lo / kBlk, sink = cdiv(from, (int64_t)kBlk);
+  return all - first + (sink < first ? sink : first);
 }
 
-// Whether the calls take this shape: the queries answer 0 for others, as their products could wrap.
-bool shape_taken(int64_t BH, int64_t G, int64_t D) {
-  return BH >= 1 && BH <= kMaxRows && G >= 1 && G <= kMaxRows && (D == 64 || D == 128);
+// Slots of partial results of a call, as dense_slots, but one per row at least where others join them.
+int64_t part_slots(int64_t BH, int64_t G, int64_t nb, bool lens, bool join) {
+  const int64_t slots = dense_slots(BH, G, nb, lens);
+  return join && slots < BH ? BH : slots;
 }
 
-// The cap as the kernels take it, in a range where scale / softcap and its products stay normal: below
-// 2^-64 every weight is 1 either way, and above 2^90 (0: none) scores below 2^78 do not notice a cap.
-float kernel_cap(float softcap) {
-  return softcap > 0x1p90f ? 0.0f : softcap > 0.0f && softcap < 0x1p-64f ? 0x1p-64f : softcap;
+// Bytes for calls of up to so many positions.
+size_t dense_bytes(int64_t BH, int64_t G, int64_t D, int64_t positions, bool join) {
+  if (positions > kMaxCap) positions = kMaxCap;
+  const int64_t nb = cdiv(positions, (int64_t)kBlk) + 1;  // a window may begin inside a block
+  const int64_t one = part_slots(BH, G, nb, false, join), own = part_slots(BH, G, nb, true, join);
+  return part_bytes(BH, G, D, one > own ? one : own);
 }
 
-// An upper bound of a row's positions that the host knows.
-int64_t dense_positions(const int32_t *lens, int64_t n, int64_t cap, int64_t window) {
-  const int64_t most = lens ? cap : n;
-  return window > 0 && window < most ? window : most;
+// Sets up and launches the splits; their join only where the results are not the caller's to join.
+int dense_call(AttnArgs &a, const char *what, int64_t D, bool i8, void *workspace, size_t workspace_bytes, hipStream_t st) {
+  const bool lens = a.lens != nullptr;
+  const int64_t nb = dense_blocks(a.lens, a.n, a.cap, a.window, a.sinks), all = dense_slots(a.BH, a.G, nb, lens);
+  const int64_t slots = part_slots(a.BH, a.G, nb, lens, a.join);
+  a.groups = head_groups(a.G);
+  a.nsplit = all < 1 ? 1 : lens ? all : cdiv(nb, cdiv(nb, all / a.BH));  // as many as shares of that size fill
+  const size_t need = part_bytes(a.BH, a.G, D, slots);
+  if (need && (!workspace || workspace_bytes < need))
+    return fail(FATHOM_ERR_WORKSPACE, "%s: workspace %zu bytes, need %zu", what, workspace_bytes, need);
+  if (need && reinterpret_cast<uintptr_t>(workspace) & 15)
+    return fail(FATHOM_ERR_INVALID, "%s: the workspace must be 16-byte aligned", what);
+  place(a, workspace, D, slots, lens && all > 0);
+  return run_dense(a, a.BH, D, i8, one_group(nb), st);
+}
+
+int attention(const char *what, const void *q, int q_dtype, const void *k8, const void *v8, const float *k_scale,
+              const float *v_scale, int code_dtype, int64_t BH, int64_t G, int64_t D, int64_t cap, const int32_t *lens, int64_t n,
+              int64_t window, int64_t sinks, float scale, float softcap, const float *slopes, float *out, void *workspace,
+              size_t workspace_bytes, void *stream) {
+  int rc = check_store(what, k8, v8, k_scale, v_scale, code_dtype, BH, cap, D);
+  if (!rc) rc = check_query(what, q, q_dtype, G, cap, lens, n, softcap, out);
+  if (rc) return rc;
+  if (window < 0) return fail(FATHOM_ERR_INVALID, "%s: window %lld", what, (long long)window);
+  if (sinks < 0) return fail(FATHOM_ERR_INVALID, "%s: sinks %lld", what, (long long)sinks);
+  AttnArgs a{q, q_dtype, (const uint8_t *)k8, (const uint8_t *)v8, k_scale, v_scale, G, cap, cdiv(cap, kBlk), lens, n, window,
+             sinks, nullptr, 0, scale, kernel_cap(softcap), slopes, out, nullptr, nullptr, nullptr, 1, BH, 1, false};
+  return dense_call(a, what, D, code_dtype == FATHOM_DT_I8, workspace, workspace_bytes, (hipStream_t)stream);
 }
 
 }  // namespace
+
+size_t tail_bytes(int64_t BH, int64_t G, int64_t D, int64_t positions) { return dense_bytes(BH, G, D, positions, true); }
+
+int tail_attention(Tail &t, const char *what, const void *q, int q_dtype, const void *k8, const void *v8, const float *k_scale,
+                   const float *v_scale, bool i8, int64_t BH, int64_t G, int64_t D, int64_t cap, const int32_t *lens, int64_t n,
+                   float scale, float softcap, const float *slopes, void *workspace, size_t workspace_bytes, hipStream_t st) {
+  AttnArgs a{q, q_dtype, (const uint8_t *)k8, (const uint8_t *)v8, k_scale, v_scale, G, cap, cdiv(cap, kBlk), lens, n, 0,
+             0, nullptr, 0, scale, kernel_cap(softcap), slopes, nullptr, nullptr, nullptr, nullptr, 1, BH, 1, true};
+  const int rc = dense_call(a, what, D, i8, workspace, workspace_bytes, st);
+  t = Tail{a.part, a.ml, a.where, a.nsplit};
+  return rc;
+}
+
 }  // namespace rows8
 }  // namespace fathom
 
@@ -1140,10 +1073,7 @@ using namespace fathom::rows8;
 
 extern "C" size_t fathom_rows8_attention_workspace_bytes(int64_t BH, int64_t G, int64_t D, int64_t positions) {
   if (!shape_taken(BH, G, D) || positions < 1) return 0;
-  if (positions > kMaxCap) positions = kMaxCap;
-  const int64_t nb = cdiv(positions, (int64_t)kBlk) + 1;  // a window may begin inside a block
-  const int64_t one = dense_slots(BH, G, nb, false), own = dense_slots(BH, G, nb, true), slots = one > own ? one : own;
-  return part_bytes(BH, G, D, slots);
+  return dense_bytes(BH, G, D, positions, false);
 }
 
 extern "C" int fathom_rows8_attention(const void *q, int q_dtype, const void *k8, const void *v8, const float *k_scale,
@@ -1151,25 +1081,17 @@ extern "C" int fathom_rows8_attention(const void *q, int q_dtype, const void *k8
                                       const int32_t *lens, int64_t n, int64_t window, float scale, float softcap,
                                       const float *slopes, float *out, void *workspace, size_t workspace_bytes,
                                       void *stream) {
-  int rc = check_store("rows8_attention", k8, v8, k_scale, v_scale, code_dtype, BH, cap, D);
-  if (!rc) rc = check_query("rows8_attention", q, q_dtype, G, cap, lens, n, softcap, out);
-  if (rc) return rc;
-  if (window < 0) return fail(FATHOM_ERR_INVALID, "rows8_attention: window %lld", (long long)window);
-  AttnArgs a{q, q_dtype, (const uint8_t *)k8, (const uint8_t *)v8, k_scale, v_scale, G, cap, cdiv(cap, kBlk), lens, n, window,
-             nullptr, 0, scale, kernel_cap(softcap), slopes, out, nullptr, nullptr, nullptr, 1, BH, 1};
-  const int64_t most = dense_positions(lens, n, cap, window);
-  const int64_t nb = lens ? cdiv(most, (int64_t)kBlk) + (window > 0) : cdiv(n, (int64_t)kBlk) - (n - most) / kBlk;
-  const int64_t slots = dense_slots(BH, G, nb, lens != nullptr);
-  a.BH = BH;
-  a.groups = head_groups(G);
-  a.nsplit = slots < 1 ? 1 : lens ? slots : cdiv(nb, cdiv(nb, slots / BH));  // as many as shares of that size fill
-  const size_t need = part_bytes(BH, G, D, slots);
-  if (need && (!workspace || workspace_bytes < need))
-    return fail(FATHOM_ERR_WORKSPACE, "rows8_attention: workspace %zu bytes, need %zu", workspace_bytes, need);
-  if (need && reinterpret_cast<uintptr_t>(workspace) & 15)
-    return fail(FATHOM_ERR_INVALID, "rows8_attention: the workspace must be 16-byte aligned");
-  place(a, workspace, D, slots, lens != nullptr);
-  return run_dense(a, BH, D, code_dtype == FATHOM_DT_I8, one_group(nb), (hipStream_t)stream);
+  return attention("rows8_attention", q, q_dtype, k8, v8, k_scale, v_scale, code_dtype, BH, G, D, cap, lens, n, window, 0, scale,
+                   softcap, slopes, out, workspace, workspace_bytes, stream);
+}
+
+extern "C" int fathom_rows8_sink_attention(const void *q, int q_dtype, const void *k8, const void *v8, const float *k_scale,
+                                           const float *v_scale, int code_dtype, int64_t BH, int64_t G, int64_t D, int64_t cap,
+                                           const int32_t *lens, int64_t n, int64_t window, int64_t sinks, float scale,
+                                           float softcap, const float *slopes, float *out, void *workspace,
+                                           size_t workspace_bytes, void *stream) {
+  return attention("rows8_sink_attention", q, q_dtype, k8, v8, k_scale, v_scale, code_dtype, BH, G, D, cap, lens, n, window,
+                   sinks, scale, softcap, slopes, out, workspace, workspace_bytes, stream);
 }
 
 extern "C" size_t fathom_rows8_gather_attention_workspace_bytes(int64_t BH, int64_t G, int64_t D, int64_t k) {
@@ -1192,7 +1114,7 @@ extern "C" int fathom_rows8_gather_attention(const void *q, int q_dtype, const i
   if (k < 0 || k > 0x7FFFFFFF / G) return fail(FATHOM_ERR_INVALID, "rows8_gather_attention: G=%lld k=%lld", (long long)G, (long long)k);
   if (k > 0 && !idx) return fail(FATHOM_ERR_INVALID, "rows8_gather_attention: null index pointer");
   AttnArgs a{q, q_dtype, (const uint8_t *)k8, (const uint8_t *)v8, k_scale, v_scale, G, cap, cdiv(cap, kBlk), lens, n, 0,
-             idx, k, scale, kernel_cap(softcap), slopes, out, nullptr, nullptr, nullptr, 1, BH, 1};
+             0, idx, k, scale, kernel_cap(softcap), slopes, out, nullptr, nullptr, nullptr, 1, BH, 1, false};
   a.nsplit = list_splits(BH * G, k);
   const int64_t slots = a.nsplit > 1 ? BH * a.nsplit : 0;
   const size_t need = part_bytes(BH, G, D, slots);

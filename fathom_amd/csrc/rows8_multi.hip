@@ -1,0 +1,231 @@
+// Chunk attention and shared-prefix attention over the 8-bit K/V row store: entry
+// points, shares of the work, and the join of partial results.
+#include "rows8_multi.hpp"
+
+namespace fathom {
+namespace rows8 {
+namespace {
+
+constexpr int kJoinThreads = 256;
+constexpr int64_t kMaxTiles = 65535;  // grid y
+
+// Joins a query's splits, and its sequence's own tokens behind a shared prefix: one workgroup per query, D / 4 lanes
+// take 16 bytes of every (1024 / D)-th split.
+template <int D, int OUT>
+__global__ __launch_bounds__(kJoinThreads) void join_kernel(MultiArgs a, Tail tail) {
+  constexpr int kLanes = D / 4, kGroups = kJoinThreads / kLanes, kWaves = kJoinThreads / kWave;
+  __shared__ float4 acc[kGroups][kLanes];
+  __shared__ float red[2][kWaves];
+  const int tid = threadIdx.x, lane = tid % kLanes, grp = tid / kLanes;
+  const int64_t m = blockIdx.x, r = blockIdx.y, y = m / a.rows, g = m % a.G, o = m / a.G;
+  const int nb = tile_span(a, r, y * a.rows).nb, per = (nb + a.nsplit - 1) / a.nsplit;
+  const int own = per ? (nb + per - 1) / per : 0;  // splits that have blocks
+  const int64_t at = (r * a.tiles + y) * a.nsplit * a.rows + m % a.rows;
+  int more = 0;
+  int64_t slot = 0;
+  if (a.shared) {
+    const int64_t row = o * a.BH + r;
+    const int2 w = tail.where ? tail.where[row] : make_int2((int)(row * tail.nsplit), (int)tail.nsplit);
+    slot = (int64_t)w.x * a.G + g;
+    more = w.y;
+  }
+  const int ns = own + more;
+  auto ml = [&](int s) { return s < own ? a.ml[at + (int64_t)s * a.rows] : tail.ml[slot + (int64_t)(s - own) * a.G]; };
+  float big = kLowest;
+  for (int s = tid; s < ns; s += kJoinThreads) big = fmaxf(big, ml(s).x);
+#pragma unroll
+  for (int x = 32; x > 0; x >>= 1) big = fmaxf(big, __shfl_xor(big, x));
+  if ((tid & 63) == 0) red[0][tid >> 6] = big;
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < kWaves; ++k) big = fmaxf(big, red[0][k]);
+  float l = 0.0f;
+  for (int s = tid; s < ns; s += kJoinThreads) {
+    const float2 x = ml(s);
+    l = fmaf(x.y, __builtin_amdgcn_exp2f(x.x - big), l);
+  }
+  l = wave_sum_f(l);
+  if ((tid & 63) == 0) red[1][tid >> 6] = l;
+  float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  for (int s = grp; s < ns; s += kGroups) {
+    const float *p = s < own ? a.part + (at + (int64_t)s * a.rows) * D : tail.part + (slot + (int64_t)(s - own) * a.G) * D;
+    const float4 u = reinterpret_cast<const float4 *>(p)[lane];
+    const float f = __builtin_amdgcn_exp2f(ml(s).x - big);
+    v.x = fmaf(u.x, f, v.x);
+    v.y = fmaf(u.y, f, v.y);
+    v.z = fmaf(u.z, f, v.z);
+    v.w = fmaf(u.w, f, v.w);
+  }
+  acc[grp][lane] = v;
+  __syncthreads();
+  if (tid >= D) return;
+  float sum = 0.0f;
+  l = 0.0f;
+#pragma unroll
+  for (int k = 0; k < kGroups; ++k) sum += reinterpret_cast<const float *>(acc[k])[tid];
+#pragma unroll
+  for (int k = 0; k < kWaves; ++k) l += red[1][k];
+  const float out = l == 0.0f ? 0.0f : sum / l;
+  const int64_t to = (a.shared ? (o * a.BH + r) * a.G + g : (r * a.G + g) * a.O + o) * D + tid;
+  if constexpr (OUT == FATHOM_DT_F32) static_cast<float *>(a.out)[to] = out;
+  else if constexpr (OUT == FATHOM_DT_F16) static_cast<uint16_t *>(a.out)[to] = float_to_f16_bits(out);
+  else static_cast<uint16_t *>(a.out)[to] = float_to_bf16_bits(out);
+}
+
+template <int D>
+void launch_join(const MultiArgs &a, const Tail &t, int out, hipStream_t st) {
+  const dim3 grid((unsigned)((int64_t)a.G * a.O), (unsigned)a.BH);
+  if (out == FATHOM_DT_F32) join_kernel<D, FATHOM_DT_F32><<<grid, kJoinThreads, 0, st>>>(a, t);
+  else if (out == FATHOM_DT_F16) join_kernel<D, FATHOM_DT_F16><<<grid, kJoinThreads, 0, st>>>(a, t);
+  else join_kernel<D, FATHOM_DT_BF16><<<grid, kJoinThreads, 0, st>>>(a, t);
+}
+
+// Queries of a tile: one wave's, where a row has no more.
+int tile_rows(int64_t M) { return M <= 32 ? 32 : 128; }
+
+// Splits of what a tile sees, up to nb blocks: as many workgroups as are at work at once, each with a few blocks.
+int64_t tile_splits(int64_t BH, int64_t M, int64_t D, int64_t nb) {
+  const int rows = tile_rows(M);
+  const int64_t tiles = BH * cdiv(M, (int64_t)rows), places = rows == 32 ? (D == 128 ? 1280 : 2048) : 512;
+  const int64_t room = places / tiles, most = cdiv(nb, (int64_t)4);
+  const int64_t ns = room < most ? room : most;
+  return ns < 1 ? 1 : ns;
+}
+
+// Blocks that a tile sees at most, of rows of up to n tokens.
+int64_t tile_blocks(int64_t n, int64_t T, int64_t window, int64_t sinks) {
+  const int64_t all = cdiv(n, (int64_t)kBlk);
+  if (window <= 0 || window >= n) return all;
+  const int64_t some = cdiv(window + T - 1, (int64_t)kBlk) + 1 + cdiv(sinks < n ? sinks : n, (int64_t)kBlk);
+  return some < all ? some : all;
+}
+
+size_t multi_bytes(int64_t BH, int64_t M, int64_t D, int64_t ns) {
+  const int rows = tile_rows(M);
+  return (size_t)(BH * cdiv(M, (int64_t)rows) * ns * rows * (D + 2)) * sizeof(float);
+}
+
+bool queries_taken(int64_t BH, int64_t G, int64_t O) {
+  return O >= 1 && O <= kMaxCap && G <= kMaxTiles * 32 / O && BH * G * O <= (int64_t)1 << 40;
+}
+
+void place(MultiArgs &a, void *workspace, int64_t D) {
+  const int64_t rows = a.BH * a.tiles * a.nsplit * a.rows;
+  a.part = static_cast<float *>(workspace);
+  a.ml = reinterpret_cast<float2 *>(a.part + rows * D);
+}
+
+int run_multi(const MultiArgs &a, int q_dtype, int64_t D, bool i8, hipStream_t st) {
+  if (D == 128 && i8) launch_multi_d128_int8(a, q_dtype, st);
+  else if (D == 128) launch_multi_d128_e4m3(a, q_dtype, st);
+  else if (i8) launch_multi_d64_int8(a, q_dtype, st);
+  else launch_multi_d64_e4m3(a, q_dtype, st);
+  return launch_status("rows8 multi_kernel");
+}
+
+int run_join(const MultiArgs &a, const Tail &t, int out, int64_t D, hipStream_t st) {
+  if (D == 128) launch_join<128>(a, t, out, st);
+  else launch_join<64>(a, t, out, st);
+  return launch_status("rows8 join_kernel");
+}
+
+}  // namespace
+}  // namespace rows8
+}  // namespace fathom
+
+using namespace fathom;
+using namespace fathom::rows8;
+
+extern "C" size_t fathom_rows8_chunk_attention_workspace_bytes(int64_t BH, int64_t G, int64_t T, int64_t D, int64_t positions) {
+  if (!shape_taken(BH, G, D) || !queries_taken(BH, G, T) || positions < 1) return 0;
+  if (positions > kMaxCap) positions = kMaxCap;
+  const int64_t ns = tile_splits(BH, G * T, D, cdiv(positions, (int64_t)kBlk) + 1);
+  return ns > 1 ? multi_bytes(BH, G * T, D, ns) : 0;
+}
+
+extern "C" int fathom_rows8_chunk_attention(const void *q, int q_dtype, int64_t q_row_stride, int64_t q_head_stride,
+                                            int64_t q_tok_stride, const void *k8, const void *v8, const float *k_scale,
+                                            const float *v_scale, int code_dtype, int64_t BH, int64_t G, int64_t T, int64_t D,
+                                            int64_t cap, const int32_t *lens, int64_t n, int64_t window, int64_t sinks,
+                                            float scale, float softcap, const float *slopes, void *out, void *workspace,
+                                            size_t workspace_bytes, void *stream) {
+  const char *what = "rows8_chunk_attention";
+  int rc = check_store(what, k8, v8, k_scale, v_scale, code_dtype, BH, cap, D);
+  if (rc) return rc;
+  if (T < 0) return fail(FATHOM_ERR_INVALID, "%s: T=%lld", what, (long long)T);
+  if (T == 0) return FATHOM_OK;
+  rc = check_query(what, q, q_dtype, G, cap, lens, n, softcap, out);
+  if (rc) return rc;
+  if (!queries_taken(BH, G, T)) return fail(FATHOM_ERR_INVALID, "%s: G=%lld T=%lld, at most %lld queries per row", what, (long long)G, (long long)T, (long long)kMaxTiles * 32);
+  if (window < 0) return fail(FATHOM_ERR_INVALID, "%s: window %lld", what, (long long)window);
+  if (sinks < 0) return fail(FATHOM_ERR_INVALID, "%s: sinks %lld", what, (long long)sinks);
+  const int64_t size = q_dtype == FATHOM_DT_F32 ? 4 : 2;
+  if (((q_row_stride | q_head_stride | q_tok_stride) * size) & 15 || reinterpret_cast<uintptr_t>(out) & 15)
+    return fail(FATHOM_ERR_INVALID, "%s: the strides of q and out must be multiples of 16 bytes", what);
+  if (window >= cap) window = 0;
+  if (sinks > cap) sinks = cap;
+  MultiArgs a{q, q_row_stride, q_head_stride, q_tok_stride, (const uint8_t *)k8, (const uint8_t *)v8, k_scale, v_scale, cap,
+              cdiv(cap, kBlk), lens, n, (int)G, (int)T, (int)window, (int)sinks, false, nullptr, 0, 0, BH, scale,
+              kernel_cap(softcap), slopes, out, nullptr, nullptr, 1, 1, tile_rows(G * T)};
+  a.tiles = (int)cdiv(G * T, (int64_t)a.rows);
+  a.nsplit = (int)tile_splits(BH, G * T, D, tile_blocks(lens ? cap : n, T, window, sinks));
+  if (a.nsplit > 1) {
+    const size_t need = multi_bytes(BH, G * T, D, a.nsplit);
+    if (!workspace || workspace_bytes < need)
+      return fail(FATHOM_ERR_WORKSPACE, "%s: workspace %zu bytes, need %zu", what, workspace_bytes, need);
+    if (reinterpret_cast<uintptr_t>(workspace) & 15)
+      return fail(FATHOM_ERR_INVALID, "%s: the workspace must be 16-byte aligned", what);
+    place(a, workspace, D);
+  }
+  rc = run_multi(a, q_dtype, D, code_dtype == FATHOM_DT_I8, (hipStream_t)stream);
+  return rc || a.nsplit == 1 ? rc : run_join(a, Tail{}, q_dtype, D, (hipStream_t)stream);
+}
+
+extern "C" size_t fathom_rows8_shared_attention_workspace_bytes(int64_t prefix_BH, int64_t sequences, int64_t G, int64_t D,
+                                                                int64_t prefix_positions, int64_t positions) {
+  if (!shape_taken(prefix_BH, G, D) || !queries_taken(prefix_BH, G, sequences) || sequences > kMaxRows / prefix_BH) return 0;
+  if (prefix_positions > kMaxCap) prefix_positions = kMaxCap;
+  if (prefix_positions < 0) prefix_positions = 0;
+  const int64_t ns = tile_splits(prefix_BH, G * sequences, D, cdiv(prefix_positions, (int64_t)kBlk));
+  return multi_bytes(prefix_BH, G * sequences, D, ns) + tail_bytes(prefix_BH * sequences, G, D, positions < 0 ? 0 : positions);
+}
+
+extern "C" int fathom_rows8_shared_attention(const void *q, int q_dtype, const void *prefix_k8, const void *prefix_v8,
+                                             const float *prefix_k_scale, const float *prefix_v_scale, int64_t prefix_BH,
+                                             int64_t prefix_cap, const int32_t *prefix_lens, int64_t prefix_n, const void *k8,
+                                             const void *v8, const float *k_scale, const float *v_scale, int code_dtype,
+                                             int64_t sequences, int64_t G, int64_t D, int64_t cap, const int32_t *lens, int64_t n,
+                                             float scale, float softcap, const float *slopes, float *out, void *workspace,
+                                             size_t workspace_bytes, void *stream) {
+  const char *what = "rows8_shared_attention";
+  int rc = check_store(what, prefix_k8, prefix_v8, prefix_k_scale, prefix_v_scale, code_dtype, prefix_BH, prefix_cap, D);
+  if (rc) return rc;
+  if (sequences < 1 || sequences > kMaxRows / prefix_BH)
+    return fail(FATHOM_ERR_INVALID, "%s: %lld sequences of %lld rows, at most 65535 rows", what, (long long)sequences, (long long)prefix_BH);
+  const int64_t BH = prefix_BH * sequences;
+  rc = check_store(what, k8, v8, k_scale, v_scale, code_dtype, BH, cap, D);
+  if (!rc) rc = check_query(what, q, q_dtype, G, cap, lens, n, softcap, out);
+  if (rc) return rc;
+  if (!prefix_lens && (prefix_n < 0 || prefix_n > prefix_cap))
+    return fail(FATHOM_ERR_INVALID, "%s: prefix length %lld outside [0, cap=%lld]", what, (long long)prefix_n, (long long)prefix_cap);
+  if (!queries_taken(prefix_BH, G, sequences))
+    return fail(FATHOM_ERR_INVALID, "%s: %lld sequences, G=%lld, at most %lld queries per row", what, (long long)sequences, (long long)G, (long long)kMaxTiles * 32);
+  MultiArgs a{q, G * D, D, prefix_BH * G * D, (const uint8_t *)prefix_k8, (const uint8_t *)prefix_v8, prefix_k_scale,
+              prefix_v_scale, prefix_cap, cdiv(prefix_cap, kBlk), prefix_lens, prefix_n, (int)G, (int)sequences, 0, 0, true,
+              lens, n, cap, prefix_BH, scale, kernel_cap(softcap), slopes, out, nullptr, nullptr, 1, 1, tile_rows(G * sequences)};
+  a.tiles = (int)cdiv(G * sequences, (int64_t)a.rows);
+  a.nsplit = (int)tile_splits(prefix_BH, G * sequences, D, cdiv(prefix_lens ? prefix_cap : prefix_n, (int64_t)kBlk));
+  const size_t first = multi_bytes(prefix_BH, G * sequences, D, a.nsplit);
+  if (!workspace || workspace_bytes < first)
+    return fail(FATHOM_ERR_WORKSPACE, "%s: workspace %zu bytes, need more than %zu", what, workspace_bytes, first);
+  if (reinterpret_cast<uintptr_t>(workspace) & 15)
+    return fail(FATHOM_ERR_INVALID, "%s: the workspace must be 16-byte aligned", what);
+  place(a, workspace, D);
+  const bool i8 = code_dtype == FATHOM_DT_I8;
+  const hipStream_t st = (hipStream_t)stream;
+  Tail t;
+  rc = tail_attention(t, what, q, q_dtype, k8, v8, k_scale, v_scale, i8, BH, G, D, cap, lens, n, scale, softcap, slopes,
+                      static_cast<char *>(workspace) + first, workspace_bytes - first, st);
+  if (!rc) rc = run_multi(a, q_dtype, D, i8, st);
+  return rc ? rc : run_join(a, t, FATHOM_DT_F32, D, st);
+}

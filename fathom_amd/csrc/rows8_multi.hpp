@@ -1,0 +1,504 @@
+// Attention of many queries over one K/V row of the 8-bit store, on the matrix
+// cores: the kernel of chunk attention (a row's last T tokens, each over what it
+// sees) and of a shared prefix (a batch's single tokens over the row that they share).
+//
+// For a query at place p of its row, with c the codes:
+//   u_t = scale s_K(t) (q . cK_t)
+//   z_t = softcap tanh(u_t / softcap) (u_t without a cap) + slope (t - p)
+//   out = sum_t e^(z_t - m) s_V(t) cV_t / sum_t e^(z_t - m)
+// over the tokens t < end, end = p + 1 (the prefix's length where it is shared), without those of
+// [sinks, p + 1 - window).
+#pragma once
+
+#include "rows8_core.hpp"
+
+namespace fathom {
+namespace rows8 {
+
+struct MultiArgs {
+  const void *q;  // query (o, g) of row r at r q_row + g q_head + o q_out, in elements: o a token, or a sequence of the batch
+  int64_t q_row, q_head, q_out;
+  const uint8_t *k8, *v8;
+  const float *ks, *vs;
+  int64_t cap, nblk;
+  const int32_t *lens;  // of the store's rows, or n
+  int64_t n;
+  int G, O, window, sinks;  // M = G O queries of a row
+  bool shared;
+  const int32_t *tails;  // shared: tokens of sequence (o, r) behind the prefix, [O, BH], or tail_n
+  int64_t tail_n, tail_cap;
+  int64_t BH;
+  float scale, softcap;
+  const float *slopes;  // [BH, G]; shared: [O, BH, G]
+  void *out;            // [BH, G, O, D] of the queries' type; shared: written by the join, [O, BH, G, D] float32
+  float2 *ml;           // [BH, tiles, nsplit, rows of a tile] a split's (m, l)
+  float *part;          // [..., D] its weighted rows
+  int nsplit, tiles, rows;
+};
+
+// What a tile of `rows` queries from the first one m0 of row r sees: blocks [0, sink) and, `skip` blocks further, up to
+// nb in all; `end` the last token's successor, len the row's length.
+struct TileSpan {
+  int len, end, sink, skip, nb;
+  __device__ __forceinline__ int block(int i) const { return i < sink ? i : i + skip; }
+};
+__device__ __forceinline__ TileSpan tile_span(const MultiArgs &a, int64_t r, int64_t m0) {
+  TileSpan s;
+  s.len = (int)row_length(a.lens, a.n, a.cap, r);
+  int first = 0;  // the first token of the tile's windows
+  s.end = s.len;
+  if (!a.shared) {
+    const int64_t M = (int64_t)a.G * a.O, last = m0 + a.rows < M ? m0 + a.rows : M;
+    const int64_t lo = (int64_t)s.len - a.O + 1 + m0 / a.G - a.window;
+    const int64_t end = (int64_t)s.len - a.O + 1 + (last - 1) / a.G;
+    s.end = end < 0 ? 0 : (int)end;
+    first = a.window > 0 && lo > 0 ? (int)lo : 0;
+  }
+  const int sinks = a.sinks < first ? a.sinks : first, from = first / kBlk;
+  s.sink = (sinks + kBlk - 1) / kBlk;
+  s.sink = s.sink < from ? s.sink : from;
+  s.skip = from - s.sink;
+  s.nb = (s.end + kBlk - 1) / kBlk - s.skip;
+  if (s.nb < 0) s.nb = 0;
+  return s;
+}
+
+#ifdef FATHOM_ROWS8_MULTI_KERNEL
+namespace {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+
+// A weight is 2^(z - base), the base a whole number that is raised where a score passes it by kMost, to kStart below
+// the score, so that the rows' sums are scaled anew only where a score has grown by 2^3 (a row's first blocks).
+// The largest weight times scale is held between 2^10 and 2^15, so f16 (to 2^-24) ends at 2^-34 of it.
+constexpr float kMost = 15.0f, kStart = 12.0f;
+constexpr float kLeastWeight = -100.0f;  // a block counts with that weight at least in the choice of its values' scale
+
+__device__ __forceinline__ float power(float e) { return ldexpf(1.0f, (int)__builtin_amdgcn_fmed3f(e, -300.0f, 300.0f)); }
+
+// Bytes 0, 1 (HI: 2, 3) of a dword of codes as two bf16 values (exact); int8 codes as pair16 takes them.
+template <bool I8, bool HI>
+__device__ __forceinline__ uint32_t pair_bf16(uint32_t w) {
+  if constexpr (I8) {  // under 0x4B0000 a byte u is the float 2^23 + u
+    const float x = __uint_as_float(__builtin_amdgcn_perm(0x4B000000u, w, HI ? 0x070C0C02u : 0x070C0C00u)) - 8388736.0f;
+    const float y = __uint_as_float(__builtin_amdgcn_perm(0x4B000000u, w, HI ? 0x070C0C03u : 0x070C0C01u)) - 8388736.0f;
+    return __builtin_bit_cast(uint32_t, bf16x2{(__bf16)x, (__bf16)y});
+  } else {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)w, 1.0f, HI));
+  }
+}
+
+__device__ __forceinline__ void barrier_lds() {  // waits for LDS only: loads of the next tile stay on their way
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
+__device__ __forceinline__ float other_half(float v) {  // of lane l ^ 32
+  const uint32_t x = __float_as_uint(v);
+  const auto p = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+  return __uint_as_float((threadIdx.x & 32) ? p[0] : p[1]);
+}
+
+// A workgroup of W waves takes a tile of 32 W queries of one row, or one split of what
+// they see; each wave has 32 of the queries.  The tile's queries are consecutive in (o, g), so
+// that a chunk's tile is a few tokens of all heads.  Per 64-token block of the row:
+//   the codes are requested a block ahead, converted once per workgroup and kept in LDS as 16-bit
+//     numbers (exact): K by tokens, V transposed, both with their 16-byte pieces in an order
+//     that keeps the lanes' reads on different banks;
+//   S^T = K q^T (v_mfma_f32_32x32x16): lane l holds query l & 31 and 32 of the block's scores, so
+//     that maximum and sum need one exchange, between l and l ^ 32.  The queries are exact: bf16 and f16 in
+//     their own type, float32 as three bf16 parts; bf16 parts are taken from q 2^-e, e the exponent of the row's largest.
+//   O^T += V^T p^T with the weights in the layout that the scores come in, which fixes the order of the tokens in the
+//     transposed V.  A weight is one f16 (PREC: two, 22 bits) of p s_V 2^-E, E the exponent of the largest p s_V so
+//     far, so that blocks of small values with large weights count fully.
+template <int D, bool I8, int QT, bool PREC, int W>
+__global__ __launch_bounds__(W *kWave, 2) void multi_kernel(MultiArgs a) {
+  constexpr bool kBf16 = QT != FATHOM_DT_F16;
+  constexpr int kParts = QT == FATHOM_DT_F32 ? 3 : 1, kSteps = D / 16, kTiles = D / 32;
+  constexpr int kThreads = W * kWave, kBufs = W == 1 ? 1 : 2, kRows = 32 * W;
+  constexpr int kKeys = kBlk * D / 16 / kThreads;        // 16-byte pieces of K per thread
+  constexpr int kCh = D == 64 && W == 4 ? 4 : 8;         // channels of V per thread and item of four tokens
+  constexpr int kItems = kBlk / 4 * D / kCh / kThreads;  // items per thread
+  typedef typename std::conditional<kBf16, bf16x8, f16x8>::type frag;
+  __shared__ __attribute__((aligned(16))) uint16_t kt[kBufs][kBlk * D], vt[kBufs][kBlk * D];
+  __shared__ int odd[kBufs];  // the last block (+ 1) in this buffer that holds a NaN in V
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane & 31, half = lane >> 5;
+  const int64_t r = blockIdx.x;
+  const int y = (int)(gridDim.y - 1 - blockIdx.y);  // the tiles that see most come first
+  const int64_t m0 = (int64_t)y * kRows, M = (int64_t)a.G * a.O;
+  const TileSpan span = tile_span(a, r, m0);
+  const int per = (span.nb + a.nsplit - 1) / a.nsplit;
+  const int first = (int)blockIdx.z * per, last = first + per < span.nb ? first + per : span.nb;
+  if (blockIdx.z > 0 && first >= span.nb) return;
+
+  // ---- the lane's query
+  const int64_t mine = m0 + 32 * wave + col, m = mine < M ? mine : M - 1;
+  const int64_t o_at = m / a.G, g = m % a.G;
+  int end = span.len, lo = 0;
+  float back = 0.0f;  // the bias takes t - (end - 1) - back
+  if (a.shared) {
+    back = (float)(int)row_length(a.tails, a.tail_n, a.tail_cap, o_at * a.BH + r);
+  } else {
+    const int64_t e = (int64_t)span.len - a.O + 1 + o_at;
+    end = e < 0 ? 0 : (int)e;
+    lo = a.window > 0 && end > a.window ? end - a.window : 0;
+  }
+  const int from = a.sinks < lo ? a.sinks : lo;  // tokens of [from, lo) take no part
+  const float slope = !a.slopes ? 0.0f : a.slopes[a.shared ? (o_at * a.BH + r) * a.G + g : r * a.G + g] * kLog2e;
+  frag qf[kParts][kSteps];
+  int ex = 0;
+  {
+    const int64_t at = r * a.q_row + g * a.q_head + o_at * a.q_out + 8 * half;
+    float x[kSteps][8], big = 0.0f;
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      if constexpr (QT == FATHOM_DT_F16) {
+        qf[0][s] = *reinterpret_cast<const f16x8 *>(static_cast<const uint16_t *>(a.q) + at + 16 * s);
+      } else {
+        load8_q(a.q, QT, at + 16 * s, x[s]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) big = fmaxf(big, fabsf(x[s][e]));
+      }
+    }
+    if constexpr (kBf16) {
+      big = fmaxf(big, other_half(big));
+      if (big > 0.0f && big < INFINITY) frexpf(big, &ex);
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          float v = ldexpf(x[s][e], -ex);
+#pragma unroll
+          for (int k = 0; k < kParts; ++k) {
+            const __bf16 b = (__bf16)v;
+            qf[k][s][e] = b;
+            v = fabsf(v) < INFINITY ? v - (float)b : 0.0f;
+          }
+        }
+    }
+  }
+  // the scores' factor, scale log2 e or scale / softcap, as a fraction and a power of two
+  float cm = a.softcap > 0.0f ? __builtin_amdgcn_fmed3f(a.scale / a.softcap, -3.0e38f, 3.0e38f) : a.scale * kLog2e;
+  if (cm != 0.0f && fabsf(cm) < INFINITY) {
+    int e;
+    cm = frexpf(cm, &e);
+    ex += e;
+  }
+
+  // ---- staging
+  u32x4 kr[kKeys];
+  typedef typename std::conditional<kCh == 8, u32x2v, uint32_t>::type vpiece;
+  vpiece vr[kItems][4];
+  typedef const __attribute__((address_space(4))) float *scalar_ptr;
+  const scalar_ptr ksp = (scalar_ptr)(a.ks + r * a.nblk), vsp = (scalar_ptr)(a.vs + r * a.nblk);
+  float ks_next = 0.0f, vs_next = 0.0f;
+  auto load = [&](int i) {
+    if (i >= last) return;
+    const int b = span.block(i);
+    const RowsWith<0> k(a.k8, r * a.cap, b, span.end, D), v(a.v8, r * a.cap, b, span.end, D);
+#pragma unroll
+    for (int x = 0; x < kKeys; ++x) kr[x] = k.load16(16 * (x * kThreads + tid));
+#pragma unroll
+    for (int x = 0; x < kItems; ++x) {
+      const int item = x * kThreads + tid, at = item / (D / kCh) * 4 * D + item % (D / kCh) * kCh;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v.load(at + j * D, vr[x][j]);
+    }
+    ks_next = ksp[b];
+    vs_next = vsp[b];
+  };
+  auto stage = [&](int buf, int i) {
+    if (i >= last) return;
+#pragma unroll
+    for (int x = 0; x < kKeys; ++x) {
+      const int at = x * kThreads + tid, tok = at / (D / 16), piece = at % (D / 16);
+      uint32_t w[8];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t c = flip_sign<I8>(kr[x][e]);
+        if constexpr (kBf16) {
+          w[2 * e] = pair_bf16<I8, false>(c);
+          w[2 * e + 1] = pair_bf16<I8, true>(c);
+        } else {
+          w[2 * e] = __builtin_bit_cast(uint32_t, pair16<I8, false>(c));
+          w[2 * e + 1] = __builtin_bit_cast(uint32_t, pair16<I8, true>(c));
+        }
+      }
+      char *row = reinterpret_cast<char *>(kt[buf]) + tok * 2 * D;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        *reinterpret_cast<u32x4 *>(row + 16 * ((2 * piece + h) ^ (tok & (D / 8 - 1)))) = u32x4{w[4 * h], w[4 * h + 1], w[4 * h + 2], w[4 * h + 3]};
+    }
+    uint32_t nan = 0;
+#pragma unroll
+    for (int x = 0; x < kItems; ++x) {
+      const int item = x * kThreads + tid, quad = item / (D / kCh), ch0 = item % (D / kCh) * kCh;
+      // tokens 4 quad ..: half (quad >> 1 & 1) of the piece that lane half quad & 1 reads for 16 tokens
+      const int piece = (quad >> 3) * 4 + (quad >> 2 & 1) * 2 + (quad & 1);
+      char *base = reinterpret_cast<char *>(vt[buf]) + 8 * (quad >> 1 & 1);
+#pragma unroll
+      for (int d = 0; d < kCh / 4; ++d) {
+        uint32_t w[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          uint32_t c;
+          if constexpr (kCh == 8) c = vr[x][j][d];
+          else c = vr[x][j];
+          if constexpr (!I8) nan |= (c & 0x7F7F7F7Fu) + 0x01010101u;
+          w[j] = flip_sign<I8>(c);
+        }
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {  // channels 4 d + 2 p, + 1
+          const uint32_t ab = __builtin_amdgcn_perm(w[1], w[0], p ? 0x07030602u : 0x05010400u);
+          const uint32_t cd = __builtin_amdgcn_perm(w[3], w[2], p ? 0x07030602u : 0x05010400u);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int ch = ch0 + 4 * d + 2 * p + h;
+            const u32x2v v = {__builtin_bit_cast(uint32_t, h ? pair16<I8, true>(ab) : pair16<I8, false>(ab)),
+                              __builtin_bit_cast(uint32_t, h ? pair16<I8, true>(cd) : pair16<I8, false>(cd))};
+            *reinterpret_cast<u32x2v *>(base + ch * 2 * kBlk + 16 * (piece ^ ((ch ^ ch >> 3) & 7))) = v;
+          }
+        }
+      }
+    }
+    if (!I8 && (nan & 0x80808080u)) odd[buf] = i + 1;
+  };
+
+  f32x16 o[kTiles];
+#pragma unroll
+  for (int d = 0; d < kTiles; ++d)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[d][e] = 0.0f;
+  float base = kLowest, l = 0.0f, E = -1000.0f;
+
+  auto block = [&](int buf, int i, float ks, float vs) {
+    const int t0 = span.block(i) * kBlk;
+    if (!__any(t0 < end && (t0 + kBlk > lo || t0 < from))) return;
+    const bool edge = !__all(t0 + kBlk <= end && (t0 >= lo || t0 + kBlk <= from));
+    // ---- scores
+    f32x16 s[2];
+    const char *kb = reinterpret_cast<const char *>(kt[buf]);
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[x][e] = 0.0f;
+      const int tok = 32 * x + col;
+#pragma unroll
+      for (int c = 0; c < kSteps; ++c) {
+        const frag k = *reinterpret_cast<const frag *>(kb + tok * 2 * D + 16 * ((2 * c + half) ^ (tok & (D / 8 - 1))));
+#pragma unroll
+        for (int p = kParts - 1; p >= 0; --p) {
+          if constexpr (kBf16) s[x] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k, qf[p][c], s[x], 0, 0, 0);
+          else s[x] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qf[p][c], s[x], 0, 0, 0);
+        }
+      }
+    }
+    float f = ldexpf(fabsf(ks) * fabsf(cm), ex);
+    // never infinite: a score of 0 has to stay one; nor 0 without a cap: a score of -inf has to stay one too
+    f = fabsf(ks) < INFINITY ? __builtin_amdgcn_fmed3f(f, a.softcap > 0.0f ? 0.0f : 1.2e-38f, 3.0e38f) : f;
+    if ((ks < 0.0f) != (cm < 0.0f)) {
+#pragma unroll
+      for (int x = 0; x < 2; ++x) s[x] = -s[x];
+    }
+    const int at = t0 + 4 * half;  // register e of s[x] is token at + 32 x + 8 (e / 4) + e % 4
+    if (a.softcap > 0.0f) {
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[x][e] = tanh_any(s[x][e] * f);
+      f = a.softcap * kLog2e;
+    }
+    if (a.slopes) {
+      const float b = (float)(at - (end - 1)) - back;
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[x][e] = fmaf(s[x][e], f, slope * (b + (float)(32 * x + 8 * (e / 4) + e % 4)));
+      f = 1.0f;
+    }
+    uint32_t seen = 0xFFFFFFFFu;  // bit 16 x + e
+    if (edge) {
+      seen = 0;
+#pragma unroll
+      for (int b = 0; b < 32; ++b) {
+        const int t = at + 32 * (b / 16) + 8 * (b % 16 / 4) + b % 4;
+        seen |= (t < end && (t >= lo || t < from) ? 1u : 0u) << b;
+      }
+      asm volatile("" : "+v"(seen));
+#pragma unroll
+      for (int b = 0; b < 32; ++b) s[b / 16][b % 16] = seen >> b & 1 ? s[b / 16][b % 16] : -INFINITY;
+    }
+    float mx = -INFINITY;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) mx = fmaxf(mx, fmaxf(s[0][e], s[1][e]));
+    mx *= f;
+    if (__any(fabsf(mx) >= kLarge && fabsf(mx) < INFINITY)) {
+#pragma unroll
+      for (int x = 0; x < 2; ++x) s[x] *= f;
+      f = 1.0f;
+    }
+    const float ev = (float)((int)((__float_as_uint(vs) >> 23) & 0xFF) - 127);  // |s_V| < 2^(ev + 1)
+    if (__any(mx - base > kMost || fmaxf(mx - base, kLeastWeight) + ev - (kMost - 1.0f) > E)) {
+      mx = fmaxf(mx, other_half(mx));
+      const float to = mx - base > kMost ? floorf(mx) - kStart : base, up = to - base;
+      const float most = ceilf(fmaxf(mx - to, kLeastWeight) + ev) - (kStart - 1.0f);
+      const float was = E;
+      E = fmaxf(was - up, most);
+      l *= power(-up);
+      const float by = power(was - E - up);
+#pragma unroll
+      for (int d = 0; d < kTiles; ++d) o[d] *= by;
+      base = to;
+    }
+    const float wv = ldexpf(vs, -(int)E);
+    const char *vb = reinterpret_cast<const char *>(vt[buf]);
+    auto values = [&](int d, int x, int c) {
+      const int ch = 32 * d + col, piece = 4 * x + 2 * c + half;
+      return *reinterpret_cast<const f16x8 *>(vb + ch * 2 * kBlk + 16 * (piece ^ ((ch ^ ch >> 3) & 7)));
+    };
+    // A NaN in V counts for the queries that see its token, and for no other: counted apart, it is no value there
+    const bool nans = !I8 && edge && odd[buf] == i + 1;
+    if (nans) {
+#pragma unroll 1
+      for (int d = 0; d < kTiles; ++d) {
+        f32x16 hits;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) hits[e] = 0.0f;
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const f16x8 v = values(d, x, c);
+            f16x8 is, sees;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              is[e] = v[e] != v[e] ? (_Float16)1.0f : (_Float16)0.0f;
+              sees[e] = seen >> (16 * x + 8 * c + e) & 1 ? (_Float16)1.0f : (_Float16)0.0f;
+            }
+            hits = __builtin_amdgcn_mfma_f32_32x32x16_f16(is, sees, hits, 0, 0, 0);
+          }
+#pragma unroll
+        for (int k = 0; k < kTiles; ++k)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) o[k][e] = k == d && hits[e] > 0.0f ? NAN : o[k][e];
+      }
+    }
+    // ---- weights and products, 16 tokens at a time
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        float w[8], ps[4];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e] = __builtin_amdgcn_exp2f(fmaf(s[x][8 * c + e], f, -base));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) ps[e] = w[2 * e] + w[2 * e + 1];  // added together first: alone, most weights
+        l += (ps[0] + ps[1]) + (ps[2] + ps[3]);                      // would be lost beside a large sum
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e] *= wv;
+        if (edge) {  // a scale that is not finite counts only where its tokens are seen
+#pragma unroll
+          for (int e = 0; e < 8; ++e) w[e] = seen >> (16 * x + 8 * c + e) & 1 ? w[e] : 0.0f;
+        }
+        const f16x8 p = join8(split16(w[0], w[1], 0.0f), split16(w[2], w[3], 0.0f), split16(w[4], w[5], 0.0f), split16(w[6], w[7], 0.0f));
+        f16x8 rest;
+        if constexpr (PREC)
+          rest = join8(split16(w[0], w[1], -1.0f), split16(w[2], w[3], -1.0f), split16(w[4], w[5], -1.0f), split16(w[6], w[7], -1.0f));
+#pragma unroll
+        for (int d = 0; d < kTiles; ++d) {
+          f16x8 v = values(d, x, c);
+          if (nans) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = v[e] != v[e] ? (_Float16)0.0f : v[e];
+          }
+          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p, o[d], 0, 0, 0);
+          if constexpr (PREC) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, rest, o[d], 0, 0, 0);
+        }
+      }
+  };
+
+  if (tid < kBufs) odd[tid] = 0;
+  load(first);
+  float ks = ks_next, vs = vs_next;
+  barrier_lds();  // `odd` is cleared before a thread sets it
+  stage(0, first);
+  load(first + 1);
+  barrier_lds();
+  for (int i = first; i < last; ++i) {
+    const int buf = kBufs == 2 ? (i - first) & 1 : 0;
+    block(buf, i, ks, vs);
+    ks = ks_next;
+    vs = vs_next;
+    if constexpr (kBufs == 1) barrier_lds();
+    stage(kBufs == 2 ? buf ^ 1 : 0, i + 1);
+    load(i + 2);
+    barrier_lds();
+  }
+
+  l += other_half(l);
+  if (mine >= M) return;
+  if (a.nsplit > 1 || a.shared) {
+    const int64_t at = ((r * a.tiles + y) * a.nsplit + blockIdx.z) * kRows + 32 * wave + col;
+    if (half == 0) a.ml[at] = make_float2(base + kStart, ldexpf(l, -(int)kStart));
+#pragma unroll
+    for (int d = 0; d < kTiles; ++d)
+#pragma unroll
+      for (int e = 0; e < 16; e += 4) {
+        float4 v;
+        v.x = ldexpf(o[d][e], (int)(E - kStart));
+        v.y = ldexpf(o[d][e + 1], (int)(E - kStart));
+        v.z = ldexpf(o[d][e + 2], (int)(E - kStart));
+        v.w = ldexpf(o[d][e + 3], (int)(E - kStart));
+        *reinterpret_cast<float4 *>(a.part + at * D + 32 * d + 2 * e + 4 * half) = v;
+      }
+    return;
+  }
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  const int64_t at = ((r * a.G + g) * a.O + o_at) * D + 4 * half;
+#pragma unroll
+  for (int d = 0; d < kTiles; ++d)
+#pragma unroll
+    for (int e = 0; e < 16; e += 4) {
+      float v[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[k] = l == 0.0f ? 0.0f : ldexpf(o[d][e + k] * inv, (int)E);
+      const int64_t to = at + 32 * d + 2 * e;
+      if constexpr (QT == FATHOM_DT_F32) {
+        *reinterpret_cast<float4 *>(static_cast<float *>(a.out) + to) = make_float4(v[0], v[1], v[2], v[3]);
+      } else {
+        const u32x2v w = {pack2<QT>(v[0], v[1]), pack2<QT>(v[2], v[3])};
+        *reinterpret_cast<u32x2v *>(static_cast<uint16_t *>(a.out) + to) = w;
+      }
+    }
+}
+
+template <int D, bool I8, int QT, bool PREC>
+void launch_multi(const MultiArgs &a, hipStream_t st) {
+  const dim3 grid((unsigned)a.BH, (unsigned)a.tiles, (unsigned)a.nsplit);
+  if (a.rows == 32) multi_kernel<D, I8, QT, PREC, 1><<<grid, kWave, 0, st>>>(a);
+  else multi_kernel<D, I8, QT, PREC, 4><<<grid, 4 * kWave, 0, st>>>(a);
+}
+template <int D, bool I8>
+void launch_multi(const MultiArgs &a, int q_dtype, hipStream_t st) {
+  if (q_dtype == FATHOM_DT_F32) launch_multi<D, I8, FATHOM_DT_F32, true>(a, st);
+  else if (q_dtype == FATHOM_DT_F16 && a.shared) launch_multi<D, I8, FATHOM_DT_F16, true>(a, st);
+  else if (q_dtype == FATHOM_DT_F16) launch_multi<D, I8, FATHOM_DT_F16, false>(a, st);
+  else if (a.shared) launch_multi<D, I8, FATHOM_DT_BF16, true>(a, st);
+  else launch_multi<D, I8, FATHOM_DT_BF16, false>(a, st);
+}
+
+}  // namespace
+#endif
+
+// Launches multi_kernel; one for each head size and code type, as they take long to compile.
+void launch_multi_d64_e4m3(const MultiArgs &a, int q_dtype, hipStream_t st);
+void launch_multi_d64_int8(const MultiArgs &a, int q_dtype, hipStream_t st);
+void launch_multi_d128_e4m3(const MultiArgs &a, int q_dtype, hipStream_t st);
+void launch_multi_d128_int8(const MultiArgs &a, int q_dtype, hipStream_t st);
+
+}  // namespace rows8
+}  // namespace fathom

@@ -1,0 +1,5 @@
+// multi_kernel for heads of 128 and e4m3 codes.
+#define FATHOM_ROWS8_MULTI_KERNEL
+#include "rows8_multi.hpp"
+
+void fathom::rows8::launch_multi_d128_e4m3(const MultiArgs &a, int q_dtype, hipStream_t st) { launch_multi<128, false>(a, q_dtype, st); }

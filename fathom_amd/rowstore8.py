@@ -45,6 +45,19 @@ def _rows(x):
     return x, sr, st
 
 
+def _heads(q):
+    """Queries [BH, G, T, d] of a float type, with the strides of rows, heads and tokens: any, but dense channels, each
+    at a multiple of 16 bytes (a copy is made of others)."""
+    if q.dtype not in _KDT:
+        q = q.float()
+    size = 4 if q.dtype == _F32 else 2
+    st = [s if n > 1 else 0 for s, n in zip(q.stride()[:3], q.shape[:3])]
+    if q.stride(3) != 1 or (q.data_ptr() | st[0] * size | st[1] * size | st[2] * size) & 15:
+        q = torch.empty(q.shape, dtype=q.dtype, device=q.device).copy_(q)
+        st = q.stride()[:3]
+    return q, st[0], st[1], st[2]
+
+
 class RowStore8:
     """The K/V rows of one layer in 8 bits; see the module's text.
 
@@ -136,6 +149,10 @@ class RowStore8:
         if at % 16:
             q = q.clone()
             at = q.data_ptr()
+        return q, at, *self._scores(shape, scale, softcap, slopes)
+
+    def _scores(self, shape, scale, softcap, slopes):
+        """The scale, cap and slopes of a call whose queries have this shape."""
         softcap = 0.0 if softcap is None else float(softcap)
         if not 0.0 <= softcap < math.inf:
             raise ValueError(f"softcap {softcap} must be positive and finite (None or 0: no cap)")
@@ -146,18 +163,18 @@ class RowStore8:
                 self._elsewhere(slopes)
             if slopes.dtype != _F32 or slopes.shape != shape[:2] or not slopes.is_contiguous():
                 slopes = slopes.float().expand(shape[:2]).contiguous()
-        return q, at, self.d ** -0.5 if scale is None else float(scale), softcap, slopes
+        return self.d ** -0.5 if scale is None else float(scale), softcap, slopes
 
-    def _workspace(self, query, G, positions):
+    def _workspace(self, query, G, positions, *queries):
         """The call's workspace (or None), its address and size, for at least `positions`: sizes grow with them, so one query
         serves up to the next power of two."""
         if positions < 1:
             return None, None, 0
         bits = (positions - 1).bit_length()
-        key = query, self.BH, G, self.d, bits
+        key = query, self.BH, G, *queries, self.d, bits
         nbytes = _SIZES.get(key)
         if nbytes is None:
-            nbytes = _SIZES[key] = getattr(_lib.lib(), query)(self.BH, G, self.d, 1 << bits)
+            nbytes = _SIZES[key] = getattr(_lib.lib(), query)(self.BH, G, *queries, self.d, 1 << bits)
         if not nbytes:
             return None, None, 0
         ws = torch.empty((nbytes,), dtype=torch.uint8, device=self.device)
@@ -186,6 +203,64 @@ class RowStore8:
         V, vr, vt = _rows(V)
         self._call("fathom_rows8_write", K.data_ptr(), V.data_ptr(), _KDT[K.dtype], kr, kt, vr, vt, rows_at, at, self.BH,
                    K.shape[1], self.d, self.cap, self._code, *self._store())
+
+    def write_rotated(self, q, K, V, inv_freq, pos=0, offset=0, q_weight=None, k_weight=None, eps=1e-6, keys=False):
+        """What a layer does with its projections, in one pass: norms of each query and key head, the position rotation,
+        and `write` of the rotated keys and of V.  q [BH, G, T, d], K, V [BH, T, d], all of one type.  Returns the
+        rotated queries [BH, G, T, d], or with keys=True (queries, keys [BH, T, d]), both of q's type; the store's codes are
+        made from the keys before that rounding.
+
+        With weights (q_weight, k_weight [d]; None: no norm) x becomes x / sqrt(mean(x^2) + eps) * weight.  Token i
+        of a row stands at position t = pos + i + offset; with inv_freq [r / 2] (float32; r <= d a multiple of
+        16; None: no rotation) channels c and c + r / 2 become (x_c cos - x_{c+r/2} sin, x_{c+r/2} cos + x_c sin) of
+        the angle t inv_freq[c], which is formed in float64; channels behind r stay.  offset is an int or integers [BH]:
+        what stands before the store's first token, as a shared prefix does.  Views as in `write`; with a tensor `pos`,
+        rows whose tokens do not all fit are rotated but not written."""
+        for t in (q, K, V):
+            if t.device != self.device:
+                self._elsewhere(t)
+        BH, d = self.BH, self.d
+        if K.dim() != 3 or K.shape != V.shape or K.shape[0] != BH or K.shape[2] != d:
+            raise ValueError(f"K {tuple(K.shape)} and V {tuple(V.shape)} must be alike, [{BH}, T, {d}]")
+        T = K.shape[1]
+        if q.dim() != 4 or q.shape[0] != BH or q.shape[1] < 1 or q.shape[2] != T or q.shape[3] != d:
+            raise ValueError(f"q {tuple(q.shape)} must be [{BH}, G, {T}, {d}]")
+        if not q.dtype == K.dtype == V.dtype or not q.dtype.is_floating_point:
+            raise ValueError(f"q {q.dtype}, K {K.dtype} and V {V.dtype} must be of one float type")
+        turned = 0
+        if inv_freq is not None:
+            if inv_freq.device != self.device:
+                self._elsewhere(inv_freq)
+            turned = 2 * inv_freq.numel()
+            if inv_freq.dim() != 1 or turned > d or turned % 16 or not inv_freq.dtype.is_floating_point:
+                raise ValueError(f"inv_freq {inv_freq.dtype} {tuple(inv_freq.shape)} must be float32 [r / 2], r <= {d} a multiple of 16")
+            if inv_freq.dtype != _F32 or not inv_freq.is_contiguous():
+                inv_freq = inv_freq.float().contiguous()
+        weights = [q_weight, k_weight]
+        given = [w for w in weights if w is not None]
+        for w in given:
+            if w.device != self.device:
+                self._elsewhere(w)
+            if w.shape != (d,) or not w.dtype.is_floating_point:
+                raise ValueError(f"a weight {w.dtype} {tuple(w.shape)} must be floats [{d}]")
+        w_dtype = given[0].dtype if given and given[0].dtype == given[-1].dtype and given[0].dtype in _KDT else _F32
+        weights = [w if w is None else w.to(w_dtype).contiguous() for w in weights]
+        eps = float(eps)
+        if not 0.0 <= eps < math.inf:
+            raise ValueError(f"eps {eps} must be finite and not negative")
+        rows, rows_at, at = self._per_row(pos, "pos")
+        shifts, shifts_at, shift = self._per_row(offset, "offset")
+        q, qr, qh, qt = _heads(q)
+        K, kr, kt = _rows(K)
+        V, vr, vt = _rows(V)
+        G = q.shape[1]
+        out = torch.empty((BH, G, T, d), dtype=q.dtype, device=self.device)
+        k_out = torch.empty((BH, T, d), dtype=q.dtype, device=self.device) if keys else None
+        self._call("fathom_rows8_write_rotated", q.data_ptr(), K.data_ptr(), V.data_ptr(), _KDT[q.dtype], qr, qh, qt, kr, kt, vr,
+                   vt, rows_at, at, shifts_at, shift, inv_freq.data_ptr() if turned else None, turned,
+                   *(None if w is None else w.data_ptr() for w in weights), _KDT[w_dtype], eps, BH, G, T, d, self.cap,
+                   self._code, *self._store(), out.data_ptr(), None if k_out is None else k_out.data_ptr())
+        return (out, k_out) if keys else out
 
     def _read(self, idx_at, rows_at, at, R, dtype):
         if dtype not in _KDT:
@@ -216,9 +291,9 @@ class RowStore8:
         return self._read(idx.data_ptr(), None, 0, idx.shape[1], dtype)
 
     # ------------------------------------------------------------------ attention
-    def attention(self, q, length, window=0, scale=None, softcap=None, slopes=None):
+    def attention(self, q, length, window=0, scale=None, softcap=None, slopes=None, sinks=0):
         """Attention of one token per row, q [BH, G, d] (float32, float16 or bfloat16),
-        over the row's first `length` tokens, or the last `window` of them (0: all):
+        over the row's first `length` tokens, or the last `window` of them (0: all) and the first `sinks`:
         softmax(z) . V in float32 [BH, G, d], with
           z_t = scale q . K_t, capped to softcap tanh(z_t / softcap) if softcap is given,
                 then biased by slopes[bh, g] (t - (length - 1)) if slopes are given
@@ -227,14 +302,15 @@ class RowStore8:
         as within [0, cap].  A row without tokens gives zeros."""
         q, q_at, scale, softcap, slopes = self._query(q, scale, softcap, slopes)
         lens, lens_at, n = self._per_row(length, "length")
-        G, window = q.shape[1], max(min(int(window), _FAR), -1)  # the library refuses negative ones
+        G, window, sinks = q.shape[1], max(min(int(window), _FAR), -1), max(min(int(sinks), _FAR), -1)  # the library refuses negative ones
         positions = n if lens is None else self.cap
-        positions = max(min(positions, window) if window > 0 else positions, 0)
+        positions = max(min(positions, window + -(-sinks // BLK) * BLK) if window > 0 else positions, 0)
         ws, ws_at, nbytes = self._workspace("fathom_rows8_attention_workspace_bytes", G, positions)
         out = torch.empty_like(q, dtype=_F32)
-        self._call("fathom_rows8_attention", q_at, _KDT[q.dtype], *self._store(), self._code, self.BH, G, self.d, self.cap,
-                   lens_at, n, window, scale, softcap, None if slopes is None else slopes.data_ptr(), out.data_ptr(), ws_at,
-                   nbytes)
+        extra = (sinks,) if sinks else ()
+        self._call("fathom_rows8_sink_attention" if sinks else "fathom_rows8_attention", q_at, _KDT[q.dtype], *self._store(),
+                   self._code, self.BH, G, self.d, self.cap, lens_at, n, window, *extra, scale, softcap,
+                   None if slopes is None else slopes.data_ptr(), out.data_ptr(), ws_at, nbytes)
         return out
 
     def gather_attention(self, q, idx, length=None, scale=None, softcap=None, slopes=None):
@@ -259,4 +335,58 @@ class RowStore8:
         self._call("fathom_rows8_gather_attention", q_at, _KDT[q.dtype], idx.data_ptr(), *self._store(), self._code, self.BH, G,
                    k, self.d, self.cap, lens_at, n, scale, softcap, None if slopes is None else slopes.data_ptr(),
                    out.data_ptr(), ws_at, nbytes)
+        return out
+
+    def chunk_attention(self, q, length, window=0, sinks=0, scale=None, softcap=None, slopes=None):
+        """Attention of the last T tokens of each row, q [BH, G, T, d] (float32, float16 or bfloat16, any strides), each
+        over the tokens up to its own: a prompt, a piece of one, or drafted tokens, once `write` or `write_rotated` has
+        their keys and values.  Token i of a row of `length` tokens stands at place p = length - T + i and sees tokens
+        t <= p, with a window only the last `window` of them and the first `sinks`.  Scores as in `attention`, with the
+        bias slopes[bh, g] (t - p).  [BH, G, T, d] in q's type; a token before the row's first (p < 0) gives zeros, so
+        rows of fewer than T tokens are padded in front."""
+        if q.device != self.device:
+            self._elsewhere(q)
+        shape = q.shape
+        if len(shape) != 4 or shape[0] != self.BH or shape[1] < 1 or shape[3] != self.d:
+            raise ValueError(f"q {tuple(shape)} must be [{self.BH}, G, T, {self.d}]")
+        scale, softcap, slopes = self._scores(shape, scale, softcap, slopes)
+        lens, lens_at, n = self._per_row(length, "length")
+        q, qr, qh, qt = _heads(q)
+        G, T = shape[1], shape[2]
+        window, sinks = max(min(int(window), _FAR), -1), max(min(int(sinks), _FAR), -1)
+        positions = n if lens is None else self.cap
+        positions = max(min(positions, window + T + -(-sinks // BLK) * BLK) if window > 0 else positions, 0)
+        ws, ws_at, nbytes = self._workspace("fathom_rows8_chunk_attention_workspace_bytes", G, positions, T)
+        out = torch.empty(shape, dtype=q.dtype, device=self.device)
+        self._call("fathom_rows8_chunk_attention", q.data_ptr(), _KDT[q.dtype], qr, qh, qt, *self._store(), self._code, self.BH, G, T,
+                   self.d, self.cap, lens_at, n, window, sinks, scale, softcap, None if slopes is None else slopes.data_ptr(),
+                   out.data_ptr(), ws_at, nbytes)
+        return out
+
+    def shared_attention(self, q, length, prefix, prefix_length, scale=None, softcap=None, slopes=None):
+        """`attention` for a batch whose sequences begin with the same tokens: `prefix`, a RowStore8 of H rows, holds
+        them once, this store's rows [B, H] hold what follows (`length` tokens, ints or integers [B H]).  Row (b, h) attends to
+        the first prefix_length (int, or integers [H]) tokens of the prefix's row h and then its own, in one
+        softmax; the prefix is read once for all B.  q [B H, G, d]; [B H, G, d] float32."""
+        if not isinstance(prefix, RowStore8) or prefix.device != self.device:
+            raise ValueError(f"the prefix must be a RowStore8 on {self.device}")
+        H = prefix.BH
+        if prefix.d != self.d or prefix._code != self._code or self.BH % H:
+            raise ValueError(f"a prefix of {H} rows of {prefix.d} {prefix.k8.dtype} codes does not fit {self.BH} rows of "
+                             f"{self.d} {self.k8.dtype}")
+        q, q_at, scale, softcap, slopes = self._query(q, scale, softcap, slopes)
+        lens, lens_at, n = self._per_row(length, "length")
+        plens, plens_at, pn = prefix._per_row(prefix_length, "prefix_length")
+        G = q.shape[1]
+        bits = [max(min(v, _FAR), 1) - 1 for v in (pn if plens is None else prefix.cap, n if lens is None else self.cap)]
+        key = "shared", H, self.BH, G, self.d, bits[0].bit_length(), bits[1].bit_length()
+        nbytes = _SIZES.get(key)
+        if nbytes is None:
+            nbytes = _SIZES[key] = _lib.lib().fathom_rows8_shared_attention_workspace_bytes(
+                H, self.BH // H, G, self.d, 1 << bits[0].bit_length(), 1 << bits[1].bit_length())
+        ws = torch.empty((nbytes,), dtype=torch.uint8, device=self.device)
+        out = torch.empty_like(q, dtype=_F32)
+        self._call("fathom_rows8_shared_attention", q_at, _KDT[q.dtype], *prefix._store(), H, prefix.cap, plens_at, pn,
+                   *self._store(), self._code, self.BH // H, G, self.d, self.cap, lens_at, n, scale, softcap,
+                   None if slopes is None else slopes.data_ptr(), out.data_ptr(), ws.data_ptr(), nbytes)
         return out

@@ -381,6 +381,30 @@ int fathom_rows8_write(const void *K, const void *V, int dtype, int64_t k_row_st
                        float *v_scale, void *stream);
 
 /*
+ * A layer's queries and keys on their way into the store: norms, position
+ * rotation and fathom_rows8_write's quantisation, in one launch.  q (element (bh,
+ * g, i, c) at bh * q_row_stride + g * q_head_stride + i * q_tok_stride + c), K and
+ * V as for fathom_rows8_write, all of dtype; every base and stride a multiple of 16
+ * bytes.  Token i of a row stands at position t = p + offset + i, with p as above
+ * and offset from offset[bh] (int32, device) or offset_value (within 32 bits)
+ * where offset is NULL.  Each head of q and K is divided by sqrt(mean(x^2) +
+ * eps) and multiplied by q_weight, k_weight [D] (of weight_dtype; NULL: no norm);
+ * channels c and c + rotated / 2, c < rotated / 2, are turned by the angle t *
+ * inv_freq[c] (inv_freq [rotated / 2] float32; rotated a multiple of 16, 0: no
+ * rotation), formed in float64: (x_c cos - x_{c + rotated/2} sin,
+ * x_{c + rotated/2} cos + x_c sin).  q_out [BH, G, T, D] and, unless NULL, k_out
+ * [BH, T, D] of dtype take the results; K's codes are made from the float32 values.
+ * Rows of `pos` that do not fit are rotated but not written.  T <= 2^27.
+ */
+int fathom_rows8_write_rotated(const void *q, const void *K, const void *V, int dtype, int64_t q_row_stride,
+                               int64_t q_head_stride, int64_t q_tok_stride, int64_t k_row_stride, int64_t k_tok_stride,
+                               int64_t v_row_stride, int64_t v_tok_stride, const int32_t *pos, int64_t pos_value,
+                               const int32_t *offset, int64_t offset_value, const float *inv_freq, int64_t rotated,
+                               const void *q_weight, const void *k_weight, int weight_dtype, float eps, int64_t BH,
+                               int64_t G, int64_t T, int64_t D, int64_t cap, int code_dtype, void *k8, void *v8,
+                               float *k_scale, float *v_scale, void *q_out, void *k_out, void *stream);
+
+/*
  * Values of R tokens per row, K, V [BH, R, D] of dtype (16-byte aligned): token
  * idx[bh, r] (int64, device) where idx is given, else pos[bh] + r (int32,
  * device), or pos_value + r where pos is NULL too.  Tokens outside [0, cap) give
@@ -416,6 +440,18 @@ int fathom_rows8_attention(const void *q, int q_dtype, const void *k8, const voi
                            const float *slopes, float *out, void *workspace, size_t workspace_bytes, void *stream);
 
 /*
+ * The same over the last `window` tokens and the first `sinks` ones, [0, min(sinks,
+ * len - window)): a layer that attends to its last tokens and keeps a few first
+ * ones visible.  Without a window every token takes part anyway.  The workspace is
+ * fathom_rows8_attention_workspace_bytes for window + sinks positions, sinks
+ * rounded up to a multiple of 64, or the longest length where that is less.
+ */
+int fathom_rows8_sink_attention(const void *q, int q_dtype, const void *k8, const void *v8, const float *k_scale,
+                                const float *v_scale, int code_dtype, int64_t BH, int64_t G, int64_t D, int64_t cap,
+                                const int32_t *lens, int64_t n, int64_t window, int64_t sinks, float scale, float softcap,
+                                const float *slopes, float *out, void *workspace, size_t workspace_bytes, void *stream);
+
+/*
  * The same attention over listed tokens, t = idx[bh, g, j] for j < k (int64,
  * device; a token listed twice counts twice).  Tokens outside [0, len) take no
  * part (fathom_gather_attention's zero rows score 0 instead).
@@ -427,6 +463,54 @@ int fathom_rows8_gather_attention(const void *q, int q_dtype, const int64_t *idx
                                   const float *k_scale, const float *v_scale, int code_dtype, int64_t BH, int64_t G,
                                   int64_t k, int64_t D, int64_t cap, const int32_t *lens, int64_t n, float scale,
                                   float softcap, const float *slopes, float *out, void *workspace,
+                                  size_t workspace_bytes, void *stream);
+
+/*
+ * Attention of the last T tokens of each row, each over what it sees: with len as
+ * above, query (bh, g, i) (at bh * q_row_stride + g * q_head_stride + i *
+ * q_tok_stride elements; base and strides multiples of 16 bytes) stands at place
+ * p = len - T + i of its row and sees tokens t <= p, with a window only those t >
+ * p - window and t < sinks.  Scores, cap, bias (slopes[bh, g] * (t - p)) as
+ * above; a query that sees nothing (p < 0) gives zeros.  out [BH, G, T, D] of
+ * q_dtype (16-byte aligned).  Queries take part exactly (channels below 2^-126 of
+ * their row's largest aside), scores and sums are float32.  With q_dtype
+ * FATHOM_DT_F32 a weight has 22 bits, else 11, down to 2^-34 of the largest weight
+ * times scale of V.
+ * G * T <= 65535 * 32.
+ * workspace: fathom_rows8_chunk_attention_workspace_bytes(BH, G, T, D, positions)
+ * bytes, 16-byte aligned, positions = the longest length the host knows, or with a
+ * window the smaller of that and window + T + sinks, sinks rounded up to a multiple
+ * of 64.  The query never falls as positions grow.
+ */
+size_t fathom_rows8_chunk_attention_workspace_bytes(int64_t BH, int64_t G, int64_t T, int64_t D, int64_t positions);
+int fathom_rows8_chunk_attention(const void *q, int q_dtype, int64_t q_row_stride, int64_t q_head_stride,
+                                 int64_t q_tok_stride, const void *k8, const void *v8, const float *k_scale,
+                                 const float *v_scale, int code_dtype, int64_t BH, int64_t G, int64_t T, int64_t D,
+                                 int64_t cap, const int32_t *lens, int64_t n, int64_t window, int64_t sinks, float scale,
+                                 float softcap, const float *slopes, void *out, void *workspace, size_t workspace_bytes,
+                                 void *stream);
+
+/*
+ * Attention of one token per row where the rows of a batch begin with the same
+ * tokens: row (s, h) of `sequences` x prefix_BH rows attends to the first
+ * prefix_lens[h] (or prefix_n) tokens of row h of the prefix's store and to the
+ * first lens[s, h] (or n) tokens of its own, as if they followed each other in one
+ * row.  The prefix is read once for all sequences.  q, out [sequences * prefix_BH,
+ * G, D] contiguous, out float32; both stores have the same D and code_dtype.
+ * Precision as fathom_rows8_chunk_attention's with a weight of 22 bits for the
+ * prefix, fathom_rows8_attention's for the rest.
+ * workspace: fathom_rows8_shared_attention_workspace_bytes(prefix_BH, sequences,
+ * G, D, prefix_positions, positions) bytes, 16-byte aligned, of the longest
+ * lengths that the host knows.  The query falls with neither.
+ */
+size_t fathom_rows8_shared_attention_workspace_bytes(int64_t prefix_BH, int64_t sequences, int64_t G, int64_t D,
+                                                     int64_t prefix_positions, int64_t positions);
+int fathom_rows8_shared_attention(const void *q, int q_dtype, const void *prefix_k8, const void *prefix_v8,
+                                  const float *prefix_k_scale, const float *prefix_v_scale, int64_t prefix_BH,
+                                  int64_t prefix_cap, const int32_t *prefix_lens, int64_t prefix_n, const void *k8,
+                                  const void *v8, const float *k_scale, const float *v_scale, int code_dtype,
+                                  int64_t sequences, int64_t G, int64_t D, int64_t cap, const int32_t *lens, int64_t n,
+                                  float scale, float softcap, const float *slopes, float *out, void *workspace,
                                   size_t workspace_bytes, void *stream);
 
 /*

@@ -125,3 +125,42 @@ def attention(q, K, V, toks, length, scale, softcap=0.0, slope=None):
     rel = 2 * dz + (len(toks) / 8 + 64) * U + 2.0 ** -20
     blocks = np.nan_to_num(np.abs(np.pad(V, ((0, -len(V) % BLK), (0, 0))))).reshape(-1, BLK * D).max(1)
     return w @ v, rel * weight + len(toks) * 2.0 ** -37 * (w * blocks[np.asarray(toks) // BLK]).max()
+
+
+def rotated(x, t, inv_freq, weight, eps=0.0):
+    """Rows x [..., T, D] at positions t [T] in float64: x / sqrt(mean(x^2) + eps) * weight (None: as they are), then
+    channels c and c + r / 2, r = 2 len(inv_freq), turned by t inv_freq[c]."""
+    x = np.asarray(x, np.float64)
+    if weight is not None:
+        x = x / np.sqrt((x ** 2).mean(-1, keepdims=True) + eps) * np.asarray(weight, np.float64)
+    half = len(inv_freq)
+    angle = np.asarray(t, np.float64)[:, None] * np.asarray(inv_freq, np.float64)
+    a, b = x[..., :half], x[..., half:2 * half]
+    return np.concatenate([a * np.cos(angle) - b * np.sin(angle), b * np.cos(angle) + a * np.sin(angle), x[..., 2 * half:]], -1)
+
+
+def sees(p, n, window=0, sinks=0):
+    """The tokens of [0, n) that a query at place p sees."""
+    t = np.arange(min(n, p + 1)) if p >= 0 else np.arange(0)
+    return t if window <= 0 else t[(t > p - window) | (t < sinks)]
+
+
+def many_attention(q, K, V, toks, length, scale, softcap=0.0, slope=None, weight_bits=22, parts=1):
+    """`attention` of one query that is one of many (chunk_attention, a shared prefix), with the bound of those kernels.
+
+    Their products are those of `parts` exact parts of the query, D each, in one chain, so D counts that many times; a score's
+    factor is rounded three times more.  A weight has `weight_bits` bits, and ends half of 2^-24 / 2^10 below the largest w
+    s, at the largest code, which is at most twice the largest |V| of its block."""
+    out, err = attention(q, K, V, toks, length, scale, softcap, slope)
+    if len(toks) == 0:
+        return out, err
+    k, v = K[toks], V[toks]
+    z = k @ q * scale
+    a = (np.abs(k) @ np.abs(q)).max() * abs(scale)
+    z = softcap * np.tanh(z / softcap) if softcap else z
+    z = z + (slope * (np.asarray(toks, np.float64) - (length - 1)) if slope is not None else 0.0)
+    w = np.exp(z - z.max())
+    w = w / w.sum()
+    blocks = np.nan_to_num(np.abs(np.pad(V, ((0, -len(V) % BLK), (0, 0))))).reshape(-1, BLK * V.shape[1]).max(1)
+    extra = 2 * ((parts - 1) * q.shape[0] + 4) * U * a + 2.0 ** -weight_bits
+    return out, err + extra * (w @ np.abs(v)) + len(toks) * 2.0 ** -34 * (w * blocks[np.asarray(toks) // BLK]).max()

@@ -1,0 +1,468 @@
+"""Chunk attention, shared prefixes and windows with sinks over the 8-bit K/V row store on the GPU, against the oracle in
+float64 within its bound of the kernels' arithmetic."""
+import numpy as np
+import pytest
+import torch
+
+from fathom_amd.rowstore8 import RowStore8
+from oracle import rows8_oracle as R
+from test_gpu_rows8 import BLK, CODES, DEV, _f32, _from_numpy, _rand
+
+pytestmark = pytest.mark.gpu
+HALF = {torch.float32: 2.0 ** -24, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}  # half a step of each type
+# half a step below each type's smallest normal number, where steps no longer shrink with the value: float16's are 2^-24
+FLOOR = {torch.float32: 2.0 ** -150, torch.float16: 2.0 ** -25, torch.bfloat16: 2.0 ** -134}
+BITS = {torch.float32: 22, torch.float16: 11, torch.bfloat16: 11}  # of a chunk's weights
+PARTS = {torch.float32: 3, torch.float16: 1, torch.bfloat16: 1}
+
+
+def _filled(BH, cap, D, code, seed=0, garbage_behind=None):
+    """A store whose blocks were written at once, its numpy copy; bytes and scales behind `garbage_behind` [BH] are of any kind."""
+    o = {"k8": np.zeros((BH, cap, D), np.uint8), "v8": np.zeros((BH, cap, D), np.uint8)}
+    o["ks"], o["vs"] = np.zeros((2, BH, -(-cap // BLK)), np.float32)
+    R.write(o, _f32(_rand((BH, cap, D), seed + 1)), _f32(_rand((BH, cap, D), seed + 2)), 0, code)
+    if garbage_behind is not None:
+        rng = np.random.default_rng(seed + 3)
+        for b, n in enumerate(garbage_behind):
+            for c in ("k8", "v8"):
+                o[c][b, n:] = rng.integers(0, 256, (cap - n, D), dtype=np.uint8)
+            for s in ("ks", "vs"):
+                o[s][b, -(-n // BLK):] = np.nan
+    return _from_numpy(o, code), o
+
+
+def _values(o, code):
+    return R.values(o["k8"], o["ks"], code), R.values(o["v8"], o["vs"], code)
+
+
+def _check_chunk(got, q, o, code, lens, window=0, sinks=0, scale=None, softcap=0.0, slopes=None, every=1):
+    """got [BH, G, T, d] against the oracle, every `every`-th token."""
+    BH, G, T, D = got.shape
+    K, V = _values(o, code)
+    scale = D ** -0.5 if scale is None else scale
+    got, half = got.double().cpu().numpy(), HALF[q.dtype]
+    qf = q.double().cpu().numpy()
+    for b in range(BH):
+        n = int(lens[b])
+        for i in range(0, T, every):
+            p = n - T + i
+            toks = R.sees(p, n, window, sinks)
+            for g in range(G):
+                ref, tol = R.many_attention(qf[b, g, i], K[b], V[b], toks, p + 1, scale, softcap,
+                                            None if slopes is None else float(slopes[b, g]), BITS[q.dtype], PARTS[q.dtype])
+                off = np.abs(got[b, g, i] - ref) - (tol + np.maximum((np.abs(ref) + tol) * half, FLOOR[q.dtype]))
+                assert (off <= 0).all(), f"row {b} head {g} token {i} (place {p} of {n}): {off.max():.3g} over {tol.max():.3g}"
+
+
+# ----------------------------------------------------------------------------- chunks
+@pytest.mark.parametrize("code", ["e4m3", "int8"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("G, T, lens", [(1, 1, [1, 64, 65]), (4, 8, [8, 0, 200]), (3, 43, [300, 43, 42]), (5, 131, [131, 333, 60])])
+def test_chunk(code, dtype, D, G, T, lens):
+    """One wave's tiles and four waves', whole and ragged, rows shorter than the chunk and empty ones."""
+    st, o = _filled(3, 333, D, code, garbage_behind=lens)
+    q = _rand((3 * G, T, D), 5, dtype).view(3, G, T, D)
+    got = st.chunk_attention(q.to(DEV), torch.tensor(lens, device=DEV))
+    assert got.dtype == dtype and got.shape == q.shape
+    _check_chunk(got, q, o, code, lens, every=3 if T > 20 else 1)
+
+
+@pytest.mark.parametrize("code, dtype, D", [("e4m3", torch.bfloat16, 128), ("int8", torch.float16, 64), ("e4m3", torch.float32, 64),
+                                            ("int8", torch.float32, 128)])
+@pytest.mark.parametrize("window, sinks", [(1, 0), (1, 1), (64, 4), (63, 64), (100, 65), (130, 200), (500, 3), (10 ** 9, 7), (7, 10 ** 9)])
+def test_chunk_windows_and_sinks(code, dtype, D, window, sinks):
+    G, T, n = 4, 70, 400
+    st, o = _filled(2, n, D, code, seed=3)
+    q = _rand((2 * G, T, D), 6, dtype).view(2, G, T, D)
+    got = st.chunk_attention(q.to(DEV), n, window=window, sinks=sinks)
+    _check_chunk(got, q, o, code, [n, n], window, sinks, every=5)
+    lens = [250, 90]
+    got = st.chunk_attention(q.to(DEV), torch.tensor(lens, device=DEV), window=window, sinks=sinks)
+    _check_chunk(got, q, o, code, lens, window, sinks, every=7)
+
+
+@pytest.mark.parametrize("code, dtype, D", [("e4m3", torch.bfloat16, 128), ("int8", torch.float32, 64)])
+@pytest.mark.parametrize("softcap, slopes, scale", [(30.0, False, None), (0.0, True, None), (5.0, True, 0.3), (2.0, False, -0.2),
+                                                    (0.0, False, 0.0), (0.0, True, -0.1), (1e-25, False, None), (1e29, False, None)])
+def test_chunk_caps_and_slopes(code, dtype, D, softcap, slopes, scale):
+    G, T, n = 3, 50, 300
+    st, o = _filled(2, n, D, code, seed=9)
+    q = _rand((2 * G, T, D), 7, dtype).view(2, G, T, D)
+    sl = 2.0 ** -torch.arange(1.0, 2 * G + 1).view(2, G) if slopes else None
+    got = st.chunk_attention(q.to(DEV), n, scale=scale, softcap=softcap, slopes=None if sl is None else sl.to(DEV))
+    cap = softcap if softcap < 1e27 else 0.0
+    _check_chunk(got, q, o, code, [n, n], scale=scale, softcap=max(cap, 2.0 ** -64) if cap else 0.0, slopes=sl, every=4)
+    if sl is not None:
+        for shaped in (sl[0], sl[:, :1].double()):  # [G]; a view that expands
+            one = st.chunk_attention(q.to(DEV), n, scale=scale, softcap=softcap, slopes=shaped.to(DEV))
+            _check_chunk(one, q, o, code, [n, n], scale=scale, softcap=softcap, slopes=shaped.expand(2, G), every=25)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("BH, G, T, n", [(1, 1, 1, 40000), (2, 4, 3, 20011), (1, 7, 40, 9000), (3, 2, 8, 4097)])
+def test_chunk_in_splits(dtype, BH, G, T, n):
+    """Few queries over long rows: the row is shared out over workgroups and joined."""
+    st, o = _filled(BH, n, 128, "e4m3", seed=11)
+    q = _rand((BH * G, T, 128), 8, dtype).view(BH, G, T, 128)
+    _check_chunk(st.chunk_attention(q.to(DEV), n), q, o, "e4m3", [n] * BH, every=9)
+    lens = [n - 5000 * b if b else 70 for b in range(BH)]
+    got = st.chunk_attention(q.to(DEV), torch.tensor(lens, device=DEV))
+    _check_chunk(got, q, o, "e4m3", lens, every=9)
+    lens = [0] * BH
+    assert not st.chunk_attention(q.to(DEV), torch.tensor(lens, device=DEV)).any()
+
+
+def test_chunk_of_one_token_is_the_single_token_attention():
+    st, o = _filled(4, 700, 128, "int8", seed=21)
+    q = _rand((4 * 6, 1, 128), 9).view(4, 6, 128)
+    for n, w, s in ((700, 0, 0), (333, 100, 5), (64, 0, 0)):
+        one = st.attention(q.to(DEV), n, window=w, sinks=s).double()
+        many = st.chunk_attention(q.to(DEV)[:, :, None], n, window=w, sinks=s)[:, :, 0].double()
+        assert float((one - many).abs().max()) <= 1e-5 * float(one.abs().max())  # two float32 evaluations, each checked above
+
+
+def test_chunk_query_layouts():
+    """Token-major projections, padded heads, a shifted base, float64: the results of the plain layout, bit for bit."""
+    st, _ = _filled(2, 200, 64, "e4m3", seed=5)
+    q = _rand((2 * 4, 33, 64), 3, torch.bfloat16).view(2, 4, 33, 64).to(DEV)
+    ref = st.chunk_attention(q, 150)
+    token_major = q.permute(0, 2, 1, 3).contiguous().permute(0, 2, 1, 3)
+    padded = torch.zeros(2, 4, 33, 80, dtype=q.dtype, device=DEV)
+    padded[..., 8:72] = q
+    odd = torch.zeros(q.numel() + 1, dtype=q.dtype, device=DEV)[1:].view(q.shape).copy_(q)
+    strided = torch.zeros(2, 4, 33, 128, dtype=q.dtype, device=DEV)[..., ::2].copy_(q)
+    for x in (token_major, padded[..., 8:72], odd, strided, q.transpose(0, 1).contiguous().transpose(0, 1)):
+        assert torch.equal(x, q) and torch.equal(st.chunk_attention(x, 150), ref)
+    wide = st.chunk_attention(q.double(), 150)
+    assert wide.dtype == torch.float32 and torch.equal(wide, st.chunk_attention(q.float(), 150))
+    assert st.chunk_attention(q[:, :, :0], 150).shape == (2, 4, 0, 64)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_chunk_what_a_query_does_not_see_does_not_count(dtype):
+    """NaN codes, infinite and NaN scales in later tokens and between sinks and window leave a query as it is; the
+    queries that see them are NaN."""
+    G, T, n, D = 4, 100, 300, 128
+    st, o = _filled(1, n, D, "e4m3", seed=31)
+    q = _rand((G, T, D), 4, dtype).view(1, G, T, D).to(DEV)
+    clean = {w: st.chunk_attention(q, n, window=w, sinks=3) for w in (0, 64)}
+    at = 230  # place 230: queries from 30 on see it, with a window of 64 those from 30 to 93
+    for what in ("v", "k"):
+        bad, _ = _filled(1, n, D, "e4m3", seed=31)
+        codes = (bad.v8 if what == "v" else bad.k8).view(torch.uint8)
+        codes[0, at, 5] = 0x7F
+        codes[0, at, 77] = 0xFF
+        for w, last in ((0, T), (64, 94)):
+            got = bad.chunk_attention(q, n, window=w, sinks=3)
+            hit = torch.zeros(T, dtype=torch.bool, device=DEV)
+            hit[at - (n - T):last] = True
+            chans = torch.zeros(D, dtype=torch.bool, device=DEV)
+            chans[[5, 77]] = True
+            nan = (hit[:, None] & (chans if what == "v" else torch.ones_like(chans))).expand(1, G, T, D)
+            assert torch.equal(got.isnan(), nan)
+            assert torch.equal(got[~nan], clean[w][~nan])
+    for value in (float("inf"), float("nan")):  # scales of the block from 256: queries from 56 on see it
+        for s in ("k_scale", "v_scale"):
+            bad, _ = _filled(1, n, D, "e4m3", seed=31)
+            getattr(bad, s)[0, 4] = value
+            got = bad.chunk_attention(q, n)
+            assert torch.equal(got[:, :, :56], clean[0][:, :, :56])
+            # an infinite score of either sign, or NaN; those of -inf alone leave the other tokens' attention
+            dots = torch.matmul(q[0].double(), bad.k8[0, 256:].double().t().contiguous())
+            seen = torch.arange(n - 256, device=DEV) <= torch.arange(T, device=DEV)[:, None] - 56
+            finite = ((dots < 0) | ~seen).all(-1) if s == "k_scale" and value > 0 else ~seen.any(-1).expand(G, T)
+            assert torch.equal(got[0].isfinite().all(-1), finite)
+
+
+@pytest.mark.parametrize("code", ["e4m3", "int8"])
+def test_chunk_blocks_of_any_scale(code):
+    """Scales of K and V that differ by many powers of two, negative ones, zeros, weights far below the largest that carry the
+    output because the large one's values are small."""
+    G, T, n, D = 2, 40, 64 * 6, 128
+    _, o = _filled(2, n, D, code, seed=41)
+    o["vs"][0] *= np.float32(2.0) ** np.array([-90, 0, 30, -3, 0, 60], np.float32)
+    o["vs"][1] *= np.float32(2.0) ** np.array([60, 0, -30, 3, 0, -60], np.float32)
+    o["ks"][0, 1] *= -1
+    o["vs"][1, 2] *= -1
+    o["ks"][1, 3] = o["vs"][0, 1] = 0.0
+    o["vs"][1, 4] = np.float32(1e-42)
+    st = _from_numpy(o, code)
+    for dtype in (torch.bfloat16, torch.float32):
+        q = (_rand((2 * G, T, D), 8) * 4).to(dtype).view(2, G, T, D)
+        _check_chunk(st.chunk_attention(q.to(DEV), n), q, o, code, [n, n], every=3)
+    # one token takes nearly all of the weight and has no value
+    st, o = _filled(1, n, D, code, seed=43)
+    q = torch.zeros(1, 1, 3, D)
+    q[..., 0] = 1.0
+    o["k8"][0, :, 0] = 0
+    o["k8"][0, 0, 0] = R.encode(np.array([100.0]), code)[0]
+    o["ks"][0] = 1.0
+    o["v8"][0, 0] = 0
+    st = _from_numpy(o, code)
+    for scale in (0.05, 0.15, 0.2):  # e^5, e^15, e^20 times the others' weight
+        for dtype in (torch.bfloat16, torch.float16, torch.float32):
+            _check_chunk(st.chunk_attention(q.to(dtype).to(DEV), n, scale=scale), q.to(dtype), o, code, [n], scale=scale)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_chunk_large_scores_and_queries_of_any_size(dtype):
+    """Scores of +-2^10 to 2^40 (one token takes all), queries whose channels span the type, rows of zeros."""
+    G, T, n, D = 2, 35, 200, 64
+    st, o = _filled(1, n, D, "e4m3", seed=51)
+    q = _rand((G, T, D), 2).view(1, G, T, D)
+    for power in (10, 20, 40):
+        big = (q * 2.0 ** power).to(dtype)
+        got = st.chunk_attention(big.to(DEV), n).double().cpu().numpy()
+        K, V = _values(o, "e4m3")
+        z = np.einsum("gtd,nd->gtn", big[0].double().numpy(), K[0]) * D ** -0.5
+        for g in range(G):
+            for i in range(T):
+                zz = np.sort(z[g, i, :n - T + i + 1])
+                if zz[-1] - zz[-2] < 40 + 2.0 ** -20 * abs(zz[-1]):
+                    continue  # the second largest counts too
+                ref = V[0][int(z[g, i, :n - T + i + 1].argmax())]
+                # the one weight as it is held, the value's product with it, the inverse of the sum and its product, the result
+                assert np.allclose(got[0, g, i], ref, rtol=2.0 ** -BITS[dtype] + 4 * R.U + HALF[dtype], atol=1e-9)
+    assert np.isfinite(got).all()
+    tiny = q.clone()
+    tiny[0, 0] *= 1e-30
+    tiny[0, 0, :, 3] = 1.0
+    tiny[0, 1] = 0.0
+    tiny = tiny.to(dtype)
+    _check_chunk(st.chunk_attention(tiny.to(DEV), n), tiny, o, "e4m3", [n], every=4)
+    huge = (q.sign() * torch.finfo(dtype).max).to(dtype)
+    assert st.chunk_attention(huge.to(DEV), n, scale=1e-38).isfinite().all()
+
+
+# ----------------------------------------------------------------------------- windows with sinks, single tokens
+@pytest.mark.parametrize("code, D, G", [("e4m3", 128, 4), ("int8", 64, 12), ("int8", 128, 9)])
+@pytest.mark.parametrize("window, sinks, n", [(1, 1, 2), (64, 4, 333), (100, 64, 1000), (100, 65, 1000), (333, 300, 2000), (1500, 40, 2000),
+                                              (64, 1999, 2000), (2000, 5, 2000), (128, 10 ** 12, 1999)])
+def test_window_with_sinks(code, D, G, window, sinks, n):
+    st, o = _filled(3, 2000, D, code, seed=61, garbage_behind=[n, n, n])
+    K, V = _values(o, code)
+    q = _rand((3, G, D), 5)
+    sl = 2.0 ** -torch.arange(1.0, 3 * G + 1).view(3, G)
+    lens = [n, n // 2, 1]
+    for length, L in ((n, [n] * 3), (torch.tensor(lens, device=DEV), lens)):
+        for cap, slopes in ((0.0, None), (20.0, sl)):
+            got = st.attention(q.to(DEV), length, window=window, sinks=sinks, softcap=cap, slopes=None if slopes is None else slopes.to(DEV))
+            for b in range(3):
+                for g in range(G):
+                    ref, tol = R.attention(q[b, g].double().numpy(), K[b], V[b], R.sees(L[b] - 1, L[b], window, sinks), L[b], D ** -0.5, cap,
+                                           None if slopes is None else float(slopes[b, g]))
+                    assert (np.abs(got[b, g].double().cpu().numpy() - ref) <= tol).all(), (b, g)
+
+
+def test_window_with_sinks_in_splits():
+    st, o = _filled(2, 30000, 128, "e4m3", seed=62)
+    K, V = _values(o, "e4m3")
+    q = _rand((2, 3, 128), 5)
+    for n, window, sinks in ((30000, 9000, 8000), (25111, 20000, 70), (30000, 64, 29000)):
+        for length in (n, torch.tensor([n, n - 64], device=DEV)):
+            got = st.attention(q.to(DEV), length, window=window, sinks=sinks).double().cpu().numpy()
+            for b in range(2):
+                L = n if isinstance(length, int) else n - 64 * b
+                for g in range(3):
+                    ref, tol = R.attention(q[b, g].double().numpy(), K[b], V[b], R.sees(L - 1, L, window, sinks), L, 128 ** -0.5)
+                    assert (np.abs(got[b, g] - ref) <= tol).all()
+
+
+def test_sinks_leave_other_calls_as_they_are():
+    """No sinks, or sinks that the window reaches: the bits of the call without the argument."""
+    st, _ = _filled(2, 3000, 128, "e4m3", seed=63)
+    q = _rand((2, 4, 128), 5).to(DEV)
+    for n, window in ((3000, 0), (3000, 700), (100, 64), (3000, 3000)):
+        ref = st.attention(q, n, window=window)
+        assert torch.equal(ref, st.attention(q, n, window=window, sinks=0))
+        if not window or window >= n:
+            assert torch.equal(ref, st.attention(q, n, window=window, sinks=77))
+
+
+def test_tokens_between_sinks_and_window_do_not_count():
+    st, o = _filled(1, 1000, 128, "e4m3", seed=64)
+    q = _rand((1, 4, 128), 5).to(DEV)
+    ref = st.attention(q, 1000, window=100, sinks=10)
+    for c in (st.k8, st.v8):
+        c.view(torch.uint8)[0, 10:900] = 0x7F
+    for s in (st.k_scale, st.v_scale):
+        s[0, 1:14] = float("nan")  # blocks of tokens 64 .. 895
+    assert torch.equal(ref, st.attention(q, 1000, window=100, sinks=10))
+    many = st.chunk_attention(q[:, :, None], 1000, window=100, sinks=10)
+    assert many.isfinite().all()
+
+
+# ----------------------------------------------------------------------------- shared prefixes
+def _check_shared(got, q, o, po, code, lens, plens, scale=None, softcap=0.0, slopes=None, rows=None):
+    BH, G, D = q.shape
+    H = po["k8"].shape[0]
+    K, V = _values(o, code)
+    PK, PV = _values(po, code)
+    scale = D ** -0.5 if scale is None else scale
+    got, qf = got.double().cpu().numpy(), q.double().cpu().numpy()
+    for r in rows or range(BH):
+        n, P = int(lens[r]), int(plens[r % H])
+        # whole blocks, so that the bound's blocks are the stores'
+        pad = -P % BLK
+        k, v = (np.concatenate([p[r % H][:P], np.zeros((pad, D)), x[r][:n]]) for p, x in ((PK, K), (PV, V)))
+        toks = np.concatenate([np.arange(P), P + pad + np.arange(n)])
+        for g in range(G):
+            s = None if slopes is None else float(slopes[r, g])
+            bias = pad  # the padding is no distance: places are those of the joined row
+            if s is not None and pad:
+                k2, v2 = np.concatenate([PK[r % H][:P], K[r][:n]]), np.concatenate([PV[r % H][:P], V[r][:n]])
+                ref, tol = R.many_attention(qf[r, g], k2, v2, np.arange(P + n), P + n, scale, softcap, s, 22, PARTS[q.dtype])
+                tol = 2 * tol  # its blocks are shifted against the stores': one of them has parts of two
+            else:
+                ref, tol = R.many_attention(qf[r, g], k, v, toks, P + bias + n, scale, softcap, s, 22, PARTS[q.dtype])
+            off = np.abs(got[r, g] - ref) - tol
+            assert (off <= 0).all(), f"row {r} head {g}: {off.max():.3g} over {tol.max():.3g}"
+
+
+@pytest.mark.parametrize("code", ["e4m3", "int8"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("B, H, G, P, n", [(1, 1, 1, 1, 1), (3, 2, 4, 200, 70), (9, 1, 5, 777, 130), (4, 3, 12, 64, 64)])
+def test_shared(code, dtype, D, B, H, G, P, n):
+    lens = [(n * (i % 4)) // 3 for i in range(B * H)]  # some rows without tokens of their own
+    pst, po = _filled(H, P + 50, D, code, seed=71, garbage_behind=[P] * H)
+    st, o = _filled(B * H, n, D, code, seed=72, garbage_behind=lens)
+    q = _rand((B * H, G, D), 6, dtype)
+    got = st.shared_attention(q.to(DEV), torch.tensor(lens, device=DEV), pst, P)
+    assert got.dtype == torch.float32
+    _check_shared(got, q, o, po, code, lens, [P] * H)
+    same = st.shared_attention(q.to(DEV), torch.tensor(lens, device=DEV), pst, torch.tensor([P] * H, device=DEV))
+    _check_shared(same, q, o, po, code, lens, [P] * H)
+
+
+@pytest.mark.parametrize("softcap, slopes, scale", [(20.0, True, None), (0.0, True, 0.2), (3.0, False, -0.1)])
+def test_shared_caps_and_slopes(softcap, slopes, scale):
+    B, H, G, D = 5, 2, 3, 128
+    lens, plens = [40, 0, 7, 64, 100, 3, 0, 0, 99, 1], [130, 64]
+    pst, po = _filled(H, 192, D, "int8", seed=73)
+    st, o = _filled(B * H, 100, D, "int8", seed=74)
+    q = _rand((B * H, G, D), 6)
+    sl = 2.0 ** -torch.arange(1.0, B * H * G + 1).fmod(9).view(B * H, G) if slopes else None
+    got = st.shared_attention(q.to(DEV), torch.tensor(lens, device=DEV), pst, torch.tensor(plens, device=DEV), scale=scale, softcap=softcap,
+                              slopes=None if sl is None else sl.to(DEV))
+    _check_shared(got, q, o, po, "int8", lens, plens, scale, softcap, sl)
+
+
+@pytest.mark.parametrize("B, H, G, P, n, dtype", [(2, 1, 4, 30000, 3000, torch.float32), (33, 2, 4, 5000, 40, torch.bfloat16),
+                                                  (70, 1, 1, 9999, 1200, torch.float16)])
+def test_shared_in_splits(B, H, G, P, n, dtype):
+    pst, po = _filled(H, P, 128, "e4m3", seed=75)
+    st, o = _filled(B * H, n, 128, "e4m3", seed=76)
+    q = _rand((B * H, G, 128), 6, dtype)
+    rows = list(range(0, B * H, max(1, B * H // 5)))
+    got = st.shared_attention(q.to(DEV), n, pst, P)
+    _check_shared(got, q, o, po, "e4m3", [n] * B * H, [P] * H, rows=rows)
+    lens = [n * i // (B * H) for i in range(B * H)]
+    got = st.shared_attention(q.to(DEV), torch.tensor(lens, device=DEV), pst, P)
+    _check_shared(got, q, o, po, "e4m3", lens, [P] * H, rows=rows)
+
+
+def test_shared_ends():
+    """No prefix is the attention over the row's own tokens, no own tokens that over the prefix; nothing gives zeros."""
+    st, _ = _filled(4, 300, 128, "e4m3", seed=77)
+    pst, _ = _filled(2, 300, 128, "e4m3", seed=78)
+    q = _rand((4, 4, 128), 6).to(DEV)
+    close = lambda a, b: float((a - b).abs().max()) <= 1e-5 * float(b.abs().max())  # noqa: E731
+    assert close(st.shared_attention(q, 300, pst, 0), st.attention(q, 300))
+    assert close(st.shared_attention(q, 0, pst, 222), torch.cat([pst.attention(q[2 * b:2 * b + 2], 222) for b in range(2)]))
+    assert not st.shared_attention(q, 0, pst, 0).any()
+    zero = torch.zeros(4, dtype=torch.int32, device=DEV)
+    assert not st.shared_attention(q, zero, pst, zero[:2]).any()
+
+
+# ----------------------------------------------------------------------------- calls
+def test_calls_repeat_bit_for_bit_on_any_stream():
+    st, _ = _filled(4, 5000, 128, "e4m3", seed=81)
+    pst, _ = _filled(2, 5000, 128, "e4m3", seed=82)
+    q4 = _rand((8, 8, 128), 6, torch.bfloat16).view(4, 2, 8, 128).to(DEV)
+    q3 = q4[:, :, 0].contiguous()
+    calls = [lambda: st.chunk_attention(q4, 5000), lambda: st.shared_attention(q3, 3000, pst, 5000),
+             lambda: st.attention(q3, 5000, window=900, sinks=70)]
+    torch.cuda.synchronize()
+    for f in calls:
+        ref = f()
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            other = f()
+        torch.cuda.current_stream().wait_stream(s)
+        assert torch.equal(ref, other) and torch.equal(ref, f())
+
+
+def test_captured_calls_follow_their_lengths():
+    """Graphs of each call, replayed in turn with lengths that change between replays, equal the eager calls."""
+    st, _ = _filled(4, 5000, 128, "e4m3", seed=83)
+    pst, _ = _filled(2, 3000, 128, "e4m3", seed=84)
+    q4 = _rand((8, 8, 128), 6, torch.bfloat16).view(4, 2, 8, 128).to(DEV)
+    q3 = q4[:, :, 0].contiguous()
+    lens = torch.full((4,), 5000, dtype=torch.int32, device=DEV)
+    plens = torch.full((2,), 3000, dtype=torch.int32, device=DEV)
+    calls = [lambda: st.chunk_attention(q4, lens), lambda: st.shared_attention(q3, lens, pst, plens),
+             lambda: st.attention(q3, lens, window=900, sinks=70), lambda: st.chunk_attention(q4, lens, window=333, sinks=4)]
+    for f in calls:
+        f()
+    torch.cuda.synchronize()
+    graphs = []
+    for f in calls:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = f()
+        graphs.append((g, out))
+    for L, P in (([5000, 1, 64, 0], [3000, 100]), ([7, 4999, 2500, 5000], [0, 1]), ([5000] * 4, [3000] * 2)):
+        lens.copy_(torch.tensor(L))
+        plens.copy_(torch.tensor(P))
+        for g, _ in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        for (g, out), f in zip(graphs, calls):
+            assert torch.equal(out, f())
+
+
+def test_offsets_past_32_bits():
+    """Rows of 2^24 + 100 tokens: codes of the second one begin past 2^31 bytes, its last tokens past 2^32."""
+    cap, D = (1 << 24) + 100, 128
+    st = RowStore8.empty(2, cap, torch.int8, D, DEV)
+    K, V = _rand((2, 300, D), 1, torch.bfloat16), _rand((2, 300, D), 2, torch.bfloat16)
+    st.write(K.to(DEV), V.to(DEV), cap - 300)
+    o = {"k8": np.zeros((2, 384, D), np.uint8), "v8": np.zeros((2, 384, D), np.uint8)}
+    o["ks"], o["vs"] = np.zeros((2, 2, 6), np.float32)
+    lead = (cap - 300) % BLK
+    R.write(o, _f32(K), _f32(V), lead, "int8")
+    n, window = lead + 300, 200
+    q = _rand((2 * 2, 20, D), 3, torch.bfloat16).view(2, 2, 20, D)
+    got = st.chunk_attention(q.to(DEV), cap, window=window)
+    _check_chunk(got, q, o, "int8", [n, n], window, every=3)
+    one = st.attention(q[:, :, -1].contiguous().to(DEV), cap, window=window, sinks=0)
+    assert float((one - got[:, :, -1].float()).abs().max()) <= 2.0 ** -7 * float(one.abs().max())
+
+
+def test_refusals():
+    st, _ = _filled(4, 100, 128, "e4m3")
+    other, _ = _filled(3, 100, 128, "e4m3")
+    ints, _ = _filled(2, 100, 128, "int8")
+    short, _ = _filled(2, 100, 64, "e4m3")
+    pst, _ = _filled(2, 100, 128, "e4m3")
+    q = torch.zeros(4, 2, 8, 128, dtype=torch.bfloat16, device=DEV)
+    q3 = q[:, :, 0].contiguous()
+    for bad in (q[:3], q[..., :64], q3, q[:, :0], q.cpu()):
+        with pytest.raises(ValueError):
+            st.chunk_attention(bad, 100)
+    for kw in (dict(length=101), dict(length=-1), dict(length=100, window=-1), dict(length=100, sinks=-1), dict(length=100, softcap=-1.0),
+               dict(length=torch.zeros(3, dtype=torch.int32, device=DEV)), dict(length=torch.zeros(4, device=DEV)), dict(length=1 << 63)):
+        with pytest.raises(ValueError):
+            st.chunk_attention(q, **kw)
+    with pytest.raises(ValueError):
+        st.attention(q3, 100, window=10, sinks=-1)
+    for prefix in (other, ints, short, None, q3):
+        with pytest.raises(ValueError):
+            st.shared_attention(q3, 100, prefix, 100)
+    for kw in (dict(length=101, prefix_length=5), dict(length=5, prefix_length=101), dict(length=5, prefix_length=-1),
+               dict(length=5, prefix_length=torch.zeros(4, dtype=torch.int32, device=DEV))):
+        with pytest.raises(ValueError):
+            st.shared_attention(q3, prefix=pst, **kw)

@@ -74,7 +74,7 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 // the score, so that the rows' sums are scaled anew only where a score has grown by 2^3 (a row's first blocks).
 // The largest weight times scale is held between 2^10 and 2^15, so f16 (to 2^-24) ends at 2^-34 of it.
 constexpr float kMost = 15.0f, kStart = 12.0f;
-constexpr float kLeastWeight = -100.0f;  // a block counts with that weight at least in the choice of its values' scale
+constexpr float kLeastWeight = -112.0f;  // a block counts with that weight at least in the choice of its values' scale: it stays finite
 
 __device__ __forceinline__ float power(float e) { return ldexpf(1.0f, (int)__builtin_amdgcn_fmed3f(e, -300.0f, 300.0f)); }
 
@@ -88,6 +88,32 @@ __device__ __forceinline__ uint32_t pair_bf16(uint32_t w) {
   } else {
     return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)w, 1.0f, HI));
   }
+}
+
+__device__ __forceinline__ uint32_t dword_of(uint32_t v, int) { return v; }
+__device__ __forceinline__ uint32_t dword_of(u32x2v v, int d) { return v[d]; }
+// The top bits of a dword's bytes that hold an e4m3 NaN (0x7F, 0xFF).
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u; }
+__device__ __forceinline__ void clear_nans(uint32_t &w) { w &= ~((nan_bytes(w) >> 7) * 0xFFu); }
+__device__ __forceinline__ void clear_nans(u32x2v &w) {
+  w[0] &= ~((nan_bytes(w[0]) >> 7) * 0xFFu);
+  w[1] &= ~((nan_bytes(w[1]) >> 7) * 0xFFu);
+}
+
+// tanh_any without a branch: the compiler would make one of its select, for every score by itself.
+__device__ __forceinline__ float tanh_both(float u) {
+  const float t = __builtin_amdgcn_exp2f(fabsf(u) * (-2.0f * kLog2e));
+  const float n = 1.0f - t, d = 1.0f + t, r = __builtin_amdgcn_rcpf(d);
+  float far = n * r;
+  far = fmaf(fmaf(-far, d, n), r, far);
+  const uint32_t near = fabsf(u) < 0.5f ? 0xFFFFFFFFu : 0u;
+  return __uint_as_float((__float_as_uint(tanh_small(u)) & near) | (__float_as_uint(copysignf(far, u)) & ~near));
+}
+
+// Two floats as f16, to nearest, and what that leaves of them.
+__device__ __forceinline__ f16x2 round16(float x, float y) {
+  typedef float f32x2v __attribute__((ext_vector_type(2)));
+  return __builtin_convertvector(f32x2v{x, y}, f16x2);
 }
 
 __device__ __forceinline__ void barrier_lds() {  // waits for LDS only: loads of the next tile stay on their way
@@ -114,7 +140,7 @@ __device__ __forceinline__ float other_half(float v) {  // of lane l ^ 32
 //   O^T += V^T p^T with the weights in the layout that the scores come in, which fixes the order of the tokens in the
 //     transposed V.  A weight is one f16 (PREC: two, 22 bits) of p s_V 2^-E, E the exponent of the largest p s_V so
 //     far, so that blocks of small values with large weights count fully.
-template <int D, bool I8, int QT, bool PREC, int W>
+template <int D, bool I8, int QT, bool PREC, bool EXTRA, int W>
 __global__ __launch_bounds__(W *kWave, 2) void multi_kernel(MultiArgs a) {
   constexpr bool kBf16 = QT != FATHOM_DT_F16;
   constexpr int kParts = QT == FATHOM_DT_F32 ? 3 : 1, kSteps = D / 16, kTiles = D / 32;
@@ -124,7 +150,7 @@ __global__ __launch_bounds__(W *kWave, 2) void multi_kernel(MultiArgs a) {
   constexpr int kItems = kBlk / 4 * D / kCh / kThreads;  // items per thread
   typedef typename std::conditional<kBf16, bf16x8, f16x8>::type frag;
   __shared__ __attribute__((aligned(16))) uint16_t kt[kBufs][kBlk * D], vt[kBufs][kBlk * D];
-  __shared__ int odd[kBufs];  // the last block (+ 1) in this buffer that holds a NaN in V
+  __shared__ int odd[2];  // the first and the last block that hold a NaN in V
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 31, half = lane >> 5;
   const int64_t r = blockIdx.x;
@@ -148,7 +174,7 @@ __global__ __launch_bounds__(W *kWave, 2) void multi_kernel(MultiArgs a) {
     lo = a.window > 0 && end > a.window ? end - a.window : 0;
   }
   const int from = a.sinks < lo ? a.sinks : lo;  // tokens of [from, lo) take no part
-  const float slope = !a.slopes ? 0.0f : a.slopes[a.shared ? (o_at * a.BH + r) * a.G + g : r * a.G + g] * kLog2e;
+  const float slope = !EXTRA || !a.slopes ? 0.0f : a.slopes[a.shared ? (o_at * a.BH + r) * a.G + g : r * a.G + g] * kLog2e;
   frag qf[kParts][kSteps];
   int ex = 0;
   {
@@ -182,7 +208,7 @@ __global__ __launch_bounds__(W *kWave, 2) void multi_kernel(MultiArgs a) {
     }
   }
   // the scores' factor, scale log2 e or scale / softcap, as a fraction and a power of two
-  float cm = a.softcap > 0.0f ? __builtin_amdgcn_fmed3f(a.scale / a.softcap, -3.0e38f, 3.0e38f) : a.scale * kLog2e;
+  float cm = EXTRA && a.softcap > 0.0f ? __builtin_amdgcn_fmed3f(a.scale / a.softcap, -3.0e38f, 3.0e38f) : a.scale * kLog2e;
   if (cm != 0.0f && fabsf(cm) < INFINITY) {
     int e;
     cm = frexpf(cm, &e);
@@ -210,9 +236,15 @@ __global__ __launch_bounds__(W *kWave, 2) void multi_kernel(MultiArgs a) {
     }
     ks_next = ksp[b];
     vs_next = vsp[b];
+    if (!(fabsf(vs_next) < INFINITY)) vs_next = 0.0f;  // counted behind the loop
+  };
+  auto mark = [&](int i) {
+    atomicMin(&odd[0], i);
+    atomicMax(&odd[1], i);
   };
   auto stage = [&](int buf, int i) {
     if (i >= last) return;
+    if (tid == 0 && !(fabsf(vsp[span.block(i)]) < INFINITY)) mark(i);
 #pragma unroll
     for (int x = 0; x < kKeys; ++x) {
       const int at = x * kThreads + tid, tok = at / (D / 16), piece = at % (D / 16);
@@ -233,7 +265,18 @@ __global__ __launch_bounds__(W *kWave, 2) void multi_kernel(MultiArgs a) {
       for (int h = 0; h < 2; ++h)
         *reinterpret_cast<u32x4 *>(row + 16 * ((2 * piece + h) ^ (tok & (D / 8 - 1)))) = u32x4{w[4 * h], w[4 * h + 1], w[4 * h + 2], w[4 * h + 3]};
     }
-    uint32_t nan = 0;
+    if constexpr (!I8) {  // a NaN in V is staged as 0, and counted behind the loop
+      uint32_t nan = 0;
+#pragma unroll
+      for (int x = 0; x < 4 * kItems; ++x)
+#pragma unroll
+        for (int d = 0; d < kCh / 4; ++d) nan |= nan_bytes(dword_of(vr[x / 4][x % 4], d));
+      if (__builtin_expect(nan != 0, 0)) {
+        mark(i);
+#pragma unroll
+        for (int x = 0; x < 4 * kItems; ++x) clear_nans(vr[x / 4][x % 4]);
+      }
+    }
 #pragma unroll
     for (int x = 0; x < kItems; ++x) {
       const int item = x * kThreads + tid, quad = item / (D / kCh), ch0 = item % (D / kCh) * kCh;
@@ -244,13 +287,7 @@ __global__ __launch_bounds__(W *kWave, 2) void multi_kernel(MultiArgs a) {
       for (int d = 0; d < kCh / 4; ++d) {
         uint32_t w[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          uint32_t c;
-          if constexpr (kCh == 8) c = vr[x][j][d];
-          else c = vr[x][j];
-          if constexpr (!I8) nan |= (c & 0x7F7F7F7Fu) + 0x01010101u;
-          w[j] = flip_sign<I8>(c);
-        }
+        for (int j = 0; j < 4; ++j) w[j] = flip_sign<I8>(dword_of(vr[x][j], d));
 #pragma unroll
         for (int p = 0; p < 2; ++p) {  // channels 4 d + 2 p, + 1
           const uint32_t ab = __builtin_amdgcn_perm(w[1], w[0], p ? 0x07030602u : 0x05010400u);
@@ -265,7 +302,6 @@ __global__ __launch_bounds__(W *kWave, 2) void multi_kernel(MultiArgs a) {
         }
       }
     }
-    if (!I8 && (nan & 0x80808080u)) odd[buf] = i + 1;
   };
 
   f32x16 o[kTiles];
@@ -275,44 +311,77 @@ __global__ __launch_bounds__(W *kWave, 2) void multi_kernel(MultiArgs a) {
     for (int e = 0; e < 16; ++e) o[d][e] = 0.0f;
   float base = kLowest, l = 0.0f, E = -1000.0f;
 
+  // Bit 16 x + e: whether the query sees token at + 32 x + 8 (e / 4) + e % 4.
+  auto seen_of = [&](int at) {
+    uint32_t seen = 0;
+#pragma unroll
+    for (int b = 0; b < 32; ++b) {
+      const int t = at + 32 * (b / 16) + 8 * (b % 16 / 4) + b % 4;
+      seen |= (t < end && (t >= lo || t < from) ? 1u : 0u) << b;
+    }
+    asm volatile("" : "+v"(seen));  // a register of the lane: as masks for every token it would fill the scalar ones
+    return seen;
+  };
   auto block = [&](int buf, int i, float ks, float vs) {
     const int t0 = span.block(i) * kBlk;
     if (!__any(t0 < end && (t0 + kBlk > lo || t0 < from))) return;
     const bool edge = !__all(t0 + kBlk <= end && (t0 >= lo || t0 + kBlk <= from));
-    // ---- scores
+    // ---- scores; operands are read four products ahead
     f32x16 s[2];
-    const char *kb = reinterpret_cast<const char *>(kt[buf]);
+    const char *kb = reinterpret_cast<const char *>(kt[buf]) + col * 2 * D;
+    frag kf[2][4];
+    auto keys = [&](int n) {  // of steps 4 n ..: tokens 32 (4 n / kSteps) ..
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {
+      for (int c = 0; c < 4; ++c) {
+        const int x = 4 * n / kSteps, piece = 2 * (4 * n % kSteps + c) + half;
+        kf[n & 1][c] = *reinterpret_cast<const frag *>(kb + 64 * D * x + 16 * (piece ^ (col & (D / 8 - 1))));
+      }
+    };
+    keys(0);
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
 #pragma unroll
       for (int e = 0; e < 16; ++e) s[x][e] = 0.0f;
-      const int tok = 32 * x + col;
 #pragma unroll
-      for (int c = 0; c < kSteps; ++c) {
-        const frag k = *reinterpret_cast<const frag *>(kb + tok * 2 * D + 16 * ((2 * c + half) ^ (tok & (D / 8 - 1))));
+    for (int n = 0; n < kSteps / 2; ++n) {
+      if (n + 1 < kSteps / 2) keys(n + 1);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
 #pragma unroll
         for (int p = kParts - 1; p >= 0; --p) {
-          if constexpr (kBf16) s[x] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k, qf[p][c], s[x], 0, 0, 0);
-          else s[x] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qf[p][c], s[x], 0, 0, 0);
+          const int x = 4 * n / kSteps, step = 4 * n % kSteps + c;
+          if constexpr (kBf16) s[x] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[n & 1][c], qf[p][step], s[x], 0, 0, 0);
+          else s[x] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[n & 1][c], qf[p][step], s[x], 0, 0, 0);
         }
-      }
     }
+    const char *vb = reinterpret_cast<const char *>(vt[buf]);
+    f16x8 vf[2][kTiles];
+    auto values = [&](int n) {  // of tokens 16 n ..
+#pragma unroll
+      for (int d = 0; d < kTiles; ++d) {
+        const int ch = 32 * d + col, piece = 2 * n + half;
+        vf[n & 1][d] = *reinterpret_cast<const f16x8 *>(vb + ch * 2 * kBlk + 16 * (piece ^ ((ch ^ ch >> 3) & 7)));
+      }
+    };
+    values(0);
     float f = ldexpf(fabsf(ks) * fabsf(cm), ex);
     // never infinite: a score of 0 has to stay one; nor 0 without a cap: a score of -inf has to stay one too
-    f = fabsf(ks) < INFINITY ? __builtin_amdgcn_fmed3f(f, a.softcap > 0.0f ? 0.0f : 1.2e-38f, 3.0e38f) : f;
+    f = fabsf(ks) < INFINITY ? __builtin_amdgcn_fmed3f(f, EXTRA && a.softcap > 0.0f ? 0.0f : 1.2e-38f, 3.0e38f) : f;
     if ((ks < 0.0f) != (cm < 0.0f)) {
+      asm volatile("");  // a branch, not selects in every block
 #pragma unroll
       for (int x = 0; x < 2; ++x) s[x] = -s[x];
     }
     const int at = t0 + 4 * half;  // register e of s[x] is token at + 32 x + 8 (e / 4) + e % 4
-    if (a.softcap > 0.0f) {
+    if (EXTRA && a.softcap > 0.0f) {
 #pragma unroll
       for (int x = 0; x < 2; ++x)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) s[x][e] = tanh_any(s[x][e] * f);
+        for (int e = 0; e < 16; ++e) s[x][e] = tanh_both(s[x][e] * f);
       f = a.softcap * kLog2e;
     }
-    if (a.slopes) {
+    if (EXTRA && a.slopes) {
       const float b = (float)(at - (end - 1)) - back;
 #pragma unroll
       for (int x = 0; x < 2; ++x)
@@ -320,21 +389,15 @@ __global__ __launch_bounds__(W *kWave, 2) void multi_kernel(MultiArgs a) {
         for (int e = 0; e < 16; ++e) s[x][e] = fmaf(s[x][e], f, slope * (b + (float)(32 * x + 8 * (e / 4) + e % 4)));
       f = 1.0f;
     }
-    uint32_t seen = 0xFFFFFFFFu;  // bit 16 x + e
     if (edge) {
-      seen = 0;
-#pragma unroll
-      for (int b = 0; b < 32; ++b) {
-        const int t = at + 32 * (b / 16) + 8 * (b % 16 / 4) + b % 4;
-        seen |= (t < end && (t >= lo || t < from) ? 1u : 0u) << b;
-      }
-      asm volatile("" : "+v"(seen));
+      const uint32_t seen = seen_of(at);
 #pragma unroll
       for (int b = 0; b < 32; ++b) s[b / 16][b % 16] = seen >> b & 1 ? s[b / 16][b % 16] : -INFINITY;
     }
     float mx = -INFINITY;
 #pragma unroll
-    for (int e = 0; e < 16; ++e) mx = fmaxf(mx, fmaxf(s[0][e], s[1][e]));
+    for (int e = 0; e < 16; ++e)  // NaN stays: its weights are NaN anyhow (fmaxf would first quieten every operand)
+      mx = __builtin_elementwise_maximum(__builtin_elementwise_maximum(mx, s[0][e]), s[1][e]);
     mx *= f;
     if (__any(fabsf(mx) >= kLarge && fabsf(mx) < INFINITY)) {
 #pragma unroll
@@ -343,7 +406,7 @@ __global__ __launch_bounds__(W *kWave, 2) void multi_kernel(MultiArgs a) {
     }
     const float ev = (float)((int)((__float_as_uint(vs) >> 23) & 0xFF) - 127);  // |s_V| < 2^(ev + 1)
     if (__any(mx - base > kMost || fmaxf(mx - base, kLeastWeight) + ev - (kMost - 1.0f) > E)) {
-      mx = fmaxf(mx, other_half(mx));
+      mx = __builtin_elementwise_maximum(mx, other_half(mx));
       const float to = mx - base > kMost ? floorf(mx) - kStart : base, up = to - base;
       const float most = ceilf(fmaxf(mx - to, kLeastWeight) + ev) - (kStart - 1.0f);
       const float was = E;
@@ -354,77 +417,69 @@ __global__ __launch_bounds__(W *kWave, 2) void multi_kernel(MultiArgs a) {
       for (int d = 0; d < kTiles; ++d) o[d] *= by;
       base = to;
     }
-    const float wv = ldexpf(vs, -(int)E);
-    const char *vb = reinterpret_cast<const char *>(vt[buf]);
-    auto values = [&](int d, int x, int c) {
-      const int ch = 32 * d + col, piece = 4 * x + 2 * c + half;
-      return *reinterpret_cast<const f16x8 *>(vb + ch * 2 * kBlk + 16 * (piece ^ ((ch ^ ch >> 3) & 7)));
-    };
-    // A NaN in V counts for the queries that see its token, and for no other: counted apart, it is no value there
-    const bool nans = !I8 && edge && odd[buf] == i + 1;
-    if (nans) {
-#pragma unroll 1
+    // ---- weights and products, 16 tokens at a time.  The factor of V goes into the exponent, and out of the sum again.
+    // A block's weights are added together first: alone, most would be lost beside a large sum.
+    const float wv = ldexpf(fabsf(vs), -(int)E);
+    // Where it is so small that weights which count in the sum would be lost in the products' operands, they are added apart;
+    // below 2^-64 all of those are 0: the block has no value to add.
+    const bool small = !(wv >= (PREC ? 0x1p-64f : 0x1p-6f)), none = !(wv >= 0x1p-64f);
+    if (__builtin_expect(__any(small), 0)) {
+      float sum = 0.0f;
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) sum += __builtin_amdgcn_exp2f(fmaf(s[x][e], f, -base));
+      l += small ? sum : 0.0f;
+      if (__all(none)) return;
+    }
+    if (vs < 0.0f) {  // not written by this store's writer
+      asm volatile("");
+#pragma unroll
+      for (int d = 0; d < kTiles; ++d) o[d] = -o[d];
+    }
+    const float zero = none ? INFINITY : base - __builtin_amdgcn_logf(wv), back_by = small ? 0.0f : __builtin_amdgcn_rcpf(wv);
+    float sum = 0.0f;
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      if (n < 3) values(n + 1);
+      float w[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) w[e] = __builtin_amdgcn_exp2f(fmaf(s[n / 2][8 * (n % 2) + e], f, -zero));
+      f16x2 hi[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) hi[e] = round16(w[2 * e], w[2 * e + 1]);
+      if constexpr (PREC) {
+        sum += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+      } else {  // the weights as they are held, so that they divide out
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum = __builtin_amdgcn_fdot2(hi[e], f16x2{(_Float16)1.0f, (_Float16)1.0f}, sum, false);
+      }
+      const f16x8 p = join8(hi[0], hi[1], hi[2], hi[3]);
+      f16x8 rest;
+      if constexpr (PREC) {
+        f16x2 lo[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) lo[e] = round16(w[2 * e] - (float)hi[e].x, w[2 * e + 1] - (float)hi[e].y);
+        rest = join8(lo[0], lo[1], lo[2], lo[3]);
+      }
+#pragma unroll
       for (int d = 0; d < kTiles; ++d) {
-        f32x16 hits;
-#pragma unroll
-        for (int e = 0; e < 16; ++e) hits[e] = 0.0f;
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            const f16x8 v = values(d, x, c);
-            f16x8 is, sees;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              is[e] = v[e] != v[e] ? (_Float16)1.0f : (_Float16)0.0f;
-              sees[e] = seen >> (16 * x + 8 * c + e) & 1 ? (_Float16)1.0f : (_Float16)0.0f;
-            }
-            hits = __builtin_amdgcn_mfma_f32_32x32x16_f16(is, sees, hits, 0, 0, 0);
-          }
-#pragma unroll
-        for (int k = 0; k < kTiles; ++k)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) o[k][e] = k == d && hits[e] > 0.0f ? NAN : o[k][e];
+        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[n & 1][d], p, o[d], 0, 0, 0);
+        if constexpr (PREC) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[n & 1][d], rest, o[d], 0, 0, 0);
       }
     }
-    // ---- weights and products, 16 tokens at a time
+    l = fmaf(sum, back_by, l);
+    if (vs < 0.0f) {
+      asm volatile("");
 #pragma unroll
-    for (int x = 0; x < 2; ++x)
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        float w[8], ps[4];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) w[e] = __builtin_amdgcn_exp2f(fmaf(s[x][8 * c + e], f, -base));
-#pragma unroll
-        for (int e = 0; e < 4; ++e) ps[e] = w[2 * e] + w[2 * e + 1];  // added together first: alone, most weights
-        l += (ps[0] + ps[1]) + (ps[2] + ps[3]);                      // would be lost beside a large sum
-#pragma unroll
-        for (int e = 0; e < 8; ++e) w[e] *= wv;
-        if (edge) {  // a scale that is not finite counts only where its tokens are seen
-#pragma unroll
-          for (int e = 0; e < 8; ++e) w[e] = seen >> (16 * x + 8 * c + e) & 1 ? w[e] : 0.0f;
-        }
-        const f16x8 p = join8(split16(w[0], w[1], 0.0f), split16(w[2], w[3], 0.0f), split16(w[4], w[5], 0.0f), split16(w[6], w[7], 0.0f));
-        f16x8 rest;
-        if constexpr (PREC)
-          rest = join8(split16(w[0], w[1], -1.0f), split16(w[2], w[3], -1.0f), split16(w[4], w[5], -1.0f), split16(w[6], w[7], -1.0f));
-#pragma unroll
-        for (int d = 0; d < kTiles; ++d) {
-          f16x8 v = values(d, x, c);
-          if (nans) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = v[e] != v[e] ? (_Float16)0.0f : v[e];
-          }
-          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, p, o[d], 0, 0, 0);
-          if constexpr (PREC) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, rest, o[d], 0, 0, 0);
-        }
-      }
+      for (int d = 0; d < kTiles; ++d) o[d] = -o[d];
+    }
   };
 
-  if (tid < kBufs) odd[tid] = 0;
+  if (tid < 2) odd[tid] = tid ? -1 : 0x7FFFFFFF;
   load(first);
   float ks = ks_next, vs = vs_next;
-  barrier_lds();  // `odd` is cleared before a thread sets it
+  barrier_lds();  // `odd` is set before a thread changes it
   stage(0, first);
   load(first + 1);
   barrier_lds();
@@ -437,6 +492,38 @@ __global__ __launch_bounds__(W *kWave, 2) void multi_kernel(MultiArgs a) {
     stage(kBufs == 2 ? buf ^ 1 : 0, i + 1);
     load(i + 2);
     barrier_lds();
+  }
+
+  // A NaN in V makes the results of the queries that see its token NaN in its channel, and no others; a scale of V that is
+  // not finite in every channel.  Of the blocks between the first and the last that hold such, the product of what is NaN and
+  // what is seen says where.
+  if (__builtin_expect(odd[1] >= 0, 0)) {
+#pragma unroll 1
+    for (int i = odd[0]; i <= odd[1]; ++i) {
+      const int at = span.block(i) * kBlk + 4 * half;
+      const uint32_t seen = seen_of(at);
+      const bool whole = !(fabsf(vsp[span.block(i)]) < INFINITY);
+#pragma unroll
+      for (int d = 0; d < kTiles; ++d) {
+        f32x16 hits;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) hits[e] = 0.0f;
+#pragma unroll 1
+        for (int b = 0; b < 32; b += 8) {
+          f16x8 is, sees;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const int t = at + 2 * b + 8 * (e / 4) + e % 4;
+            const uint32_t c = t < span.end ? a.v8[(r * a.cap + t) * D + 32 * d + col] : 0u;
+            is[e] = whole || (!I8 && (c & 0x7F) == 0x7F) ? (_Float16)1.0f : (_Float16)0.0f;
+            sees[e] = seen >> (b + e) & 1 ? (_Float16)1.0f : (_Float16)0.0f;
+          }
+          hits = __builtin_amdgcn_mfma_f32_32x32x16_f16(is, sees, hits, 0, 0, 0);
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[d][e] = hits[e] > 0.0f ? NAN : o[d][e];
+      }
+    }
   }
 
   l += other_half(l);
@@ -476,11 +563,16 @@ __global__ __launch_bounds__(W *kWave, 2) void multi_kernel(MultiArgs a) {
     }
 }
 
-template <int D, bool I8, int QT, bool PREC>
+template <int D, bool I8, int QT, bool PREC, bool EXTRA>
 void launch_multi(const MultiArgs &a, hipStream_t st) {
   const dim3 grid((unsigned)a.BH, (unsigned)a.tiles, (unsigned)a.nsplit);
-  if (a.rows == 32) multi_kernel<D, I8, QT, PREC, 1><<<grid, kWave, 0, st>>>(a);
-  else multi_kernel<D, I8, QT, PREC, 4><<<grid, 4 * kWave, 0, st>>>(a);
+  if (a.rows == 32) multi_kernel<D, I8, QT, PREC, EXTRA, 1><<<grid, kWave, 0, st>>>(a);
+  else multi_kernel<D, I8, QT, PREC, EXTRA, 4><<<grid, 4 * kWave, 0, st>>>(a);
+}
+template <int D, bool I8, int QT, bool PREC>
+void launch_multi(const MultiArgs &a, hipStream_t st) {
+  if (a.softcap > 0.0f || a.slopes) launch_multi<D, I8, QT, PREC, true>(a, st);
+  else launch_multi<D, I8, QT, PREC, false>(a, st);
 }
 template <int D, bool I8>
 void launch_multi(const MultiArgs &a, int q_dtype, hipStream_t st) {

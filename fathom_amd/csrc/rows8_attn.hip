@@ -241,14 +241,6 @@ struct VPiece<8> {
 __device__ __forceinline__ uint32_t dword_of(uint32_t v, int) { return v; }
 __device__ __forceinline__ uint32_t dword_of(VPiece<8>::type v, int d) { return v[d]; }
 
-// Of a query channel x (the head's largest in [2^12, 2^14)): whether two f16 may hold fewer than 19 bits
-// of it, and what they leave of such a one, times 2^38 (at most 2^13: they end at 2^-24).
-__device__ __forceinline__ bool small_channel(float x) { return fabsf(x) < 0x1p-6f && x != 0.0f; }
-__device__ __forceinline__ float rest_of(float x) {
-  const float left = x - (float)(_Float16)x;
-  return small_channel(x) ? ldexpf(left - (float)(_Float16)left, 38) : 0.0f;
-}
-
 // v + the value of the lane 8 columns away in the same row of 16 lanes (row_ror:8).
 __device__ __forceinline__ float add_other_half(float v) {
   return v + dpp<kXor8>(v);

@@ -138,6 +138,14 @@ __device__ __forceinline__ f16x2 split16(float x, float y, float keep) {
   return __builtin_convertvector(f32x2{fmaf((float)hi.x, keep, x), fmaf((float)hi.y, keep, y)}, f16x2);
 }
 
+// Of a query channel x (the head's largest in [2^12, 2^14)): whether two f16 may hold fewer than 19 bits
+// of it, and what they leave of such a one, times 2^38 (at most 2^13: they end at 2^-24).
+__device__ __forceinline__ bool small_channel(float x) { return fabsf(x) < 0x1p-6f && x != 0.0f; }
+__device__ __forceinline__ float rest_of(float x) {
+  const float left = x - (float)(_Float16)x;
+  return small_channel(x) ? ldexpf(left - (float)(_Float16)left, 38) : 0.0f;
+}
+
 // A caller's cap as the kernels take it, in a range where scale / softcap and its products stay normal: below
 // 2^-64 every weight is 1 either way, and above 2^90 (0: none) scores below 2^78 do not notice a cap.
 inline float kernel_cap(float softcap) {

@@ -17,10 +17,11 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(MultiArgs a, Tail ta
   __shared__ float4 acc[kGroups][kLanes];
   __shared__ float red[2][kWaves];
   const int tid = threadIdx.x, lane = tid % kLanes, grp = tid / kLanes;
-  const int64_t m = blockIdx.x, r = blockIdx.y, y = m / a.rows, g = m % a.G, o = m / a.G;
-  const int nb = tile_span(a, r, y * a.rows).nb, per = (nb + a.nsplit - 1) / a.nsplit;
-  const int own = per ? (nb + per - 1) / per : 0;  // splits that have blocks
-  const int64_t at = (r * a.tiles + y) * a.nsplit * a.rows + m % a.rows;
+  const int m = (int)blockIdx.x, y = m / a.rows;
+  const int64_t r = blockIdx.y, g = m % a.G, o = m / a.G;
+  const int2 from = a.where[r * a.tiles + y];
+  const int own = from.y;  // splits of the tile
+  const int64_t at = (int64_t)from.x * a.rows + m % a.rows;
   int more = 0;
   int64_t slot = 0;
   if (a.shared) {
@@ -83,13 +84,21 @@ void launch_join(const MultiArgs &a, const Tail &t, int out, hipStream_t st) {
 // Queries of a tile: one wave's, where a row has no more.
 int tile_rows(int64_t M) { return M <= 32 ? 32 : 128; }
 
-// Splits of what a tile sees, up to nb blocks: as many workgroups as are at work at once, each with a few blocks.
-int64_t tile_splits(int64_t BH, int64_t M, int64_t D, int64_t nb) {
+// Shares that tiles of up to nb blocks are cut into (at most that many and one per tile more); 0: a workgroup takes each tile.
+// `places` workgroups are at work at once (of 32 queries of D = 128 one per CU, else two).  Few tiles are cut so that all places
+// have the same to do.  So are tiles that see very different lengths (`even` is false), up to twice the places, in rounds of
+// shares of a quarter of the mean and less; more tiles even out by themselves, those that see most first.
+int64_t tile_shares(int64_t BH, int64_t M, int64_t D, int64_t nb, bool even) {
   const int rows = tile_rows(M);
-  const int64_t tiles = BH * cdiv(M, (int64_t)rows), places = rows == 32 ? (D == 128 ? 1280 : 2048) : 512;
-  const int64_t room = places / tiles, most = cdiv(nb, (int64_t)4);
-  const int64_t ns = room < most ? room : most;
-  return ns < 1 ? 1 : ns;
+  const int64_t tiles = BH * cdiv(M, (int64_t)rows), places = rows == 32 && D == 128 ? 256 : 512;
+  if (nb <= 4 || tiles >= 2 * places || (even && tiles > places / 2)) return 0;
+  const int64_t rounds = cdiv(4 * tiles, places), shares = places * rounds - tiles, most = tiles * cdiv(nb, (int64_t)4);
+  return most < shares ? most : shares;
+}
+// The same for a prefix, whose tiles always leave partial results.
+int64_t prefix_shares(int64_t BH, int64_t M, int64_t D, int64_t nb) {
+  const int64_t shares = tile_shares(BH, M, D, nb, true), tiles = BH * cdiv(M, (int64_t)tile_rows(M));
+  return shares > tiles ? shares : tiles;
 }
 
 // Blocks that a tile sees at most, of rows of up to n tokens.
@@ -100,19 +109,24 @@ int64_t tile_blocks(int64_t n, int64_t T, int64_t window, int64_t sinks) {
   return some < all ? some : all;
 }
 
-size_t multi_bytes(int64_t BH, int64_t M, int64_t D, int64_t ns) {
+// Bytes of the partial results of so many shares and of the tiles' slots.
+size_t multi_bytes(int64_t BH, int64_t M, int64_t D, int64_t shares) {
   const int rows = tile_rows(M);
-  return (size_t)(BH * cdiv(M, (int64_t)rows) * ns * rows * (D + 2)) * sizeof(float);
+  const int64_t tiles = BH * cdiv(M, (int64_t)rows);
+  return (size_t)((shares + tiles) * rows * (D + 2) + cdiv(2 * tiles, (int64_t)4) * 4) * sizeof(float);
 }
 
+// Whether a call takes so many queries: of a row at most 65535 tiles of 32, in all so many that a grid of two workgroups per
+// tile stays below 2^32 threads.
 bool queries_taken(int64_t BH, int64_t G, int64_t O) {
-  return O >= 1 && O <= kMaxCap && G <= kMaxTiles * 32 / O && BH * G * O <= (int64_t)1 << 40;
+  return O >= 1 && O <= kMaxCap && G <= kMaxTiles * 32 / O && BH * G * O <= (int64_t)1 << 27;
 }
 
 void place(MultiArgs &a, void *workspace, int64_t D) {
-  const int64_t rows = a.BH * a.tiles * a.nsplit * a.rows;
+  const int64_t rows = (a.shares + a.BH * a.tiles) * a.rows;
   a.part = static_cast<float *>(workspace);
   a.ml = reinterpret_cast<float2 *>(a.part + rows * D);
+  a.where = reinterpret_cast<int2 *>(a.ml + rows);
 }
 
 int run_multi(const MultiArgs &a, int q_dtype, int64_t D, bool i8, hipStream_t st) {
@@ -139,8 +153,8 @@ using namespace fathom::rows8;
 extern "C" size_t fathom_rows8_chunk_attention_workspace_bytes(int64_t BH, int64_t G, int64_t T, int64_t D, int64_t positions) {
   if (!shape_taken(BH, G, D) || !queries_taken(BH, G, T) || positions < 1) return 0;
   if (positions > kMaxCap) positions = kMaxCap;
-  const int64_t ns = tile_splits(BH, G * T, D, cdiv(positions, (int64_t)kBlk) + 1);
-  return ns > 1 ? multi_bytes(BH, G * T, D, ns) : 0;
+  const int64_t shares = tile_shares(BH, G * T, D, cdiv(positions, (int64_t)kBlk) + 1, false);
+  return shares ? multi_bytes(BH, G * T, D, shares) : 0;
 }
 
 extern "C" int fathom_rows8_chunk_attention(const void *q, int q_dtype, int64_t q_row_stride, int64_t q_head_stride,
@@ -156,7 +170,7 @@ extern "C" int fathom_rows8_chunk_attention(const void *q, int q_dtype, int64_t 
   if (T == 0) return FATHOM_OK;
   rc = check_query(what, q, q_dtype, G, cap, lens, n, softcap, out);
   if (rc) return rc;
-  if (!queries_taken(BH, G, T)) return fail(FATHOM_ERR_INVALID, "%s: G=%lld T=%lld, at most %lld queries per row", what, (long long)G, (long long)T, (long long)kMaxTiles * 32);
+  if (!queries_taken(BH, G, T)) return fail(FATHOM_ERR_INVALID, "%s: G=%lld T=%lld, at most %lld queries per row and 2^27 in all", what, (long long)G, (long long)T, (long long)kMaxTiles * 32);
   if (window < 0) return fail(FATHOM_ERR_INVALID, "%s: window %lld", what, (long long)window);
   if (sinks < 0) return fail(FATHOM_ERR_INVALID, "%s: sinks %lld", what, (long long)sinks);
   const int64_t size = q_dtype == FATHOM_DT_F32 ? 4 : 2;
@@ -166,11 +180,12 @@ extern "C" int fathom_rows8_chunk_attention(const void *q, int q_dtype, int64_t 
   if (sinks > cap) sinks = cap;
   MultiArgs a{q, q_row_stride, q_head_stride, q_tok_stride, (const uint8_t *)k8, (const uint8_t *)v8, k_scale, v_scale, cap,
               cdiv(cap, kBlk), lens, n, (int)G, (int)T, (int)window, (int)sinks, false, nullptr, 0, 0, BH, scale,
-              kernel_cap(softcap), slopes, out, nullptr, nullptr, 1, 1, tile_rows(G * T)};
+              kernel_cap(softcap), slopes, out, nullptr, nullptr, nullptr, 0, 1, tile_rows(G * T)};
   a.tiles = (int)cdiv(G * T, (int64_t)a.rows);
-  a.nsplit = (int)tile_splits(BH, G * T, D, tile_blocks(lens ? cap : n, T, window, sinks));
-  if (a.nsplit > 1) {
-    const size_t need = multi_bytes(BH, G * T, D, a.nsplit);
+  const int64_t most = lens ? cap : n;
+  a.shares = (int)tile_shares(BH, G * T, D, tile_blocks(most, T, window, sinks), window > 0 || most >= 4 * T);
+  if (a.shares) {
+    const size_t need = multi_bytes(BH, G * T, D, a.shares);
     if (!workspace || workspace_bytes < need)
       return fail(FATHOM_ERR_WORKSPACE, "%s: workspace %zu bytes, need %zu", what, workspace_bytes, need);
     if (reinterpret_cast<uintptr_t>(workspace) & 15)
@@ -178,7 +193,7 @@ extern "C" int fathom_rows8_chunk_attention(const void *q, int q_dtype, int64_t 
     place(a, workspace, D);
   }
   rc = run_multi(a, q_dtype, D, code_dtype == FATHOM_DT_I8, (hipStream_t)stream);
-  return rc || a.nsplit == 1 ? rc : run_join(a, Tail{}, q_dtype, D, (hipStream_t)stream);
+  return rc || !a.shares ? rc : run_join(a, Tail{}, q_dtype, D, (hipStream_t)stream);
 }
 
 extern "C" size_t fathom_rows8_shared_attention_workspace_bytes(int64_t prefix_BH, int64_t sequences, int64_t G, int64_t D,
@@ -186,8 +201,8 @@ extern "C" size_t fathom_rows8_shared_attention_workspace_bytes(int64_t prefix_B
   if (!shape_taken(prefix_BH, G, D) || !queries_taken(prefix_BH, G, sequences) || sequences > kMaxRows / prefix_BH) return 0;
   if (prefix_positions > kMaxCap) prefix_positions = kMaxCap;
   if (prefix_positions < 0) prefix_positions = 0;
-  const int64_t ns = tile_splits(prefix_BH, G * sequences, D, cdiv(prefix_positions, (int64_t)kBlk));
-  return multi_bytes(prefix_BH, G * sequences, D, ns) + tail_bytes(prefix_BH * sequences, G, D, positions < 0 ? 0 : positions);
+  const int64_t shares = prefix_shares(prefix_BH, G * sequences, D, cdiv(prefix_positions, (int64_t)kBlk));
+  return multi_bytes(prefix_BH, G * sequences, D, shares) + tail_bytes(prefix_BH * sequences, G, D, positions < 0 ? 0 : positions);
 }
 
 extern "C" int fathom_rows8_shared_attention(const void *q, int q_dtype, const void *prefix_k8, const void *prefix_v8,
@@ -209,13 +224,13 @@ extern "C" int fathom_rows8_shared_attention(const void *q, int q_dtype, const v
   if (!prefix_lens && (prefix_n < 0 || prefix_n > prefix_cap))
     return fail(FATHOM_ERR_INVALID, "%s: prefix length %lld outside [0, cap=%lld]", what, (long long)prefix_n, (long long)prefix_cap);
   if (!queries_taken(prefix_BH, G, sequences))
-    return fail(FATHOM_ERR_INVALID, "%s: %lld sequences, G=%lld, at most %lld queries per row", what, (long long)sequences, (long long)G, (long long)kMaxTiles * 32);
+    return fail(FATHOM_ERR_INVALID, "%s: %lld sequences, G=%lld, at most %lld queries per row and 2^27 in all", what, (long long)sequences, (long long)G, (long long)kMaxTiles * 32);
   MultiArgs a{q, G * D, D, prefix_BH * G * D, (const uint8_t *)prefix_k8, (const uint8_t *)prefix_v8, prefix_k_scale,
               prefix_v_scale, prefix_cap, cdiv(prefix_cap, kBlk), prefix_lens, prefix_n, (int)G, (int)sequences, 0, 0, true,
-              lens, n, cap, prefix_BH, scale, kernel_cap(softcap), slopes, out, nullptr, nullptr, 1, 1, tile_rows(G * sequences)};
+              lens, n, cap, prefix_BH, scale, kernel_cap(softcap), slopes, out, nullptr, nullptr, nullptr, 1, 1, tile_rows(G * sequences)};
   a.tiles = (int)cdiv(G * sequences, (int64_t)a.rows);
-  a.nsplit = (int)tile_splits(prefix_BH, G * sequences, D, cdiv(prefix_lens ? prefix_cap : prefix_n, (int64_t)kBlk));
-  const size_t first = multi_bytes(prefix_BH, G * sequences, D, a.nsplit);
+  a.shares = (int)prefix_shares(prefix_BH, G * sequences, D, cdiv(prefix_lens ? prefix_cap : prefix_n, (int64_t)kBlk));
+  const size_t first = multi_bytes(prefix_BH, G * sequences, D, a.shares);
   if (!workspace || workspace_bytes < first)
     return fail(FATHOM_ERR_WORKSPACE, "%s: workspace %zu bytes, need more than %zu", what, workspace_bytes, first);
   if (reinterpret_cast<uintptr_t>(workspace) & 15)

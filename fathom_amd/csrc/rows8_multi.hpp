@@ -31,9 +31,10 @@ struct MultiArgs {
   float scale, softcap;
   const float *slopes;  // [BH, G]; shared: [O, BH, G]
   void *out;            // [BH, G, O, D] of the queries' type; shared: written by the join, [O, BH, G, D] float32
-  float2 *ml;           // [BH, tiles, nsplit, rows of a tile] a split's (m, l)
-  float *part;          // [..., D] its weighted rows
-  int nsplit, tiles, rows;
+  float2 *ml;           // [slots, rows of a tile] a split's (m, l)
+  float *part;          // [slots, rows, D] its weighted rows
+  int2 *where;          // [BH, tiles] a tile's first slot and its splits; null: one workgroup takes a tile
+  int shares, tiles, rows;
 };
 
 // What a tile of `rows` queries from the first one m0 of row r sees: blocks [0, sink) and, `skip` blocks further, up to
@@ -42,15 +43,16 @@ struct TileSpan {
   int len, end, sink, skip, nb;
   __device__ __forceinline__ int block(int i) const { return i < sink ? i : i + skip; }
 };
-__device__ __forceinline__ TileSpan tile_span(const MultiArgs &a, int64_t r, int64_t m0) {
+__device__ __forceinline__ TileSpan tile_span(const MultiArgs &a, int64_t r, int m0) {
   TileSpan s;
   s.len = (int)row_length(a.lens, a.n, a.cap, r);
   int first = 0;  // the first token of the tile's windows
   s.end = s.len;
   if (!a.shared) {
-    const int64_t M = (int64_t)a.G * a.O, last = m0 + a.rows < M ? m0 + a.rows : M;
-    const int64_t lo = (int64_t)s.len - a.O + 1 + m0 / a.G - a.window;
-    const int64_t end = (int64_t)s.len - a.O + 1 + (last - 1) / a.G;
+    const int M = a.G * a.O, last = m0 + a.rows < M ? m0 + a.rows : M;
+    const int64_t place = (int64_t)s.len - a.O + 1;
+    const int64_t lo = place + (int)((unsigned)m0 / (unsigned)a.G) - a.window;
+    const int64_t end = place + (int)((unsigned)(last - 1) / (unsigned)a.G);
     s.end = end < 0 ? 0 : (int)end;
     first = a.window > 0 && lo > 0 ? (int)lo : 0;
   }
@@ -73,6 +75,8 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 // A weight is 2^(z - base), the base a whole number that is raised where a score passes it by kMost, to kStart below
 // the score, so that the rows' sums are scaled anew only where a score has grown by 2^3 (a row's first blocks).
 // The largest weight times scale is held between 2^10 and 2^15, so f16 (to 2^-24) ends at 2^-34 of it.
+constexpr int kMultiWaves = 4, kMultiThreads = kMultiWaves * kWave;
+constexpr uint32_t kLeastBlocks = 4;  // of a workgroup's share
 constexpr float kMost = 15.0f, kStart = 12.0f;
 constexpr float kLeastWeight = -112.0f;  // a block counts with that weight at least in the choice of its values' scale: it stays finite
 
@@ -128,42 +132,117 @@ __device__ __forceinline__ float other_half(float v) {  // of lane l ^ 32
   return __uint_as_float((threadIdx.x & 32) ? p[0] : p[1]);
 }
 
-// A workgroup of W waves takes a tile of 32 W queries of one row, or one split of what
-// they see; each wave has 32 of the queries.  The tile's queries are consecutive in (o, g), so
+// Four floats at element `at` of an output of type DT.
+template <int DT>
+__device__ __forceinline__ void store4(void *out, int64_t at, const float (&v)[4]) {
+  if constexpr (DT == FATHOM_DT_F32) {
+    *reinterpret_cast<float4 *>(static_cast<float *>(out) + at) = make_float4(v[0], v[1], v[2], v[3]);
+  } else {
+    const u32x2v w = {pack2<DT>(v[0], v[1]), pack2<DT>(v[2], v[3])};
+    *reinterpret_cast<u32x2v *>(static_cast<uint16_t *>(out) + at) = w;
+  }
+}
+
+// The part of a workgroup where tiles are shared out: its tile (of all rows'), split, the tile's splits (0: the call needs
+// no such workgroup) and blocks per split.
+struct Share {
+  int tile, split, active, per;
+};
+struct FindTile {
+  uint64_t total[kMultiWaves];
+  uint32_t wave[kMultiWaves];
+  int share[4];
+};
+// Every workgroup takes `per` blocks, so that the tile that sees most does not hold the call up: each sums all tiles'
+// blocks, which gives `per`, and finds its tile in the prefix sums of ceil(blocks / per).  Those are at most
+// `shares` + tiles, the grid.  A thread takes some tiles in a row; workgroup 0 writes down where all begin.
+__device__ __forceinline__ Share find_tile(const MultiArgs &a, int w, FindTile &sh) {
+  const int tid = threadIdx.x, wave = tid >> 6, n = (int)a.BH * a.tiles;
+  const int c = (n + kMultiThreads - 1) / kMultiThreads, i0 = tid * c;
+  auto blocks = [&](int i) {
+    const int r = i / a.tiles;
+    return i < n ? (uint32_t)tile_span(a, r, (i - r * a.tiles) * a.rows).nb : 0u;
+  };
+  uint64_t sum = 0;  // tiles of one row count its blocks each
+  for (int i = 0; i < c; ++i) sum += blocks(i0 + i);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
+  if ((tid & 63) == 0) sh.total[wave] = sum;
+  if (tid == 0) sh.share[2] = 0;
+  __syncthreads();
+  uint64_t total = 0;
+#pragma unroll
+  for (int v = 0; v < kMultiWaves; ++v) total += sh.total[v];
+  const uint64_t even = (total + a.shares - 1) / a.shares;
+  const uint32_t per = even > kLeastBlocks ? (uint32_t)even : kLeastBlocks;
+  uint32_t own = 0;
+  for (int i = 0; i < c; ++i) own += (blocks(i0 + i) + per - 1) / per;
+  uint32_t upto = wave_incl_scan_u32(own);
+  if ((tid & 63) == 63) sh.wave[wave] = upto;
+  __syncthreads();
+  for (int v = 0; v < wave; ++v) upto += sh.wave[v];
+  uint32_t at = upto - own;
+  if (w == 0 || ((uint32_t)w >= at && (uint32_t)w < upto))
+    for (int i = 0; i < c; ++i) {
+      const uint32_t act = (blocks(i0 + i) + per - 1) / per;
+      if ((uint32_t)w >= at && (uint32_t)w < at + act) {
+        sh.share[0] = i0 + i;
+        sh.share[1] = w - (int)at;
+        sh.share[2] = (int)act;
+      }
+      if (w == 0 && i0 + i < n) a.where[i0 + i] = make_int2((int)at, (int)act);
+      at += act;
+    }
+  __syncthreads();
+  return Share{__builtin_amdgcn_readfirstlane(sh.share[0]), __builtin_amdgcn_readfirstlane(sh.share[1]),
+               __builtin_amdgcn_readfirstlane(sh.share[2]), __builtin_amdgcn_readfirstlane((int)per)};
+}
+
+// A workgroup of four waves takes a tile of 128 queries of one row, or one split of what they see; each wave has 32 of the
+// queries.  Where a row has no more than 32 queries every wave has them all, and the waves take blocks in turn.  The tile's queries are consecutive in (o, g), so
 // that a chunk's tile is a few tokens of all heads.  Per 64-token block of the row:
 //   the codes are requested a block ahead, converted once per workgroup and kept in LDS as 16-bit
 //     numbers (exact): K by tokens, V transposed, both with their 16-byte pieces in an order
 //     that keeps the lanes' reads on different banks;
 //   S^T = K q^T (v_mfma_f32_32x32x16): lane l holds query l & 31 and 32 of the block's scores, so
-//     that maximum and sum need one exchange, between l and l ^ 32.  The queries are exact: bf16 and f16 in
-//     their own type, float32 as three bf16 parts; bf16 parts are taken from q 2^-e, e the exponent of the row's largest.
+//     that maximum and sum need one exchange, between l and l ^ 32.  bf16 and f16 queries are operands as they are (bf16
+//     ones times 2^-e, e the exponent of the query's largest channel); float32 ones are two f16, 22 bits, and where a wave has channels
+//     below 2^-18 of their query's largest, what is left of those takes a third product, times 2^38, first.
 //   O^T += V^T p^T with the weights in the layout that the scores come in, which fixes the order of the tokens in the
 //     transposed V.  A weight is one f16 (PREC: two, 22 bits) of p s_V 2^-E, E the exponent of the largest p s_V so
 //     far, so that blocks of small values with large weights count fully.
-template <int D, bool I8, int QT, bool PREC, bool EXTRA, int W>
-__global__ __launch_bounds__(W *kWave, 2) void multi_kernel(MultiArgs a) {
-  constexpr bool kBf16 = QT != FATHOM_DT_F16;
-  constexpr int kParts = QT == FATHOM_DT_F32 ? 3 : 1, kSteps = D / 16, kTiles = D / 32;
-  constexpr int kThreads = W * kWave, kBufs = W == 1 ? 1 : 2, kRows = 32 * W;
+template <int D, bool I8, int QT, bool PREC, bool EXTRA, int RW>
+__global__ __launch_bounds__(kMultiThreads, RW == 1 && D == 128 ? 1 : 2) void multi_kernel(MultiArgs a) {
+  constexpr bool kBf16 = QT == FATHOM_DT_BF16;
+  constexpr int kParts = QT == FATHOM_DT_F32 ? 2 : 1, kSteps = D / 16, kTiles = D / 32;
+  constexpr int kThreads = RW * kWave, kBufs = RW == 1 ? 1 : 2, kRows = 32 * RW;  // threads that share a block
+  constexpr int kGroups = kMultiWaves / RW;                                      // of them in a workgroup
   constexpr int kKeys = kBlk * D / 16 / kThreads;        // 16-byte pieces of K per thread
-  constexpr int kCh = D == 64 && W == 4 ? 4 : 8;         // channels of V per thread and item of four tokens
+  constexpr int kCh = D == 64 && RW == 4 ? 4 : 8;        // channels of V per thread and item of four tokens
   constexpr int kItems = kBlk / 4 * D / kCh / kThreads;  // items per thread
   typedef typename std::conditional<kBf16, bf16x8, f16x8>::type frag;
-  __shared__ __attribute__((aligned(16))) uint16_t kt[kBufs][kBlk * D], vt[kBufs][kBlk * D];
-  __shared__ int odd[2];  // the first and the last block that hold a NaN in V
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  __shared__ __attribute__((aligned(16))) uint16_t lds[kGroups][kBufs][2][kBlk * D];
+  __shared__ int odd[kGroups][2];  // the first and the last block that hold a NaN in V
+  __shared__ FindTile find;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int group = wave / RW, tid = threadIdx.x % kThreads;
   const int col = lane & 31, half = lane >> 5;
-  const int64_t r = blockIdx.x;
-  const int y = (int)(gridDim.y - 1 - blockIdx.y);  // the tiles that see most come first
-  const int64_t m0 = (int64_t)y * kRows, M = (int64_t)a.G * a.O;
+  Share share{(int)(gridDim.y - 1 - blockIdx.y), 0, 1, 0};  // the tiles that see most come first
+  int64_t r = blockIdx.x;
+  if (a.where) {  // uniform over the workgroup
+    share = find_tile(a, (int)blockIdx.x, find);
+    if (share.active == 0) return;
+    r = share.tile / a.tiles;
+    share.tile %= a.tiles;
+  }
+  const int m0 = share.tile * kRows, M = a.G * a.O;
   const TileSpan span = tile_span(a, r, m0);
-  const int per = (span.nb + a.nsplit - 1) / a.nsplit;
-  const int first = (int)blockIdx.z * per, last = first + per < span.nb ? first + per : span.nb;
-  if (blockIdx.z > 0 && first >= span.nb) return;
+  const int first = share.split * share.per;
+  const int last = share.split + 1 < share.active ? first + share.per : span.nb;
 
   // ---- the lane's query
-  const int64_t mine = m0 + 32 * wave + col, m = mine < M ? mine : M - 1;
-  const int64_t o_at = m / a.G, g = m % a.G;
+  const int mine = m0 + 32 * (wave % RW) + col, m = mine < M ? mine : M - 1;
+  const int64_t o_at = (unsigned)m / (unsigned)a.G, g = m - (int)o_at * a.G;
   int end = span.len, lo = 0;
   float back = 0.0f;  // the bias takes t - (end - 1) - back
   if (a.shared) {
@@ -177,36 +256,38 @@ __global__ __launch_bounds__(W *kWave, 2) void multi_kernel(MultiArgs a) {
   const float slope = !EXTRA || !a.slopes ? 0.0f : a.slopes[a.shared ? (o_at * a.BH + r) * a.G + g : r * a.G + g] * kLog2e;
   frag qf[kParts][kSteps];
   int ex = 0;
-  {
-    const int64_t at = r * a.q_row + g * a.q_head + o_at * a.q_out + 8 * half;
+  const int64_t q_at = r * a.q_row + g * a.q_head + o_at * a.q_out + 8 * half;
+  bool far = false;  // float32: some channel of the wave's queries is small, as small_channel has it
+  if constexpr (QT == FATHOM_DT_F16) {
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) qf[0][s] = *reinterpret_cast<const f16x8 *>(static_cast<const uint16_t *>(a.q) + q_at + 16 * s);
+  } else {
     float x[kSteps][8], big = 0.0f;
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
-      if constexpr (QT == FATHOM_DT_F16) {
-        qf[0][s] = *reinterpret_cast<const f16x8 *>(static_cast<const uint16_t *>(a.q) + at + 16 * s);
-      } else {
-        load8_q(a.q, QT, at + 16 * s, x[s]);
+      load8_q(a.q, QT, q_at + 16 * s, x[s]);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) big = fmaxf(big, fabsf(x[s][e]));
-      }
+      for (int e = 0; e < 8; ++e) big = fmaxf(big, fabsf(x[s][e]));
     }
-    if constexpr (kBf16) {
-      big = fmaxf(big, other_half(big));
-      if (big > 0.0f && big < INFINITY) frexpf(big, &ex);
+    big = fmaxf(big, other_half(big));
+    if (big > 0.0f && big < INFINITY) frexpf(big, &ex);
+    if constexpr (!kBf16) ex -= 14;  // the largest |q| of the query in [2^13, 2^14)
 #pragma unroll
-      for (int s = 0; s < kSteps; ++s)
+    for (int s = 0; s < kSteps; ++s)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          float v = ldexpf(x[s][e], -ex);
-#pragma unroll
-          for (int k = 0; k < kParts; ++k) {
-            const __bf16 b = (__bf16)v;
-            qf[k][s][e] = b;
-            v = fabsf(v) < INFINITY ? v - (float)b : 0.0f;
-          }
+      for (int e = 0; e < 8; ++e) {
+        const float v = ldexpf(x[s][e], -ex);
+        if constexpr (kBf16) {
+          qf[0][s][e] = (__bf16)v;
+        } else {
+          qf[0][s][e] = (_Float16)v;
+          qf[1][s][e] = (_Float16)(v - (float)(_Float16)v);
+          far |= small_channel(v);
         }
-    }
+      }
+    far = __any(far);
   }
+  const int exq = ex;
   // the scores' factor, scale log2 e or scale / softcap, as a fraction and a power of two
   float cm = EXTRA && a.softcap > 0.0f ? __builtin_amdgcn_fmed3f(a.scale / a.softcap, -3.0e38f, 3.0e38f) : a.scale * kLog2e;
   if (cm != 0.0f && fabsf(cm) < INFINITY) {
@@ -239,8 +320,8 @@ __global__ __launch_bounds__(W *kWave, 2) void multi_kernel(MultiArgs a) {
     if (!(fabsf(vs_next) < INFINITY)) vs_next = 0.0f;  // counted behind the loop
   };
   auto mark = [&](int i) {
-    atomicMin(&odd[0], i);
-    atomicMax(&odd[1], i);
+    atomicMin(&odd[group][0], i);
+    atomicMax(&odd[group][1], i);
   };
   auto stage = [&](int buf, int i) {
     if (i >= last) return;
@@ -260,7 +341,7 @@ __global__ __launch_bounds__(W *kWave, 2) void multi_kernel(MultiArgs a) {
           w[2 * e + 1] = __builtin_bit_cast(uint32_t, pair16<I8, true>(c));
         }
       }
-      char *row = reinterpret_cast<char *>(kt[buf]) + tok * 2 * D;
+      char *row = reinterpret_cast<char *>(lds[group][buf][0]) + tok * 2 * D;
 #pragma unroll
       for (int h = 0; h < 2; ++h)
         *reinterpret_cast<u32x4 *>(row + 16 * ((2 * piece + h) ^ (tok & (D / 8 - 1)))) = u32x4{w[4 * h], w[4 * h + 1], w[4 * h + 2], w[4 * h + 3]};
@@ -282,7 +363,7 @@ __global__ __launch_bounds__(W *kWave, 2) void multi_kernel(MultiArgs a) {
       const int item = x * kThreads + tid, quad = item / (D / kCh), ch0 = item % (D / kCh) * kCh;
       // tokens 4 quad ..: half (quad >> 1 & 1) of the piece that lane half quad & 1 reads for 16 tokens
       const int piece = (quad >> 3) * 4 + (quad >> 2 & 1) * 2 + (quad & 1);
-      char *base = reinterpret_cast<char *>(vt[buf]) + 8 * (quad >> 1 & 1);
+      char *base = reinterpret_cast<char *>(lds[group][buf][1]) + 8 * (quad >> 1 & 1);
 #pragma unroll
       for (int d = 0; d < kCh / 4; ++d) {
         uint32_t w[4];
@@ -328,7 +409,7 @@ __global__ __launch_bounds__(W *kWave, 2) void multi_kernel(MultiArgs a) {
     const bool edge = !__all(t0 + kBlk <= end && (t0 >= lo || t0 + kBlk <= from));
     // ---- scores; operands are read four products ahead
     f32x16 s[2];
-    const char *kb = reinterpret_cast<const char *>(kt[buf]) + col * 2 * D;
+    const char *kb = reinterpret_cast<const char *>(lds[group][buf][0]) + col * 2 * D;
     frag kf[2][4];
     auto keys = [&](int n) {  // of steps 4 n ..: tokens 32 (4 n / kSteps) ..
 #pragma unroll
@@ -337,11 +418,30 @@ __global__ __launch_bounds__(W *kWave, 2) void multi_kernel(MultiArgs a) {
         kf[n & 1][c] = *reinterpret_cast<const frag *>(kb + 64 * D * x + 16 * (piece ^ (col & (D / 8 - 1))));
       }
     };
-    keys(0);
 #pragma unroll
     for (int x = 0; x < 2; ++x)
 #pragma unroll
       for (int e = 0; e < 16; ++e) s[x][e] = 0.0f;
+    if constexpr (QT == FATHOM_DT_F32) {
+      if (__builtin_expect(far, 0)) {  // what two f16 leave of small channels, formed anew from the queries
+#pragma unroll 1
+        for (int c = 0; c < kSteps; ++c) {
+          float x[8];
+          load8_q(a.q, QT, q_at + 16 * c, x);
+          f16x8 left;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) left[e] = (_Float16)rest_of(ldexpf(x[e], -exq));
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const f16x8 k = *reinterpret_cast<const f16x8 *>(kb + 64 * D * h + 16 * ((2 * c + half) ^ (col & (D / 8 - 1))));
+            s[h] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, left, s[h], 0, 0, 0);
+          }
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) s[h] *= 0x1p-38f;
+      }
+    }
+    keys(0);
 #pragma unroll
     for (int n = 0; n < kSteps / 2; ++n) {
       if (n + 1 < kSteps / 2) keys(n + 1);
@@ -355,7 +455,7 @@ __global__ __launch_bounds__(W *kWave, 2) void multi_kernel(MultiArgs a) {
           else s[x] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[n & 1][c], qf[p][step], s[x], 0, 0, 0);
         }
     }
-    const char *vb = reinterpret_cast<const char *>(vt[buf]);
+    const char *vb = reinterpret_cast<const char *>(lds[group][buf][1]);
     f16x8 vf[2][kTiles];
     auto values = [&](int n) {  // of tokens 16 n ..
 #pragma unroll
@@ -476,30 +576,41 @@ __global__ __launch_bounds__(W *kWave, 2) void multi_kernel(MultiArgs a) {
     }
   };
 
-  if (tid < 2) odd[tid] = tid ? -1 : 0x7FFFFFFF;
-  load(first);
+  // Groups of one wave need no barrier: its LDS operations are in order.
+  auto sync = [&]() {
+    if constexpr (RW == 1) {
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
+      __builtin_amdgcn_wave_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
+    } else {
+      barrier_lds();
+    }
+  };
+  if (tid < 2) odd[group][tid] = tid ? -1 : 0x7FFFFFFF;
+  load(first + group);
   float ks = ks_next, vs = vs_next;
-  barrier_lds();  // `odd` is set before a thread changes it
-  stage(0, first);
-  load(first + 1);
-  barrier_lds();
-  for (int i = first; i < last; ++i) {
-    const int buf = kBufs == 2 ? (i - first) & 1 : 0;
+  sync();  // `odd` is set before a thread changes it
+  stage(0, first + group);
+  load(first + group + kGroups);
+  sync();
+  int buf = 0;
+  for (int i = first + group; i < last; i += kGroups) {
     block(buf, i, ks, vs);
     ks = ks_next;
     vs = vs_next;
-    if constexpr (kBufs == 1) barrier_lds();
-    stage(kBufs == 2 ? buf ^ 1 : 0, i + 1);
-    load(i + 2);
-    barrier_lds();
+    if constexpr (kBufs == 1) sync();
+    else buf ^= 1;
+    stage(buf, i + kGroups);
+    load(i + 2 * kGroups);
+    sync();
   }
 
   // A NaN in V makes the results of the queries that see its token NaN in its channel, and no others; a scale of V that is
   // not finite in every channel.  Of the blocks between the first and the last that hold such, the product of what is NaN and
   // what is seen says where.
-  if (__builtin_expect(odd[1] >= 0, 0)) {
+  if (__builtin_expect(odd[group][1] >= 0, 0)) {
 #pragma unroll 1
-    for (int i = odd[0]; i <= odd[1]; ++i) {
+    for (int i = odd[group][0]; i <= odd[group][1]; i += kGroups) {
       const int at = span.block(i) * kBlk + 4 * half;
       const uint32_t seen = seen_of(at);
       const bool whole = !(fabsf(vsp[span.block(i)]) < INFINITY);
@@ -527,10 +638,12 @@ __global__ __launch_bounds__(W *kWave, 2) void multi_kernel(MultiArgs a) {
   }
 
   l += other_half(l);
-  if (mine >= M) return;
-  if (a.nsplit > 1 || a.shared) {
-    const int64_t at = ((r * a.tiles + y) * a.nsplit + blockIdx.z) * kRows + 32 * wave + col;
-    if (half == 0) a.ml[at] = make_float2(base + kStart, ldexpf(l, -(int)kStart));
+  const bool parts = a.where != nullptr;
+  const int64_t slot = parts ? ((int64_t)blockIdx.x * kRows) : 0;
+  if constexpr (RW == 1) {  // ---- the waves' sums over their blocks, in the LDS that held those
+    __shared__ float wm[kMultiWaves][32], wl[kMultiWaves][32];
+    constexpr int kPitch = D + 4;
+    float *mine_at = reinterpret_cast<float *>(lds[group][0][0]) + col * kPitch + 4 * half;
 #pragma unroll
     for (int d = 0; d < kTiles; ++d)
 #pragma unroll
@@ -540,34 +653,71 @@ __global__ __launch_bounds__(W *kWave, 2) void multi_kernel(MultiArgs a) {
         v.y = ldexpf(o[d][e + 1], (int)(E - kStart));
         v.z = ldexpf(o[d][e + 2], (int)(E - kStart));
         v.w = ldexpf(o[d][e + 3], (int)(E - kStart));
-        *reinterpret_cast<float4 *>(a.part + at * D + 32 * d + 2 * e + 4 * half) = v;
+        *reinterpret_cast<float4 *>(mine_at + 32 * d + 2 * e) = v;
       }
+    if (half == 0) {
+      wm[wave][col] = base + kStart;
+      wl[wave][col] = ldexpf(l, -(int)kStart);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int x = threadIdx.x; x < 32 * D / 4; x += kMultiThreads) {
+      const int row = x / (D / 4), c = 4 * (x % (D / 4));
+      if (m0 + row >= M) break;
+      float big = wm[0][row];
+#pragma unroll
+      for (int v = 1; v < kMultiWaves; ++v) big = fmaxf(big, wm[v][row]);
+      float L = 0.0f, out[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int v = 0; v < kMultiWaves; ++v) {
+        const float f = __builtin_amdgcn_exp2f(wm[v][row] - big);
+        const float4 u = *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(lds[v][0][0]) + row * kPitch + c);
+        L = fmaf(wl[v][row], f, L);
+        out[0] = fmaf(u.x, f, out[0]);
+        out[1] = fmaf(u.y, f, out[1]);
+        out[2] = fmaf(u.z, f, out[2]);
+        out[3] = fmaf(u.w, f, out[3]);
+      }
+      if (parts) {
+        if (c == 0) a.ml[slot + row] = make_float2(big, L);
+        *reinterpret_cast<float4 *>(a.part + (slot + row) * D + c) = make_float4(out[0], out[1], out[2], out[3]);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) out[k] = L == 0.0f ? 0.0f : out[k] / L;
+        const int at_o = (unsigned)(m0 + row) / (unsigned)a.G, at_g = m0 + row - at_o * a.G;
+        store4<QT>(a.out, ((r * a.G + at_g) * a.O + at_o) * D + c, out);
+      }
+    }
     return;
   }
+  if (mine >= M) return;
+  const int row = 32 * wave + col;
+  if (parts && half == 0) a.ml[slot + row] = make_float2(base + kStart, ldexpf(l, -(int)kStart));
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  const int64_t at = ((r * a.G + g) * a.O + o_at) * D + 4 * half;
+  const int64_t out_at = ((r * a.G + g) * a.O + o_at) * D + 4 * half;
 #pragma unroll
   for (int d = 0; d < kTiles; ++d)
 #pragma unroll
     for (int e = 0; e < 16; e += 4) {
+      const int c = 32 * d + 2 * e;
       float v[4];
+      if (parts) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) v[k] = l == 0.0f ? 0.0f : ldexpf(o[d][e + k] * inv, (int)E);
-      const int64_t to = at + 32 * d + 2 * e;
-      if constexpr (QT == FATHOM_DT_F32) {
-        *reinterpret_cast<float4 *>(static_cast<float *>(a.out) + to) = make_float4(v[0], v[1], v[2], v[3]);
+        for (int k = 0; k < 4; ++k) v[k] = ldexpf(o[d][e + k], (int)(E - kStart));
+        *reinterpret_cast<float4 *>(a.part + (slot + row) * D + c + 4 * half) = make_float4(v[0], v[1], v[2], v[3]);
       } else {
-        const u32x2v w = {pack2<QT>(v[0], v[1]), pack2<QT>(v[2], v[3])};
-        *reinterpret_cast<u32x2v *>(static_cast<uint16_t *>(a.out) + to) = w;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = l == 0.0f ? 0.0f : ldexpf(o[d][e + k] * inv, (int)E);
+        store4<QT>(a.out, out_at + c, v);
       }
     }
 }
 
 template <int D, bool I8, int QT, bool PREC, bool EXTRA>
 void launch_multi(const MultiArgs &a, hipStream_t st) {
-  const dim3 grid((unsigned)a.BH, (unsigned)a.tiles, (unsigned)a.nsplit);
-  if (a.rows == 32) multi_kernel<D, I8, QT, PREC, EXTRA, 1><<<grid, kWave, 0, st>>>(a);
-  else multi_kernel<D, I8, QT, PREC, EXTRA, 4><<<grid, 4 * kWave, 0, st>>>(a);
+  const dim3 grid = a.where ? dim3((unsigned)(a.shares + a.BH * a.tiles)) : dim3((unsigned)a.BH, (unsigned)a.tiles);
+  if (a.rows == 32) multi_kernel<D, I8, QT, PREC, EXTRA, 1><<<grid, kMultiThreads, 0, st>>>(a);
+  else multi_kernel<D, I8, QT, PREC, EXTRA, 4><<<grid, kMultiThreads, 0, st>>>(a);
 }
 template <int D, bool I8, int QT, bool PREC>
 void launch_multi(const MultiArgs &a, hipStream_t st) {

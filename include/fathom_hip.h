@@ -472,11 +472,11 @@ int fathom_rows8_gather_attention(const void *q, int q_dtype, const int64_t *idx
  * p = len - T + i of its row and sees tokens t <= p, with a window only those t >
  * p - window and t < sinks.  Scores, cap, bias (slopes[bh, g] * (t - p)) as
  * above; a query that sees nothing (p < 0) gives zeros.  out [BH, G, T, D] of
- * q_dtype (16-byte aligned).  Queries take part exactly (channels below 2^-126 of
- * their row's largest aside), scores and sums are float32.  With q_dtype
+ * q_dtype (16-byte aligned).  bf16 and f16 queries take part exactly, float32 ones
+ * as fathom_rows8_attention's; scores and sums are float32.  With q_dtype
  * FATHOM_DT_F32 a weight has 22 bits, else 11, down to 2^-34 of the largest weight
  * times scale of V.
- * G * T <= 65535 * 32.
+ * G * T <= 65535 * 32, BH * G * T <= 2^27.
  * workspace: fathom_rows8_chunk_attention_workspace_bytes(BH, G, T, D, positions)
  * bytes, 16-byte aligned, positions = the longest length the host knows, or with a
  * window the smaller of that and window + T + sinks, sinks rounded up to a multiple
@@ -496,7 +496,8 @@ int fathom_rows8_chunk_attention(const void *q, int q_dtype, int64_t q_row_strid
  * prefix_lens[h] (or prefix_n) tokens of row h of the prefix's store and to the
  * first lens[s, h] (or n) tokens of its own, as if they followed each other in one
  * row.  The prefix is read once for all sequences.  q, out [sequences * prefix_BH,
- * G, D] contiguous, out float32; both stores have the same D and code_dtype.
+ * G, D] contiguous, out float32; both stores have the same D and code_dtype;
+ * sequences * G <= 65535 * 32, sequences * prefix_BH * G <= 2^27.
  * Precision as fathom_rows8_chunk_attention's with a weight of 22 bits for the
  * prefix, fathom_rows8_attention's for the rest.
  * workspace: fathom_rows8_shared_attention_workspace_bytes(prefix_BH, sequences,

@@ -216,6 +216,9 @@ __global__ __launch_bounds__(kMultiThreads, RW == 1 && D == 128 ? 1 : 2) void mu
   constexpr bool kBf16 = QT == FATHOM_DT_BF16;
   constexpr int kParts = QT == FATHOM_DT_F32 ? 2 : 1, kSteps = D / 16, kTiles = D / 32;
   constexpr int kThreads = RW * kWave, kBufs = RW == 1 ? 1 : 2, kRows = 32 * RW;  // threads that share a block
+  // operands read ahead: float32 queries take twice the registers (of 256; one more spilled register in the loop waits for all
+  // loads on their way)
+  constexpr int kAhead = kParts == 2 && D == 128 ? 2 : 4, kVBufs = kParts == 2 && D == 128 ? 1 : 2;
   constexpr int kGroups = kMultiWaves / RW;                                      // of them in a workgroup
   constexpr int kKeys = kBlk * D / 16 / kThreads;        // 16-byte pieces of K per thread
   constexpr int kCh = D == 64 && RW == 4 ? 4 : 8;        // channels of V per thread and item of four tokens
@@ -407,14 +410,14 @@ __global__ __launch_bounds__(kMultiThreads, RW == 1 && D == 128 ? 1 : 2) void mu
     const int t0 = span.block(i) * kBlk;
     if (!__any(t0 < end && (t0 + kBlk > lo || t0 < from))) return;
     const bool edge = !__all(t0 + kBlk <= end && (t0 >= lo || t0 + kBlk <= from));
-    // ---- scores; operands are read four products ahead
+    // ---- scores; operands are read kAhead products ahead
     f32x16 s[2];
     const char *kb = reinterpret_cast<const char *>(lds[group][buf][0]) + col * 2 * D;
-    frag kf[2][4];
-    auto keys = [&](int n) {  // of steps 4 n ..: tokens 32 (4 n / kSteps) ..
+    frag kf[2][kAhead];
+    auto keys = [&](int n) {  // of steps kAhead n ..: tokens 32 (kAhead n / kSteps) ..
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const int x = 4 * n / kSteps, piece = 2 * (4 * n % kSteps + c) + half;
+      for (int c = 0; c < kAhead; ++c) {
+        const int x = kAhead * n / kSteps, piece = 2 * (kAhead * n % kSteps + c) + half;
         kf[n & 1][c] = *reinterpret_cast<const frag *>(kb + 64 * D * x + 16 * (piece ^ (col & (D / 8 - 1))));
       }
     };
@@ -443,28 +446,28 @@ __global__ __launch_bounds__(kMultiThreads, RW == 1 && D == 128 ? 1 : 2) void mu
     }
     keys(0);
 #pragma unroll
-    for (int n = 0; n < kSteps / 2; ++n) {
-      if (n + 1 < kSteps / 2) keys(n + 1);
+    for (int n = 0; n < 2 * kSteps / kAhead; ++n) {
+      if (n + 1 < 2 * kSteps / kAhead) keys(n + 1);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int c = 0; c < 4; ++c)
+      for (int c = 0; c < kAhead; ++c)
 #pragma unroll
         for (int p = kParts - 1; p >= 0; --p) {
-          const int x = 4 * n / kSteps, step = 4 * n % kSteps + c;
+          const int x = kAhead * n / kSteps, step = kAhead * n % kSteps + c;
           if constexpr (kBf16) s[x] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[n & 1][c], qf[p][step], s[x], 0, 0, 0);
           else s[x] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[n & 1][c], qf[p][step], s[x], 0, 0, 0);
         }
     }
     const char *vb = reinterpret_cast<const char *>(lds[group][buf][1]);
-    f16x8 vf[2][kTiles];
+    f16x8 vf[kVBufs][kTiles];
     auto values = [&](int n) {  // of tokens 16 n ..
 #pragma unroll
       for (int d = 0; d < kTiles; ++d) {
         const int ch = 32 * d + col, piece = 2 * n + half;
-        vf[n & 1][d] = *reinterpret_cast<const f16x8 *>(vb + ch * 2 * kBlk + 16 * (piece ^ ((ch ^ ch >> 3) & 7)));
+        vf[n % kVBufs][d] = *reinterpret_cast<const f16x8 *>(vb + ch * 2 * kBlk + 16 * (piece ^ ((ch ^ ch >> 3) & 7)));
       }
     };
-    values(0);
+    if (kVBufs == 2) values(0);
     float f = ldexpf(fabsf(ks) * fabsf(cm), ex);
     // never infinite: a score of 0 has to stay one; nor 0 without a cap: a score of -inf has to stay one too
     f = fabsf(ks) < INFINITY ? __builtin_amdgcn_fmed3f(f, EXTRA && a.softcap > 0.0f ? 0.0f : 1.2e-38f, 3.0e38f) : f;
@@ -475,18 +478,38 @@ __global__ __launch_bounds__(kMultiThreads, RW == 1 && D == 128 ? 1 : 2) void mu
     }
     const int at = t0 + 4 * half;  // register e of s[x] is token at + 32 x + 8 (e / 4) + e % 4
     if (EXTRA && a.softcap > 0.0f) {
+      float big = 0.0f;
 #pragma unroll
       for (int x = 0; x < 2; ++x)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) s[x][e] = tanh_both(s[x][e] * f);
+        for (int e = 0; e < 16; ++e) {
+          s[x][e] *= f;
+          big = __builtin_elementwise_maximum(big, fabsf(s[x][e]));
+        }
+      if (__all(big < 0.5f)) {  // most blocks: scores well below the cap
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) s[x][e] = tanh_small(s[x][e]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 32; e += 4) {
+#pragma unroll
+          for (int k = e; k < e + 4; ++k) s[k / 16][k % 16] = tanh_both(s[k / 16][k % 16]);
+          if (e < 28)  // four after four: all at once would spill a hundred registers
+            asm volatile("" : "+v"(s[e / 16][e % 16]), "+v"(s[e / 16][e % 16 + 1]), "+v"(s[e / 16][e % 16 + 2]), "+v"(s[e / 16][e % 16 + 3]),
+                              "+v"(s[(e + 4) / 16][(e + 4) % 16]), "+v"(s[(e + 5) / 16][(e + 5) % 16]),
+                              "+v"(s[(e + 6) / 16][(e + 6) % 16]), "+v"(s[(e + 7) / 16][(e + 7) % 16]));
+        }
+      }
       f = a.softcap * kLog2e;
     }
     if (EXTRA && a.slopes) {
-      const float b = (float)(at - (end - 1)) - back;
+      const float b = slope * ((float)(at - (end - 1)) - back);
 #pragma unroll
       for (int x = 0; x < 2; ++x)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) s[x][e] = fmaf(s[x][e], f, slope * (b + (float)(32 * x + 8 * (e / 4) + e % 4)));
+        for (int e = 0; e < 16; ++e) s[x][e] = fmaf(s[x][e], f, fmaf((float)(32 * x + 8 * (e / 4) + e % 4), slope, b));
       f = 1.0f;
     }
     if (edge) {
@@ -541,7 +564,8 @@ __global__ __launch_bounds__(kMultiThreads, RW == 1 && D == 128 ? 1 : 2) void mu
     float sum = 0.0f;
 #pragma unroll
     for (int n = 0; n < 4; ++n) {
-      if (n < 3) values(n + 1);
+      if (kVBufs == 1) values(n);
+      else if (n < 3) values(n + 1);
       float w[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) w[e] = __builtin_amdgcn_exp2f(fmaf(s[n / 2][8 * (n % 2) + e], f, -zero));
@@ -564,8 +588,8 @@ __global__ __launch_bounds__(kMultiThreads, RW == 1 && D == 128 ? 1 : 2) void mu
       }
 #pragma unroll
       for (int d = 0; d < kTiles; ++d) {
-        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[n & 1][d], p, o[d], 0, 0, 0);
-        if constexpr (PREC) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[n & 1][d], rest, o[d], 0, 0, 0);
+        o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[n % kVBufs][d], p, o[d], 0, 0, 0);
+        if constexpr (PREC) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[n % kVBufs][d], rest, o[d], 0, 0, 0);
       }
     }
     l = fmaf(sum, back_by, l);

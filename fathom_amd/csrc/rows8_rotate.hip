@@ -6,8 +6,8 @@
 //   (y_c, y_{c + r/2}) = (a cos - b sin, b cos + a sin), a = x'_c, b = x'_{c + r/2}, angle t inv_freq[c], c < r / 2
 //   y_c = x'_c                                          for c >= r
 // for each query head and for K (the rotate-half convention of scripts/common.py:44-47); K's y and V
-// are quantised as rows8_write does.  All in float32 but the angle, which is formed and reduced to
-// [-pi, pi] in float64: t inv_freq is exact there up to 2^29 tokens.
+// are quantised as rows8_write does.  All in float32 but the angle, which is formed and reduced in
+// float64.
 #include "rows8.hpp"
 
 namespace fathom {
@@ -116,19 +116,27 @@ __device__ __forceinline__ void load_weights(const void *w, int dt, Pairs c, flo
   }
 }
 
-// cos and sin of position t for the thread's pairs.
+// cos and sin of position t for the thread's pairs: the angle in quarter turns n + f, |f| <= 1/2, in float64, then
+// x = f pi / 2 in float32 and sin x = x + x^3 P(x^2), cos x = 1 - x^2 / 2 + x^4 Q(x^2), P and Q least-squares fits of
+// degree 2 on |x| <= pi / 4, each off by less than a step of float32.
 __device__ __forceinline__ void turn_of(const RotateArgs &a, Pairs c, int64_t t, float (&cs)[8], float (&sn)[8]) {
-  constexpr double kPi = 3.14159265358979323846, kPiRest = 1.2246467991473532e-16;  // pi in two parts
+  constexpr double kQuarters = 0.63661977236758134308, kWhole = 6755399441055744.0;  // 2 / pi; 1.5 2^52: a sum's low bits are n
+  float inv[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) inv[i] = c.turned ? a.inv_freq[c.a + i] : 0.0f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    cs[i] = 1.0f;
-    sn[i] = 0.0f;
-    if (c.turned) {
-      const double angle = (double)t * (double)a.inv_freq[c.a + i];
-      const double n = 2.0 * rint(angle * (0.5 / kPi));
-      const double left = fma(-n, kPiRest, fma(-n, kPi, angle));
-      sincosf((float)left, &sn[i], &cs[i]);
-    }
+    const double q = (double)t * ((double)inv[i] * kQuarters), m = q + kWhole;
+    const uint32_t n = (uint32_t)__double2loint(m);
+    const float x = (float)(q - (m - kWhole)) * 1.57079632679489661923f, w = x * x;
+    float p = fmaf(w, -0.00019515919848345220f, 0.00833216588944196700f);
+    p = fmaf(p, w, -0.16666655242443085f);
+    const float s = fmaf(x * w, p, x);
+    float k = fmaf(w, 2.4435816158074886e-5f, -0.0013887340901419520f);
+    k = fmaf(k, w, 0.04166664555668831f);
+    k = fmaf(fmaf(k, w, -0.5f), w, 1.0f);
+    sn[i] = __uint_as_float(__float_as_uint(n & 1 ? k : s) ^ (n & 2) << 30);
+    cs[i] = __uint_as_float(__float_as_uint(n & 1 ? s : k) ^ ((n + 1) & 2) << 30);
   }
 }
 
@@ -166,11 +174,17 @@ __global__ __launch_bounds__(kThreads) void rotate_kernel(RotateArgs a) {
     load_weights(a.weight[0], a.weight_dtype, c, w);
     const int64_t i = (int64_t)((int)blockIdx.x - 2 * a.kv_blocks) * a.q_tokens + slot % a.q_tokens;
     if (i >= a.T) return;  // whole rows' lanes
+    const int64_t step = L::kSlots / a.q_tokens, at = bh * a.q_row + i * a.q_tok;
+    int64_t g = slot / a.q_tokens;
+    Raw<DT> next{};
+    if (g < a.G) next = load_pairs<DT>(a.q, at + g * a.q_head, c);
     float cs[8], sn[8];
     turn_of(a, c, p + i + shift, cs, sn);
-    for (int64_t g = slot / a.q_tokens; g < a.G; g += L::kSlots / a.q_tokens) {
+    for (; g < a.G; g += step) {  // the next head is requested first
+      const Raw<DT> now = next;
+      if (g + step < a.G) next = load_pairs<DT>(a.q, at + (g + step) * a.q_head, c);
       float x[16];
-      unpack_pairs<DT>(load_pairs<DT>(a.q, bh * a.q_row + g * a.q_head + i * a.q_tok, c), x);
+      unpack_pairs<DT>(now, x);
       if (a.weight[0]) norm<D>(x, w, a.eps);
       turn(x, cs, sn);
       store_pairs<DT>(a.q_out, ((bh * a.G + g) * a.T + i) * D, c, x);

@@ -7,7 +7,7 @@
 //   y_c = x'_c                                          for c >= r
 // for each query head and for K (the rotate-half convention of scripts/common.py:44-47); K's y and V
 // are quantised as rows8_write does.  All in float32 but the angle, which is formed and reduced in
-// float64.
+// fixed point (see turn_of).
 #include "rows8.hpp"
 
 namespace fathom {
@@ -18,6 +18,8 @@ typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kThreads = 256;
+constexpr int kHeads = 4;           // of a workgroup of queries, which turn by the same angles
+constexpr int64_t kFill = 2048;     // workgroups of queries: fewer heads each where there would not be as many
 constexpr int64_t kMaxRotate = 1 << 27;  // tokens of a call: its grid stays below 2^32 threads
 
 struct RotateArgs {
@@ -36,6 +38,8 @@ struct RotateArgs {
   void *q_out, *k_out;
   int kv_blocks;  // workgroups of K, and of V, per row; the others take queries
   int q_tokens;   // tokens of a workgroup of queries, a power of two
+  int q_heads;    // and its heads, of consecutive workgroups
+  int q_parts;    // workgroups that share its tokens
 };
 
 // A thread holds sixteen channels of a row, as eight pairs that turn together: channels a .. a + 7 and b .. b + 7.
@@ -116,19 +120,26 @@ __device__ __forceinline__ void load_weights(const void *w, int dt, Pairs c, flo
   }
 }
 
-// cos and sin of position t for the thread's pairs: the angle in quarter turns n + f, |f| <= 1/2, in float64, then
-// x = f pi / 2 in float32 and sin x = x + x^3 P(x^2), cos x = 1 - x^2 / 2 + x^4 Q(x^2), P and Q least-squares fits of
-// degree 2 on |x| <= pi / 4, each off by less than a step of float32.
-__device__ __forceinline__ void turn_of(const RotateArgs &a, Pairs c, int64_t t, float (&cs)[8], float (&sn)[8]) {
-  constexpr double kQuarters = 0.63661977236758134308, kWhole = 6755399441055744.0;  // 2 / pi; 1.5 2^52: a sum's low bits are n
-  float inv[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) inv[i] = c.turned ? a.inv_freq[c.a + i] : 0.0f;
+// A frequency as turns per token, in fractions of 2^-64 of a turn: inv / (2 pi) in two float64, whole turns dropped.
+__device__ __forceinline__ uint64_t turns_of(float inv) {
+  constexpr double kTurn = 0.15915494309189534561, kRest = -9.8393383659123640e-18;  // 1 / (2 pi) in two parts
+  const double hi = (double)inv * kTurn, lo = fma((double)inv, kTurn, -hi) + (double)inv * kRest;
+  const double part = (hi - floor(hi)) * 0x1p32, whole = floor(part);
+  return ((uint64_t)(uint32_t)whole << 32) + (uint64_t)(int64_t)rint((part - whole) * 0x1p32 + lo * 0x1p64);
+}
+
+// cos and sin of position t for the thread's pairs.  The angle is the product of t and the pair's turns, modulo whole turns by
+// itself: its upper word is exact to 2^-31 of a turn whatever t.  In quarter turns n + f, |f| <= 1/2, x = f pi / 2: sin x = x + x^3
+// P(x^2), cos x = 1 - x^2 / 2 + x^4 Q(x^2), P and Q least-squares fits of degree 2 on |x| <= pi / 4, off by less than a step of
+// float32 each.  (Angles in float64, half as fast: 8 x 32768 tokens of 4 heads 176 us; 163.)
+__device__ __forceinline__ void turn_of(const uint64_t (&turns)[8], Pairs c, int64_t t, float (&cs)[8], float (&sn)[8]) {
+  const uint32_t lo = (uint32_t)t, hi = (uint32_t)((uint64_t)t >> 32);
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const double q = (double)t * ((double)inv[i] * kQuarters), m = q + kWhole;
-    const uint32_t n = (uint32_t)__double2loint(m);
-    const float x = (float)(q - (m - kWhole)) * 1.57079632679489661923f, w = x * x;
+    const uint32_t f0 = (uint32_t)turns[i], f1 = (uint32_t)(turns[i] >> 32);
+    const uint32_t phase = __umulhi(lo, f0) + lo * f1 + hi * f0;  // 2^-32 of a turn
+    const uint32_t n = (phase + 0x20000000u) >> 30;
+    const float x = (float)(int32_t)(phase - (n << 30)) * 1.4629180792671596e-9f, w = x * x;  // 2 pi / 2^32
     float p = fmaf(w, -0.00019515919848345220f, 0.00833216588944196700f);
     p = fmaf(p, w, -0.16666655242443085f);
     const float s = fmaf(x * w, p, x);
@@ -137,6 +148,10 @@ __device__ __forceinline__ void turn_of(const RotateArgs &a, Pairs c, int64_t t,
     k = fmaf(fmaf(k, w, -0.5f), w, 1.0f);
     sn[i] = __uint_as_float(__float_as_uint(n & 1 ? k : s) ^ (n & 2) << 30);
     cs[i] = __uint_as_float(__float_as_uint(n & 1 ? s : k) ^ ((n + 1) & 2) << 30);
+    if (!c.turned) {
+      sn[i] = 0.0f;
+      cs[i] = 1.0f;
+    }
   }
 }
 
@@ -169,20 +184,28 @@ __global__ __launch_bounds__(kThreads) void rotate_kernel(RotateArgs a) {
   const int64_t p = a.pos ? (int64_t)a.pos[bh] : a.pos_value;
   const int64_t shift = a.offset ? (int64_t)a.offset[bh] : a.offset_value;
   const Pairs c = pairs_of<D>(a.turn);
+  __shared__ uint64_t shared_turns[D / 2];
+  if (2 * tid < a.turn) shared_turns[tid] = turns_of(a.inv_freq[tid]);
+  __syncthreads();
+  uint64_t turns[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) turns[i] = c.turned ? shared_turns[c.a + i] : 0;
   float w[16];
   if ((int)blockIdx.x >= 2 * a.kv_blocks) {  // ---- queries: a token's heads share its angles
     load_weights(a.weight[0], a.weight_dtype, c, w);
-    const int64_t i = (int64_t)((int)blockIdx.x - 2 * a.kv_blocks) * a.q_tokens + slot % a.q_tokens;
+    const int unit = (int)blockIdx.x - 2 * a.kv_blocks, part = unit % a.q_parts;
+    const int64_t i = (int64_t)(unit / a.q_parts) * a.q_tokens + slot % a.q_tokens;
     if (i >= a.T) return;  // whole rows' lanes
     const int64_t step = L::kSlots / a.q_tokens, at = bh * a.q_row + i * a.q_tok;
-    int64_t g = slot / a.q_tokens;
+    const int64_t last = (int64_t)(part + 1) * a.q_heads, end = last < a.G ? last : a.G;
+    int64_t g = (int64_t)part * a.q_heads + slot / a.q_tokens;
     Raw<DT> next{};
-    if (g < a.G) next = load_pairs<DT>(a.q, at + g * a.q_head, c);
+    if (g < end) next = load_pairs<DT>(a.q, at + g * a.q_head, c);
     float cs[8], sn[8];
-    turn_of(a, c, p + i + shift, cs, sn);
-    for (; g < a.G; g += step) {  // the next head is requested first
+    turn_of(turns, c, p + i + shift, cs, sn);
+    for (; g < end; g += step) {  // the next head is requested first
       const Raw<DT> now = next;
-      if (g + step < a.G) next = load_pairs<DT>(a.q, at + (g + step) * a.q_head, c);
+      if (g + step < end) next = load_pairs<DT>(a.q, at + (g + step) * a.q_head, c);
       float x[16];
       unpack_pairs<DT>(now, x);
       if (a.weight[0]) norm<D>(x, w, a.eps);
@@ -216,7 +239,7 @@ __global__ __launch_bounds__(kThreads) void rotate_kernel(RotateArgs a) {
     if (!kv) {
       if (a.weight[1]) norm<D>(x[i], w, a.eps);
       float cs[8], sn[8];
-      turn_of(a, c, p + j + shift, cs, sn);
+      turn_of(turns, c, p + j + shift, cs, sn);
       turn(x[i], cs, sn);
       if (a.k_out && j >= 0 && j < a.T) store_pairs<DT>(a.k_out, (bh * a.T + j) * D, c, x[i]);
     }
@@ -262,7 +285,12 @@ void launch_rotate(RotateArgs a, int64_t BH, hipStream_t st) {
   a.kv_blocks = (int)cdiv(a.T + kBlk - 1, kBlk);  // T tokens touch at most so many
   a.q_tokens = 1;
   while (a.q_tokens < a.T && a.q_tokens < Lane<D>::kSlots) a.q_tokens *= 2;
-  const int64_t all = 2 * (int64_t)a.kv_blocks + cdiv(a.T, a.q_tokens);
+  const int64_t units = cdiv(a.T, a.q_tokens), slots = Lane<D>::kSlots / a.q_tokens;  // heads of a pass
+  int64_t heads = kHeads;
+  while (heads > 1 && units * BH * cdiv(a.G, heads) < kFill) heads /= 2;
+  a.q_heads = (int)(heads > slots ? heads : slots);
+  a.q_parts = (int)cdiv(a.G, (int64_t)a.q_heads);
+  const int64_t all = 2 * (int64_t)a.kv_blocks + units * a.q_parts;
   rotate_kernel<D, DT, I8><<<dim3((unsigned)all, (unsigned)BH), kThreads, 0, st>>>(a);
 }
 

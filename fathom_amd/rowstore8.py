@@ -51,11 +51,12 @@ def _heads(q):
     if q.dtype not in _KDT:
         q = q.float()
     size = 4 if q.dtype == _F32 else 2
-    st = [s if n > 1 else 0 for s, n in zip(q.stride()[:3], q.shape[:3])]
-    if q.stride(3) != 1 or (q.data_ptr() | st[0] * size | st[1] * size | st[2] * size) & 15:
+    (BH, G, T, _), (sr, sh, st, sd) = q.shape, q.stride()
+    sr, sh, st = sr if BH > 1 else 0, sh if G > 1 else 0, st if T > 1 else 0  # the stride of a single one says nothing
+    if sd != 1 or (q.data_ptr() | sr * size | sh * size | st * size) & 15:
         q = torch.empty(q.shape, dtype=q.dtype, device=q.device).copy_(q)
-        st = q.stride()[:3]
-    return q, st[0], st[1], st[2]
+        sr, sh, st, _ = q.stride()
+    return q, sr, sh, st
 
 
 class RowStore8:
@@ -216,35 +217,41 @@ class RowStore8:
         the angle t inv_freq[c], which is formed in float64; channels behind r stay.  offset is an int or integers [BH]:
         what stands before the store's first token, as a shared prefix does.  Views as in `write`; with a tensor `pos`,
         rows whose tokens do not all fit are rotated but not written."""
+        dev, BH, d = self.device, self.BH, self.d
         for t in (q, K, V):
-            if t.device != self.device:
+            if t.device != dev:
                 self._elsewhere(t)
-        BH, d = self.BH, self.d
-        if K.dim() != 3 or K.shape != V.shape or K.shape[0] != BH or K.shape[2] != d:
-            raise ValueError(f"K {tuple(K.shape)} and V {tuple(V.shape)} must be alike, [{BH}, T, {d}]")
-        T = K.shape[1]
-        if q.dim() != 4 or q.shape[0] != BH or q.shape[1] < 1 or q.shape[2] != T or q.shape[3] != d:
-            raise ValueError(f"q {tuple(q.shape)} must be [{BH}, G, {T}, {d}]")
-        if not q.dtype == K.dtype == V.dtype or not q.dtype.is_floating_point:
-            raise ValueError(f"q {q.dtype}, K {K.dtype} and V {V.dtype} must be of one float type")
-        turned = 0
+        shape, k_shape, dtype = q.shape, K.shape, q.dtype
+        if len(k_shape) != 3 or k_shape != V.shape or k_shape[0] != BH or k_shape[2] != d:
+            raise ValueError(f"K {tuple(k_shape)} and V {tuple(V.shape)} must be alike, [{BH}, T, {d}]")
+        T = k_shape[1]
+        if len(shape) != 4 or shape[0] != BH or shape[1] < 1 or shape[2] != T or shape[3] != d:
+            raise ValueError(f"q {tuple(shape)} must be [{BH}, G, {T}, {d}]")
+        if not dtype == K.dtype == V.dtype or not dtype.is_floating_point:
+            raise ValueError(f"q {dtype}, K {K.dtype} and V {V.dtype} must be of one float type")
+        turned, inv_at = 0, None
         if inv_freq is not None:
-            if inv_freq.device != self.device:
+            if inv_freq.device != dev:
                 self._elsewhere(inv_freq)
             turned = 2 * inv_freq.numel()
             if inv_freq.dim() != 1 or turned > d or turned % 16 or not inv_freq.dtype.is_floating_point:
                 raise ValueError(f"inv_freq {inv_freq.dtype} {tuple(inv_freq.shape)} must be float32 [r / 2], r <= {d} a multiple of 16")
             if inv_freq.dtype != _F32 or not inv_freq.is_contiguous():
                 inv_freq = inv_freq.float().contiguous()
-        weights = [q_weight, k_weight]
-        given = [w for w in weights if w is not None]
-        for w in given:
-            if w.device != self.device:
-                self._elsewhere(w)
-            if w.shape != (d,) or not w.dtype.is_floating_point:
-                raise ValueError(f"a weight {w.dtype} {tuple(w.shape)} must be floats [{d}]")
-        w_dtype = given[0].dtype if given and given[0].dtype == given[-1].dtype and given[0].dtype in _KDT else _F32
-        weights = [w if w is None else w.to(w_dtype).contiguous() for w in weights]
+            inv_at = inv_freq.data_ptr()
+        w_dtype, weights_at = _F32, (None, None)
+        if q_weight is not None or k_weight is not None:
+            given = [w for w in (q_weight, k_weight) if w is not None]
+            for w in given:
+                if w.device != dev:
+                    self._elsewhere(w)
+                if w.shape != (d,) or not w.dtype.is_floating_point:
+                    raise ValueError(f"a weight {w.dtype} {tuple(w.shape)} must be floats [{d}]")
+            if given[0].dtype == given[-1].dtype and given[0].dtype in _KDT:
+                w_dtype = given[0].dtype
+            weights = [w if w is None or (w.dtype == w_dtype and w.is_contiguous()) else w.to(w_dtype).contiguous()
+                       for w in (q_weight, k_weight)]
+            weights_at = [None if w is None else w.data_ptr() for w in weights]
         eps = float(eps)
         if not 0.0 <= eps < math.inf:
             raise ValueError(f"eps {eps} must be finite and not negative")
@@ -253,12 +260,10 @@ class RowStore8:
         q, qr, qh, qt = _heads(q)
         K, kr, kt = _rows(K)
         V, vr, vt = _rows(V)
-        G = q.shape[1]
-        out = torch.empty((BH, G, T, d), dtype=q.dtype, device=self.device)
-        k_out = torch.empty((BH, T, d), dtype=q.dtype, device=self.device) if keys else None
+        out = torch.empty(shape, dtype=q.dtype, device=dev)
+        k_out = torch.empty(k_shape, dtype=q.dtype, device=dev) if keys else None
         self._call("fathom_rows8_write_rotated", q.data_ptr(), K.data_ptr(), V.data_ptr(), _KDT[q.dtype], qr, qh, qt, kr, kt, vr,
-                   vt, rows_at, at, shifts_at, shift, inv_freq.data_ptr() if turned else None, turned,
-                   *(None if w is None else w.data_ptr() for w in weights), _KDT[w_dtype], eps, BH, G, T, d, self.cap,
+                   vt, rows_at, at, shifts_at, shift, inv_at, turned, *weights_at, _KDT[w_dtype], eps, BH, shape[1], T, d, self.cap,
                    self._code, *self._store(), out.data_ptr(), None if k_out is None else k_out.data_ptr())
         return (out, k_out) if keys else out
 

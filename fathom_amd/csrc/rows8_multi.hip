@@ -183,7 +183,7 @@ extern "C" int fathom_rows8_chunk_attention(const void *q, int q_dtype, int64_t 
               kernel_cap(softcap), slopes, out, nullptr, nullptr, nullptr, 0, 1, tile_rows(G * T)};
   a.tiles = (int)cdiv(G * T, (int64_t)a.rows);
   const int64_t most = lens ? cap : n;
-  a.shares = (int)tile_shares(BH, G * T, D, tile_blocks(most, T, window, sinks), window > 0 || most >= 4 * T);
+  a.shares = (int)tile_shares(BH, G * T, D, tile_blocks(most, T, window, sinks), !lens && (window > 0 || most >= 4 * T));
   if (a.shares) {
     const size_t need = multi_bytes(BH, G * T, D, a.shares);
     if (!workspace || workspace_bytes < need)

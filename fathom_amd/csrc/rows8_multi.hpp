@@ -205,8 +205,8 @@ __device__ __forceinline__ Share find_tile(const MultiArgs &a, int w, FindTile &
 //     numbers (exact): K by tokens, V transposed, both with their 16-byte pieces in an order
 //     that keeps the lanes' reads on different banks;
 //   S^T = K q^T (v_mfma_f32_32x32x16): lane l holds query l & 31 and 32 of the block's scores, so
-//     that maximum and sum need one exchange, between l and l ^ 32.  bf16 and f16 queries are operands as they are (bf16
-//     ones times 2^-e, e the exponent of the query's largest channel); float32 ones are two f16, 22 bits, and where a wave has channels
+//     that maximum and sum need one exchange, between l and l ^ 32.  bf16 and f16 queries are operands as they are;
+//     float32 ones are two f16, 22 bits, and where a wave has channels
 //     below 2^-18 of their query's largest, what is left of those takes a third product, times 2^38, first.
 //   O^T += V^T p^T with the weights in the layout that the scores come in, which fixes the order of the tokens in the
 //     transposed V.  A weight is one f16 (PREC: two, 22 bits) of p s_V 2^-E, E the exponent of the largest p s_V so
@@ -216,9 +216,10 @@ __global__ __launch_bounds__(kMultiThreads, RW == 1 && D == 128 ? 1 : 2) void mu
   constexpr bool kBf16 = QT == FATHOM_DT_BF16;
   constexpr int kParts = QT == FATHOM_DT_F32 ? 2 : 1, kSteps = D / 16, kTiles = D / 32;
   constexpr int kThreads = RW * kWave, kBufs = RW == 1 ? 1 : 2, kRows = 32 * RW;  // threads that share a block
-  // operands read ahead: float32 queries take twice the registers (of 256; one more spilled register in the loop waits for all
-  // loads on their way)
-  constexpr int kAhead = kParts == 2 && D == 128 ? 2 : 4, kVBufs = kParts == 2 && D == 128 ? 1 : 2;
+  // Operands read ahead.  Fewer where registers are short (float32 queries take twice as many, caps and biases some), as
+  // a spilled register's way back waits for all loads on theirs: 32 x 8 x 4 queries over 32768 tokens 121 us; 84.
+  constexpr bool kLean = D == 128 && (kParts == 2 || EXTRA);
+  constexpr int kAhead = kLean ? 2 : 4, kVBufs = kLean ? 1 : 2;
   constexpr int kGroups = kMultiWaves / RW;                                      // of them in a workgroup
   constexpr int kKeys = kBlk * D / 16 / kThreads;        // 16-byte pieces of K per thread
   constexpr int kCh = D == 64 && RW == 4 ? 4 : 8;        // channels of V per thread and item of four tokens
@@ -261,9 +262,29 @@ __global__ __launch_bounds__(kMultiThreads, RW == 1 && D == 128 ? 1 : 2) void mu
   int ex = 0;
   const int64_t q_at = r * a.q_row + g * a.q_head + o_at * a.q_out + 8 * half;
   bool far = false;  // float32: some channel of the wave's queries is small, as small_channel has it
-  if constexpr (QT == FATHOM_DT_F16) {
+  if constexpr (QT != FATHOM_DT_F32) {
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s) qf[0][s] = *reinterpret_cast<const f16x8 *>(static_cast<const uint16_t *>(a.q) + q_at + 16 * s);
+    for (int s = 0; s < kSteps; ++s) qf[0][s] = *reinterpret_cast<const frag *>(static_cast<const uint16_t *>(a.q) + q_at + 16 * s);
+    if constexpr (kBf16) {  // times a power of two where products could pass float32's range: the largest |q| at 2^100 or more
+      uint32_t big = 0;
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+        const u32x4 w = __builtin_bit_cast(u32x4, qf[0][s]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t x = w[e] << 16 & 0x7FFF0000u, y = w[e] & 0x7FFF0000u;
+          big = big > x ? big : x;
+          big = big > y ? big : y;
+        }
+      }
+      if (__builtin_expect(__any(big >= 0x71800000u), 0)) {
+        ex = 60;
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) qf[0][s][e] = (__bf16)ldexpf((float)qf[0][s][e], -60);
+      }
+    }
   } else {
     float x[kSteps][8], big = 0.0f;
 #pragma unroll
@@ -273,20 +294,18 @@ __global__ __launch_bounds__(kMultiThreads, RW == 1 && D == 128 ? 1 : 2) void mu
       for (int e = 0; e < 8; ++e) big = fmaxf(big, fabsf(x[s][e]));
     }
     big = fmaxf(big, other_half(big));
-    if (big > 0.0f && big < INFINITY) frexpf(big, &ex);
-    if constexpr (!kBf16) ex -= 14;  // the largest |q| of the query in [2^13, 2^14)
+    if (big > 0.0f && big < INFINITY) {
+      frexpf(big, &ex);
+      ex -= 14;  // the largest |q| of the query in [2^13, 2^14)
+    }
 #pragma unroll
     for (int s = 0; s < kSteps; ++s)
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const float v = ldexpf(x[s][e], -ex);
-        if constexpr (kBf16) {
-          qf[0][s][e] = (__bf16)v;
-        } else {
-          qf[0][s][e] = (_Float16)v;
-          qf[1][s][e] = (_Float16)(v - (float)(_Float16)v);
-          far |= small_channel(v);
-        }
+        qf[0][s][e] = (_Float16)v;
+        qf[1][s][e] = (_Float16)(v - (float)(_Float16)v);
+        far |= small_channel(v);
       }
     far = __any(far);
   }
@@ -395,16 +414,14 @@ __global__ __launch_bounds__(kMultiThreads, RW == 1 && D == 128 ? 1 : 2) void mu
     for (int e = 0; e < 16; ++e) o[d][e] = 0.0f;
   float base = kLowest, l = 0.0f, E = -1000.0f;
 
-  // Bit 16 x + e: whether the query sees token at + 32 x + 8 (e / 4) + e % 4.
+  // Bit 16 x + e: whether the query sees token at + 32 x + 8 (e / 4) + e % 4.  Those places rise with the bit, so the bits
+  // of tokens before t are the lowest ones, four for each eight tokens.
   auto seen_of = [&](int at) {
-    uint32_t seen = 0;
-#pragma unroll
-    for (int b = 0; b < 32; ++b) {
-      const int t = at + 32 * (b / 16) + 8 * (b % 16 / 4) + b % 4;
-      seen |= (t < end && (t >= lo || t < from) ? 1u : 0u) << b;
-    }
-    asm volatile("" : "+v"(seen));  // a register of the lane: as masks for every token it would fill the scalar ones
-    return seen;
+    auto before = [&](int t) {
+      const int n = t - at, bits = n <= 0 ? 0 : 4 * (n >> 3) + ((n & 7) < 4 ? n & 7 : 4);
+      return bits >= 32 ? 0xFFFFFFFFu : (1u << bits) - 1u;
+    };
+    return before(end) & ~(before(lo) & ~before(from));
   };
   auto block = [&](int buf, int i, float ks, float vs) {
     const int t0 = span.block(i) * kBlk;
@@ -513,9 +530,13 @@ __global__ __launch_bounds__(kMultiThreads, RW == 1 && D == 128 ? 1 : 2) void mu
       f = 1.0f;
     }
     if (edge) {
+      asm volatile("");  // a branch, not selects in every block
       const uint32_t seen = seen_of(at);
 #pragma unroll
-      for (int b = 0; b < 32; ++b) s[b / 16][b % 16] = seen >> b & 1 ? s[b / 16][b % 16] : -INFINITY;
+      for (int b = 0; b < 32; ++b) {
+        const uint32_t keep = (uint32_t)((int32_t)(seen << (31 - b)) >> 31), x = __float_as_uint(s[b / 16][b % 16]);
+        s[b / 16][b % 16] = __uint_as_float((x & keep) | (0xFF800000u & ~keep));  // else -infinity
+      }
     }
     float mx = -INFINITY;
 #pragma unroll
@@ -731,7 +752,7 @@ __global__ __launch_bounds__(kMultiThreads, RW == 1 && D == 128 ? 1 : 2) void mu
         *reinterpret_cast<float4 *>(a.part + (slot + row) * D + c + 4 * half) = make_float4(v[0], v[1], v[2], v[3]);
       } else {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] = l == 0.0f ? 0.0f : ldexpf(o[d][e + k] * inv, (int)E);
+        for (int k = 0; k < 4; ++k) v[k] = ldexpf(o[d][e + k] * inv, (int)E);
         store4<QT>(a.out, out_at + c, v);
       }
     }

@@ -19,7 +19,8 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(MultiArgs a, Tail ta
   const int tid = threadIdx.x, lane = tid % kLanes, grp = tid / kLanes;
   const int m = (int)blockIdx.x, y = m / a.rows;
   const int64_t r = blockIdx.y, g = m % a.G, o = m / a.G;
-  const int2 from = a.where[r * a.tiles + y];
+  const int tile = (int)r * a.tiles + y;
+  const int2 from = a.splits ? make_int2(tile * a.splits, a.splits) : a.where[tile];
   const int own = from.y;  // splits of the tile
   const int64_t at = (int64_t)from.x * a.rows + m % a.rows;
   int more = 0;
@@ -49,9 +50,11 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(MultiArgs a, Tail ta
   if ((tid & 63) == 0) red[1][tid >> 6] = l;
   float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   for (int s = grp; s < ns; s += kGroups) {
+    const float2 x = ml(s);
+    if (x.y == 0.0f) continue;  // no weight, and perhaps nothing written
     const float *p = s < own ? a.part + (at + (int64_t)s * a.rows) * D : tail.part + (slot + (int64_t)(s - own) * a.G) * D;
     const float4 u = reinterpret_cast<const float4 *>(p)[lane];
-    const float f = __builtin_amdgcn_exp2f(ml(s).x - big);
+    const float f = __builtin_amdgcn_exp2f(x.x - big);
     v.x = fmaf(u.x, f, v.x);
     v.y = fmaf(u.y, f, v.y);
     v.z = fmaf(u.z, f, v.z);
@@ -86,14 +89,22 @@ int tile_rows(int64_t M) { return M <= 32 ? 32 : 128; }
 
 // Shares that tiles of up to nb blocks are cut into (at most that many and one per tile more); 0: a workgroup takes each tile.
 // `places` workgroups are at work at once (of 32 queries of D = 128 one per CU, else two).  Few tiles are cut so that all places
-// have the same to do.  So are tiles that see very different lengths (`even` is false), up to twice the places, in rounds of
-// shares of a quarter of the mean and less; more tiles even out by themselves, those that see most first.
+// have the same to do.  So are tiles that see very different lengths (`even` is false), up to twice the places: into a few
+// rounds, as every tile's last share is shorter; of shares, a workgroup's partial results cost about four blocks.  More tiles
+// even out by themselves, those that see most first.  (32 ragged rows of 572 tokens, 576 tiles: 509 us a workgroup per tile, 283
+// in five rounds.)
 int64_t tile_shares(int64_t BH, int64_t M, int64_t D, int64_t nb, bool even) {
   const int rows = tile_rows(M);
   const int64_t tiles = BH * cdiv(M, (int64_t)rows), places = rows == 32 && D == 128 ? 256 : 512;
   if (nb <= 4 || tiles >= 2 * places || (even && tiles > places / 2)) return 0;
-  const int64_t rounds = cdiv(4 * tiles, places), shares = places * rounds - tiles, most = tiles * cdiv(nb, (int64_t)4);
+  const int64_t rounds = cdiv(3 * tiles, places), most = tiles * cdiv(nb, (int64_t)4);
+  const int64_t shares = rounds == 1 ? places - tiles : places * rounds - tiles * 5 / 8;
   return most < shares ? most : shares;
+}
+// Splits of each of so many tiles that all have the same to do: as many as there are places, of four blocks and more.
+int64_t tile_splits(int64_t tiles, int64_t shares, int64_t nb) {
+  const int64_t room = (shares + tiles) / tiles, most = cdiv(nb, (int64_t)4);
+  return most < 1 ? 1 : room < most ? room : most;
 }
 // The same for a prefix, whose tiles always leave partial results.
 int64_t prefix_shares(int64_t BH, int64_t M, int64_t D, int64_t nb) {
@@ -127,6 +138,7 @@ void place(MultiArgs &a, void *workspace, int64_t D) {
   a.part = static_cast<float *>(workspace);
   a.ml = reinterpret_cast<float2 *>(a.part + rows * D);
   a.where = reinterpret_cast<int2 *>(a.ml + rows);
+  a.parts = true;
 }
 
 int run_multi(const MultiArgs &a, int q_dtype, int64_t D, bool i8, hipStream_t st) {
@@ -180,10 +192,12 @@ extern "C" int fathom_rows8_chunk_attention(const void *q, int q_dtype, int64_t 
   if (sinks > cap) sinks = cap;
   MultiArgs a{q, q_row_stride, q_head_stride, q_tok_stride, (const uint8_t *)k8, (const uint8_t *)v8, k_scale, v_scale, cap,
               cdiv(cap, kBlk), lens, n, (int)G, (int)T, (int)window, (int)sinks, false, nullptr, 0, 0, BH, scale,
-              kernel_cap(softcap), slopes, out, nullptr, nullptr, nullptr, 0, 1, tile_rows(G * T)};
+              kernel_cap(softcap), slopes, out, nullptr, nullptr, nullptr, 0, 1, tile_rows(G * T), 0, false};
   a.tiles = (int)cdiv(G * T, (int64_t)a.rows);
   const int64_t most = lens ? cap : n;
-  a.shares = (int)tile_shares(BH, G * T, D, tile_blocks(most, T, window, sinks), !lens && (window > 0 || most >= 4 * T));
+  const int64_t nb = tile_blocks(most, T, window, sinks);
+  const bool even = !lens && (window > 0 || most >= 4 * T);
+  a.shares = (int)tile_shares(BH, G * T, D, nb, even);
   if (a.shares) {
     const size_t need = multi_bytes(BH, G * T, D, a.shares);
     if (!workspace || workspace_bytes < need)
@@ -191,6 +205,7 @@ extern "C" int fathom_rows8_chunk_attention(const void *q, int q_dtype, int64_t 
     if (reinterpret_cast<uintptr_t>(workspace) & 15)
       return fail(FATHOM_ERR_INVALID, "%s: the workspace must be 16-byte aligned", what);
     place(a, workspace, D);
+    if (!lens && even) a.splits = (int)tile_splits(BH * a.tiles, a.shares, nb);
   }
   rc = run_multi(a, q_dtype, D, code_dtype == FATHOM_DT_I8, (hipStream_t)stream);
   return rc || !a.shares ? rc : run_join(a, Tail{}, q_dtype, D, (hipStream_t)stream);
@@ -227,7 +242,7 @@ extern "C" int fathom_rows8_shared_attention(const void *q, int q_dtype, const v
     return fail(FATHOM_ERR_INVALID, "%s: %lld sequences, G=%lld, at most %lld queries per row and 2^27 in all", what, (long long)sequences, (long long)G, (long long)kMaxTiles * 32);
   MultiArgs a{q, G * D, D, prefix_BH * G * D, (const uint8_t *)prefix_k8, (const uint8_t *)prefix_v8, prefix_k_scale,
               prefix_v_scale, prefix_cap, cdiv(prefix_cap, kBlk), prefix_lens, prefix_n, (int)G, (int)sequences, 0, 0, true,
-              lens, n, cap, prefix_BH, scale, kernel_cap(softcap), slopes, out, nullptr, nullptr, nullptr, 1, 1, tile_rows(G * sequences)};
+              lens, n, cap, prefix_BH, scale, kernel_cap(softcap), slopes, out, nullptr, nullptr, nullptr, 1, 1, tile_rows(G * sequences), 0, false};
   a.tiles = (int)cdiv(G * sequences, (int64_t)a.rows);
   a.shares = (int)prefix_shares(prefix_BH, G * sequences, D, cdiv(prefix_lens ? prefix_cap : prefix_n, (int64_t)kBlk));
   const size_t first = multi_bytes(prefix_BH, G * sequences, D, a.shares);
@@ -236,6 +251,7 @@ extern "C" int fathom_rows8_shared_attention(const void *q, int q_dtype, const v
   if (reinterpret_cast<uintptr_t>(workspace) & 15)
     return fail(FATHOM_ERR_INVALID, "%s: the workspace must be 16-byte aligned", what);
   place(a, workspace, D);
+  if (!prefix_lens) a.splits = (int)tile_splits(prefix_BH * a.tiles, a.shares, cdiv(prefix_n, (int64_t)kBlk));
   const bool i8 = code_dtype == FATHOM_DT_I8;
   const hipStream_t st = (hipStream_t)stream;
   Tail t;

@@ -33,8 +33,10 @@ struct MultiArgs {
   void *out;            // [BH, G, O, D] of the queries' type; shared: written by the join, [O, BH, G, D] float32
   float2 *ml;           // [slots, rows of a tile] a split's (m, l)
   float *part;          // [slots, rows, D] its weighted rows
-  int2 *where;          // [BH, tiles] a tile's first slot and its splits; null: one workgroup takes a tile
+  int2 *where;          // [BH, tiles] a tile's first slot and its splits, where they are shared out on the device; else null
   int shares, tiles, rows;
+  int splits;  // of every tile, where that is the same for all: tile t's slots begin at t splits; 0: see `where`
+  bool parts;  // partial results are written, for the join
 };
 
 // What a tile of `rows` queries from the first one m0 of row r sees: blocks [0, sink) and, `skip` blocks further, up to
@@ -233,16 +235,18 @@ __global__ __launch_bounds__(kMultiThreads, RW == 1 && D == 128 ? 1 : 2) void mu
   const int col = lane & 31, half = lane >> 5;
   Share share{(int)(gridDim.y - 1 - blockIdx.y), 0, 1, 0};  // the tiles that see most come first
   int64_t r = blockIdx.x;
-  if (a.where) {  // uniform over the workgroup
-    share = find_tile(a, (int)blockIdx.x, find);
+  if (a.parts) {  // uniform over the workgroup
+    if (a.splits) share = Share{(int)blockIdx.x / a.splits, (int)blockIdx.x % a.splits, a.splits, 0};
+    else share = find_tile(a, (int)blockIdx.x, find);
     if (share.active == 0) return;
     r = share.tile / a.tiles;
     share.tile %= a.tiles;
   }
   const int m0 = share.tile * kRows, M = a.G * a.O;
   const TileSpan span = tile_span(a, r, m0);
+  if (a.splits) share.per = (span.nb + a.splits - 1) / a.splits;
   const int first = share.split * share.per;
-  const int last = share.split + 1 < share.active ? first + share.per : span.nb;
+  const int end_of = first + share.per, last = share.split + 1 < share.active && end_of < span.nb ? end_of : span.nb;
 
   // ---- the lane's query
   const int mine = m0 + 32 * (wave % RW) + col, m = mine < M ? mine : M - 1;
@@ -683,7 +687,7 @@ __global__ __launch_bounds__(kMultiThreads, RW == 1 && D == 128 ? 1 : 2) void mu
   }
 
   l += other_half(l);
-  const bool parts = a.where != nullptr;
+  const bool parts = a.parts;
   const int64_t slot = parts ? ((int64_t)blockIdx.x * kRows) : 0;
   if constexpr (RW == 1) {  // ---- the waves' sums over their blocks, in the LDS that held those
     __shared__ float wm[kMultiWaves][32], wl[kMultiWaves][32];
@@ -760,7 +764,9 @@ __global__ __launch_bounds__(kMultiThreads, RW == 1 && D == 128 ? 1 : 2) void mu
 
 template <int D, bool I8, int QT, bool PREC, bool EXTRA>
 void launch_multi(const MultiArgs &a, hipStream_t st) {
-  const dim3 grid = a.where ? dim3((unsigned)(a.shares + a.BH * a.tiles)) : dim3((unsigned)a.BH, (unsigned)a.tiles);
+  const dim3 grid = a.splits  ? dim3((unsigned)(a.splits * a.BH * a.tiles))
+                    : a.parts ? dim3((unsigned)(a.shares + a.BH * a.tiles))
+                              : dim3((unsigned)a.BH, (unsigned)a.tiles);
   if (a.rows == 32) multi_kernel<D, I8, QT, PREC, EXTRA, 1><<<grid, kMultiThreads, 0, st>>>(a);
   else multi_kernel<D, I8, QT, PREC, EXTRA, 4><<<grid, kMultiThreads, 0, st>>>(a);
 }

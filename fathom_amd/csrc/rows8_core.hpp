@@ -101,6 +101,7 @@ struct RowsWith {
   __device__ __forceinline__ void load(int off, u32x2 &v) const {
     v = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rsrc, off, 0, AUX));
   }
+  __device__ __forceinline__ void load(int off, uint16_t &v) const { v = __builtin_amdgcn_raw_buffer_load_b16(rsrc, off, 0, AUX); }
   __device__ __forceinline__ void load(int off, uint32_t &v) const { v = __builtin_amdgcn_raw_buffer_load_b32(rsrc, off, 0, AUX); }
 };
 typedef RowsWith<kStream> RowsOf;

@@ -88,15 +88,15 @@ void launch_join(const MultiArgs &a, const Tail &t, int out, hipStream_t st) {
 int tile_rows(int64_t M) { return M <= 32 ? 32 : 128; }
 
 // Shares that tiles of up to nb blocks are cut into (at most that many and one per tile more); 0: a workgroup takes each tile.
-// `places` workgroups are at work at once (of 32 queries of D = 128 one per CU, else two).  Few tiles are cut so that all places
+// `places` workgroups are at work at once, two per CU.  Few tiles are cut so that all places
 // have the same to do.  So are tiles that see very different lengths (`even` is false), up to twice the places: into a few
 // rounds, as every tile's last share is shorter; of shares, a workgroup's partial results cost about four blocks.  More tiles
 // even out by themselves, those that see most first.  (32 ragged rows of 572 tokens, 576 tiles: 509 us a workgroup per tile, 283
 // in five rounds.)
 int64_t tile_shares(int64_t BH, int64_t M, int64_t D, int64_t nb, bool even) {
   const int rows = tile_rows(M);
-  const int64_t tiles = BH * cdiv(M, (int64_t)rows), places = rows == 32 && D == 128 ? 256 : 512;
-  if (nb <= 4 || tiles >= 2 * places || (even && tiles > places / 2)) return 0;
+  const int64_t tiles = BH * cdiv(M, (int64_t)rows), places = 512;
+  if (nb <= (rows == 32 ? 16 : 4) || tiles >= 2 * places || (even && tiles > places / 2)) return 0;
   const int64_t rounds = cdiv(3 * tiles, places), most = tiles * cdiv(nb, (int64_t)4);
   const int64_t shares = rounds == 1 ? places - tiles : places * rounds - tiles * 5 / 8;
   return most < shares ? most : shares;

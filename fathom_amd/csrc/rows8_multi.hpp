@@ -97,10 +97,16 @@ __device__ __forceinline__ uint32_t pair_bf16(uint32_t w) {
 }
 
 __device__ __forceinline__ uint32_t dword_of(uint32_t v, int) { return v; }
+__device__ __forceinline__ uint32_t dword_of(uint16_t v, int) { return v; }
 __device__ __forceinline__ uint32_t dword_of(u32x2v v, int d) { return v[d]; }
 // The top bits of a dword's bytes that hold an e4m3 NaN (0x7F, 0xFF).
 __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u; }
 __device__ __forceinline__ void clear_nans(uint32_t &w) { w &= ~((nan_bytes(w) >> 7) * 0xFFu); }
+__device__ __forceinline__ void clear_nans(uint16_t &w) {
+  uint32_t x = w;
+  clear_nans(x);
+  w = (uint16_t)x;
+}
 __device__ __forceinline__ void clear_nans(u32x2v &w) {
   w[0] &= ~((nan_bytes(w[0]) >> 7) * 0xFFu);
   w[1] &= ~((nan_bytes(w[1]) >> 7) * 0xFFu);
@@ -214,20 +220,22 @@ __device__ __forceinline__ Share find_tile(const MultiArgs &a, int w, FindTile &
 //     transposed V.  A weight is one f16 (PREC: two, 22 bits) of p s_V 2^-E, E the exponent of the largest p s_V so
 //     far, so that blocks of small values with large weights count fully.
 template <int D, bool I8, int QT, bool PREC, bool EXTRA, int RW>
-__global__ __launch_bounds__(kMultiThreads, RW == 1 && D == 128 ? 1 : 2) void multi_kernel(MultiArgs a) {
+__global__ __launch_bounds__(kMultiThreads, RW == 1 && D == 128 && QT == FATHOM_DT_F32 ? 1 : 2) void multi_kernel(MultiArgs a) {
   constexpr bool kBf16 = QT == FATHOM_DT_BF16;
   constexpr int kParts = QT == FATHOM_DT_F32 ? 2 : 1, kSteps = D / 16, kTiles = D / 32;
-  constexpr int kThreads = RW * kWave, kBufs = RW == 1 ? 1 : 2, kRows = 32 * RW;  // threads that share a block
+  constexpr bool kDirect = RW == 1;  // operands straight from the codes, without LDS
+  constexpr int kThreads = RW * kWave, kBufs = 2, kRows = 32 * RW;  // threads that share a block
   // Operands read ahead.  Fewer where registers are short (float32 queries take twice as many, caps and biases some), as
   // a spilled register's way back waits for all loads on theirs: 32 x 8 x 4 queries over 32768 tokens 121 us; 84.
-  constexpr bool kLean = D == 128 && (kParts == 2 || EXTRA);
+  constexpr bool kLean = kDirect || (D == 128 && (kParts == 2 || EXTRA));
   constexpr int kAhead = kLean ? 2 : 4, kVBufs = kLean ? 1 : 2;
   constexpr int kGroups = kMultiWaves / RW;                                      // of them in a workgroup
-  constexpr int kKeys = kBlk * D / 16 / kThreads;        // 16-byte pieces of K per thread
-  constexpr int kCh = D == 64 && RW == 4 ? 4 : 8;        // channels of V per thread and item of four tokens
-  constexpr int kItems = kBlk / 4 * D / kCh / kThreads;  // items per thread
+  constexpr int kKeys = kBlk * D / 16 / kThreads;                  // 16-byte pieces of K per thread
+  constexpr int kCh = kDirect ? D / 32 : D == 64 ? 4 : 8;          // channels of V per thread and item of four tokens
+  constexpr int kItems = kBlk / 4 * D / kCh / kThreads;            // items per thread
   typedef typename std::conditional<kBf16, bf16x8, f16x8>::type frag;
-  __shared__ __attribute__((aligned(16))) uint16_t lds[kGroups][kBufs][2][kBlk * D];
+  constexpr int kPitch = D + 4, kCodes = 2 * kBlk * D;  // of a row of sums; bytes of a block's K, or V, as 16-bit numbers
+  __shared__ __attribute__((aligned(16))) char lds[kGroups][kDirect ? 32 * kPitch * 4 : 2 * kBufs * kCodes];
   __shared__ int odd[kGroups][2];  // the first and the last block that hold a NaN in V
   __shared__ FindTile find;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -264,11 +272,12 @@ __global__ __launch_bounds__(kMultiThreads, RW == 1 && D == 128 ? 1 : 2) void mu
   const float slope = !EXTRA || !a.slopes ? 0.0f : a.slopes[a.shared ? (o_at * a.BH + r) * a.G + g : r * a.G + g] * kLog2e;
   frag qf[kParts][kSteps];
   int ex = 0;
-  const int64_t q_at = r * a.q_row + g * a.q_head + o_at * a.q_out + 8 * half;
+  const int64_t q_at = r * a.q_row + g * a.q_head + o_at * a.q_out;
+  auto channel = [&](int s) { return kDirect ? 32 * (s / 2) + 16 * half + 8 * (s % 2) : 16 * s + 8 * half; };  // of step s, eight of them
   bool far = false;  // float32: some channel of the wave's queries is small, as small_channel has it
   if constexpr (QT != FATHOM_DT_F32) {
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s) qf[0][s] = *reinterpret_cast<const frag *>(static_cast<const uint16_t *>(a.q) + q_at + 16 * s);
+    for (int s = 0; s < kSteps; ++s) qf[0][s] = *reinterpret_cast<const frag *>(static_cast<const uint16_t *>(a.q) + q_at + channel(s));
     if constexpr (kBf16) {  // times a power of two where products could pass float32's range: the largest |q| at 2^100 or more
       uint32_t big = 0;
 #pragma unroll
@@ -293,7 +302,7 @@ __global__ __launch_bounds__(kMultiThreads, RW == 1 && D == 128 ? 1 : 2) void mu
     float x[kSteps][8], big = 0.0f;
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
-      load8_q(a.q, QT, q_at + 16 * s, x[s]);
+      load8_q(a.q, QT, q_at + channel(s), x[s]);
 #pragma unroll
       for (int e = 0; e < 8; ++e) big = fmaxf(big, fabsf(x[s][e]));
     }
@@ -324,34 +333,56 @@ __global__ __launch_bounds__(kMultiThreads, RW == 1 && D == 128 ? 1 : 2) void mu
 
   // ---- staging
   u32x4 kr[kKeys];
-  typedef typename std::conditional<kCh == 8, u32x2v, uint32_t>::type vpiece;
+  typedef typename std::conditional<kCh == 8, u32x2v, typename std::conditional<kCh == 4, uint32_t, uint16_t>::type>::type vpiece;
   vpiece vr[kItems][4];
   typedef const __attribute__((address_space(4))) float *scalar_ptr;
   const scalar_ptr ksp = (scalar_ptr)(a.ks + r * a.nblk), vsp = (scalar_ptr)(a.vs + r * a.nblk);
   float ks_next = 0.0f, vs_next = 0.0f;
-  auto load = [&](int i) {
-    if (i >= last) return;
-    const int b = span.block(i);
-    const RowsWith<0> k(a.k8, r * a.cap, b, span.end, D), v(a.v8, r * a.cap, b, span.end, D);
+  auto load_keys = [&](int i) __attribute__((always_inline)) {
+    const int b = i < last ? span.block(i) : 0;
+    const RowsWith<0> k(a.k8, r * a.cap, b, i < last ? span.end : 0, D);
 #pragma unroll
-    for (int x = 0; x < kKeys; ++x) kr[x] = k.load16(16 * (x * kThreads + tid));
+    for (int x = 0; x < kKeys; ++x)  // direct: every other piece of token 32 (x / (kSteps / 2)) + col
+      kr[x] = k.load16(kDirect ? (32 * (x / (kSteps / 2)) + col) * D + 32 * (x % (kSteps / 2)) + 16 * half : 16 * (x * kThreads + tid));
+    ks_next = ksp[b];
+    vs_next = vsp[b];
+  };
+  auto load_values = [&](int i) __attribute__((always_inline)) {
+    // A load of 128 channels' values covers two whole lines: as streams they leave the caches to K, whose lines take four loads
+    // each (8 rows of 262144 tokens, 4 x 4 queries: 105 us; 89.  With K as streams too 118).
+    const RowsWith<kDirect && D == 128 ? kStream : 0> v(a.v8, r * a.cap, i < last ? span.block(i) : 0, i < last ? span.end : 0, D);
 #pragma unroll
-    for (int x = 0; x < kItems; ++x) {
-      const int item = x * kThreads + tid, at = item / (D / kCh) * 4 * D + item % (D / kCh) * kCh;
+    for (int x = 0; x < kItems; ++x) {  // direct: channels kCh col .. of tokens 8 x + 4 half ..
+      const int item = x * kThreads + tid, at = kDirect ? (8 * x + 4 * half) * D + kCh * col : item / (D / kCh) * 4 * D + item % (D / kCh) * kCh;
 #pragma unroll
       for (int j = 0; j < 4; ++j) v.load(at + j * D, vr[x][j]);
     }
-    ks_next = ksp[b];
-    vs_next = vsp[b];
-    if (!(fabsf(vs_next) < INFINITY)) vs_next = 0.0f;  // counted behind the loop
   };
-  auto mark = [&](int i) {
+  auto load = [&](int i) __attribute__((always_inline)) {
+    load_keys(i);
+    load_values(i);
+  };
+  auto mark = [&](int i) __attribute__((always_inline)) {
     atomicMin(&odd[group][0], i);
     atomicMax(&odd[group][1], i);
   };
-  auto stage = [&](int buf, int i) {
+  // A NaN among the thread's codes of V counts as 0, and is counted behind the loop.
+  auto clear_values = [&](int i) __attribute__((always_inline)) {
+    if constexpr (!I8) {
+      uint32_t nan = 0;
+#pragma unroll
+      for (int x = 0; x < 4 * kItems; ++x)
+#pragma unroll
+        for (int d = 0; d < (kCh + 3) / 4; ++d) nan |= nan_bytes(dword_of(vr[x / 4][x % 4], d));
+      if (__builtin_expect(nan != 0, 0)) {
+        mark(i);
+#pragma unroll
+        for (int x = 0; x < 4 * kItems; ++x) clear_nans(vr[x / 4][x % 4]);
+      }
+    }
+  };
+  auto stage = [&](int buf, int i) __attribute__((always_inline)) {
     if (i >= last) return;
-    if (tid == 0 && !(fabsf(vsp[span.block(i)]) < INFINITY)) mark(i);
 #pragma unroll
     for (int x = 0; x < kKeys; ++x) {
       const int at = x * kThreads + tid, tok = at / (D / 16), piece = at % (D / 16);
@@ -367,29 +398,18 @@ __global__ __launch_bounds__(kMultiThreads, RW == 1 && D == 128 ? 1 : 2) void mu
           w[2 * e + 1] = __builtin_bit_cast(uint32_t, pair16<I8, true>(c));
         }
       }
-      char *row = reinterpret_cast<char *>(lds[group][buf][0]) + tok * 2 * D;
+      char *row = lds[group] + 2 * buf * kCodes + tok * 2 * D;
 #pragma unroll
       for (int h = 0; h < 2; ++h)
         *reinterpret_cast<u32x4 *>(row + 16 * ((2 * piece + h) ^ (tok & (D / 8 - 1)))) = u32x4{w[4 * h], w[4 * h + 1], w[4 * h + 2], w[4 * h + 3]};
     }
-    if constexpr (!I8) {  // a NaN in V is staged as 0, and counted behind the loop
-      uint32_t nan = 0;
-#pragma unroll
-      for (int x = 0; x < 4 * kItems; ++x)
-#pragma unroll
-        for (int d = 0; d < kCh / 4; ++d) nan |= nan_bytes(dword_of(vr[x / 4][x % 4], d));
-      if (__builtin_expect(nan != 0, 0)) {
-        mark(i);
-#pragma unroll
-        for (int x = 0; x < 4 * kItems; ++x) clear_nans(vr[x / 4][x % 4]);
-      }
-    }
+    clear_values(i);
 #pragma unroll
     for (int x = 0; x < kItems; ++x) {
       const int item = x * kThreads + tid, quad = item / (D / kCh), ch0 = item % (D / kCh) * kCh;
       // tokens 4 quad ..: half (quad >> 1 & 1) of the piece that lane half quad & 1 reads for 16 tokens
       const int piece = (quad >> 3) * 4 + (quad >> 2 & 1) * 2 + (quad & 1);
-      char *base = reinterpret_cast<char *>(lds[group][buf][1]) + 8 * (quad >> 1 & 1);
+      char *base = lds[group] + (2 * buf + 1) * kCodes + 8 * (quad >> 1 & 1);
 #pragma unroll
       for (int d = 0; d < kCh / 4; ++d) {
         uint32_t w[4];
@@ -420,27 +440,40 @@ __global__ __launch_bounds__(kMultiThreads, RW == 1 && D == 128 ? 1 : 2) void mu
 
   // Bit 16 x + e: whether the query sees token at + 32 x + 8 (e / 4) + e % 4.  Those places rise with the bit, so the bits
   // of tokens before t are the lowest ones, four for each eight tokens.
-  auto seen_of = [&](int at) {
+  auto seen_of = [&](int at) __attribute__((always_inline)) {
     auto before = [&](int t) {
       const int n = t - at, bits = n <= 0 ? 0 : 4 * (n >> 3) + ((n & 7) < 4 ? n & 7 : 4);
       return bits >= 32 ? 0xFFFFFFFFu : (1u << bits) - 1u;
     };
     return before(end) & ~(before(lo) & ~before(from));
   };
-  auto block = [&](int buf, int i, float ks, float vs) {
-    const int t0 = span.block(i) * kBlk;
-    if (!__any(t0 < end && (t0 + kBlk > lo || t0 < from))) return;
-    const bool edge = !__all(t0 + kBlk <= end && (t0 >= lo || t0 + kBlk <= from));
-    // ---- scores; operands are read kAhead products ahead
-    f32x16 s[2];
-    const char *kb = reinterpret_cast<const char *>(lds[group][buf][0]) + col * 2 * D;
+  // ---- scores; operands are read kAhead products ahead
+  f32x16 s[2];
+  auto scores = [&](int buf) __attribute__((always_inline)) {
+    const char *kb = lds[group] + 2 * buf * kCodes + col * 2 * D;
     frag kf[2][kAhead];
-    auto keys = [&](int n) {  // of steps kAhead n ..: tokens 32 (kAhead n / kSteps) ..
+    auto key = [&](int x, int c) __attribute__((always_inline)) {  // of tokens 32 x .., step c
+      if constexpr (kDirect) {
+        uint32_t w[4];
 #pragma unroll
-      for (int c = 0; c < kAhead; ++c) {
-        const int x = kAhead * n / kSteps, piece = 2 * (kAhead * n % kSteps + c) + half;
-        kf[n & 1][c] = *reinterpret_cast<const frag *>(kb + 64 * D * x + 16 * (piece ^ (col & (D / 8 - 1))));
+        for (int e = 0; e < 2; ++e) {
+          const uint32_t code = flip_sign<I8>(kr[x * (kSteps / 2) + c / 2][2 * (c & 1) + e]);
+          if constexpr (kBf16) {
+            w[2 * e] = pair_bf16<I8, false>(code);
+            w[2 * e + 1] = pair_bf16<I8, true>(code);
+          } else {
+            w[2 * e] = __builtin_bit_cast(uint32_t, pair16<I8, false>(code));
+            w[2 * e + 1] = __builtin_bit_cast(uint32_t, pair16<I8, true>(code));
+          }
+        }
+        return __builtin_bit_cast(frag, u32x4{w[0], w[1], w[2], w[3]});
+      } else {
+        return *reinterpret_cast<const frag *>(kb + 64 * D * x + 16 * ((2 * c + half) ^ (col & (D / 8 - 1))));
       }
+    };
+    auto keys = [&](int n) __attribute__((always_inline)) {  // of products kAhead n ..: the block's two halves in turn
+#pragma unroll
+      for (int c = 0; c < kAhead; ++c) kf[n & 1][c] = key((kAhead * n + c) % 2, (kAhead * n + c) / 2);
     };
 #pragma unroll
     for (int x = 0; x < 2; ++x)
@@ -448,18 +481,21 @@ __global__ __launch_bounds__(kMultiThreads, RW == 1 && D == 128 ? 1 : 2) void mu
       for (int e = 0; e < 16; ++e) s[x][e] = 0.0f;
     if constexpr (QT == FATHOM_DT_F32) {
       if (__builtin_expect(far, 0)) {  // what two f16 leave of small channels, formed anew from the queries
-#pragma unroll 1
-        for (int c = 0; c < kSteps; ++c) {
+        auto left = [&](int c) __attribute__((always_inline)) {
           float x[8];
-          load8_q(a.q, QT, q_at + 16 * c, x);
-          f16x8 left;
+          load8_q(a.q, QT, q_at + channel(c), x);
+          f16x8 v;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) left[e] = (_Float16)rest_of(ldexpf(x[e], -exq));
+          for (int e = 0; e < 8; ++e) v[e] = (_Float16)rest_of(ldexpf(x[e], -exq));
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const f16x8 k = *reinterpret_cast<const f16x8 *>(kb + 64 * D * h + 16 * ((2 * c + half) ^ (col & (D / 8 - 1))));
-            s[h] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, left, s[h], 0, 0, 0);
-          }
+          for (int h = 0; h < 2; ++h) s[h] = __builtin_amdgcn_mfma_f32_32x32x16_f16(key(h, c), v, s[h], 0, 0, 0);
+        };
+        if constexpr (kDirect) {  // the registers of K need constant places
+#pragma unroll
+          for (int c = 0; c < kSteps; ++c) left(c);
+        } else {
+#pragma unroll 1
+          for (int c = 0; c < kSteps; ++c) left(c);
         }
 #pragma unroll
         for (int h = 0; h < 2; ++h) s[h] *= 0x1p-38f;
@@ -474,18 +510,43 @@ __global__ __launch_bounds__(kMultiThreads, RW == 1 && D == 128 ? 1 : 2) void mu
       for (int c = 0; c < kAhead; ++c)
 #pragma unroll
         for (int p = kParts - 1; p >= 0; --p) {
-          const int x = kAhead * n / kSteps, step = kAhead * n % kSteps + c;
+          const int x = (kAhead * n + c) % 2, step = (kAhead * n + c) / 2;
           if constexpr (kBf16) s[x] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[n & 1][c], qf[p][step], s[x], 0, 0, 0);
           else s[x] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[n & 1][c], qf[p][step], s[x], 0, 0, 0);
         }
     }
-    const char *vb = reinterpret_cast<const char *>(lds[group][buf][1]);
+  };
+  // ---- their weights, and the values' products
+  auto block = [&](int buf, int i, float ks, float vs) __attribute__((always_inline)) {
+    const int t0 = span.block(i) * kBlk;
+    const bool edge = !__all(t0 + kBlk <= end && (t0 >= lo || t0 + kBlk <= from));
+    const char *vb = lds[group] + (2 * buf + 1) * kCodes;
     f16x8 vf[kVBufs][kTiles];
-    auto values = [&](int n) {  // of tokens 16 n ..
+    auto values = [&](int n) __attribute__((always_inline)) {  // of tokens 16 n ..
+      if constexpr (kDirect) {
+        f16x2 v[2][2][kTiles];  // of tokens 8 x + 4 half + 2 y, + 1 and channel kTiles col + d
 #pragma unroll
-      for (int d = 0; d < kTiles; ++d) {
-        const int ch = 32 * d + col, piece = 2 * n + half;
-        vf[n % kVBufs][d] = *reinterpret_cast<const f16x8 *>(vb + ch * 2 * kBlk + 16 * (piece ^ ((ch ^ ch >> 3) & 7)));
+        for (int x = 0; x < 2; ++x) {
+          uint32_t w[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) w[j] = flip_sign<I8>(dword_of(vr[2 * n + x][j], 0));
+#pragma unroll
+          for (int y = 0; y < 2; ++y)
+#pragma unroll
+            for (int d = 0; d < kTiles; d += 2) {
+              const uint32_t ab = __builtin_amdgcn_perm(w[2 * y + 1], w[2 * y], d ? 0x07030602u : 0x05010400u);
+              v[x][y][d] = pair16<I8, false>(ab);
+              v[x][y][d + 1] = pair16<I8, true>(ab);
+            }
+        }
+#pragma unroll
+        for (int d = 0; d < kTiles; ++d) vf[n % kVBufs][d] = join8(v[0][0][d], v[0][1][d], v[1][0][d], v[1][1][d]);
+      } else {
+#pragma unroll
+        for (int d = 0; d < kTiles; ++d) {
+          const int ch = 32 * d + col, piece = 2 * n + half;
+          vf[n % kVBufs][d] = *reinterpret_cast<const f16x8 *>(vb + ch * 2 * kBlk + 16 * (piece ^ ((ch ^ ch >> 3) & 7)));
+        }
       }
     };
     if (kVBufs == 2) values(0);
@@ -535,6 +596,7 @@ __global__ __launch_bounds__(kMultiThreads, RW == 1 && D == 128 ? 1 : 2) void mu
     }
     if (edge) {
       asm volatile("");  // a branch, not selects in every block
+      if constexpr (kDirect) clear_values(i);  // what all queries see makes NaN by itself
       const uint32_t seen = seen_of(at);
 #pragma unroll
       for (int b = 0; b < 32; ++b) {
@@ -589,6 +651,7 @@ __global__ __launch_bounds__(kMultiThreads, RW == 1 && D == 128 ? 1 : 2) void mu
     float sum = 0.0f;
 #pragma unroll
     for (int n = 0; n < 4; ++n) {
+      if (kDirect) __builtin_amdgcn_sched_barrier(0);
       if (kVBufs == 1) values(n);
       else if (n < 3) values(n + 1);
       float w[8];
@@ -625,33 +688,51 @@ __global__ __launch_bounds__(kMultiThreads, RW == 1 && D == 128 ? 1 : 2) void mu
     }
   };
 
-  // Groups of one wave need no barrier: its LDS operations are in order.
-  auto sync = [&]() {
-    if constexpr (RW == 1) {
-      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
-      __builtin_amdgcn_wave_barrier();
-      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
-    } else {
-      barrier_lds();
-    }
-  };
   if (tid < 2) odd[group][tid] = tid ? -1 : 0x7FFFFFFF;
   load(first + group);
-  float ks = ks_next, vs = vs_next;
-  sync();  // `odd` is set before a thread changes it
-  stage(0, first + group);
-  load(first + group + kGroups);
-  sync();
-  int buf = 0;
-  for (int i = first + group; i < last; i += kGroups) {
-    block(buf, i, ks, vs);
-    ks = ks_next;
-    vs = vs_next;
-    if constexpr (kBufs == 1) sync();
-    else buf ^= 1;
-    stage(buf, i + kGroups);
-    load(i + 2 * kGroups);
-    sync();
+  __syncthreads();  // `odd` is set before a thread changes it
+  // Of a block that none of the wave's queries sees, nothing is formed.
+  auto seen = [&](int i) __attribute__((always_inline)) {
+    const int t0 = span.block(i) * kBlk;
+    return __any(t0 < end && (t0 + kBlk > lo || t0 < from)) != 0;
+  };
+  // A block's scale of V, and 0 for one that is not finite: that is counted behind the loop.
+  auto scale_of = [&](int i, float vs) __attribute__((always_inline)) {
+    if (fabsf(vs) < INFINITY) return vs;
+    if (lane == 0) mark(i);
+    return 0.0f;
+  };
+  if constexpr (kDirect) {  // the next block's K is requested once the scores are formed, its V once the products are
+    for (int i = first + group; i < last; i += kGroups) {
+      const float ks = ks_next, vs = scale_of(i, vs_next);
+      const bool some = seen(i);
+      if (some) scores(0);
+      __builtin_amdgcn_sched_barrier(0);
+      load_keys(i + kGroups);
+      __builtin_amdgcn_sched_barrier(0);
+      if (some) block(0, i, ks, vs);
+      __builtin_amdgcn_sched_barrier(0);
+      load_values(i + kGroups);
+    }
+    __syncthreads();
+  } else {
+    float ks = ks_next, vs = vs_next;
+    stage(0, first);
+    load(first + 1);
+    barrier_lds();
+    for (int i = first; i < last; ++i) {
+      const int buf = (i - first) & 1;
+      vs = scale_of(i, vs);
+      if (seen(i)) {
+        scores(buf);
+        block(buf, i, ks, vs);
+      }
+      ks = ks_next;
+      vs = vs_next;
+      stage(buf ^ 1, i + 1);
+      load(i + 2);
+      barrier_lds();
+    }
   }
 
   // A NaN in V makes the results of the queries that see its token NaN in its channel, and no others; a scale of V that is
@@ -674,7 +755,7 @@ __global__ __launch_bounds__(kMultiThreads, RW == 1 && D == 128 ? 1 : 2) void mu
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
             const int t = at + 2 * b + 8 * (e / 4) + e % 4;
-            const uint32_t c = t < span.end ? a.v8[(r * a.cap + t) * D + 32 * d + col] : 0u;
+            const uint32_t c = t < span.end ? a.v8[(r * a.cap + t) * D + (kDirect ? kTiles * col + d : 32 * d + col)] : 0u;
             is[e] = whole || (!I8 && (c & 0x7F) == 0x7F) ? (_Float16)1.0f : (_Float16)0.0f;
             sees[e] = seen >> (b + e) & 1 ? (_Float16)1.0f : (_Float16)0.0f;
           }
@@ -689,21 +770,17 @@ __global__ __launch_bounds__(kMultiThreads, RW == 1 && D == 128 ? 1 : 2) void mu
   l += other_half(l);
   const bool parts = a.parts;
   const int64_t slot = parts ? ((int64_t)blockIdx.x * kRows) : 0;
-  if constexpr (RW == 1) {  // ---- the waves' sums over their blocks, in the LDS that held those
+  if constexpr (kDirect) {  // ---- the waves' sums over their blocks
     __shared__ float wm[kMultiWaves][32], wl[kMultiWaves][32];
-    constexpr int kPitch = D + 4;
-    float *mine_at = reinterpret_cast<float *>(lds[group][0][0]) + col * kPitch + 4 * half;
+    typedef float piece __attribute__((ext_vector_type(kTiles)));
+    float *mine_at = reinterpret_cast<float *>(lds[group]) + col * kPitch;
 #pragma unroll
-    for (int d = 0; d < kTiles; ++d)
+    for (int e = 0; e < 16; ++e) {  // register e of o[d] is channel kTiles (8 (e / 4) + 4 half + e % 4) + d
+      piece v;
 #pragma unroll
-      for (int e = 0; e < 16; e += 4) {
-        float4 v;
-        v.x = ldexpf(o[d][e], (int)(E - kStart));
-        v.y = ldexpf(o[d][e + 1], (int)(E - kStart));
-        v.z = ldexpf(o[d][e + 2], (int)(E - kStart));
-        v.w = ldexpf(o[d][e + 3], (int)(E - kStart));
-        *reinterpret_cast<float4 *>(mine_at + 32 * d + 2 * e) = v;
-      }
+      for (int d = 0; d < kTiles; ++d) v[d] = ldexpf(o[d][e], (int)(E - kStart));
+      *reinterpret_cast<piece *>(mine_at + kTiles * (8 * (e / 4) + 4 * half + e % 4)) = v;
+    }
     if (half == 0) {
       wm[wave][col] = base + kStart;
       wl[wave][col] = ldexpf(l, -(int)kStart);
@@ -720,7 +797,7 @@ __global__ __launch_bounds__(kMultiThreads, RW == 1 && D == 128 ? 1 : 2) void mu
 #pragma unroll
       for (int v = 0; v < kMultiWaves; ++v) {
         const float f = __builtin_amdgcn_exp2f(wm[v][row] - big);
-        const float4 u = *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(lds[v][0][0]) + row * kPitch + c);
+        const float4 u = *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(lds[v]) + row * kPitch + c);
         L = fmaf(wl[v][row], f, L);
         out[0] = fmaf(u.x, f, out[0]);
         out[1] = fmaf(u.y, f, out[1]);

@@ -247,17 +247,20 @@ __device__ __forceinline__ float add_other_half(float v) {
 }
 
 // The blocks of a row that a call takes: the first `sink` ones and, `skip` blocks further, those of the window, nb in
-// all.  Tokens of them that take no part: [from, lo), and from len on.
+// all.  Tokens of them that take no part: [from, lo), and from len on.  Without sinks, from = sink = 0.
+template <bool SINKS>
 struct Span {
   int len, lo, from, sink, skip, nb;
-  __device__ __forceinline__ int block(int i) const { return i < sink ? i : i + skip; }  // the i-th of them
+  __device__ __forceinline__ int block(int i) const { return SINKS && i < sink ? i : i + skip; }  // the i-th of them
 };
-__device__ __forceinline__ Span row_span(const AttnArgs &a, int64_t bh) {
-  Span s;
+template <bool SINKS>
+__device__ __forceinline__ Span<SINKS> row_span(const AttnArgs &a, int64_t bh) {
+  Span<SINKS> s;
   s.len = (int)row_length(a.lens, a.n, a.cap, bh);
   s.lo = a.window > 0 && s.len > a.window ? s.len - (int)a.window : 0;
-  s.from = a.sinks < s.lo ? (int)a.sinks : s.lo;
-  const int first = s.lo / kBlk, sink = (s.from + kBlk - 1) / kBlk;
+  const int first = s.lo / kBlk;
+  s.from = !SINKS ? 0 : a.sinks < s.lo ? (int)a.sinks : s.lo;
+  const int sink = (s.from + kBlk - 1) / kBlk;
   s.sink = sink < first ? sink : first;  // the last sinks may be in the window's first block
   s.skip = first - s.sink;
   s.nb = (s.len + kBlk - 1) / kBlk - s.skip;
@@ -274,8 +277,9 @@ struct Part {
 // blocks, which gives `per`, and finds its row in the prefix sums of ceil(blocks /
 // per).  Those are at most kDenseTotal / kDenseWaves / head groups + BH, the grid.  (32
 // bits hold the sums: 2^31 blocks of D = 64 are 17 TB.)
+template <bool SINKS>
 __device__ __forceinline__ uint32_t blocks_of(const AttnArgs &a, int r) {
-  return r < (int)a.BH ? (uint32_t)row_span(a, r).nb : 0u;
+  return r < (int)a.BH ? (uint32_t)row_span<SINKS>(a, r).nb : 0u;
 }
 // Blocks per workgroup.  A row's last workgroup may have less to do: with few rows the
 // share leaves room for those, so that all of the call's workgroups are at work at once.
@@ -290,9 +294,10 @@ __device__ __forceinline__ uint32_t groups_of(const AttnArgs &a, int r, uint32_t
 }
 
 // Up to 64 rows: a lane per row, each wave for itself.
+template <bool SINKS>
 __device__ __forceinline__ Part find_part(const AttnArgs &a, uint32_t w) {
   const int lane = threadIdx.x & 63;
-  const uint32_t nb = blocks_of(a, lane), per = share_of(a, __builtin_amdgcn_readlane(wave_incl_scan_u32(nb), 63));
+  const uint32_t nb = blocks_of<SINKS>(a, lane), per = share_of(a, __builtin_amdgcn_readlane(wave_incl_scan_u32(nb), 63));
   const uint32_t act = groups_of(a, lane, nb, per), upto = wave_incl_scan_u32(act);
   const uint64_t past = __ballot(upto > w);
   if (!past) return Part{a.BH, 0, 0, 0};  // the call needs no such workgroup
@@ -307,12 +312,13 @@ struct FindShared {
   uint32_t wave[2][kDenseWaves];
   int part[4];
 };
+template <bool SINKS>
 __device__ __forceinline__ Part find_part_wide(const AttnArgs &a, uint32_t w, FindShared &sh) {
   constexpr int kThreads = kDenseWaves * kWave;
   const int tid = threadIdx.x, wave = tid >> 6;
   const int c = ((int)a.BH + kThreads - 1) / kThreads, r0 = tid * c;
   uint32_t sum = 0;
-  for (int i = 0; i < c; ++i) sum += blocks_of(a, r0 + i);
+  for (int i = 0; i < c; ++i) sum += blocks_of<SINKS>(a, r0 + i);
   sum = wave_incl_scan_u32(sum);
   if ((tid & 63) == 63) sh.wave[0][wave] = sum;
   if (tid == 0) sh.part[0] = (int)a.BH;
@@ -322,7 +328,7 @@ __device__ __forceinline__ Part find_part_wide(const AttnArgs &a, uint32_t w, Fi
   for (int v = 0; v < kDenseWaves; ++v) total += sh.wave[0][v];
   const uint32_t per = share_of(a, total);
   uint32_t mine = 0;
-  for (int i = 0; i < c; ++i) mine += groups_of(a, r0 + i, blocks_of(a, r0 + i), per);
+  for (int i = 0; i < c; ++i) mine += groups_of(a, r0 + i, blocks_of<SINKS>(a, r0 + i), per);
   uint32_t upto = wave_incl_scan_u32(mine);
   if ((tid & 63) == 63) sh.wave[1][wave] = upto;
   __syncthreads();
@@ -330,7 +336,7 @@ __device__ __forceinline__ Part find_part_wide(const AttnArgs &a, uint32_t w, Fi
   uint32_t at = upto - mine;
   if (w >= at && w < upto)
     for (int i = 0; i < c; ++i) {
-      const uint32_t act = groups_of(a, r0 + i, blocks_of(a, r0 + i), per);
+      const uint32_t act = groups_of(a, r0 + i, blocks_of<SINKS>(a, r0 + i), per);
       if (w < at + act) {
         sh.part[0] = r0 + i;
         sh.part[1] = (int)(w - at);
@@ -372,6 +378,7 @@ __device__ __forceinline__ Part find_part_wide(const AttnArgs &a, uint32_t w, Fi
 //     tokens and pairs two tokens' bytes with one v_perm.
 // Rows are read through buffer descriptors that end at the row's length: what lies
 // behind it reads as zeros.
+// SINKS is a parameter as its masks cost calls without sinks 1 to 6 % (1 x 1000 tokens 10.5 us; 11.2).
 //
 // Bound: HBM, 2 D bytes per token and group of 16 heads: more heads read the rows once for each (8 x 65536
 // tokens of 32 heads 46 to 53 us, 1.4 times the rows' bytes from HBM; of 12 heads 34, with cap and bias 39).
@@ -380,7 +387,7 @@ __device__ __forceinline__ Part find_part_wide(const AttnArgs &a, uint32_t w, Fi
 // NG = 1), a third of the time that its rows take.  8 x 1048576 tokens of 4 heads (2.15 GB) 304 us, 7.1 TB/s; 32 x
 // 32768 (0.27 GB) 46 us with the join of the splits; one dot product per lane group and no matrix
 // cores: 917 and 127 us.  Short rows are bound by latency: the launch, the rows' way from HBM, one block's arithmetic.
-template <int D, bool I8, int NG, bool EXTRA, int NW>
+template <int D, bool I8, int NG, bool EXTRA, int NW, bool SINKS>
 __global__ __launch_bounds__(NW *kWave, 2) void dense_kernel(AttnArgs a) {
   constexpr int kHalves = D / 64;  // 16-byte pieces of a row per lane
   constexpr int kSteps = D / 32;   // matrix instructions along the channels
@@ -393,17 +400,17 @@ __global__ __launch_bounds__(NW *kWave, 2) void dense_kernel(AttnArgs a) {
   int64_t slot = (int64_t)blockIdx.z * a.nsplit + blockIdx.x;  // of the partial results
   if (NW == kDenseWaves && a.where) {  // uniform over the workgroup
     if (a.BH <= kWave) {
-      part = find_part(a, blockIdx.x);
+      part = find_part<SINKS>(a, blockIdx.x);
     } else {
       __shared__ FindShared find;
-      part = find_part_wide(a, blockIdx.x, find);
+      part = find_part_wide<SINKS>(a, blockIdx.x, find);
     }
     if (part.bh >= a.BH) return;
     slot = blockIdx.x;
     if (part.split == 0 && blockIdx.y == 0 && tid == 0) a.where[part.bh] = make_int2((int)blockIdx.x, part.active);
   }
   const int64_t bh = part.bh;
-  const Span span = row_span(a, bh);
+  const Span<SINKS> span = row_span<SINKS>(a, bh);
   const int lo = span.lo, len = span.len;
   if (!a.where) part.per = (span.nb + part.active - 1) / part.active;
   const int first = part.split * part.per;  // of the row's blocks in the order of span.block
@@ -646,11 +653,22 @@ __global__ __launch_bounds__(NW *kWave, 2) void dense_kernel(AttnArgs a) {
         f = 1.0f;
       }
       if (edge) {
-        const uint32_t none = left_out();
+        if constexpr (SINKS) {
+          const uint32_t none = left_out();
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+          for (int i = 0; i < 4; ++i)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) s[n][i][j] = none >> (4 * i + j) & 1 ? -INFINITY : s[n][i][j];
+            for (int j = 0; j < 4; ++j) s[n][i][j] = none >> (4 * i + j) & 1 ? -INFINITY : s[n][i][j];
+        } else {
+          asm volatile("");  // a branch, not selects in every block
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const int t = in_block + 16 * i + j;
+              s[n][i][j] = t >= lo && t < len ? s[n][i][j] : -INFINITY;
+            }
+        }
       }
       float mx = -INFINITY;
 #pragma unroll
@@ -686,12 +704,12 @@ __global__ __launch_bounds__(NW *kWave, 2) void dense_kernel(AttnArgs a) {
 #pragma unroll
     for (int n = 0; n < NG; ++n) wv[n] = ldexpf(vs, 14 - (int)ceilf(R[n]));
     if (edge) {  // a token outside has no value either (its codes may be NaN)
-      const uint32_t none = left_out();
+      const uint32_t none = SINKS ? left_out() : 0;
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          if (none >> (4 * i + j) & 1) vr[i][j] = vpiece{};
+          if (SINKS ? none >> (4 * i + j) & 1 : in_block + 16 * i + j < lo) vr[i][j] = vpiece{};
     }
     // ---- weights and products, 32 tokens at a time
 #pragma unroll
@@ -966,8 +984,11 @@ int run_list(AttnArgs a, int64_t BH, int64_t D, bool i8, hipStream_t st) {
 template <int D, bool I8, int NG, int NW>
 void launch_dense(const AttnArgs &a, int64_t BH, hipStream_t st) {
   const dim3 grid((unsigned)a.nsplit, (unsigned)head_groups(a.G), a.where ? 1u : (unsigned)BH);
-  if (a.softcap > 0.0f || a.slopes) dense_kernel<D, I8, NG, true, NW><<<grid, NW * kWave, 0, st>>>(a);
-  else dense_kernel<D, I8, NG, false, NW><<<grid, NW * kWave, 0, st>>>(a);
+  const bool extra = a.softcap > 0.0f || a.slopes, sinks = a.sinks > 0 && a.window > 0;
+  if (extra && sinks) dense_kernel<D, I8, NG, true, NW, true><<<grid, NW * kWave, 0, st>>>(a);
+  else if (extra) dense_kernel<D, I8, NG, true, NW, false><<<grid, NW * kWave, 0, st>>>(a);
+  else if (sinks) dense_kernel<D, I8, NG, false, NW, true><<<grid, NW * kWave, 0, st>>>(a);
+  else dense_kernel<D, I8, NG, false, NW, false><<<grid, NW * kWave, 0, st>>>(a);
 }
 
 template <int D, bool I8>

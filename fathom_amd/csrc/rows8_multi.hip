@@ -84,8 +84,19 @@ void launch_join(const MultiArgs &a, const Tail &t, int out, hipStream_t st) {
   else join_kernel<D, FATHOM_DT_BF16><<<grid, kJoinThreads, 0, st>>>(a, t);
 }
 
-// Queries of a tile: one wave's, where a row has no more.
-int tile_rows(int64_t M) { return M <= 32 ? 32 : 128; }
+// Queries of a tile of rows that see up to nb blocks: one wave's, where a row has no more; eight waves', which stage a block for
+// twice the queries (8 x 4 x 2048 over 65536 tokens 2.22 ms; by fours 2.44), where that leaves no more of their places empty or the
+// queries are many, and there is work for all CUs in shares of four blocks (512 queries of 4 rows over 4096 tokens 42 us; 38).
+// `four`: float32 queries and calls with a cap or bias take four waves.  Their registers or a block's longer way leave eight
+// to wait for the slowest (f32, 8 x 4 x 1024 over 16384 tokens 797 us; 728.  Capped and biased, 4 x 12 x 3001 behind a window of
+// 4096: 535; 464).
+int tile_rows(int64_t BH, int64_t M, int64_t nb, bool four) {
+  if (M <= 32) return 32;
+  const int64_t eights = cdiv(M, (int64_t)256);
+  return !four && (M >= 2048 || eights * 2 == cdiv(M, (int64_t)128)) && BH * eights * cdiv(nb, (int64_t)4) >= 256 ? 256 : 128;
+}
+
+bool takes_four(const MultiArgs &a, int q_dtype) { return q_dtype == FATHOM_DT_F32 || a.softcap > 0.0f || a.slopes; }
 
 // Shares that tiles of up to nb blocks are cut into (at most that many and one per tile more); 0: a workgroup takes each tile.
 // `places` workgroups are at work at once, two per CU.  Few tiles are cut so that all places
@@ -93,9 +104,8 @@ int tile_rows(int64_t M) { return M <= 32 ? 32 : 128; }
 // rounds, as every tile's last share is shorter; of shares, a workgroup's partial results cost about four blocks.  More tiles
 // even out by themselves, those that see most first.  (32 ragged rows of 572 tokens, 576 tiles: 509 us a workgroup per tile, 283
 // in five rounds.)
-int64_t tile_shares(int64_t BH, int64_t M, int64_t D, int64_t nb, bool even) {
-  const int rows = tile_rows(M);
-  const int64_t tiles = BH * cdiv(M, (int64_t)rows), places = 512;
+int64_t tile_shares(int64_t BH, int64_t M, int rows, int64_t nb, bool even) {
+  const int64_t tiles = BH * cdiv(M, (int64_t)rows), places = rows == 256 ? 256 : 512;
   if (nb <= (rows == 32 ? 16 : 4) || tiles >= 2 * places || (even && tiles > places / 2)) return 0;
   const int64_t rounds = cdiv(3 * tiles, places), most = tiles * cdiv(nb, (int64_t)4);
   const int64_t shares = rounds == 1 ? places - tiles : places * rounds - tiles * 5 / 8;
@@ -107,8 +117,8 @@ int64_t tile_splits(int64_t tiles, int64_t shares, int64_t nb) {
   return most < 1 ? 1 : room < most ? room : most;
 }
 // The same for a prefix, whose tiles always leave partial results.
-int64_t prefix_shares(int64_t BH, int64_t M, int64_t D, int64_t nb) {
-  const int64_t shares = tile_shares(BH, M, D, nb, true), tiles = BH * cdiv(M, (int64_t)tile_rows(M));
+int64_t prefix_shares(int64_t BH, int64_t M, int rows, int64_t nb) {
+  const int64_t shares = tile_shares(BH, M, rows, nb, true), tiles = BH * cdiv(M, (int64_t)rows);
   return shares > tiles ? shares : tiles;
 }
 
@@ -121,8 +131,7 @@ int64_t tile_blocks(int64_t n, int64_t T, int64_t window, int64_t sinks) {
 }
 
 // Bytes of the partial results of so many shares and of the tiles' slots.
-size_t multi_bytes(int64_t BH, int64_t M, int64_t D, int64_t shares) {
-  const int rows = tile_rows(M);
+size_t multi_bytes(int64_t BH, int64_t M, int rows, int64_t D, int64_t shares) {
   const int64_t tiles = BH * cdiv(M, (int64_t)rows);
   return (size_t)((shares + tiles) * rows * (D + 2) + cdiv(2 * tiles, (int64_t)4) * 4) * sizeof(float);
 }
@@ -165,8 +174,13 @@ using namespace fathom::rows8;
 extern "C" size_t fathom_rows8_chunk_attention_workspace_bytes(int64_t BH, int64_t G, int64_t T, int64_t D, int64_t positions) {
   if (!shape_taken(BH, G, D) || !queries_taken(BH, G, T) || positions < 1) return 0;
   if (positions > kMaxCap) positions = kMaxCap;
-  const int64_t shares = tile_shares(BH, G * T, D, cdiv(positions, (int64_t)kBlk) + 1, false);
-  return shares ? multi_bytes(BH, G * T, D, shares) : 0;
+  size_t most = 0;  // of whichever tiles a call takes
+  for (const int rows : {32, 128, 256}) {
+    if ((rows == 32) != (G * T <= 32)) continue;
+    const int64_t shares = tile_shares(BH, G * T, rows, cdiv(positions, (int64_t)kBlk) + 1, false);
+    if (shares) most = std::max(most, multi_bytes(BH, G * T, rows, D, shares));
+  }
+  return most;
 }
 
 extern "C" int fathom_rows8_chunk_attention(const void *q, int q_dtype, int64_t q_row_stride, int64_t q_head_stride,
@@ -192,14 +206,15 @@ extern "C" int fathom_rows8_chunk_attention(const void *q, int q_dtype, int64_t 
   if (sinks > cap) sinks = cap;
   MultiArgs a{q, q_row_stride, q_head_stride, q_tok_stride, (const uint8_t *)k8, (const uint8_t *)v8, k_scale, v_scale, cap,
               cdiv(cap, kBlk), lens, n, (int)G, (int)T, (int)window, (int)sinks, false, nullptr, 0, 0, BH, scale,
-              kernel_cap(softcap), slopes, out, nullptr, nullptr, nullptr, 0, 1, tile_rows(G * T), 0, false};
-  a.tiles = (int)cdiv(G * T, (int64_t)a.rows);
+              kernel_cap(softcap), slopes, out, nullptr, nullptr, nullptr, 0, 1, 0, 0, false};
   const int64_t most = lens ? cap : n;
   const int64_t nb = tile_blocks(most, T, window, sinks);
+  a.rows = tile_rows(BH, G * T, nb, takes_four(a, q_dtype));
+  a.tiles = (int)cdiv(G * T, (int64_t)a.rows);
   const bool even = !lens && (window > 0 || most >= 4 * T);
-  a.shares = (int)tile_shares(BH, G * T, D, nb, even);
+  a.shares = (int)tile_shares(BH, G * T, a.rows, nb, even);
   if (a.shares) {
-    const size_t need = multi_bytes(BH, G * T, D, a.shares);
+    const size_t need = multi_bytes(BH, G * T, a.rows, D, a.shares);
     if (!workspace || workspace_bytes < need)
       return fail(FATHOM_ERR_WORKSPACE, "%s: workspace %zu bytes, need %zu", what, workspace_bytes, need);
     if (reinterpret_cast<uintptr_t>(workspace) & 15)
@@ -216,8 +231,13 @@ extern "C" size_t fathom_rows8_shared_attention_workspace_bytes(int64_t prefix_B
   if (!shape_taken(prefix_BH, G, D) || !queries_taken(prefix_BH, G, sequences) || sequences > kMaxRows / prefix_BH) return 0;
   if (prefix_positions > kMaxCap) prefix_positions = kMaxCap;
   if (prefix_positions < 0) prefix_positions = 0;
-  const int64_t shares = prefix_shares(prefix_BH, G * sequences, D, cdiv(prefix_positions, (int64_t)kBlk));
-  return multi_bytes(prefix_BH, G * sequences, D, shares) + tail_bytes(prefix_BH * sequences, G, D, positions < 0 ? 0 : positions);
+  size_t most = 0;  // of whichever tiles a call takes
+  for (const int rows : {32, 128, 256}) {
+    if ((rows == 32) != (G * sequences <= 32)) continue;
+    const int64_t shares = prefix_shares(prefix_BH, G * sequences, rows, cdiv(prefix_positions, (int64_t)kBlk));
+    most = std::max(most, multi_bytes(prefix_BH, G * sequences, rows, D, shares));
+  }
+  return most + tail_bytes(prefix_BH * sequences, G, D, positions < 0 ? 0 : positions);
 }
 
 extern "C" int fathom_rows8_shared_attention(const void *q, int q_dtype, const void *prefix_k8, const void *prefix_v8,
@@ -242,16 +262,18 @@ extern "C" int fathom_rows8_shared_attention(const void *q, int q_dtype, const v
     return fail(FATHOM_ERR_INVALID, "%s: %lld sequences, G=%lld, at most %lld queries per row and 2^27 in all", what, (long long)sequences, (long long)G, (long long)kMaxTiles * 32);
   MultiArgs a{q, G * D, D, prefix_BH * G * D, (const uint8_t *)prefix_k8, (const uint8_t *)prefix_v8, prefix_k_scale,
               prefix_v_scale, prefix_cap, cdiv(prefix_cap, kBlk), prefix_lens, prefix_n, (int)G, (int)sequences, 0, 0, true,
-              lens, n, cap, prefix_BH, scale, kernel_cap(softcap), slopes, out, nullptr, nullptr, nullptr, 1, 1, tile_rows(G * sequences), 0, false};
+              lens, n, cap, prefix_BH, scale, kernel_cap(softcap), slopes, out, nullptr, nullptr, nullptr, 1, 1, 0, 0, false};
+  const int64_t nb = cdiv(prefix_lens ? prefix_cap : prefix_n, (int64_t)kBlk);
+  a.rows = tile_rows(prefix_BH, G * sequences, nb, takes_four(a, q_dtype));
   a.tiles = (int)cdiv(G * sequences, (int64_t)a.rows);
-  a.shares = (int)prefix_shares(prefix_BH, G * sequences, D, cdiv(prefix_lens ? prefix_cap : prefix_n, (int64_t)kBlk));
-  const size_t first = multi_bytes(prefix_BH, G * sequences, D, a.shares);
+  a.shares = (int)prefix_shares(prefix_BH, G * sequences, a.rows, nb);
+  const size_t first = multi_bytes(prefix_BH, G * sequences, a.rows, D, a.shares);
   if (!workspace || workspace_bytes < first)
     return fail(FATHOM_ERR_WORKSPACE, "%s: workspace %zu bytes, need more than %zu", what, workspace_bytes, first);
   if (reinterpret_cast<uintptr_t>(workspace) & 15)
     return fail(FATHOM_ERR_INVALID, "%s: the workspace must be 16-byte aligned", what);
   place(a, workspace, D);
-  if (!prefix_lens) a.splits = (int)tile_splits(prefix_BH * a.tiles, a.shares, cdiv(prefix_n, (int64_t)kBlk));
+  if (!prefix_lens) a.splits = (int)tile_splits(prefix_BH * a.tiles, a.shares, nb);
   const bool i8 = code_dtype == FATHOM_DT_I8;
   const hipStream_t st = (hipStream_t)stream;
   Tail t;

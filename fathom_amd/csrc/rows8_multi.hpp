@@ -77,7 +77,6 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 // A weight is 2^(z - base), the base a whole number that is raised where a score passes it by kMost, to kStart below
 // the score, so that the rows' sums are scaled anew only where a score has grown by 2^3 (a row's first blocks).
 // The largest weight times scale is held between 2^10 and 2^15, so f16 (to 2^-24) ends at 2^-34 of it.
-constexpr int kMultiWaves = 4, kMultiThreads = kMultiWaves * kWave;
 constexpr uint32_t kLeastBlocks = 4;  // of a workgroup's share
 constexpr float kMost = 15.0f, kStart = 12.0f;
 constexpr float kLeastWeight = -112.0f;  // a block counts with that weight at least in the choice of its values' scale: it stays finite
@@ -157,16 +156,17 @@ struct Share {
   int tile, split, active, per;
 };
 struct FindTile {
-  uint64_t total[kMultiWaves];
-  uint32_t wave[kMultiWaves];
+  uint64_t total[8];
+  uint32_t wave[8];
   int share[4];
 };
 // Every workgroup takes `per` blocks, so that the tile that sees most does not hold the call up: each sums all tiles'
 // blocks, which gives `per`, and finds its tile in the prefix sums of ceil(blocks / per).  Those are at most
 // `shares` + tiles, the grid.  A thread takes some tiles in a row; workgroup 0 writes down where all begin.
+template <int WAVES>
 __device__ __forceinline__ Share find_tile(const MultiArgs &a, int w, FindTile &sh) {
   const int tid = threadIdx.x, wave = tid >> 6, n = (int)a.BH * a.tiles;
-  const int c = (n + kMultiThreads - 1) / kMultiThreads, i0 = tid * c;
+  const int c = (n + WAVES * kWave - 1) / (WAVES * kWave), i0 = tid * c;
   auto blocks = [&](int i) {
     const int r = i / a.tiles;
     return i < n ? (uint32_t)tile_span(a, r, (i - r * a.tiles) * a.rows).nb : 0u;
@@ -180,7 +180,7 @@ __device__ __forceinline__ Share find_tile(const MultiArgs &a, int w, FindTile &
   __syncthreads();
   uint64_t total = 0;
 #pragma unroll
-  for (int v = 0; v < kMultiWaves; ++v) total += sh.total[v];
+  for (int v = 0; v < WAVES; ++v) total += sh.total[v];
   const uint64_t even = (total + a.shares - 1) / a.shares;
   const uint32_t per = even > kLeastBlocks ? (uint32_t)even : kLeastBlocks;
   uint32_t own = 0;
@@ -206,21 +206,35 @@ __device__ __forceinline__ Share find_tile(const MultiArgs &a, int w, FindTile &
                __builtin_amdgcn_readfirstlane(sh.share[2]), __builtin_amdgcn_readfirstlane((int)per)};
 }
 
-// A workgroup of four waves takes a tile of 128 queries of one row, or one split of what they see; each wave has 32 of the
-// queries.  Where a row has no more than 32 queries every wave has them all, and the waves take blocks in turn.  The tile's queries are consecutive in (o, g), so
-// that a chunk's tile is a few tokens of all heads.  Per 64-token block of the row:
-//   the codes are requested a block ahead, converted once per workgroup and kept in LDS as 16-bit
-//     numbers (exact): K by tokens, V transposed, both with their 16-byte pieces in an order
-//     that keeps the lanes' reads on different banks;
-//   S^T = K q^T (v_mfma_f32_32x32x16): lane l holds query l & 31 and 32 of the block's scores, so
-//     that maximum and sum need one exchange, between l and l ^ 32.  bf16 and f16 queries are operands as they are;
-//     float32 ones are two f16, 22 bits, and where a wave has channels
-//     below 2^-18 of their query's largest, what is left of those takes a third product, times 2^38, first.
-//   O^T += V^T p^T with the weights in the layout that the scores come in, which fixes the order of the tokens in the
-//     transposed V.  A weight is one f16 (PREC: two, 22 bits) of p s_V 2^-E, E the exponent of the largest p s_V so
-//     far, so that blocks of small values with large weights count fully.
+// Whether a wave has a SIMD's registers to itself: by itself it holds both operands of a block of 128 channels, to which float32
+// queries, a cap or a bias add more than half of the registers take (4 x 4 capped queries of 8 rows of 262144 tokens 135 us
+// with 73 registers spilled; 97).  Waves that share a block do better by twos (float32, capped, 8 x 4 x 1024 over 16384 tokens
+// 888 us with 32 spilled outside the loop; 1199).
+template <int D, int QT, bool EXTRA, int RW>
+constexpr bool kWide = RW == 1 && D == 128 && (EXTRA || QT == FATHOM_DT_F32);
+
+// A workgroup takes a tile of queries of one row, or one share of what they see; each wave has 32 of them.  A tile's queries
+// are consecutive in (o, g), so that a chunk's tile is a few tokens of all heads.  RW waves share a block of the row, for 32 RW
+// queries: four, or eight (one workgroup per CU).  Where a row has no more than 32, RW is one: all four waves of a workgroup
+// have them all, and take blocks in turn.  Per 64-token block:
+//   the codes are requested a block ahead.  Several waves convert them once and keep them in LDS as 16-bit numbers (exact): K
+//     by tokens, V transposed, both with their 16-byte pieces in an order that keeps the lanes' reads on different banks.
+//     A wave by itself takes its operands straight from the codes: the order of the channels inside K's contraction is
+//     free, and so is that of V's channels over the tiles of the result, lane c's being kTiles c ..
+//   S^T = K q^T (v_mfma_f32_32x32x16): lane l holds query l & 31 and 32 of the block's scores, so that maximum and sum
+//     need one exchange, between l and l ^ 32.  bf16 and f16 queries are operands as they are; float32 ones are two f16, 22
+//     bits, and where a wave has channels below 2^-18 of their query's largest, what is left of those takes a third
+//     product, times 2^38, first.
+//   O^T += V^T p^T with the weights in the layout that the scores come in, which fixes the order of the tokens in V's
+//     operand.  A weight is one f16 (PREC: two, 22 bits) of p s_V 2^-E, E the exponent of the largest p s_V so far, so
+//     that blocks of small values with large weights count fully.
+//
+// Bound: for many queries the matrix cores and the vector instructions between them, which the two waves of a SIMD overlap
+// in part.  8 x 4 x 2048 queries over 65536 tokens (2.16 TFLOP): 2.22 ms, 970 TFLOP/s, 80 % of what an 8192^3 bf16 product
+// reaches (1200); tiles of four waves 2.44 ms, and eight with the last four half a block behind the others 2.28.  For up to 32
+// queries HBM: 8 rows of 262144 tokens (0.54 GB) 89 us, 6.0 TB/s.
 template <int D, bool I8, int QT, bool PREC, bool EXTRA, int RW>
-__global__ __launch_bounds__(kMultiThreads, RW == 1 && D == 128 && QT == FATHOM_DT_F32 ? 1 : 2) void multi_kernel(MultiArgs a) {
+__global__ __launch_bounds__((RW == 8 ? 8 : 4) * kWave, (kWide<D, QT, EXTRA, RW>) ? 1 : 2) void multi_kernel(MultiArgs a) {
   constexpr bool kBf16 = QT == FATHOM_DT_BF16;
   constexpr int kParts = QT == FATHOM_DT_F32 ? 2 : 1, kSteps = D / 16, kTiles = D / 32;
   constexpr bool kDirect = RW == 1;  // operands straight from the codes, without LDS
@@ -229,10 +243,11 @@ __global__ __launch_bounds__(kMultiThreads, RW == 1 && D == 128 && QT == FATHOM_
   // a spilled register's way back waits for all loads on theirs: 32 x 8 x 4 queries over 32768 tokens 121 us; 84.
   constexpr bool kLean = kDirect || (D == 128 && (kParts == 2 || EXTRA));
   constexpr int kAhead = kLean ? 2 : 4, kVBufs = kLean ? 1 : 2;
-  constexpr int kGroups = kMultiWaves / RW;                                      // of them in a workgroup
-  constexpr int kKeys = kBlk * D / 16 / kThreads;                  // 16-byte pieces of K per thread
-  constexpr int kCh = kDirect ? D / 32 : D == 64 ? 4 : 8;          // channels of V per thread and item of four tokens
-  constexpr int kItems = kBlk / 4 * D / kCh / kThreads;            // items per thread
+  constexpr int kWaves = RW == 8 ? 8 : 4, kGroups = kWaves / RW;  // of a workgroup
+  constexpr bool kHalves = RW == 8 && D == 64;  // half of the threads stage K, the others V
+  constexpr int kKeys = kHalves ? 1 : kBlk * D / 16 / kThreads;    // 16-byte pieces of K per thread
+  constexpr int kCh = kDirect ? D / 32 : D == 64 || RW == 8 ? 4 : 8;        // channels of V per thread and item of four tokens
+  constexpr int kItems = kHalves ? 1 : kBlk / 4 * D / kCh / kThreads;  // items per thread
   typedef typename std::conditional<kBf16, bf16x8, f16x8>::type frag;
   constexpr int kPitch = D + 4, kCodes = 2 * kBlk * D;  // of a row of sums; bytes of a block's K, or V, as 16-bit numbers
   __shared__ __attribute__((aligned(16))) char lds[kGroups][kDirect ? 32 * kPitch * 4 : 2 * kBufs * kCodes];
@@ -245,7 +260,7 @@ __global__ __launch_bounds__(kMultiThreads, RW == 1 && D == 128 && QT == FATHOM_
   int64_t r = blockIdx.x;
   if (a.parts) {  // uniform over the workgroup
     if (a.splits) share = Share{(int)blockIdx.x / a.splits, (int)blockIdx.x % a.splits, a.splits, 0};
-    else share = find_tile(a, (int)blockIdx.x, find);
+    else share = find_tile<kWaves>(a, (int)blockIdx.x, find);
     if (share.active == 0) return;
     r = share.tile / a.tiles;
     share.tile %= a.tiles;
@@ -332,6 +347,7 @@ __global__ __launch_bounds__(kMultiThreads, RW == 1 && D == 128 && QT == FATHOM_
   }
 
   // ---- staging
+  const int mine_v = kHalves ? tid % (kThreads / 2) : tid;
   u32x4 kr[kKeys];
   typedef typename std::conditional<kCh == 8, u32x2v, typename std::conditional<kCh == 4, uint32_t, uint16_t>::type>::type vpiece;
   vpiece vr[kItems][4];
@@ -353,7 +369,7 @@ __global__ __launch_bounds__(kMultiThreads, RW == 1 && D == 128 && QT == FATHOM_
     const RowsWith<kDirect && D == 128 ? kStream : 0> v(a.v8, r * a.cap, i < last ? span.block(i) : 0, i < last ? span.end : 0, D);
 #pragma unroll
     for (int x = 0; x < kItems; ++x) {  // direct: channels kCh col .. of tokens 8 x + 4 half ..
-      const int item = x * kThreads + tid, at = kDirect ? (8 * x + 4 * half) * D + kCh * col : item / (D / kCh) * 4 * D + item % (D / kCh) * kCh;
+      const int item = x * kThreads + mine_v, at = kDirect ? (8 * x + 4 * half) * D + kCh * col : item / (D / kCh) * 4 * D + item % (D / kCh) * kCh;
 #pragma unroll
       for (int j = 0; j < 4; ++j) v.load(at + j * D, vr[x][j]);
     }
@@ -383,30 +399,33 @@ __global__ __launch_bounds__(kMultiThreads, RW == 1 && D == 128 && QT == FATHOM_
   };
   auto stage = [&](int buf, int i) __attribute__((always_inline)) {
     if (i >= last) return;
+    if (!kHalves || tid < kThreads / 2) {
 #pragma unroll
-    for (int x = 0; x < kKeys; ++x) {
-      const int at = x * kThreads + tid, tok = at / (D / 16), piece = at % (D / 16);
-      uint32_t w[8];
+      for (int x = 0; x < kKeys; ++x) {
+        const int at = x * kThreads + tid, tok = at / (D / 16), piece = at % (D / 16);
+        uint32_t w[8];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const uint32_t c = flip_sign<I8>(kr[x][e]);
-        if constexpr (kBf16) {
-          w[2 * e] = pair_bf16<I8, false>(c);
-          w[2 * e + 1] = pair_bf16<I8, true>(c);
-        } else {
-          w[2 * e] = __builtin_bit_cast(uint32_t, pair16<I8, false>(c));
-          w[2 * e + 1] = __builtin_bit_cast(uint32_t, pair16<I8, true>(c));
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t c = flip_sign<I8>(kr[x][e]);
+          if constexpr (kBf16) {
+            w[2 * e] = pair_bf16<I8, false>(c);
+            w[2 * e + 1] = pair_bf16<I8, true>(c);
+          } else {
+            w[2 * e] = __builtin_bit_cast(uint32_t, pair16<I8, false>(c));
+            w[2 * e + 1] = __builtin_bit_cast(uint32_t, pair16<I8, true>(c));
+          }
         }
-      }
-      char *row = lds[group] + 2 * buf * kCodes + tok * 2 * D;
+        char *row = lds[group] + 2 * buf * kCodes + tok * 2 * D;
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-        *reinterpret_cast<u32x4 *>(row + 16 * ((2 * piece + h) ^ (tok & (D / 8 - 1)))) = u32x4{w[4 * h], w[4 * h + 1], w[4 * h + 2], w[4 * h + 3]};
+        for (int h = 0; h < 2; ++h)
+          *reinterpret_cast<u32x4 *>(row + 16 * ((2 * piece + h) ^ (tok & (D / 8 - 1)))) = u32x4{w[4 * h], w[4 * h + 1], w[4 * h + 2], w[4 * h + 3]};
+      }
     }
+    if (kHalves && tid < kThreads / 2) return;
     clear_values(i);
 #pragma unroll
     for (int x = 0; x < kItems; ++x) {
-      const int item = x * kThreads + tid, quad = item / (D / kCh), ch0 = item % (D / kCh) * kCh;
+      const int item = x * kThreads + mine_v, quad = item / (D / kCh), ch0 = item % (D / kCh) * kCh;
       // tokens 4 quad ..: half (quad >> 1 & 1) of the piece that lane half quad & 1 reads for 16 tokens
       const int piece = (quad >> 3) * 4 + (quad >> 2 & 1) * 2 + (quad & 1);
       char *base = lds[group] + (2 * buf + 1) * kCodes + 8 * (quad >> 1 & 1);
@@ -771,7 +790,7 @@ __global__ __launch_bounds__(kMultiThreads, RW == 1 && D == 128 && QT == FATHOM_
   const bool parts = a.parts;
   const int64_t slot = parts ? ((int64_t)blockIdx.x * kRows) : 0;
   if constexpr (kDirect) {  // ---- the waves' sums over their blocks
-    __shared__ float wm[kMultiWaves][32], wl[kMultiWaves][32];
+    __shared__ float wm[kWaves][32], wl[kWaves][32];
     typedef float piece __attribute__((ext_vector_type(kTiles)));
     float *mine_at = reinterpret_cast<float *>(lds[group]) + col * kPitch;
 #pragma unroll
@@ -787,15 +806,15 @@ __global__ __launch_bounds__(kMultiThreads, RW == 1 && D == 128 && QT == FATHOM_
     }
     __syncthreads();
 #pragma unroll
-    for (int x = threadIdx.x; x < 32 * D / 4; x += kMultiThreads) {
+    for (int x = threadIdx.x; x < 32 * D / 4; x += kWaves * kWave) {
       const int row = x / (D / 4), c = 4 * (x % (D / 4));
       if (m0 + row >= M) break;
       float big = wm[0][row];
 #pragma unroll
-      for (int v = 1; v < kMultiWaves; ++v) big = fmaxf(big, wm[v][row]);
+      for (int v = 1; v < kWaves; ++v) big = fmaxf(big, wm[v][row]);
       float L = 0.0f, out[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (int v = 0; v < kMultiWaves; ++v) {
+      for (int v = 0; v < kWaves; ++v) {
         const float f = __builtin_amdgcn_exp2f(wm[v][row] - big);
         const float4 u = *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(lds[v]) + row * kPitch + c);
         L = fmaf(wl[v][row], f, L);
@@ -841,11 +860,13 @@ __global__ __launch_bounds__(kMultiThreads, RW == 1 && D == 128 && QT == FATHOM_
 
 template <int D, bool I8, int QT, bool PREC, bool EXTRA>
 void launch_multi(const MultiArgs &a, hipStream_t st) {
+  constexpr bool kFour = EXTRA || QT == FATHOM_DT_F32;  // the host gives such calls no tiles of 256
   const dim3 grid = a.splits  ? dim3((unsigned)(a.splits * a.BH * a.tiles))
                     : a.parts ? dim3((unsigned)(a.shares + a.BH * a.tiles))
                               : dim3((unsigned)a.BH, (unsigned)a.tiles);
-  if (a.rows == 32) multi_kernel<D, I8, QT, PREC, EXTRA, 1><<<grid, kMultiThreads, 0, st>>>(a);
-  else multi_kernel<D, I8, QT, PREC, EXTRA, 4><<<grid, kMultiThreads, 0, st>>>(a);
+  if (a.rows == 32) multi_kernel<D, I8, QT, PREC, EXTRA, 1><<<grid, 4 * kWave, 0, st>>>(a);
+  else if (kFour || a.rows == 128) multi_kernel<D, I8, QT, PREC, EXTRA, 4><<<grid, 4 * kWave, 0, st>>>(a);
+  else multi_kernel<D, I8, QT, PREC, EXTRA, kFour ? 4 : 8><<<grid, 8 * kWave, 0, st>>>(a);
 }
 template <int D, bool I8, int QT, bool PREC>
 void launch_multi(const MultiArgs &a, hipStream_t st) {

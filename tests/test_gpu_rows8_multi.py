@@ -376,6 +376,89 @@ def test_shared_ends():
     assert not st.shared_attention(q, zero, pst, zero[:2]).any()
 
 
+# ----------------------------------------------------------------------------- tiles of eight waves, shares
+@pytest.mark.parametrize("code, dtype, D", [("e4m3", torch.bfloat16, 128), ("int8", torch.float16, 64), ("e4m3", torch.float16, 64),
+                                            ("int8", torch.bfloat16, 128), ("e4m3", torch.float32, 128)])
+@pytest.mark.parametrize("window, sinks", [(0, 0), (900, 70), (1000, 0)])
+def test_chunk_of_many_queries(code, dtype, D, window, sinks):
+    """2400 queries of a row, the last tile not full, rows of one length and of many: tiles of eight waves for 16-bit queries, of
+    four for float32 ones and with a cap."""
+    BH, G, T, n = 6, 8, 300, 1700
+    lens = [1700, 1333, 290, 0, 301, 64]
+    st, o = _filled(BH, n, D, code, seed=15, garbage_behind=lens)
+    q = _rand((BH * G, T, D), 16, dtype).view(BH, G, T, D)
+    ragged = torch.tensor(lens, device=DEV)
+    _check_chunk(st.chunk_attention(q.to(DEV), ragged, window=window, sinks=sinks), q, o, code, lens, window, sinks, every=59)
+    _check_chunk(st.chunk_attention(q.to(DEV), ragged, window=window, sinks=sinks, softcap=20.0), q, o, code, lens, window, sinks,
+                 softcap=20.0, every=83)
+    st, o = _filled(BH, n, D, code, seed=17)
+    _check_chunk(st.chunk_attention(q.to(DEV), n, window=window, sinks=sinks), q, o, code, [n] * BH, window, sinks, every=71)
+
+
+@pytest.mark.parametrize("B, H, G, P, n, dtype", [(520, 2, 4, 3800, 20, torch.bfloat16), (65, 4, 4, 16300, 3, torch.float16),
+                                                  (300, 1, 7, 9000, 10, torch.bfloat16)])
+def test_shared_by_many(B, H, G, P, n, dtype):
+    pst, po = _filled(H, P, 64, "int8", seed=91)
+    st, o = _filled(B * H, n, 64, "int8", seed=92)
+    q = _rand((B * H, G, 64), 6, dtype)
+    rows = list(range(0, B * H, B * H // 9)) + [B * H - 1]
+    lens = [n * (i % 3) // 2 for i in range(B * H)]
+    for length, prefix_length in ((torch.tensor(lens, device=DEV), P), (torch.tensor(lens, device=DEV), torch.tensor([P] * H, device=DEV))):
+        got = st.shared_attention(q.to(DEV), length, pst, prefix_length)
+        _check_shared(got, q, o, po, "int8", lens, [P] * H, rows=rows)
+    sl = torch.full((B * H, G), 2.0 ** -7)
+    got = st.shared_attention(q.to(DEV), torch.tensor(lens, device=DEV), pst, P, softcap=10.0, slopes=sl.to(DEV))
+    _check_shared(got, q, o, po, "int8", lens, [P] * H, softcap=10.0, slopes=sl, rows=rows)
+
+
+@pytest.mark.parametrize("BH, G, T, n, at", [(1, 2, 3, 30011, 29000), (1, 2, 3, 30011, 7), (6, 8, 300, 1700, 1500), (2, 4, 20, 9000, 8999)])
+def test_a_nan_in_one_of_many_shares(BH, G, T, n, at):
+    """A NaN code of V, or a scale of V that is infinite, makes the channels NaN of the queries that see it, and no others."""
+    q = _rand((BH * G, T, 128), 4, torch.bfloat16).view(BH, G, T, 128).to(DEV)
+    st, _ = _filled(BH, n, 128, "e4m3", seed=33)
+    clean = st.chunk_attention(q, n)
+    sees = torch.arange(n - T, n, device=DEV) >= at
+    st.v8.view(torch.uint8)[-1, at, 41] = 0xFF
+    got = st.chunk_attention(q, n)
+    nan = torch.zeros_like(got, dtype=torch.bool)
+    nan[-1, :, sees, 41] = True
+    assert torch.equal(got.isnan(), nan) and torch.equal(got[~nan], clean[~nan])
+    st.v_scale[-1, at // BLK] = float("inf")
+    got = st.chunk_attention(q, n)
+    nan[-1, :, torch.arange(n - T, n, device=DEV) >= at // BLK * BLK] = True
+    assert torch.equal(got.isnan(), nan) and torch.equal(got[~nan], clean[~nan])
+
+
+@pytest.mark.parametrize("code, D", [("e4m3", 128), ("int8", 64), ("int8", 128)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_caps_that_bind(code, D, dtype):
+    """Scores of many times the cap and near it, in tiles of one wave and of four, few and many of a block."""
+    n = 333
+    st, o = _filled(2, n, D, code, seed=95)
+    for G, T in ((2, 5), (3, 50)):
+        q = _rand((2 * G, T, D), 7, dtype).view(2, G, T, D)
+        q[:, :, ::3] *= 2.0 ** -6
+        for scale, cap in ((2.0, 5.0), (0.5, 3.0), (-1.0, 12.0)):
+            got = st.chunk_attention(q.to(DEV), n, scale=scale, softcap=cap)
+            _check_chunk(got, q, o, code, [n, n], scale=scale, softcap=cap, every=7)
+
+
+def test_calls_with_and_without_a_cap_in_turn():
+    """The same shapes with and without a cap take other tiles, and workspaces of one size."""
+    st, _ = _filled(6, 1700, 128, "e4m3", seed=96)
+    q = _rand((48, 300, 128), 6, torch.bfloat16).view(6, 8, 300, 128).to(DEV)
+    lens = torch.tensor([1700, 1300, 900, 500, 310, 300], dtype=torch.int32, device=DEV)
+    far = 1e29  # a cap that no score feels
+    plain, capped = st.chunk_attention(q, lens), st.chunk_attention(q, lens, softcap=far)
+    assert torch.equal(plain, capped)
+    zeros = torch.zeros(8, device=DEV)
+    biased = st.chunk_attention(q, lens, slopes=zeros)
+    # both are off by half a step of bf16 at most, from values that are off by less
+    assert float((biased.float() - plain.float()).abs().max()) <= 2 ** -7 * float(plain.float().abs().max())
+    for _ in range(2):
+        assert torch.equal(st.chunk_attention(q, lens), plain) and torch.equal(st.chunk_attention(q, lens, slopes=zeros), biased)
+
+
 # ----------------------------------------------------------------------------- calls
 def test_calls_repeat_bit_for_bit_on_any_stream():
     st, _ = _filled(4, 5000, 128, "e4m3", seed=81)

@@ -152,3 +152,25 @@ def test_oracle_rotation_closed_forms():
     assert np.allclose(got[:, 0], [-1, 0, 1]) and np.allclose(got[:, 4], [0, -1, 0]) and np.allclose(got[:, 15], 5)
     got = R.rotated(np.full((1, 4), 3.0), np.array([7]), np.zeros(0), np.array([1.0, 2.0, 0.0, -1.0]))
     assert np.allclose(got, [[1, 2, 0, -1]])
+
+
+@pytest.mark.parametrize("entry", ["chunk", "shared"])
+@pytest.mark.parametrize("BH, G, T", [(1, 4, 64), (6, 8, 300), (1, 4, 9), (2, 8, 1024), (4, 7, 33), (64, 4, 128)])
+def test_a_workspace_serves_every_kind_of_call(entry, BH, G, T):
+    """Queries of each type, with a cap, a bias or neither, take what the query's size holds; a fourth of it is refused to some.
+    (The workspace is 8 bytes off, so that no call gets to its launch.)"""
+    n = 65536
+    L = _lib.lib()
+    if entry == "chunk":
+        need = L.fathom_rows8_chunk_attention_workspace_bytes(BH, G, T, 128, n)
+        args = _chunk(BH=BH, G=G, T=T, cap=n, n=0, lens=1 << 29)
+    else:
+        need = L.fathom_rows8_shared_attention_workspace_bytes(BH, T, G, 128, n, 0)
+        args = _shared(pBH=BH, seqs=T, G=G, pcap=n, pn=0, plens=1 << 29, n=0)
+    refused = 0
+    for q_dtype in (_lib.DT_F32, _lib.DT_F16, _lib.DT_BF16):
+        for softcap, slopes in ((0.0, None), (30.0, None), (0.0, 1 << 29), (1e30, None)):
+            call = {**args, "q_dtype": q_dtype, "softcap": softcap, "slopes": slopes, "ws": (1 << 28) + 8}
+            _refused(f"fathom_rows8_{entry}_attention", {**call, "wsb": need}, _lib.ERR_INVALID, b"aligned")
+            refused += getattr(L, f"fathom_rows8_{entry}_attention")(*{**call, "wsb": need // 4}.values()) == _lib.ERR_WORKSPACE
+    assert refused

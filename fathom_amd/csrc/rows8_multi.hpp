@@ -223,8 +223,8 @@ constexpr bool kWide = RW == 1 && D == 128 && (EXTRA || QT == FATHOM_DT_F32);
 //     free, and so is that of V's channels over the tiles of the result, lane c's being kTiles c ..
 //   S^T = K q^T (v_mfma_f32_32x32x16): lane l holds query l & 31 and 32 of the block's scores, so that maximum and sum
 //     need one exchange, between l and l ^ 32.  bf16 and f16 queries are operands as they are; float32 ones are two f16, 22
-//     bits, and where a wave has channels below 2^-18 of their query's largest, what is left of those takes a third
-//     product, times 2^38, first.
+//     bits, and where a wave has channels below 2^-18 of their query's largest that could move a score by 2^-25,
+//     what is left of those, to 2^-76 of that largest, takes two more products, times 2^38.
 //   O^T += V^T p^T with the weights in the layout that the scores come in, which fixes the order of the tokens in V's
 //     operand.  A weight is one f16 (PREC: two, 22 bits) of p s_V 2^-E, E the exponent of the largest p s_V so far, so
 //     that blocks of small values with large weights count fully.
@@ -289,7 +289,9 @@ __global__ __launch_bounds__((RW == 8 ? 8 : 4) * kWave, (kWide<D, QT, EXTRA, RW>
   int ex = 0;
   const int64_t q_at = r * a.q_row + g * a.q_head + o_at * a.q_out;
   auto channel = [&](int s) { return kDirect ? 32 * (s / 2) + 16 * half + 8 * (s % 2) : 16 * s + 8 * half; };  // of step s, eight of them
-  bool far = false;  // float32: some channel of the wave's queries is small, as small_channel has it
+  // float32: times a block's scale of K, a bound of what two f16 of the wave's queries lack of their small channels, in scores times
+  // 2^25; 0 without such channels
+  float far = 0.0f;
   if constexpr (QT != FATHOM_DT_F32) {
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) qf[0][s] = *reinterpret_cast<const frag *>(static_cast<const uint16_t *>(a.q) + q_at + channel(s));
@@ -315,6 +317,7 @@ __global__ __launch_bounds__((RW == 8 ? 8 : 4) * kWave, (kWide<D, QT, EXTRA, RW>
     }
   } else {
     float x[kSteps][8], big = 0.0f;
+    int few = 0;  // small channels of the query
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
       load8_q(a.q, QT, q_at + channel(s), x[s]);
@@ -333,9 +336,13 @@ __global__ __launch_bounds__((RW == 8 ? 8 : 4) * kWave, (kWide<D, QT, EXTRA, RW>
         const float v = ldexpf(x[s][e], -ex);
         qf[0][s][e] = (_Float16)v;
         qf[1][s][e] = (_Float16)(v - (float)(_Float16)v);
-        far |= small_channel(v);
+        few += small_channel(v);
       }
-    far = __any(far);
+    few += __shfl_xor(few, 32);
+    if (few) far = ldexpf(fabsf(a.scale) * (kLog2e * (I8 ? 128.0f : 448.0f)) * (float)few, ex);  // each lacks 2^-25 at most
+#pragma unroll
+    for (int x = 32; x > 0; x >>= 1) far = fmaxf(far, __shfl_xor(far, x));
+    far = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(far)));
   }
   const int exq = ex;
   // the scores' factor, scale log2 e or scale / softcap, as a fraction and a power of two
@@ -468,7 +475,7 @@ __global__ __launch_bounds__((RW == 8 ? 8 : 4) * kWave, (kWide<D, QT, EXTRA, RW>
   };
   // ---- scores; operands are read kAhead products ahead
   f32x16 s[2];
-  auto scores = [&](int buf) __attribute__((always_inline)) {
+  auto scores = [&](int buf, float ks) __attribute__((always_inline)) {
     const char *kb = lds[group] + 2 * buf * kCodes + col * 2 * D;
     frag kf[2][kAhead];
     auto key = [&](int x, int c) __attribute__((always_inline)) {  // of tokens 32 x .., step c
@@ -498,28 +505,6 @@ __global__ __launch_bounds__((RW == 8 ? 8 : 4) * kWave, (kWide<D, QT, EXTRA, RW>
     for (int x = 0; x < 2; ++x)
 #pragma unroll
       for (int e = 0; e < 16; ++e) s[x][e] = 0.0f;
-    if constexpr (QT == FATHOM_DT_F32) {
-      if (__builtin_expect(far, 0)) {  // what two f16 leave of small channels, formed anew from the queries
-        auto left = [&](int c) __attribute__((always_inline)) {
-          float x[8];
-          load8_q(a.q, QT, q_at + channel(c), x);
-          f16x8 v;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] = (_Float16)rest_of(ldexpf(x[e], -exq));
-#pragma unroll
-          for (int h = 0; h < 2; ++h) s[h] = __builtin_amdgcn_mfma_f32_32x32x16_f16(key(h, c), v, s[h], 0, 0, 0);
-        };
-        if constexpr (kDirect) {  // the registers of K need constant places
-#pragma unroll
-          for (int c = 0; c < kSteps; ++c) left(c);
-        } else {
-#pragma unroll 1
-          for (int c = 0; c < kSteps; ++c) left(c);
-        }
-#pragma unroll
-        for (int h = 0; h < 2; ++h) s[h] *= 0x1p-38f;
-      }
-    }
     keys(0);
 #pragma unroll
     for (int n = 0; n < 2 * kSteps / kAhead; ++n) {
@@ -533,6 +518,41 @@ __global__ __launch_bounds__((RW == 8 ? 8 : 4) * kWave, (kWide<D, QT, EXTRA, RW>
           if constexpr (kBf16) s[x] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[n & 1][c], qf[p][step], s[x], 0, 0, 0);
           else s[x] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[n & 1][c], qf[p][step], s[x], 0, 0, 0);
         }
+    }
+    if constexpr (QT == FATHOM_DT_F32) {
+      // What two f16 leave of small channels, as two more, formed anew from the queries where scores could be off by 2^-25.  (32 x
+      // 8 x 4 queries over 131072 tokens, one in thirty waves with such a channel: in every block 246 us; 174.)  In sums of their
+      // own: in the others' chain the matrix cores end them 2^-46 below the largest channel, also where that meets a zero of K.
+      if (__builtin_expect(!(fabsf(ks) * far <= 1.0f), 0)) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          f32x16 t;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) t[e] = 0.0f;
+          auto left = [&](int c) __attribute__((always_inline)) {
+            float x[8];
+            load8_q(a.q, QT, q_at + channel(c), x);
+            f16x8 v[2];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const float rest = rest_of(ldexpf(x[e], -exq));
+              v[0][e] = (_Float16)rest;
+              v[1][e] = (_Float16)(rest - (float)v[0][e]);
+            }
+#pragma unroll
+            for (int p = 1; p >= 0; --p) t = __builtin_amdgcn_mfma_f32_32x32x16_f16(key(h, c), v[p], t, 0, 0, 0);
+          };
+          if constexpr (kDirect) {  // the registers of K need constant places
+#pragma unroll
+            for (int c = 0; c < kSteps; ++c) left(c);
+          } else {
+#pragma unroll 1
+            for (int c = 0; c < kSteps; ++c) left(c);
+          }
+#pragma unroll
+          for (int e = 0; e < 16; ++e) s[h][e] = fmaf(t[e], 0x1p-38f, s[h][e]);
+        }
+      }
     }
   };
   // ---- their weights, and the values' products
@@ -725,7 +745,7 @@ __global__ __launch_bounds__((RW == 8 ? 8 : 4) * kWave, (kWide<D, QT, EXTRA, RW>
     for (int i = first + group; i < last; i += kGroups) {
       const float ks = ks_next, vs = scale_of(i, vs_next);
       const bool some = seen(i);
-      if (some) scores(0);
+      if (some) scores(0, ks);
       __builtin_amdgcn_sched_barrier(0);
       load_keys(i + kGroups);
       __builtin_amdgcn_sched_barrier(0);
@@ -743,7 +763,7 @@ __global__ __launch_bounds__((RW == 8 ? 8 : 4) * kWave, (kWide<D, QT, EXTRA, RW>
       const int buf = (i - first) & 1;
       vs = scale_of(i, vs);
       if (seen(i)) {
-        scores(buf);
+        scores(buf, ks);
         block(buf, i, ks, vs);
       }
       ks = ks_next;

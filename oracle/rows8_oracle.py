@@ -150,7 +150,8 @@ def many_attention(q, K, V, toks, length, scale, softcap=0.0, slope=None, weight
 
     Their products are those of `parts` exact parts of the query, D each, in one chain, so D counts that many times; a score's
     factor is rounded three times more.  A weight has `weight_bits` bits, and ends half of 2^-24 / 2^10 below the largest w
-    s, at the largest code, which is at most twice the largest |V| of its block."""
+    s, at the largest code, which is at most twice the largest |V| of its block.  (Small channels of float32 queries may move a score by
+    2^-25 in units of log 2: a part in sixty of the 64 U that `attention` counts for joins, of which there are two.)"""
     out, err = attention(q, K, V, toks, length, scale, softcap, slope)
     if len(toks) == 0:
         return out, err

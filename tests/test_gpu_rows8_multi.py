@@ -443,6 +443,23 @@ def test_caps_that_bind(code, D, dtype):
             _check_chunk(got, q, o, code, [n, n], scale=scale, softcap=cap, every=7)
 
 
+@pytest.mark.parametrize("code, D", [("e4m3", 128), ("int8", 64)])
+@pytest.mark.parametrize("power", [-17, -20, -28, -40])
+def test_small_channels_of_float32_queries(code, D, power):
+    """Channels of 2^-17 to 2^-40 of the query's largest, which meets K's zeros, decide the scores: with two f16 parts alone those
+    would be off by 2^-8 of themselves and more."""
+    n = 200
+    _, o = _filled(2, n, D, code, seed=97)
+    o["k8"][:, :, 3] = 0
+    o["ks"] *= np.float32(2.0 ** -power)
+    st = _from_numpy(o, code)
+    for G, T in ((2, 5), (2, 40), (3, 70)):
+        q = _rand((2 * G, T, D), 8).view(2, G, T, D) * 2.0 ** power
+        q[..., 3] = 1.0
+        q[:, :, 2::3, 3] = 0.0  # some queries without the large channel
+        _check_chunk(st.chunk_attention(q.to(DEV), n), q, o, code, [n, n], every=6)
+
+
 def test_calls_with_and_without_a_cap_in_turn():
     """The same shapes with and without a cap take other tiles, and workspaces of one size."""
     st, _ = _filled(6, 1700, 128, "e4m3", seed=96)

@@ -111,14 +111,31 @@ __device__ __forceinline__ void clear_nans(u32x2v &w) {
   w[1] &= ~((nan_bytes(w[1]) >> 7) * 0xFFu);
 }
 
-// tanh_any without a branch: the compiler would make one of its select, for every score by itself.
+// tanh of |u| < 1/2, a fit of u + u^3 P(u^2): P of degree 3 is off by 2^-26, of degree 2 by 2^-20.5, which is below what a chain of 64
+// products may be off by, and far below a weight of 11 bits.
+template <bool PREC>
+__device__ __forceinline__ float tanh_near(float u) {
+  const float w = u * u;
+  float p;
+  if constexpr (PREC) {
+    p = fmaf(0.01724146865f, w, -0.05304548144f);
+    p = fmaf(p, w, 0.13325878978f);
+    p = fmaf(p, w, -0.33333143592f);
+  } else {
+    p = fmaf(-0.0447505787f, w, 0.13205356896f);
+    p = fmaf(p, w, -0.33328157663f);
+  }
+  return fmaf(u * w, p, u);
+}
+// tanh without a branch: the compiler would make one of its select, for every score by itself.
+template <bool PREC>
 __device__ __forceinline__ float tanh_both(float u) {
   const float t = __builtin_amdgcn_exp2f(fabsf(u) * (-2.0f * kLog2e));
   const float n = 1.0f - t, d = 1.0f + t, r = __builtin_amdgcn_rcpf(d);
   float far = n * r;
   far = fmaf(fmaf(-far, d, n), r, far);
   const uint32_t near = fabsf(u) < 0.5f ? 0xFFFFFFFFu : 0u;
-  return __uint_as_float((__float_as_uint(tanh_small(u)) & near) | (__float_as_uint(copysignf(far, u)) & ~near));
+  return __uint_as_float((__float_as_uint(tanh_near<PREC>(u)) & near) | (__float_as_uint(copysignf(far, u)) & ~near));
 }
 
 // Two floats as f16, to nearest, and what that leaves of them.
@@ -611,12 +628,12 @@ __global__ __launch_bounds__((RW == 8 ? 8 : 4) * kWave, (kWide<D, QT, EXTRA, RW>
 #pragma unroll
         for (int x = 0; x < 2; ++x)
 #pragma unroll
-          for (int e = 0; e < 16; ++e) s[x][e] = tanh_small(s[x][e]);
+          for (int e = 0; e < 16; ++e) s[x][e] = tanh_near<PREC>(s[x][e]);
       } else {
 #pragma unroll
         for (int e = 0; e < 32; e += 4) {
 #pragma unroll
-          for (int k = e; k < e + 4; ++k) s[k / 16][k % 16] = tanh_both(s[k / 16][k % 16]);
+          for (int k = e; k < e + 4; ++k) s[k / 16][k % 16] = tanh_both<PREC>(s[k / 16][k % 16]);
           if (e < 28)  // four after four: all at once would spill a hundred registers
             asm volatile("" : "+v"(s[e / 16][e % 16]), "+v"(s[e / 16][e % 16 + 1]), "+v"(s[e / 16][e % 16 + 2]), "+v"(s[e / 16][e % 16 + 3]),
                               "+v"(s[(e + 4) / 16][(e + 4) % 16]), "+v"(s[(e + 5) / 16][(e + 5) % 16]),

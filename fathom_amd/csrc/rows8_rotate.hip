@@ -175,7 +175,14 @@ __device__ __forceinline__ void turn(float (&x)[16], const float (&cs)[8], const
   }
 }
 
-// Workgroups of three kinds, per row: a block of K, a block of V, queries.
+// Workgroups of three kinds, per row: a block of K, a block of V, queries.  A row of D channels is D / 16 lanes', so that a
+// pair's channels are in one thread and a head's norm is a sum over 4 or 8 lanes; a block's rows stay in registers between its
+// largest value and its codes.  A workgroup's query tokens are as many as there are, up to its rows, and its heads the rest, so that
+// a token's angles are formed once for up to four heads (fewer where the call would not fill the device).
+//
+// Bound: HBM.  8 x 32768 tokens of 4 heads in bf16, D = 128, keys returned (0.81 GB in and out) 163 us, 4.9 TB/s, what a copy
+// reaches (4.97); norms and angles by themselves take less.  16 x 1777 of 7 heads, D = 64 (77 MB, much of it from L2) 19 us.
+// One token of 32 rows 8 us: the launch, the weights and frequencies on their way, then the row.
 template <int D, int DT, bool I8>
 __global__ __launch_bounds__(kThreads) void rotate_kernel(RotateArgs a) {
   typedef Lane<D> L;

@@ -212,12 +212,11 @@ class RowStore8:
         made from the keys before that rounding.
 
         With weights (q_weight, k_weight [d]; None: no norm) x becomes x / sqrt(mean(x^2) + eps) * weight.  Token i
-        of a row stands at position t = pos + i + offset; with inv_freq [r / 2] (float32, finite and below 2^50 in
-        size; r <= d a multiple of 16; None: no rotation) channels c and c + r / 2 become (x_c cos - x_{c+r/2} sin, x_{c+r/2} cos + x_c sin) of
-        the angle t inv_freq[c], whole turns of which are dropped exactly, at any t; channels
-        behind r stay.  offset is an int or integers [BH]:
-        what stands before the store's first token, as a shared prefix does.  Views as in `write`; with a tensor `pos`,
-        rows whose tokens do not all fit are rotated but not written."""
+        of a row stands at position t = pos + i + offset; with inv_freq [r / 2] (float32, finite and below 2^50 in size;
+        r <= d a multiple of 16; None: no rotation) channels c and c + r / 2 become (x_c cos - x_{c+r/2} sin,
+        x_{c+r/2} cos + x_c sin) of the angle t inv_freq[c], whose whole turns are dropped exactly at any t; channels
+        behind r stay.  offset is an int or integers [BH]: what stands before the store's first token, as a shared prefix
+        does.  Views as in `write`; with a tensor `pos`, rows whose tokens do not all fit are rotated but not written."""
         dev, BH, d = self.device, self.BH, self.d
         for t in (q, K, V):
             if t.device != dev:

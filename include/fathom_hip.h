@@ -390,9 +390,9 @@ int fathom_rows8_write(const void *K, const void *V, int dtype, int64_t k_row_st
  * where offset is NULL.  Each head of q and K is divided by sqrt(mean(x^2) +
  * eps) and multiplied by q_weight, k_weight [D] (of weight_dtype; NULL: no norm);
  * channels c and c + rotated / 2, c < rotated / 2, are turned by the angle t *
- * inv_freq[c] (inv_freq [rotated / 2] float32; rotated a multiple of 16, 0: no
- * rotation), formed in float64: (x_c cos - x_{c + rotated/2} sin,
- * x_{c + rotated/2} cos + x_c sin).  q_out [BH, G, T, D] and, unless NULL, k_out
+ * inv_freq[c] (inv_freq [rotated / 2] float32, finite and below 2^50 in size;
+ * rotated a multiple of 16, 0: no rotation), whose whole turns are dropped exactly
+ * at any t: (x_c cos - x_{c + rotated/2} sin, x_{c + rotated/2} cos + x_c sin).  q_out [BH, G, T, D] and, unless NULL, k_out
  * [BH, T, D] of dtype take the results; K's codes are made from the float32 values.
  * Rows of `pos` that do not fit are rotated but not written.  T <= 2^27.
  */
@@ -473,7 +473,8 @@ int fathom_rows8_gather_attention(const void *q, int q_dtype, const int64_t *idx
  * p - window and t < sinks.  Scores, cap, bias (slopes[bh, g] * (t - p)) as
  * above; a query that sees nothing (p < 0) gives zeros.  out [BH, G, T, D] of
  * q_dtype (16-byte aligned).  bf16 and f16 queries take part exactly, float32 ones
- * as fathom_rows8_attention's; scores and sums are float32.  With q_dtype
+ * with 22 bits, channels below 2^-18 of their head's largest too where a score could
+ * be off by 2^-25 without (to 2^-76 of it); scores and sums are float32.  With q_dtype
  * FATHOM_DT_F32 a weight has 22 bits, else 11, down to 2^-34 of the largest weight
  * times scale of V.
  * G * T <= 65535 * 32, BH * G * T <= 2^27.

@@ -8,6 +8,35 @@ namespace {
 
 constexpr int kJoinThreads = 256;
 constexpr int64_t kMaxTiles = 65535;  // grid y
+// Queries from which D / 4 lanes join each one's splits: they fill the device, and have few splits each (8 x 12 x 396 queries over 501
+// tokens in two shares 78 us with a workgroup per query; 38).
+constexpr int64_t kJoinMany = 4096;
+
+// Where the partial results of query m of row blockIdx.y lie: `own` splits of its tile and, behind a shared prefix, `more` of its
+// sequence's own tokens; `to` is its place in the output, in rows.
+struct JoinFrom {
+  int own, more;
+  int64_t at, slot, to;
+  __device__ __forceinline__ float2 ml(const MultiArgs &a, const Tail &t, int s) const {
+    return s < own ? a.ml[at + (int64_t)s * a.rows] : t.ml[slot + (int64_t)(s - own) * a.G];
+  }
+  __device__ __forceinline__ const float *part(const MultiArgs &a, const Tail &t, int s, int D) const {
+    return s < own ? a.part + (at + (int64_t)s * a.rows) * D : t.part + (slot + (int64_t)(s - own) * a.G) * D;
+  }
+};
+__device__ __forceinline__ JoinFrom join_from(const MultiArgs &a, const Tail &tail, int m) {
+  const int64_t r = blockIdx.y, g = m % a.G, o = m / a.G;
+  const int tile = (int)r * a.tiles + m / a.rows;
+  const int2 from = a.splits ? make_int2(tile * a.splits, a.splits) : a.where[tile];
+  JoinFrom f{from.y, 0, (int64_t)from.x * a.rows + m % a.rows, 0, a.shared ? (o * a.BH + r) * a.G + g : (r * a.G + g) * a.O + o};
+  if (a.shared) {
+    const int64_t row = o * a.BH + r;
+    const int2 w = tail.where ? tail.where[row] : make_int2((int)(row * tail.nsplit), (int)tail.nsplit);
+    f.slot = (int64_t)w.x * a.G + g;
+    f.more = w.y;
+  }
+  return f;
+}
 
 // Joins a query's splits, and its sequence's own tokens behind a shared prefix: one workgroup per query, D / 4 lanes
 // take 16 bytes of every (1024 / D)-th split.  The splits' weights 2^(m_s - m) are formed by all threads for the sum and again
@@ -19,22 +48,9 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(MultiArgs a, Tail ta
   __shared__ float4 acc[kGroups][kLanes];
   __shared__ float red[2][kWaves];
   const int tid = threadIdx.x, lane = tid % kLanes, grp = tid / kLanes;
-  const int m = (int)blockIdx.x, y = m / a.rows;
-  const int64_t r = blockIdx.y, g = m % a.G, o = m / a.G;
-  const int tile = (int)r * a.tiles + y;
-  const int2 from = a.splits ? make_int2(tile * a.splits, a.splits) : a.where[tile];
-  const int own = from.y;  // splits of the tile
-  const int64_t at = (int64_t)from.x * a.rows + m % a.rows;
-  int more = 0;
-  int64_t slot = 0;
-  if (a.shared) {
-    const int64_t row = o * a.BH + r;
-    const int2 w = tail.where ? tail.where[row] : make_int2((int)(row * tail.nsplit), (int)tail.nsplit);
-    slot = (int64_t)w.x * a.G + g;
-    more = w.y;
-  }
-  const int ns = own + more;
-  auto ml = [&](int s) { return s < own ? a.ml[at + (int64_t)s * a.rows] : tail.ml[slot + (int64_t)(s - own) * a.G]; };
+  const JoinFrom from = join_from(a, tail, (int)blockIdx.x);
+  const int ns = from.own + from.more;
+  auto ml = [&](int s) { return from.ml(a, tail, s); };
   float big = kLowest;
   for (int s = tid; s < ns; s += kJoinThreads) big = fmaxf(big, ml(s).x);
 #pragma unroll
@@ -54,8 +70,7 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(MultiArgs a, Tail ta
   for (int s = grp; s < ns; s += kGroups) {
     const float2 x = ml(s);
     if (x.y == 0.0f) continue;  // no weight, and perhaps nothing written
-    const float *p = s < own ? a.part + (at + (int64_t)s * a.rows) * D : tail.part + (slot + (int64_t)(s - own) * a.G) * D;
-    const float4 u = reinterpret_cast<const float4 *>(p)[lane];
+    const float4 u = reinterpret_cast<const float4 *>(from.part(a, tail, s, D))[lane];
     const float f = __builtin_amdgcn_exp2f(x.x - big);
     v.x = fmaf(u.x, f, v.x);
     v.y = fmaf(u.y, f, v.y);
@@ -72,15 +87,47 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(MultiArgs a, Tail ta
 #pragma unroll
   for (int k = 0; k < kWaves; ++k) l += red[1][k];
   const float out = l == 0.0f ? 0.0f : sum / l;
-  const int64_t to = (a.shared ? (o * a.BH + r) * a.G + g : (r * a.G + g) * a.O + o) * D + tid;
+  const int64_t to = from.to * D + tid;
   if constexpr (OUT == FATHOM_DT_F32) static_cast<float *>(a.out)[to] = out;
   else if constexpr (OUT == FATHOM_DT_F16) static_cast<uint16_t *>(a.out)[to] = float_to_f16_bits(out);
   else static_cast<uint16_t *>(a.out)[to] = float_to_bf16_bits(out);
 }
 
+// The same for many queries: D / 4 lanes per query, which take its splits one after the other with a running maximum.
+template <int D, int OUT>
+__global__ __launch_bounds__(kJoinThreads) void join_many_kernel(MultiArgs a, Tail tail) {
+  constexpr int kLanes = D / 4;
+  const int lane = threadIdx.x % kLanes, m = (int)blockIdx.x * (kJoinThreads / kLanes) + threadIdx.x / kLanes;
+  if (m >= a.G * a.O) return;
+  const JoinFrom from = join_from(a, tail, m);
+  float big = kLowest, l = 0.0f, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int s = 0; s < from.own + from.more; ++s) {
+    const float2 x = from.ml(a, tail, s);
+    const float4 u = x.y == 0.0f ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : reinterpret_cast<const float4 *>(from.part(a, tail, s, D))[lane];
+    const float top = fmaxf(big, x.x), was = __builtin_amdgcn_exp2f(big - top), f = __builtin_amdgcn_exp2f(x.x - top);
+    big = top;
+    l = fmaf(x.y, f, l * was);
+    v[0] = fmaf(u.x, f, v[0] * was);
+    v[1] = fmaf(u.y, f, v[1] * was);
+    v[2] = fmaf(u.z, f, v[2] * was);
+    v[3] = fmaf(u.w, f, v[3] * was);
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) v[k] = l == 0.0f ? 0.0f : v[k] / l;
+  store4<OUT>(a.out, from.to * D + 4 * lane, v);
+}
+
 template <int D>
 void launch_join(const MultiArgs &a, const Tail &t, int out, hipStream_t st) {
-  const dim3 grid((unsigned)((int64_t)a.G * a.O), (unsigned)a.BH);
+  const int64_t M = (int64_t)a.G * a.O;
+  if (M * a.BH >= kJoinMany) {
+    const dim3 grid((unsigned)cdiv(M, (int64_t)(1024 / D)), (unsigned)a.BH);
+    if (out == FATHOM_DT_F32) join_many_kernel<D, FATHOM_DT_F32><<<grid, kJoinThreads, 0, st>>>(a, t);
+    else if (out == FATHOM_DT_F16) join_many_kernel<D, FATHOM_DT_F16><<<grid, kJoinThreads, 0, st>>>(a, t);
+    else join_many_kernel<D, FATHOM_DT_BF16><<<grid, kJoinThreads, 0, st>>>(a, t);
+    return;
+  }
+  const dim3 grid((unsigned)M, (unsigned)a.BH);
   if (out == FATHOM_DT_F32) join_kernel<D, FATHOM_DT_F32><<<grid, kJoinThreads, 0, st>>>(a, t);
   else if (out == FATHOM_DT_F16) join_kernel<D, FATHOM_DT_F16><<<grid, kJoinThreads, 0, st>>>(a, t);
   else join_kernel<D, FATHOM_DT_BF16><<<grid, kJoinThreads, 0, st>>>(a, t);
@@ -100,15 +147,25 @@ int tile_rows(int64_t BH, int64_t M, int64_t nb, bool four) {
 
 bool takes_four(const MultiArgs &a, int q_dtype) { return q_dtype == FATHOM_DT_F32 || a.softcap > 0.0f || a.slopes; }
 
+// Workgroups that are at work at once.
+int64_t places_of(int rows) { return rows == 256 ? 256 : 512; }
+
+// Whether tiles of up to nb blocks, of rows of one length, are cut into shares: up to half as many tiles as places where more
+// than the partial results' time is won, about four blocks and with more queries more (8 x 12 x 200 queries over 501 tokens 22 us
+// a workgroup per tile, 32 cut; over 1000 tokens 45, 37); up to three quarters where rows are long (8 x 4 x 1100 over 20000 tokens 647
+// us, 478; x 1500 over 32768 1053, 1008, over 8192 278, 290).  More even out by themselves, those that see most first.
+bool shares_pay(int64_t tiles, int64_t places, int64_t nb) {
+  const int64_t won = nb * (places - tiles);
+  return 2 * tiles <= places ? won > 4 * places + 10 * tiles : 4 * tiles <= 3 * places && won > 64 * places;
+}
+
 // Shares that tiles of up to nb blocks are cut into (at most that many and one per tile more); 0: a workgroup takes each tile.
-// `places` workgroups are at work at once, two per CU.  Few tiles are cut so that all places
-// have the same to do.  So are tiles that see very different lengths (`even` is false), up to twice the places: into a few
-// rounds, as every tile's last share is shorter; of shares, a workgroup's partial results cost about four blocks.  More tiles
-// even out by themselves, those that see most first.  (32 ragged rows of 572 tokens, 576 tiles: 509 us a workgroup per tile, 283
-// in five rounds.)
-int64_t tile_shares(int64_t BH, int64_t M, int rows, int64_t nb, bool even) {
-  const int64_t tiles = BH * cdiv(M, (int64_t)rows), places = rows == 256 ? 256 : 512;
-  if (nb <= (rows == 32 ? 16 : 4) || tiles >= 2 * places || (even && tiles > places / 2)) return 0;
+// Few tiles are cut so that all places have the same to do; more of them, as those of ragged rows up to twice the places, into a
+// few rounds, as every tile's last share is shorter; of shares, a workgroup's partial results cost about four blocks.  (32 ragged
+// rows of 572 tokens of 4 heads in up to 16000: 1114 us a workgroup per tile; 414.)
+int64_t tile_shares(int64_t BH, int64_t M, int rows, int64_t nb) {
+  const int64_t tiles = BH * cdiv(M, (int64_t)rows), places = places_of(rows);
+  if (nb <= (rows == 32 ? 16 : 4) || tiles >= 2 * places) return 0;
   const int64_t rounds = cdiv(3 * tiles, places), most = tiles * cdiv(nb, (int64_t)4);
   const int64_t shares = rounds == 1 ? places - tiles : places * rounds - tiles * 5 / 8;
   return most < shares ? most : shares;
@@ -120,7 +177,8 @@ int64_t tile_splits(int64_t tiles, int64_t shares, int64_t nb) {
 }
 // The same for a prefix, whose tiles always leave partial results.
 int64_t prefix_shares(int64_t BH, int64_t M, int rows, int64_t nb) {
-  const int64_t shares = tile_shares(BH, M, rows, nb, true), tiles = BH * cdiv(M, (int64_t)rows);
+  const int64_t tiles = BH * cdiv(M, (int64_t)rows), places = places_of(rows);
+  const int64_t shares = 2 * tiles <= places || shares_pay(tiles, places, nb) ? tile_shares(BH, M, rows, nb) : 0;
   return shares > tiles ? shares : tiles;
 }
 
@@ -179,7 +237,7 @@ extern "C" size_t fathom_rows8_chunk_attention_workspace_bytes(int64_t BH, int64
   size_t most = 0;  // of whichever tiles a call takes
   for (const int rows : {32, 128, 256}) {
     if ((rows == 32) != (G * T <= 32)) continue;
-    const int64_t shares = tile_shares(BH, G * T, rows, cdiv(positions, (int64_t)kBlk) + 1, false);
+    const int64_t shares = tile_shares(BH, G * T, rows, cdiv(positions, (int64_t)kBlk) + 1);
     if (shares) most = std::max(most, multi_bytes(BH, G * T, rows, D, shares));
   }
   return most;
@@ -213,8 +271,8 @@ extern "C" int fathom_rows8_chunk_attention(const void *q, int q_dtype, int64_t 
   const int64_t nb = tile_blocks(most, T, window, sinks);
   a.rows = tile_rows(BH, G * T, nb, takes_four(a, q_dtype));
   a.tiles = (int)cdiv(G * T, (int64_t)a.rows);
-  const bool even = !lens && (window > 0 || most >= 4 * T);
-  a.shares = (int)tile_shares(BH, G * T, a.rows, nb, even);
+  const int64_t tiles = BH * a.tiles, places = places_of(a.rows);
+  a.shares = lens || shares_pay(tiles, places, nb) ? (int)tile_shares(BH, G * T, a.rows, nb) : 0;
   if (a.shares) {
     const size_t need = multi_bytes(BH, G * T, a.rows, D, a.shares);
     if (!workspace || workspace_bytes < need)
@@ -222,7 +280,8 @@ extern "C" int fathom_rows8_chunk_attention(const void *q, int q_dtype, int64_t 
     if (reinterpret_cast<uintptr_t>(workspace) & 15)
       return fail(FATHOM_ERR_INVALID, "%s: the workspace must be 16-byte aligned", what);
     place(a, workspace, D);
-    if (!lens && even) a.splits = (int)tile_splits(BH * a.tiles, a.shares, nb);
+    // tiles that see nearly the same are cut equally, without a search
+    if (!lens && (window > 0 || most >= 4 * T) && 2 * tiles <= places) a.splits = (int)tile_splits(tiles, a.shares, nb);
   }
   rc = run_multi(a, q_dtype, D, code_dtype == FATHOM_DT_I8, (hipStream_t)stream);
   return rc || !a.shares ? rc : run_join(a, Tail{}, q_dtype, D, (hipStream_t)stream);
@@ -275,7 +334,8 @@ extern "C" int fathom_rows8_shared_attention(const void *q, int q_dtype, const v
   if (reinterpret_cast<uintptr_t>(workspace) & 15)
     return fail(FATHOM_ERR_INVALID, "%s: the workspace must be 16-byte aligned", what);
   place(a, workspace, D);
-  if (!prefix_lens) a.splits = (int)tile_splits(prefix_BH * a.tiles, a.shares, nb);
+  const int64_t tiles = prefix_BH * a.tiles;
+  if (!prefix_lens && (2 * tiles <= places_of(a.rows) || a.shares == tiles)) a.splits = (int)tile_splits(tiles, a.shares, nb);
   const bool i8 = code_dtype == FATHOM_DT_I8;
   const hipStream_t st = (hipStream_t)stream;
   Tail t;

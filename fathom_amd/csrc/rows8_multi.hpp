@@ -67,6 +67,17 @@ __device__ __forceinline__ TileSpan tile_span(const MultiArgs &a, int64_t r, int
   return s;
 }
 
+// Four floats at element `at` of an output of type DT.
+template <int DT>
+__device__ __forceinline__ void store4(void *out, int64_t at, const float (&v)[4]) {
+  if constexpr (DT == FATHOM_DT_F32) {
+    *reinterpret_cast<float4 *>(static_cast<float *>(out) + at) = make_float4(v[0], v[1], v[2], v[3]);
+  } else {
+    const u32x2v w = {pack2<DT>(v[0], v[1]), pack2<DT>(v[2], v[3])};
+    *reinterpret_cast<u32x2v *>(static_cast<uint16_t *>(out) + at) = w;
+  }
+}
+
 #ifdef FATHOM_ROWS8_MULTI_KERNEL
 namespace {
 
@@ -154,17 +165,6 @@ __device__ __forceinline__ float other_half(float v) {  // of lane l ^ 32
   const uint32_t x = __float_as_uint(v);
   const auto p = __builtin_amdgcn_permlane32_swap(x, x, false, false);
   return __uint_as_float((threadIdx.x & 32) ? p[0] : p[1]);
-}
-
-// Four floats at element `at` of an output of type DT.
-template <int DT>
-__device__ __forceinline__ void store4(void *out, int64_t at, const float (&v)[4]) {
-  if constexpr (DT == FATHOM_DT_F32) {
-    *reinterpret_cast<float4 *>(static_cast<float *>(out) + at) = make_float4(v[0], v[1], v[2], v[3]);
-  } else {
-    const u32x2v w = {pack2<DT>(v[0], v[1]), pack2<DT>(v[2], v[3])};
-    *reinterpret_cast<u32x2v *>(static_cast<uint16_t *>(out) + at) = w;
-  }
 }
 
 // The part of a workgroup where tiles are shared out: its tile (of all rows'), split, the tile's splits (0: the call needs

@@ -133,22 +133,28 @@ void launch_join(const MultiArgs &a, const Tail &t, int out, hipStream_t st) {
   else join_kernel<D, FATHOM_DT_BF16><<<grid, kJoinThreads, 0, st>>>(a, t);
 }
 
+// The tiles of a call: queries of one, and workgroups that are at work at once.
+struct Tiling {
+  int rows;
+  int64_t places;
+};
+constexpr Tiling kTilings[] = {{32, 512}, {32, 256}, {128, 512}, {256, 256}};
+
+bool takes_four(const MultiArgs &a, int q_dtype) { return q_dtype == FATHOM_DT_F32 || a.softcap > 0.0f || a.slopes; }
+
 // Queries of a tile of rows that see up to nb blocks: one wave's, where a row has no more; eight waves', which stage a block for
 // twice the queries (8 x 4 x 2048 over 65536 tokens 2.22 ms; by fours 2.44), where that leaves no more of their places empty or the
 // queries are many, and there is work for all CUs in shares of four blocks (512 queries of 4 rows over 4096 tokens 42 us; 38).
 // `four`: float32 queries and calls with a cap or bias take four waves.  Their registers or a block's longer way leave eight
 // to wait for the slowest (f32, 8 x 4 x 1024 over 16384 tokens 797 us; 728.  Capped and biased, 4 x 12 x 3001 behind a window of
 // 4096: 535; 464).
-int tile_rows(int64_t BH, int64_t M, int64_t nb, bool four) {
-  if (M <= 32) return 32;
+// A wave by itself with float32 queries, a cap or a bias has a SIMD's registers at D = 128, so that half as many workgroups are
+// at work (8 rows of 262144 tokens, 4 x 4 f32 queries 119 us in twice as many shares; 105).
+Tiling tiling_of(int64_t BH, int64_t M, int64_t D, int64_t nb, bool four) {
+  if (M <= 32) return kTilings[four && D == 128 ? 1 : 0];
   const int64_t eights = cdiv(M, (int64_t)256);
-  return !four && (M >= 2048 || eights * 2 == cdiv(M, (int64_t)128)) && BH * eights * cdiv(nb, (int64_t)4) >= 256 ? 256 : 128;
+  return kTilings[!four && (M >= 2048 || eights * 2 == cdiv(M, (int64_t)128)) && BH * eights * cdiv(nb, (int64_t)4) >= 256 ? 3 : 2];
 }
-
-bool takes_four(const MultiArgs &a, int q_dtype) { return q_dtype == FATHOM_DT_F32 || a.softcap > 0.0f || a.slopes; }
-
-// Workgroups that are at work at once.
-int64_t places_of(int rows) { return rows == 256 ? 256 : 512; }
 
 // Whether tiles of up to nb blocks, of rows of one length, are cut into shares: up to half as many tiles as places where more
 // than the partial results' time is won, about four blocks and with more queries more (8 x 12 x 200 queries over 501 tokens 22 us
@@ -159,26 +165,38 @@ bool shares_pay(int64_t tiles, int64_t places, int64_t nb) {
   return 2 * tiles <= places ? won > 4 * places + 10 * tiles : 4 * tiles <= 3 * places && won > 64 * places;
 }
 
+// The same for tiles of 32 queries, whose four waves take blocks in turn, and for ragged rows of such (600 rows of up to 1500
+// tokens 27 us a workgroup per row, 53 cut; of up to 16000 201, 180).  Rows of one length that keep 7 of 10 CUs busy reach HBM's
+// rate by themselves (200 of 16000 tokens 131 us, 140 cut; 300, two on some CUs, 258, 220; 128 of 8000 60, 49).
+bool shares_pay_32(int64_t tiles, int64_t places, int64_t nb, bool ragged) {
+  if (ragged) return nb * places > 16 * places + 96 * tiles;
+  const int64_t cus = 256 * cdiv(tiles, (int64_t)256);
+  return 10 * tiles < 7 * cus && (tiles > 256 ? nb > 128 : 256 * nb > 12 * 256 + 40 * tiles);
+}
+
 // Shares that tiles of up to nb blocks are cut into (at most that many and one per tile more); 0: a workgroup takes each tile.
 // Few tiles are cut so that all places have the same to do; more of them, as those of ragged rows up to twice the places, into a
 // few rounds, as every tile's last share is shorter; of shares, a workgroup's partial results cost about four blocks.  (32 ragged
 // rows of 572 tokens of 4 heads in up to 16000: 1114 us a workgroup per tile; 414.)
-int64_t tile_shares(int64_t BH, int64_t M, int rows, int64_t nb) {
-  const int64_t tiles = BH * cdiv(M, (int64_t)rows), places = places_of(rows);
-  if (nb <= (rows == 32 ? 16 : 4) || tiles >= 2 * places) return 0;
+int64_t tile_shares(int64_t BH, int64_t M, Tiling t, int64_t nb) {
+  const int64_t tiles = BH * cdiv(M, (int64_t)t.rows), places = t.places;
+  if (nb <= (t.rows == 32 ? 16 : 4) || tiles >= 2 * places) return 0;
   const int64_t rounds = cdiv(3 * tiles, places), most = tiles * cdiv(nb, (int64_t)4);
   const int64_t shares = rounds == 1 ? places - tiles : places * rounds - tiles * 5 / 8;
   return most < shares ? most : shares;
 }
-// Splits of each of so many tiles that all have the same to do: as many as there are places, of four blocks and more.
-int64_t tile_splits(int64_t tiles, int64_t shares, int64_t nb) {
-  const int64_t room = (shares + tiles) / tiles, most = cdiv(nb, (int64_t)4);
+// Splits of each of so many tiles that all have the same to do, of four blocks and more: as many as there are places, or, of tiles of
+// 32 queries, no more than are at work at once (128 rows of 8000 tokens, f32 queries, in two rounds 66 us; 57).
+int64_t tile_splits(int64_t tiles, Tiling t, int64_t shares, int64_t nb) {
+  int64_t room = (shares + tiles) / tiles;
+  if (t.rows == 32 && tiles <= t.places) room = std::min(room, t.places / tiles);
+  const int64_t most = cdiv(nb, (int64_t)4);
   return most < 1 ? 1 : room < most ? room : most;
 }
 // The same for a prefix, whose tiles always leave partial results.
-int64_t prefix_shares(int64_t BH, int64_t M, int rows, int64_t nb) {
-  const int64_t tiles = BH * cdiv(M, (int64_t)rows), places = places_of(rows);
-  const int64_t shares = 2 * tiles <= places || shares_pay(tiles, places, nb) ? tile_shares(BH, M, rows, nb) : 0;
+int64_t prefix_shares(int64_t BH, int64_t M, Tiling t, int64_t nb) {
+  const int64_t tiles = BH * cdiv(M, (int64_t)t.rows);
+  const int64_t shares = 2 * tiles <= t.places || shares_pay(tiles, t.places, nb) ? tile_shares(BH, M, t, nb) : 0;
   return shares > tiles ? shares : tiles;
 }
 
@@ -235,10 +253,10 @@ extern "C" size_t fathom_rows8_chunk_attention_workspace_bytes(int64_t BH, int64
   if (!shape_taken(BH, G, D) || !queries_taken(BH, G, T) || positions < 1) return 0;
   if (positions > kMaxCap) positions = kMaxCap;
   size_t most = 0;  // of whichever tiles a call takes
-  for (const int rows : {32, 128, 256}) {
-    if ((rows == 32) != (G * T <= 32)) continue;
-    const int64_t shares = tile_shares(BH, G * T, rows, cdiv(positions, (int64_t)kBlk) + 1);
-    if (shares) most = std::max(most, multi_bytes(BH, G * T, rows, D, shares));
+  for (const Tiling t : kTilings) {
+    if ((t.rows == 32) != (G * T <= 32)) continue;
+    const int64_t shares = tile_shares(BH, G * T, t, cdiv(positions, (int64_t)kBlk) + 1);
+    if (shares) most = std::max(most, multi_bytes(BH, G * T, t.rows, D, shares));
   }
   return most;
 }
@@ -269,10 +287,12 @@ extern "C" int fathom_rows8_chunk_attention(const void *q, int q_dtype, int64_t 
               kernel_cap(softcap), slopes, out, nullptr, nullptr, nullptr, 0, 1, 0, 0, false};
   const int64_t most = lens ? cap : n;
   const int64_t nb = tile_blocks(most, T, window, sinks);
-  a.rows = tile_rows(BH, G * T, nb, takes_four(a, q_dtype));
+  const Tiling t = tiling_of(BH, G * T, D, nb, takes_four(a, q_dtype));
+  a.rows = t.rows;
   a.tiles = (int)cdiv(G * T, (int64_t)a.rows);
-  const int64_t tiles = BH * a.tiles, places = places_of(a.rows);
-  a.shares = lens || shares_pay(tiles, places, nb) ? (int)tile_shares(BH, G * T, a.rows, nb) : 0;
+  const int64_t tiles = BH * a.tiles;
+  const bool cut = a.rows == 32 ? shares_pay_32(tiles, t.places, nb, lens) : lens || shares_pay(tiles, t.places, nb);
+  a.shares = cut ? (int)tile_shares(BH, G * T, t, nb) : 0;
   if (a.shares) {
     const size_t need = multi_bytes(BH, G * T, a.rows, D, a.shares);
     if (!workspace || workspace_bytes < need)
@@ -281,7 +301,7 @@ extern "C" int fathom_rows8_chunk_attention(const void *q, int q_dtype, int64_t 
       return fail(FATHOM_ERR_INVALID, "%s: the workspace must be 16-byte aligned", what);
     place(a, workspace, D);
     // tiles that see nearly the same are cut equally, without a search
-    if (!lens && (window > 0 || most >= 4 * T) && 2 * tiles <= places) a.splits = (int)tile_splits(tiles, a.shares, nb);
+    if (!lens && (window > 0 || most >= 4 * T) && 2 * tiles <= t.places) a.splits = (int)tile_splits(tiles, t, a.shares, nb);
   }
   rc = run_multi(a, q_dtype, D, code_dtype == FATHOM_DT_I8, (hipStream_t)stream);
   return rc || !a.shares ? rc : run_join(a, Tail{}, q_dtype, D, (hipStream_t)stream);
@@ -293,10 +313,10 @@ extern "C" size_t fathom_rows8_shared_attention_workspace_bytes(int64_t prefix_B
   if (prefix_positions > kMaxCap) prefix_positions = kMaxCap;
   if (prefix_positions < 0) prefix_positions = 0;
   size_t most = 0;  // of whichever tiles a call takes
-  for (const int rows : {32, 128, 256}) {
-    if ((rows == 32) != (G * sequences <= 32)) continue;
-    const int64_t shares = prefix_shares(prefix_BH, G * sequences, rows, cdiv(prefix_positions, (int64_t)kBlk));
-    most = std::max(most, multi_bytes(prefix_BH, G * sequences, rows, D, shares));
+  for (const Tiling t : kTilings) {
+    if ((t.rows == 32) != (G * sequences <= 32)) continue;
+    const int64_t shares = prefix_shares(prefix_BH, G * sequences, t, cdiv(prefix_positions, (int64_t)kBlk));
+    most = std::max(most, multi_bytes(prefix_BH, G * sequences, t.rows, D, shares));
   }
   return most + tail_bytes(prefix_BH * sequences, G, D, positions < 0 ? 0 : positions);
 }
@@ -325,9 +345,10 @@ extern "C" int fathom_rows8_shared_attention(const void *q, int q_dtype, const v
               prefix_v_scale, prefix_cap, cdiv(prefix_cap, kBlk), prefix_lens, prefix_n, (int)G, (int)sequences, 0, 0, true,
               lens, n, cap, prefix_BH, scale, kernel_cap(softcap), slopes, out, nullptr, nullptr, nullptr, 1, 1, 0, 0, false};
   const int64_t nb = cdiv(prefix_lens ? prefix_cap : prefix_n, (int64_t)kBlk);
-  a.rows = tile_rows(prefix_BH, G * sequences, nb, takes_four(a, q_dtype));
+  const Tiling by = tiling_of(prefix_BH, G * sequences, D, nb, takes_four(a, q_dtype));
+  a.rows = by.rows;
   a.tiles = (int)cdiv(G * sequences, (int64_t)a.rows);
-  a.shares = (int)prefix_shares(prefix_BH, G * sequences, a.rows, nb);
+  a.shares = (int)prefix_shares(prefix_BH, G * sequences, by, nb);
   const size_t first = multi_bytes(prefix_BH, G * sequences, a.rows, D, a.shares);
   if (!workspace || workspace_bytes < first)
     return fail(FATHOM_ERR_WORKSPACE, "%s: workspace %zu bytes, need more than %zu", what, workspace_bytes, first);
@@ -335,7 +356,7 @@ extern "C" int fathom_rows8_shared_attention(const void *q, int q_dtype, const v
     return fail(FATHOM_ERR_INVALID, "%s: the workspace must be 16-byte aligned", what);
   place(a, workspace, D);
   const int64_t tiles = prefix_BH * a.tiles;
-  if (!prefix_lens && (2 * tiles <= places_of(a.rows) || a.shares == tiles)) a.splits = (int)tile_splits(tiles, a.shares, nb);
+  if (!prefix_lens && (2 * tiles <= by.places || a.shares == tiles)) a.splits = (int)tile_splits(tiles, by, a.shares, nb);
   const bool i8 = code_dtype == FATHOM_DT_I8;
   const hipStream_t st = (hipStream_t)stream;
   Tail t;

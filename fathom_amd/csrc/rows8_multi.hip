@@ -11,6 +11,8 @@ constexpr int64_t kMaxTiles = 65535;  // grid y
 // Queries from which D / 4 lanes join each one's splits: they fill the device, and have few splits each (8 x 12 x 396 queries over 501
 // tokens in two shares 78 us with a workgroup per query; 38).
 constexpr int64_t kJoinMany = 4096;
+// Below that D / 32 workgroups take a query's channels (8 queries of 320 splits 28 us with the call; 24.  512 of 16 ragged ones 27.5; 28.7).
+constexpr int64_t kJoinWide = 512;
 
 // Where the partial results of query m of row blockIdx.y lie: `own` splits of its tile and, behind a shared prefix, `more` of its
 // sequence's own tokens; `to` is its place in the output, in rows.
@@ -38,85 +40,99 @@ __device__ __forceinline__ JoinFrom join_from(const MultiArgs &a, const Tail &ta
   return f;
 }
 
-// Joins a query's splits, and its sequence's own tokens behind a shared prefix: one workgroup per query, D / 4 lanes
-// take 16 bytes of every (1024 / D)-th split.  The splits' weights 2^(m_s - m) are formed by all threads for the sum and again
-// beside each row, which is cheaper than a pass to keep them.  Bound: latency, and L2 for many (1024 queries of 64 splits, 34 MB,
-// 10 us; 128 ragged ones 6).
-template <int D, int OUT>
-__global__ __launch_bounds__(kJoinThreads) void join_kernel(MultiArgs a, Tail tail) {
-  constexpr int kLanes = D / 4, kGroups = kJoinThreads / kLanes, kWaves = kJoinThreads / kWave;
-  __shared__ float4 acc[kGroups][kLanes];
-  __shared__ float red[2][kWaves];
-  const int tid = threadIdx.x, lane = tid % kLanes, grp = tid / kLanes;
-  const JoinFrom from = join_from(a, tail, (int)blockIdx.x);
+// Splits first, first + step, .. of a query in channels c .. c + 3: their largest score and, relative to it, the sums.  Four are on
+// their way at a time (8 x 4 x 140 queries over 8000 tokens 52 us one by one; 47.5).
+struct Joined {
+  float big, l;
+  float4 v;
+};
+__device__ __forceinline__ Joined join_splits(const MultiArgs &a, const Tail &tail, const JoinFrom &from, int first, int step, int D, int c) {
   const int ns = from.own + from.more;
-  auto ml = [&](int s) { return from.ml(a, tail, s); };
-  float big = kLowest;
-  for (int s = tid; s < ns; s += kJoinThreads) big = fmaxf(big, ml(s).x);
-#pragma unroll
-  for (int x = 32; x > 0; x >>= 1) big = fmaxf(big, __shfl_xor(big, x));
-  if ((tid & 63) == 0) red[0][tid >> 6] = big;
-  __syncthreads();
-#pragma unroll
-  for (int k = 0; k < kWaves; ++k) big = fmaxf(big, red[0][k]);
-  float l = 0.0f;
-  for (int s = tid; s < ns; s += kJoinThreads) {
-    const float2 x = ml(s);
-    l = fmaf(x.y, __builtin_amdgcn_exp2f(x.x - big), l);
-  }
-  l = wave_sum_f(l);
-  if ((tid & 63) == 0) red[1][tid >> 6] = l;
+  float big = kLowest, l = 0.0f;
   float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  for (int s = grp; s < ns; s += kGroups) {
-    const float2 x = ml(s);
-    if (x.y == 0.0f) continue;  // no weight, and perhaps nothing written
-    const float4 u = reinterpret_cast<const float4 *>(from.part(a, tail, s, D))[lane];
-    const float f = __builtin_amdgcn_exp2f(x.x - big);
-    v.x = fmaf(u.x, f, v.x);
-    v.y = fmaf(u.y, f, v.y);
-    v.z = fmaf(u.z, f, v.z);
-    v.w = fmaf(u.w, f, v.w);
+  for (int s0 = first; s0 < ns; s0 += 4 * step) {
+    float2 x[4];
+    float4 u[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int s = s0 + j * step, at = s < ns ? s : s0;
+      x[j] = from.ml(a, tail, at);
+      u[j] = *reinterpret_cast<const float4 *>(from.part(a, tail, at, D) + c);
+      if (s >= ns) x[j].y = 0.0f;
+    }
+    float top = big;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) top = fmaxf(top, x[j].x);
+    const float was = __builtin_amdgcn_exp2f(big - top);
+    big = top;
+    l *= was;
+    v = make_float4(v.x * was, v.y * was, v.z * was, v.w * was);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (x[j].y == 0.0f) continue;  // no weight, and perhaps nothing written
+      const float f = __builtin_amdgcn_exp2f(x[j].x - top);
+      l = fmaf(x[j].y, f, l);
+      v.x = fmaf(u[j].x, f, v.x);
+      v.y = fmaf(u[j].y, f, v.y);
+      v.z = fmaf(u[j].z, f, v.z);
+      v.w = fmaf(u[j].w, f, v.w);
+    }
   }
-  acc[grp][lane] = v;
+  return Joined{big, l, v};
+}
+
+// Joins a query's splits, and its sequence's own tokens behind a shared prefix: a workgroup per query and CH channels, of which
+// CH / 4 lanes take every (1024 / CH)-th split.  Bound: latency, and L2 for many (1024 queries of 64 splits, 34 MB, 9 us).
+template <int D, int CH, int OUT>
+__global__ __launch_bounds__(kJoinThreads) void join_kernel(MultiArgs a, Tail tail) {
+  constexpr int kLanes = CH / 4, kGroups = kJoinThreads / kLanes;
+  __shared__ float4 acc[kGroups][kLanes];
+  __shared__ float2 sums[kGroups];
+  const int tid = threadIdx.x, lane = tid % kLanes, grp = tid / kLanes, c0 = CH * (int)blockIdx.z;
+  const JoinFrom from = join_from(a, tail, (int)blockIdx.x);
+  const Joined mine = join_splits(a, tail, from, grp, kGroups, D, c0 + 4 * lane);
+  acc[grp][lane] = mine.v;
+  if (lane == 0) sums[grp] = make_float2(mine.big, mine.l);
   __syncthreads();
-  if (tid >= D) return;
-  float sum = 0.0f;
-  l = 0.0f;
+  if (tid >= CH) return;
+  float big = kLowest, sum = 0.0f, l = 0.0f;
 #pragma unroll
-  for (int k = 0; k < kGroups; ++k) sum += reinterpret_cast<const float *>(acc[k])[tid];
+  for (int k = 0; k < kGroups; ++k) big = fmaxf(big, sums[k].x);
 #pragma unroll
-  for (int k = 0; k < kWaves; ++k) l += red[1][k];
+  for (int k = 0; k < kGroups; ++k) {
+    const float f = __builtin_amdgcn_exp2f(sums[k].x - big);
+    sum = fmaf(reinterpret_cast<const float *>(acc[k])[tid], f, sum);
+    l = fmaf(sums[k].y, f, l);
+  }
   const float out = l == 0.0f ? 0.0f : sum / l;
-  const int64_t to = from.to * D + tid;
+  const int64_t to = from.to * D + c0 + tid;
   if constexpr (OUT == FATHOM_DT_F32) static_cast<float *>(a.out)[to] = out;
   else if constexpr (OUT == FATHOM_DT_F16) static_cast<uint16_t *>(a.out)[to] = float_to_f16_bits(out);
   else static_cast<uint16_t *>(a.out)[to] = float_to_bf16_bits(out);
 }
 
-// The same for many queries: D / 4 lanes per query, which take its splits one after the other with a running maximum.
+// The same for many queries: D / 4 lanes take all of a query's splits.
 template <int D, int OUT>
 __global__ __launch_bounds__(kJoinThreads) void join_many_kernel(MultiArgs a, Tail tail) {
   constexpr int kLanes = D / 4;
   const int lane = threadIdx.x % kLanes, m = (int)blockIdx.x * (kJoinThreads / kLanes) + threadIdx.x / kLanes;
   if (m >= a.G * a.O) return;
   const JoinFrom from = join_from(a, tail, m);
-  float big = kLowest, l = 0.0f, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int s = 0; s < from.own + from.more; ++s) {
-    const float2 x = from.ml(a, tail, s);
-    const float4 u = x.y == 0.0f ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : reinterpret_cast<const float4 *>(from.part(a, tail, s, D))[lane];
-    const float top = fmaxf(big, x.x), was = __builtin_amdgcn_exp2f(big - top), f = __builtin_amdgcn_exp2f(x.x - top);
-    big = top;
-    l = fmaf(x.y, f, l * was);
-    v[0] = fmaf(u.x, f, v[0] * was);
-    v[1] = fmaf(u.y, f, v[1] * was);
-    v[2] = fmaf(u.z, f, v[2] * was);
-    v[3] = fmaf(u.w, f, v[3] * was);
-  }
+  const Joined all = join_splits(a, tail, from, 0, 1, D, 4 * lane);
+  const float v[4] = {all.v.x, all.v.y, all.v.z, all.v.w};
+  float out[4];
 #pragma unroll
-  for (int k = 0; k < 4; ++k) v[k] = l == 0.0f ? 0.0f : v[k] / l;
-  store4<OUT>(a.out, from.to * D + 4 * lane, v);
+  for (int k = 0; k < 4; ++k) out[k] = all.l == 0.0f ? 0.0f : v[k] / all.l;
+  store4<OUT>(a.out, from.to * D + 4 * lane, out);
 }
 
+template <int D, int CH>
+void launch_join(const MultiArgs &a, const Tail &t, int out, hipStream_t st) {
+  const dim3 grid((unsigned)((int64_t)a.G * a.O), (unsigned)a.BH, D / CH);
+  if (out == FATHOM_DT_F32) join_kernel<D, CH, FATHOM_DT_F32><<<grid, kJoinThreads, 0, st>>>(a, t);
+  else if (out == FATHOM_DT_F16) join_kernel<D, CH, FATHOM_DT_F16><<<grid, kJoinThreads, 0, st>>>(a, t);
+  else join_kernel<D, CH, FATHOM_DT_BF16><<<grid, kJoinThreads, 0, st>>>(a, t);
+}
 template <int D>
 void launch_join(const MultiArgs &a, const Tail &t, int out, hipStream_t st) {
   const int64_t M = (int64_t)a.G * a.O;
@@ -127,10 +143,8 @@ void launch_join(const MultiArgs &a, const Tail &t, int out, hipStream_t st) {
     else join_many_kernel<D, FATHOM_DT_BF16><<<grid, kJoinThreads, 0, st>>>(a, t);
     return;
   }
-  const dim3 grid((unsigned)M, (unsigned)a.BH);
-  if (out == FATHOM_DT_F32) join_kernel<D, FATHOM_DT_F32><<<grid, kJoinThreads, 0, st>>>(a, t);
-  else if (out == FATHOM_DT_F16) join_kernel<D, FATHOM_DT_F16><<<grid, kJoinThreads, 0, st>>>(a, t);
-  else join_kernel<D, FATHOM_DT_BF16><<<grid, kJoinThreads, 0, st>>>(a, t);
+  if (M * a.BH >= kJoinWide) launch_join<D, D>(a, t, out, st);
+  else launch_join<D, 32>(a, t, out, st);
 }
 
 // The tiles of a call: queries of one, and workgroups that are at work at once.

@@ -83,7 +83,7 @@ class RowStore8:
                 and k_scale.is_contiguous() and v_scale.is_contiguous()):
             raise ValueError("the store's tensors must be contiguous and on one device")
         self.k8, self.v8, self.k_scale, self.v_scale = k8, v8, k_scale, v_scale
-        self.device = dev
+        self.device, self._gpu = dev, dev.index
         self._code = _CODES[k8.dtype]
 
     @classmethod
@@ -123,7 +123,7 @@ class RowStore8:
             if not -_FAR < v < _FAR:
                 raise ValueError(f"{what} {v}")
             return None, None, v
-        if v.device != self.device:
+        if v.get_device() != self._gpu:
             self._elsewhere(v)
         dtype = v.dtype
         if v.shape != (self.BH,) or (dtype != _I32 and (dtype.is_floating_point or dtype.is_complex or dtype == torch.bool)):
@@ -139,7 +139,7 @@ class RowStore8:
 
     def _query(self, q, scale, softcap, slopes):
         """q as the kernels read it, with its address; the scale, cap and slopes of a call."""
-        if q.device != self.device:
+        if q.get_device() != self._gpu:
             self._elsewhere(q)
         shape = q.shape
         if len(shape) != 3 or shape[0] != self.BH or shape[2] != self.d or shape[1] < 1:
@@ -178,7 +178,7 @@ class RowStore8:
             nbytes = _SIZES[key] = getattr(_lib.lib(), query)(self.BH, G, *queries, self.d, 1 << bits)
         if not nbytes:
             return None, None, 0
-        ws = torch.empty((nbytes,), dtype=torch.uint8, device=self.device)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
         return ws, ws.data_ptr(), nbytes
 
     # ------------------------------------------------------------------ writing and reading
@@ -217,9 +217,9 @@ class RowStore8:
         x_{c+r/2} cos + x_c sin) of the angle t inv_freq[c], whose whole turns are dropped exactly at any t; channels
         behind r stay.  offset is an int or integers [BH]: what stands before the store's first token, as a shared prefix
         does.  Views as in `write`; with a tensor `pos`, rows whose tokens do not all fit are rotated but not written."""
-        dev, BH, d = self.device, self.BH, self.d
+        gpu, BH, d = self._gpu, self.BH, self.d
         for t in (q, K, V):
-            if t.device != dev:
+            if t.get_device() != gpu:
                 self._elsewhere(t)
         shape, k_shape, dtype = q.shape, K.shape, q.dtype
         if len(k_shape) != 3 or k_shape != V.shape or k_shape[0] != BH or k_shape[2] != d:
@@ -231,7 +231,7 @@ class RowStore8:
             raise ValueError(f"q {dtype}, K {K.dtype} and V {V.dtype} must be of one float type")
         turned, inv_at = 0, None
         if inv_freq is not None:
-            if inv_freq.device != dev:
+            if inv_freq.get_device() != gpu:
                 self._elsewhere(inv_freq)
             turned = 2 * inv_freq.numel()
             if inv_freq.dim() != 1 or turned > d or turned % 16 or not inv_freq.dtype.is_floating_point:
@@ -239,19 +239,17 @@ class RowStore8:
             if inv_freq.dtype != _F32 or not inv_freq.is_contiguous():
                 inv_freq = inv_freq.float().contiguous()
             inv_at = inv_freq.data_ptr()
-        w_dtype, weights_at = _F32, (None, None)
+        w_dtype, q_weight_at, k_weight_at = _F32, None, None
         if q_weight is not None or k_weight is not None:
-            given = [w for w in (q_weight, k_weight) if w is not None]
-            for w in given:
-                if w.device != dev:
-                    self._elsewhere(w)
-                if w.shape != (d,) or not w.dtype.is_floating_point:
-                    raise ValueError(f"a weight {w.dtype} {tuple(w.shape)} must be floats [{d}]")
-            if given[0].dtype == given[-1].dtype and given[0].dtype in _KDT:
-                w_dtype = given[0].dtype
-            weights = [w if w is None or (w.dtype == w_dtype and w.is_contiguous()) else w.to(w_dtype).contiguous()
-                       for w in (q_weight, k_weight)]
-            weights_at = [None if w is None else w.data_ptr() for w in weights]
+            first, last = k_weight if q_weight is None else q_weight, q_weight if k_weight is None else k_weight
+            if first.dtype == last.dtype and first.dtype in _KDT:
+                w_dtype = first.dtype
+            if q_weight is not None:
+                q_weight = self._weight(q_weight, w_dtype)
+                q_weight_at = q_weight.data_ptr()
+            if k_weight is not None:
+                k_weight = self._weight(k_weight, w_dtype)
+                k_weight_at = k_weight.data_ptr()
         eps = float(eps)
         if not 0.0 <= eps < math.inf:
             raise ValueError(f"eps {eps} must be finite and not negative")
@@ -260,19 +258,27 @@ class RowStore8:
         q, qr, qh, qt = _heads(q)
         K, kr, kt = _rows(K)
         V, vr, vt = _rows(V)
-        out = torch.empty(shape, dtype=q.dtype, device=dev)
-        k_out = torch.empty(k_shape, dtype=q.dtype, device=dev) if keys else None
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        k_out = torch.empty_like(K, memory_format=torch.contiguous_format) if keys else None
         self._call("fathom_rows8_write_rotated", q.data_ptr(), K.data_ptr(), V.data_ptr(), _KDT[q.dtype], qr, qh, qt, kr, kt, vr,
-                   vt, rows_at, at, shifts_at, shift, inv_at, turned, *weights_at, _KDT[w_dtype], eps, BH, shape[1], T, d, self.cap,
-                   self._code, *self._store(), out.data_ptr(), None if k_out is None else k_out.data_ptr())
+                   vt, rows_at, at, shifts_at, shift, inv_at, turned, q_weight_at, k_weight_at, _KDT[w_dtype], eps, BH, shape[1], T,
+                   d, self.cap, self._code, *self._store(), out.data_ptr(), None if k_out is None else k_out.data_ptr())
         return (out, k_out) if keys else out
+
+    def _weight(self, w, dtype):
+        """A norm's weights as the kernel reads them."""
+        if w.get_device() != self._gpu:
+            self._elsewhere(w)
+        if w.shape != (self.d,) or not w.dtype.is_floating_point:
+            raise ValueError(f"a weight {w.dtype} {tuple(w.shape)} must be floats [{self.d}]")
+        return w if w.dtype == dtype and w.is_contiguous() else w.to(dtype).contiguous()
 
     def _read(self, idx_at, rows_at, at, R, dtype):
         if dtype not in _KDT:
             raise ValueError(f"dtype {dtype} unsupported (float32, float16, bfloat16)")
         if R < 0:
             raise ValueError(f"{R} tokens")
-        K = torch.empty((self.BH, R, self.d), dtype=dtype, device=self.device)
+        K = torch.empty(self.BH, R, self.d, dtype=dtype, device=self.device)
         V = torch.empty_like(K)
         self._call("fathom_rows8_read", *self._store(), self._code, self.BH, self.cap, self.d, idx_at, rows_at, at, R,
                    _KDT[dtype], K.data_ptr(), V.data_ptr())
@@ -349,7 +355,7 @@ class RowStore8:
         t <= p, with a window only the last `window` of them and the first `sinks`.  Scores as in `attention`, with the
         bias slopes[bh, g] (t - p).  [BH, G, T, d] in q's type; a token before the row's first (p < 0) gives zeros, so
         rows of fewer than T tokens are padded in front."""
-        if q.device != self.device:
+        if q.get_device() != self._gpu:
             self._elsewhere(q)
         shape = q.shape
         if len(shape) != 4 or shape[0] != self.BH or shape[1] < 1 or shape[3] != self.d:
@@ -362,7 +368,7 @@ class RowStore8:
         positions = n if lens is None else self.cap
         positions = max(min(positions, window + T + -(-sinks // BLK) * BLK) if window > 0 else positions, 0)
         ws, ws_at, nbytes = self._workspace("fathom_rows8_chunk_attention_workspace_bytes", G, positions, T)
-        out = torch.empty(shape, dtype=q.dtype, device=self.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
         self._call("fathom_rows8_chunk_attention", q.data_ptr(), _KDT[q.dtype], qr, qh, qt, *self._store(), self._code, self.BH, G, T,
                    self.d, self.cap, lens_at, n, window, sinks, scale, softcap, None if slopes is None else slopes.data_ptr(),
                    out.data_ptr(), ws_at, nbytes)
@@ -389,7 +395,7 @@ class RowStore8:
         if nbytes is None:
             nbytes = _SIZES[key] = _lib.lib().fathom_rows8_shared_attention_workspace_bytes(
                 H, self.BH // H, G, self.d, 1 << bits[0].bit_length(), 1 << bits[1].bit_length())
-        ws = torch.empty((nbytes,), dtype=torch.uint8, device=self.device)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
         out = torch.empty_like(q, dtype=_F32)
         self._call("fathom_rows8_shared_attention", q_at, _KDT[q.dtype], *prefix._store(), H, prefix.cap, plens_at, pn,
                    *self._store(), self._code, self.BH // H, G, self.d, self.cap, lens_at, n, scale, softcap,

@@ -33,6 +33,9 @@ _CODES = {torch.float8_e4m3fn: _lib.DT_E4M3, torch.int8: _lib.DT_I8}
 def _rows(x):
     """Rows [BH, T, d] of a float type as the kernels read them, with their strides: any,
     but dense rows, each at a multiple of 16 bytes (a copy is made of others)."""
+    if x.dtype in _KDT and x.is_contiguous() and not x.data_ptr() & 15:
+        _, T, d = x.shape
+        return x, T * d, d
     if x.dtype not in _KDT:
         x = x.float()
     size = 4 if x.dtype == _F32 else 2
@@ -48,6 +51,9 @@ def _rows(x):
 def _heads(q):
     """Queries [BH, G, T, d] of a float type, with the strides of rows, heads and tokens: any, but dense channels, each
     at a multiple of 16 bytes (a copy is made of others)."""
+    if q.dtype in _KDT and q.is_contiguous() and not q.data_ptr() & 15:
+        _, G, T, d = q.shape
+        return q, G * T * d, T * d, d
     if q.dtype not in _KDT:
         q = q.float()
     size = 4 if q.dtype == _F32 else 2
@@ -67,23 +73,23 @@ class RowStore8:
     keeps nothing else, and methods write into them."""
 
     def __init__(self, k8, v8, k_scale, v_scale):
-        shape, dev = k8.shape, k8.device
-        if dev.type != "cuda":
+        shape, dev, gpu = k8.shape, k8.device, k8.get_device()
+        if gpu < 0:
             _need_gpu(k8)
         if len(shape) != 3 or k8.dtype not in _CODES or shape[2] not in (64, 128):
             raise ValueError(f"codes must be float8_e4m3fn or int8 [BH, cap, 64 or 128], got {k8.dtype} {tuple(shape)}")
         self.BH, self.cap, self.d = shape
         if v8.shape != shape or v8.dtype != k8.dtype:
             raise ValueError(f"v8 {v8.dtype} {tuple(v8.shape)} must be like k8 {k8.dtype} {tuple(shape)}")
-        scales = (self.BH, -(-self.cap // BLK))
+        scales = (shape[0], -(-shape[1] // BLK))
         if k_scale.shape != scales or v_scale.shape != scales or k_scale.dtype != _F32 or v_scale.dtype != _F32:
             raise ValueError(f"scales must be float32 {list(scales)}, got {k_scale.dtype} {tuple(k_scale.shape)} and "
                              f"{v_scale.dtype} {tuple(v_scale.shape)}")
-        if not (v8.device == k_scale.device == v_scale.device == dev and k8.is_contiguous() and v8.is_contiguous()
+        if not (v8.get_device() == k_scale.get_device() == v_scale.get_device() == gpu and k8.is_contiguous() and v8.is_contiguous()
                 and k_scale.is_contiguous() and v_scale.is_contiguous()):
             raise ValueError("the store's tensors must be contiguous and on one device")
         self.k8, self.v8, self.k_scale, self.v_scale = k8, v8, k_scale, v_scale
-        self.device, self._gpu = dev, dev.index
+        self.device, self._gpu = dev, gpu
         self._code = _CODES[k8.dtype]
 
     @classmethod
@@ -99,7 +105,7 @@ class RowStore8:
     # library as plain ints and are checked without building objects.
     def _call(self, name, *args):
         """The entry point on the store's device and its current stream."""
-        dev = self.device.index
+        dev = self._gpu
         fn = getattr(_lib.lib(), name)
         if _current_device() == dev:
             rc = fn(*args, _raw_stream(dev))

@@ -460,6 +460,46 @@ def test_small_channels_of_float32_queries(code, D, power):
         _check_chunk(st.chunk_attention(q.to(DEV), n), q, o, code, [n, n], every=6)
 
 
+@pytest.mark.parametrize("seed", range(10))
+def test_chunks_are_single_tokens_at_many_shapes(seed):
+    """Rows from 1 to 600, 1 to 33 heads, chunks from one token on, windows, sinks, caps, biases, lengths of each row or of all: a
+    chunk's tokens against the single-token attention, another kernel.  Both are within the oracle's bound; here with A the largest
+    |q| |K| scale of any token, and |V| <= its largest for the weighted mean of it: (4 D + 64) 2 U A for the two chains of D products
+    (of three parts in float32) and what follows, the joins, the weights' bits and their ends, half a step of the output."""
+    rng = np.random.default_rng(1000 + seed)
+    gen = torch.Generator(device=DEV).manual_seed(seed)
+    pick = lambda *x: x[rng.integers(len(x))]  # noqa: E731
+    for _ in range(12):
+        D, code, dtype = pick(64, 128), pick("e4m3", "int8"), pick(torch.bfloat16, torch.float16, torch.float32)
+        BH, G, T = pick(1, 2, 3, 5, 17, 70, 260, 600), pick(1, 2, 3, 4, 7, 8, 12, 33), pick(1, 2, 4, 5, 8, 9, 31, 33, 64, 100, 257, 700)
+        T = max(1, min(T, 40000 // (BH * G)))
+        n = max(1, min(int(2 ** rng.uniform(0, 14)), 1000000 // BH))
+        cap = n + int(rng.integers(130))
+        window = pick(0, 0, 1, 63, 64, 65, 500)
+        kw = dict(window=window, sinks=pick(0, 1, 64, 100) if window else 0, softcap=pick(None, None, 30.0, 4.0))
+        slopes = torch.exp2(-8 * torch.rand(BH, G, device=DEV, generator=gen)) if rng.random() < 0.3 else None
+        case = (D, code, str(dtype), BH, G, T, n, cap, kw, slopes is not None)
+        st = RowStore8.empty(BH, cap, CODES[code], D, DEV)
+        K, V = torch.randn(2, BH, cap, D, device=DEV, generator=gen)
+        st.write(K, V)
+        lens = torch.full((BH,), n, dtype=torch.int32, device=DEV)
+        length = n
+        if rng.random() < 0.5:
+            length = lens = torch.from_numpy(rng.integers(0, n + 1, BH).astype(np.int32)).to(DEV)
+        q = torch.randn(BH, G, T, D, device=DEV, generator=gen).to(dtype)
+        got = st.chunk_attention(q, length, slopes=slopes, **kw).double()
+        K, V = st.read(0, cap, torch.float32)
+        big = float(V.abs().max())
+        A = float(torch.bmm(q.float().abs().view(BH, G * T, D), K.abs().transpose(1, 2).contiguous()).max()) * D ** -0.5
+        rel = 2 * (4 * D + 64) * R.U * A + 2 * (n / 8 + 64) * R.U + 2 * 2.0 ** -BITS[dtype] + 2.0 ** -20 + n * 2.0 ** -33
+        for i in {0, T // 2, T - 1}:
+            seen = lens - (T - 1 - i)
+            one = st.attention(q[:, :, i].contiguous(), seen.clamp(min=0), slopes=slopes, **kw).double()
+            one[seen <= 0] = 0
+            off = (got[:, :, i] - one).abs() - rel * big - one.abs().clamp(min=2.0 ** -14) * HALF[dtype]
+            assert float(off.max()) <= 0, (case, i)
+
+
 def test_calls_with_and_without_a_cap_in_turn():
     """The same shapes with and without a cap take other tiles, and workspaces of one size."""
     st, _ = _filled(6, 1700, 128, "e4m3", seed=96)

@@ -652,6 +652,11 @@ __global__ __launch_bounds__((RW == 8 ? 8 : 4) * kWave, (kWide<D, QT, EXTRA, RW>
     }
     if (edge) {
       asm volatile("");  // a branch, not selects in every block
+      if (!(fabsf(ks) < INFINITY)) {  // behind the masks a factor of NaN would reach tokens that a query does not see
+#pragma unroll
+        for (int x = 0; x < 2; ++x) s[x] *= f;
+        f = 1.0f;
+      }
       if constexpr (kDirect) clear_values(i);  // what all queries see makes NaN by itself
       const uint32_t seen = seen_of(at);
 #pragma unroll

@@ -606,3 +606,37 @@ def test_refusals():
                dict(length=5, prefix_length=torch.zeros(4, dtype=torch.int32, device=DEV))):
         with pytest.raises(ValueError):
             st.shared_attention(q3, prefix=pst, **kw)
+
+
+# ----------------------------------------------------------------------------- what only some of a wave's queries see
+# one wave's tiles, four waves' and eight waves' (BH, G, T, n): a block's edge lies inside a wave of each
+FORMS = [(2, 4, 8, 197), (1, 2, 3, 30018), (1, 4, 100, 310), (8, 8, 300, 1241)]
+
+
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("BH, G, T, n", FORMS)
+def test_a_scale_of_k_that_is_not_finite_reaches_only_queries_that_see_it(BH, G, T, n, dtype, value):
+    D = 128
+    q = _rand((BH * G, T, D), 4, dtype).view(BH, G, T, D).to(DEV)
+    st, o = _filled(BH, n, D, "e4m3", seed=34)
+    edge = (n - T // 2) // BLK * BLK  # queries before this place do not see the block that it begins
+    assert n - T < edge < n - 1
+    clean = st.k_scale[:, edge // BLK].clone()
+    st.k_scale[:, edge // BLK] = value
+    before = edge - (n - T)
+    got = st.chunk_attention(q, n)
+    if value != value:
+        assert got[:, :, before:].isnan().all()
+    _check_chunk(got[:, :, :before], q[:, :, :before], o, "e4m3", [edge] * BH, every=max(1, before // 4))
+    _check_chunk(got[:, :, before - 1:before], q[:, :, before - 1:before], o, "e4m3", [edge] * BH)
+    # queries whose window has passed the block before that place
+    st.k_scale[:, edge // BLK] = clean
+    st.k_scale[:, edge // BLK - 1] = value
+    behind = n - T // 2
+    window, first, last = behind - edge + 1, max(edge - BLK - (n - T), 0), behind - (n - T)
+    got = st.chunk_attention(q, n, window=window, sinks=3)
+    if value != value:
+        assert got[:, :, first:last].isnan().all()
+    _check_chunk(got[:, :, :first], q[:, :, :first], o, "e4m3", [n - T + first] * BH, window, 3, every=max(1, first // 4))
+    _check_chunk(got[:, :, last:], q[:, :, last:], o, "e4m3", [n] * BH, window, 3, every=max(1, (T - last) // 4))

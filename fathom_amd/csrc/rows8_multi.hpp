@@ -701,7 +701,10 @@ __global__ __launch_bounds__((RW == 8 ? 8 : 4) * kWave, (kWide<D, QT, EXTRA, RW>
 #pragma unroll
         for (int e = 0; e < 16; ++e) sum += __builtin_amdgcn_exp2f(fmaf(s[x][e], f, -base));
       l += small ? sum : 0.0f;
-      if (__all(none)) return;
+      if (__all(none)) {
+        if constexpr (kDirect) clear_values(i);  // no product will make a NaN count
+        return;
+      }
     }
     if (vs < 0.0f) {  // not written by this store's writer
       asm volatile("");

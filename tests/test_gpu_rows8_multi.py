@@ -640,3 +640,28 @@ def test_a_scale_of_k_that_is_not_finite_reaches_only_queries_that_see_it(BH, G,
         assert got[:, :, first:last].isnan().all()
     _check_chunk(got[:, :, :first], q[:, :, :first], o, "e4m3", [n - T + first] * BH, window, 3, every=max(1, first // 4))
     _check_chunk(got[:, :, last:], q[:, :, last:], o, "e4m3", [n] * BH, window, 3, every=max(1, (T - last) // 4))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("BH, G, T", [(1, 1, 1), (2, 4, 8), (1, 4, 40), (8, 8, 300)])
+def test_a_block_of_nan_values_makes_nan(BH, G, T, dtype):
+    """V that is NaN throughout a block, or NaN among zeros, has the smallest scale there is: NaN all the same for the queries that
+    see it, wherever the block lies, as for single tokens."""
+    D, n = 128, 990 + T
+    q = _rand((BH * G, T, D), 4, dtype).view(BH, G, T, D).to(DEV)
+    K, V = _rand((BH, n, D), 1), _rand((BH, n, D), 2)
+    for zeros in (False, True):
+        for block in (0, 5, 14):
+            bad = V.clone()
+            bad[-1, block * BLK:(block + 1) * BLK] = 0.0 if zeros else float("nan")
+            bad[-1, block * BLK + 7, 33] = float("nan")
+            st = RowStore8.empty(BH, n, torch.float8_e4m3fn, D, DEV)
+            st.write(K.to(DEV), bad.to(DEV))
+            nan = torch.zeros(BH, G, T, D, dtype=torch.bool)
+            nan[-1, :, :, slice(33, 34) if zeros else slice(None)] = True
+            assert torch.equal(st.chunk_attention(q, n).isnan().cpu(), nan)
+            last = q[:, :, -1].contiguous()
+            assert torch.equal(st.attention(last, n).isnan().cpu(), nan[:, :, -1])
+            own = RowStore8.empty(BH * T, 1, torch.float8_e4m3fn, D, DEV)
+            got = own.shared_attention(q.permute(2, 0, 1, 3).reshape(BH * T, G, D), 0, st, n)
+            assert torch.equal(got.isnan().cpu().view(T, BH, G, D), nan.permute(2, 0, 1, 3))

@@ -90,6 +90,9 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 // The largest weight times scale is held between 2^10 and 2^15, so f16 (to 2^-24) ends at 2^-34 of it.
 constexpr uint32_t kLeastBlocks = 4;  // of a workgroup's share
 constexpr float kMost = 15.0f, kStart = 12.0f;
+// Bases from which 11-bit weights take scores relative to them first: below, V's factor joins the base in the exponent, where it is
+// rounded with it, by 2^-16 at most here.  (Bases of 2^17 would leave weights 2^-7 off, of 2^26 a factor of 8.)
+constexpr float kNear = 256.0f;
 constexpr float kLeastWeight = -112.0f;  // a block counts with that weight at least in the choice of its values' scale: it stays finite
 
 __device__ __forceinline__ float power(float e) { return ldexpf(1.0f, (int)__builtin_amdgcn_fmed3f(e, -300.0f, 300.0f)); }
@@ -688,20 +691,32 @@ __global__ __launch_bounds__((RW == 8 ? 8 : 4) * kWave, (kWide<D, QT, EXTRA, RW>
       for (int d = 0; d < kTiles; ++d) o[d] *= by;
       base = to;
     }
-    // ---- weights and products, 16 tokens at a time.  The factor of V goes into the exponent, and out of the sum again.
-    // A block's weights are added together first: alone, most would be lost beside a large sum.
+    // ---- weights and products, 16 tokens at a time.  A block's weights are added together first: alone, most would be lost
+    // beside a large sum.  The factor wv of V multiplies weights of 22 bits; for those of 11 it goes into the exponent, and out of
+    // the sum again.
     const float wv = ldexpf(fabsf(vs), -(int)E);
-    // Where it is so small that weights which count in the sum would be lost in the products' operands, they are added apart;
-    // below 2^-64 all of those are 0: the block has no value to add.
-    const bool small = !(wv >= (PREC ? 0x1p-64f : 0x1p-6f)), none = !(wv >= 0x1p-64f);
+    float off = base;
+    if (!PREC && __any(fabsf(base) >= kNear)) {
+      asm volatile("");  // a branch, not selects in every block
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[x][e] = fmaf(s[x][e], f, -base);
+      f = 1.0f;
+      off = 0.0f;
+    }
+    // Where that factor is so small that weights which count in the sum would be lost in the products' operands, 11-bit ones
+    // are added apart; below 2^-64 all of those are 0: the block has no value to add.
+    const bool none = !(wv >= 0x1p-64f), small = PREC ? none : !(wv >= 0x1p-6f);
     if (__builtin_expect(__any(small), 0)) {
+      const bool all = __all(none);
       float sum = 0.0f;
 #pragma unroll
       for (int x = 0; x < 2; ++x)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) sum += __builtin_amdgcn_exp2f(fmaf(s[x][e], f, -base));
-      l += small ? sum : 0.0f;
-      if (__all(none)) {
+        for (int e = 0; e < 16; ++e) sum += __builtin_amdgcn_exp2f(fmaf(s[x][e], f, -off));
+      l += small && (!PREC || all) ? sum : 0.0f;
+      if (all) {
         if constexpr (kDirect) clear_values(i);  // no product will make a NaN count
         return;
       }
@@ -711,7 +726,8 @@ __global__ __launch_bounds__((RW == 8 ? 8 : 4) * kWave, (kWide<D, QT, EXTRA, RW>
 #pragma unroll
       for (int d = 0; d < kTiles; ++d) o[d] = -o[d];
     }
-    const float zero = none ? INFINITY : base - __builtin_amdgcn_logf(wv), back_by = small ? 0.0f : __builtin_amdgcn_rcpf(wv);
+    const float zero = PREC ? off : none ? INFINITY : off - __builtin_amdgcn_logf(wv);
+    const float back_by = PREC ? 1.0f : small ? 0.0f : __builtin_amdgcn_rcpf(wv);
     float sum = 0.0f;
 #pragma unroll
     for (int n = 0; n < 4; ++n) {
@@ -721,12 +737,15 @@ __global__ __launch_bounds__((RW == 8 ? 8 : 4) * kWave, (kWide<D, QT, EXTRA, RW>
       float w[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) w[e] = __builtin_amdgcn_exp2f(fmaf(s[n / 2][8 * (n % 2) + e], f, -zero));
+      if constexpr (PREC) {
+        sum += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e] *= wv;
+      }
       f16x2 hi[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) hi[e] = round16(w[2 * e], w[2 * e + 1]);
-      if constexpr (PREC) {
-        sum += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
-      } else {  // the weights as they are held, so that they divide out
+      if constexpr (!PREC) {  // the weights as they are held, so that they divide out
 #pragma unroll
         for (int e = 0; e < 4; ++e) sum = __builtin_amdgcn_fdot2(hi[e], f16x2{(_Float16)1.0f, (_Float16)1.0f}, sum, false);
       }

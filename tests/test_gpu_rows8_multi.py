@@ -665,3 +665,41 @@ def test_a_block_of_nan_values_makes_nan(BH, G, T, dtype):
             own = RowStore8.empty(BH * T, 1, torch.float8_e4m3fn, D, DEV)
             got = own.shared_attention(q.permute(2, 0, 1, 3).reshape(BH * T, G, D), 0, st, n)
             assert torch.equal(got.isnan().cpu().view(T, BH, G, D), nan.permute(2, 0, 1, 3))
+
+
+# ----------------------------------------------------------------------------- scores far from zero
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("BH, G, T", [(1, 2, 5), (2, 4, 40), (8, 8, 300)])
+@pytest.mark.parametrize("power", [7, 10, 14, 17, 20, 24, 26, 30])
+def test_equal_scores_weigh_the_same_in_blocks_of_other_scales(dtype, BH, G, T, power):
+    """Tokens of one score, 2^power, in blocks whose scales of V differ, above all others': the mean of their values.
+
+    Their weights are one number, each held with an error e of 2^-bits at most (half a step of what it is held in) and divided by a sum
+    of those: 2 e of the mean |v|.  A factor of V that goes into the exponent of an 11-bit weight adds half a step of that exponent,
+    below 512: ln 2 2^-16, and steps of log2 and exp2 and of the products: together below 2^-15, for 22 bits 2^-21.  (At 2^7 the
+    others' weights are below e^-128 of it, which is nothing.)"""
+    D, n = 128, 64 * 18 + T
+    rng = np.random.default_rng(power)
+    o = {"k8": np.zeros((BH, n, D), np.uint8), "v8": rng.integers(1, 0x78, (BH, n, D), dtype=np.uint8)}
+    o["ks"] = np.full((BH, -(-n // BLK)), 2.0 ** (power - 10), np.float32)
+    o["vs"] = np.exp2(rng.uniform(-4, 4, o["ks"].shape)).astype(np.float32)
+    top = [np.sort(rng.choice(64 * 18, 7, replace=False)) for _ in range(BH)]
+    for b in range(BH):
+        o["k8"][b, top[b], 0] = R.encode(np.array([64.0]), "e4m3")[0]
+    st = _from_numpy(o, "e4m3")
+    q = torch.zeros(BH, G, T, D, dtype=dtype)
+    q[..., 0] = 16.0
+    V = _values(o, "e4m3")[1]
+
+    def check(got, bits, half):
+        for b in range(BH):
+            v = V[b, top[b]]
+            tol = 2 * (2.0 ** -bits + (2.0 ** -15 if bits == 11 else 2.0 ** -21)) * np.abs(v).mean(0)
+            off = np.abs(got[b].double().cpu().numpy() - v.mean(0)) - tol - half * (np.abs(v.mean(0)) + tol)
+            assert (off <= 0).all(), f"row {b}: {off.max():.3g} over {tol.max():.3g}"
+
+    check(st.chunk_attention(q.to(DEV), n, scale=1.0), BITS[dtype], HALF[dtype])
+    own, _ = _filled(BH * T, 5, D, "e4m3")  # its scores are far smaller
+    own.k_scale.mul_(2.0 ** -20)
+    got = own.shared_attention(q.permute(2, 0, 1, 3).reshape(BH * T, G, D).to(DEV), 5, st, n, scale=1.0)
+    check(got.view(T, BH, G, D).permute(1, 2, 0, 3), 22, 0.0)

@@ -851,6 +851,10 @@ __global__ __launch_bounds__((RW == 8 ? 8 : 4) * kWave, (kWide<D, QT, EXTRA, RW>
   }
 
   l += other_half(l);
+  // What leaves the wave is relative to base + kStart, so that it stays finite: to the step that this sum takes, which is another
+  // one from 2^26 on.
+  const float top = base + kStart;
+  const int down = (int)(top - base);
   const bool parts = a.parts;
   const int64_t slot = parts ? ((int64_t)blockIdx.x * kRows) : 0;
   if constexpr (kDirect) {  // ---- the waves' sums over their blocks
@@ -861,12 +865,12 @@ __global__ __launch_bounds__((RW == 8 ? 8 : 4) * kWave, (kWide<D, QT, EXTRA, RW>
     for (int e = 0; e < 16; ++e) {  // register e of o[d] is channel kTiles (8 (e / 4) + 4 half + e % 4) + d
       piece v;
 #pragma unroll
-      for (int d = 0; d < kTiles; ++d) v[d] = ldexpf(o[d][e], (int)(E - kStart));
+      for (int d = 0; d < kTiles; ++d) v[d] = ldexpf(o[d][e], (int)E - down);
       *reinterpret_cast<piece *>(mine_at + kTiles * (8 * (e / 4) + 4 * half + e % 4)) = v;
     }
     if (half == 0) {
-      wm[wave][col] = base + kStart;
-      wl[wave][col] = ldexpf(l, -(int)kStart);
+      wm[wave][col] = top;
+      wl[wave][col] = ldexpf(l, -down);
     }
     __syncthreads();
 #pragma unroll
@@ -901,7 +905,7 @@ __global__ __launch_bounds__((RW == 8 ? 8 : 4) * kWave, (kWide<D, QT, EXTRA, RW>
   }
   if (mine >= M) return;
   const int row = 32 * wave + col;
-  if (parts && half == 0) a.ml[slot + row] = make_float2(base + kStart, ldexpf(l, -(int)kStart));
+  if (parts && half == 0) a.ml[slot + row] = make_float2(top, ldexpf(l, -down));
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   const int64_t out_at = ((r * a.G + g) * a.O + o_at) * D + 4 * half;
 #pragma unroll
@@ -912,7 +916,7 @@ __global__ __launch_bounds__((RW == 8 ? 8 : 4) * kWave, (kWide<D, QT, EXTRA, RW>
       float v[4];
       if (parts) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] = ldexpf(o[d][e + k], (int)(E - kStart));
+        for (int k = 0; k < 4; ++k) v[k] = ldexpf(o[d][e + k], (int)E - down);
         *reinterpret_cast<float4 *>(a.part + (slot + row) * D + c + 4 * half) = make_float4(v[0], v[1], v[2], v[3]);
       } else {
 #pragma unroll

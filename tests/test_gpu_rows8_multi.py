@@ -703,3 +703,37 @@ def test_equal_scores_weigh_the_same_in_blocks_of_other_scales(dtype, BH, G, T, 
     own.k_scale.mul_(2.0 ** -20)
     got = own.shared_attention(q.permute(2, 0, 1, 3).reshape(BH * T, G, D).to(DEV), 5, st, n, scale=1.0)
     check(got.view(T, BH, G, D).permute(1, 2, 0, 3), 22, 0.0)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("BH, G, T", [(1, 2, 5), (1, 4, 40), (8, 8, 300)])
+def test_shares_of_scores_on_both_sides_of_a_power_of_two(dtype, BH, G, T):
+    """Scores of 2^26 - 8 in most blocks and of 2^26 + 16 in one (in units of log 2, as float32 has them): steps of 4 and of 8, where the
+    waves' and shares' maxima are apart by what is no multiple of the steps.  What the lower ones weigh together, 2^-24 each, is seen
+    in a channel of their own."""
+    D, n = 128, 64 * 20 + T
+    L = np.float32(1.44269504088896340736)
+    s = 4 * np.arange((1 << 26) // 6, (1 << 26) // 5, dtype=np.int64)
+    r = s.astype(np.float32) * L
+    low, high = (int(s[np.flatnonzero(r == np.float32(2.0 ** 26 + x))[0]]) for x in (-8, 16))
+    o = {"k8": np.zeros((BH, n, D), np.uint8), "v8": np.zeros((BH, n, D), np.uint8)}
+    o["ks"] = np.full((BH, -(-n // BLK)), 2.0 ** 10, np.float32)
+    o["vs"] = np.ones_like(o["ks"])
+    one = R.encode(np.array([1.0]), "e4m3")[0]
+    bits = lambda x: np.array([one if x >> j & 1 else 0 for j in range(2, 26)], np.uint8)  # noqa: E731
+    o["k8"][:, :, :24] = bits(low)
+    o["v8"][:, :, 3] = one
+    at = 64 * 7 + 9
+    o["k8"][:, at, :24] = bits(high)
+    o["v8"][:, at] = 0
+    o["v8"][:, at, 5] = one
+    st = _from_numpy(o, "e4m3")
+    q = torch.zeros(BH, G, T, D)
+    q[..., :24] = torch.exp2(torch.arange(2.0, 26.0) - 10)
+    q = q.to(dtype)
+    got = st.chunk_attention(q.to(DEV), n, scale=1.0).double().cpu()
+    low_ones = (n - T + torch.arange(T, dtype=torch.float64)) * 2.0 ** -24  # of the tokens up to the query's all but one
+    # the weights are powers of two; sums of n of them round 2^-24 each at most, the result half a step of its type
+    for ref, channel in ((low_ones / (1 + low_ones), 3), (1 / (1 + low_ones), 5)):
+        off = (got[..., channel] - ref).abs()
+        assert (off <= ref * (n * R.U) + torch.maximum(ref * HALF[dtype], torch.tensor(FLOOR[dtype], dtype=torch.float64))).all()

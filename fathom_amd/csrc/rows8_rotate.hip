@@ -132,7 +132,7 @@ __device__ __forceinline__ uint64_t turns_of(float inv) {
 // itself: its upper word is exact to 2^-31 of a turn whatever t.  In quarter turns n + f, |f| <= 1/2, x = f pi / 2: sin x = x + x^3
 // P(x^2), cos x = 1 - x^2 / 2 + x^4 Q(x^2), P and Q least-squares fits of degree 2 on |x| <= pi / 4, off by less than a step of
 // float32 each.  (Angles in float64, half as fast: 8 x 32768 tokens of 4 heads 176 us; 163.)
-__device__ __forceinline__ void turn_of(const uint64_t (&turns)[8], Pairs c, int64_t t, float (&cs)[8], float (&sn)[8]) {
+__device__ __forceinline__ void turn_of(const uint64_t (&turns)[8], int64_t t, float (&cs)[8], float (&sn)[8]) {
   const uint32_t lo = (uint32_t)t, hi = (uint32_t)((uint64_t)t >> 32);
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
@@ -148,10 +148,6 @@ __device__ __forceinline__ void turn_of(const uint64_t (&turns)[8], Pairs c, int
     k = fmaf(fmaf(k, w, -0.5f), w, 1.0f);
     sn[i] = __uint_as_float(__float_as_uint(n & 1 ? k : s) ^ (n & 2) << 30);
     cs[i] = __uint_as_float(__float_as_uint(n & 1 ? s : k) ^ ((n + 1) & 2) << 30);
-    if (!c.turned) {
-      sn[i] = 0.0f;
-      cs[i] = 1.0f;
-    }
   }
 }
 
@@ -166,12 +162,13 @@ __device__ __forceinline__ void norm(float (&x)[16], const float (&w)[16], float
 #pragma unroll
   for (int i = 0; i < 16; ++i) x[i] = x[i] * by * w[i];
 }
-__device__ __forceinline__ void turn(float (&x)[16], const float (&cs)[8], const float (&sn)[8]) {
+// Channels that stay are not turned by 0, which would make NaN of a finite one beside an infinite one.
+__device__ __forceinline__ void turn(float (&x)[16], Pairs c, const float (&cs)[8], const float (&sn)[8]) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const float a = x[i], b = x[8 + i];
-    x[i] = a * cs[i] - b * sn[i];
-    x[8 + i] = b * cs[i] + a * sn[i];
+    x[i] = c.turned ? a * cs[i] - b * sn[i] : a;
+    x[8 + i] = c.turned ? b * cs[i] + a * sn[i] : b;
   }
 }
 
@@ -209,14 +206,14 @@ __global__ __launch_bounds__(kThreads) void rotate_kernel(RotateArgs a) {
     Raw<DT> next{};
     if (g < end) next = load_pairs<DT>(a.q, at + g * a.q_head, c);
     float cs[8], sn[8];
-    turn_of(turns, c, p + i + shift, cs, sn);
+    turn_of(turns, p + i + shift, cs, sn);
     for (; g < end; g += step) {  // the next head is requested first
       const Raw<DT> now = next;
       if (g + step < end) next = load_pairs<DT>(a.q, at + (g + step) * a.q_head, c);
       float x[16];
       unpack_pairs<DT>(now, x);
       if (a.weight[0]) norm<D>(x, w, a.eps);
-      turn(x, cs, sn);
+      turn(x, c, cs, sn);
       store_pairs<DT>(a.q_out, ((bh * a.G + g) * a.T + i) * D, c, x);
     }
     return;
@@ -246,8 +243,8 @@ __global__ __launch_bounds__(kThreads) void rotate_kernel(RotateArgs a) {
     if (!kv) {
       if (a.weight[1]) norm<D>(x[i], w, a.eps);
       float cs[8], sn[8];
-      turn_of(turns, c, p + j + shift, cs, sn);
-      turn(x[i], cs, sn);
+      turn_of(turns, p + j + shift, cs, sn);
+      turn(x[i], c, cs, sn);
       if (a.k_out && j >= 0 && j < a.T) store_pairs<DT>(a.k_out, (bh * a.T + j) * D, c, x[i]);
     }
     if (j >= 0 && j < a.T) {

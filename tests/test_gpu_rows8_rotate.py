@@ -147,6 +147,26 @@ def test_values_that_are_not_finite():
     assert not out.any() and not st.k8.view(torch.uint8)[0].any()
 
 
+@pytest.mark.parametrize("code", ["e4m3", "int8"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("turn", [0.0, 0.25, 0.5])
+def test_channels_that_do_not_turn_keep_their_own_values(code, dtype, D, turn):
+    """Infinite and NaN channels behind r, or without a rotation, leave every other channel as it is, in the results and in the codes."""
+    BH, G, T, r = 2, 3, 70, int(D * turn)
+    q, K, V = _inputs(BH, G, T, D, dtype, seed=12)
+    for x in (q[0, 1], q[1, 2], K[0], K[1]):
+        x[3, r], x[4, r + 5], x[65, D - 1], x[66, D - 9], x[10, D // 2 + r // 2 + 1] = (float(v) for v in ("inf", "nan", "-inf", "nan", "inf"))
+    st, o = _empty(BH, 100, D, code)
+    out, keys = st.write_rotated(q.to(DEV), K.to(DEV), V.to(DEV), _inv(r).to(DEV) if r else None, 11, keys=True)
+    for got, x in ((out, q), (keys, K)):
+        torch.testing.assert_close(got[..., r:].cpu(), x[..., r:], rtol=0, atol=0, equal_nan=True)
+        assert got[..., :r].isfinite().all()
+    if dtype == torch.float32 or not r:  # the codes are made from these very keys
+        R.write(o, _f32(keys.cpu()), _f32(V), 11, code)
+        _same(st, o, code)
+
+
 def test_layouts_and_weights_of_other_types():
     """Views of a fused projection, and whatever has to be copied first, give the bits of dense tensors."""
     BH, G, T, D = 1, 4, 50, 64

@@ -388,7 +388,7 @@ class RowStore8:
         if not isinstance(prefix, RowStore8) or prefix.device != self.device:
             raise ValueError(f"the prefix must be a RowStore8 on {self.device}")
         H = prefix.BH
-        if prefix.d != self.d or prefix._code != self._code or self.BH % H:
+        if not H or prefix.d != self.d or prefix._code != self._code or self.BH % H:
             raise ValueError(f"a prefix of {H} rows of {prefix.d} {prefix.k8.dtype} codes does not fit {self.BH} rows of "
                              f"{self.d} {self.k8.dtype}")
         q, q_at, scale, softcap, slopes = self._query(q, scale, softcap, slopes)

@@ -737,3 +737,10 @@ def test_shares_of_scores_on_both_sides_of_a_power_of_two(dtype, BH, G, T):
     for ref, channel in ((low_ones / (1 + low_ones), 3), (1 / (1 + low_ones), 5)):
         off = (got[..., channel] - ref).abs()
         assert (off <= ref * (n * R.U) + torch.maximum(ref * HALF[dtype], torch.tensor(FLOOR[dtype], dtype=torch.float64))).all()
+
+
+def test_a_prefix_without_rows_is_refused():
+    st, _ = _filled(4, 100, 128, "e4m3")
+    none = RowStore8.empty(0, 100, torch.float8_e4m3fn, 128, DEV)
+    with pytest.raises(ValueError):
+        st.shared_attention(torch.zeros(4, 2, 128, device=DEV), 100, none, 100)

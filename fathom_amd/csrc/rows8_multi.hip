@@ -234,6 +234,11 @@ bool queries_taken(int64_t BH, int64_t G, int64_t O) {
   return O >= 1 && O <= kMaxCap && G <= kMaxTiles * 32 / O && BH * G * O <= (int64_t)1 << 27;
 }
 
+// The kernel keeps its factors, scale log2 e among them, in float32's range, and would make finite ones of other scales.
+int check_scale(const char *what, float scale) {
+  return fabsf(scale) <= 0x1p127f ? FATHOM_OK : fail(FATHOM_ERR_INVALID, "%s: the scale must be finite, of at most 2^127", what);
+}
+
 void place(MultiArgs &a, void *workspace, int64_t D) {
   const int64_t rows = (a.shares + a.BH * a.tiles) * a.rows;
   a.part = static_cast<float *>(workspace);
@@ -287,6 +292,8 @@ extern "C" int fathom_rows8_chunk_attention(const void *q, int q_dtype, int64_t 
   if (T < 0) return fail(FATHOM_ERR_INVALID, "%s: T=%lld", what, (long long)T);
   if (T == 0) return FATHOM_OK;
   rc = check_query(what, q, q_dtype, G, cap, lens, n, softcap, out);
+  if (rc) return rc;
+  rc = check_scale(what, scale);
   if (rc) return rc;
   if (!queries_taken(BH, G, T)) return fail(FATHOM_ERR_INVALID, "%s: G=%lld T=%lld, at most %lld queries per row and 2^27 in all", what, (long long)G, (long long)T, (long long)kMaxTiles * 32);
   if (window < 0) return fail(FATHOM_ERR_INVALID, "%s: window %lld", what, (long long)window);
@@ -350,6 +357,8 @@ extern "C" int fathom_rows8_shared_attention(const void *q, int q_dtype, const v
   const int64_t BH = prefix_BH * sequences;
   rc = check_store(what, k8, v8, k_scale, v_scale, code_dtype, BH, cap, D);
   if (!rc) rc = check_query(what, q, q_dtype, G, cap, lens, n, softcap, out);
+  if (rc) return rc;
+  rc = check_scale(what, scale);
   if (rc) return rc;
   if (!prefix_lens && (prefix_n < 0 || prefix_n > prefix_cap))
     return fail(FATHOM_ERR_INVALID, "%s: prefix length %lld outside [0, cap=%lld]", what, (long long)prefix_n, (long long)prefix_cap);

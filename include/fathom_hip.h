@@ -477,7 +477,7 @@ int fathom_rows8_gather_attention(const void *q, int q_dtype, const int64_t *idx
  * be off by 2^-25 without (to 2^-76 of it); scores and sums are float32.  With q_dtype
  * FATHOM_DT_F32 a weight has 22 bits, else 11, down to 2^-34 of the largest weight
  * times scale of V.
- * G * T <= 65535 * 32, BH * G * T <= 2^27.
+ * G * T <= 65535 * 32, BH * G * T <= 2^27, |scale| <= 2^127.
  * workspace: fathom_rows8_chunk_attention_workspace_bytes(BH, G, T, D, positions)
  * bytes, 16-byte aligned, positions = the longest length the host knows, or with a
  * window the smaller of that and window + T + sinks, sinks rounded up to a multiple
@@ -498,7 +498,7 @@ int fathom_rows8_chunk_attention(const void *q, int q_dtype, int64_t q_row_strid
  * first lens[s, h] (or n) tokens of its own, as if they followed each other in one
  * row.  The prefix is read once for all sequences.  q, out [sequences * prefix_BH,
  * G, D] contiguous, out float32; both stores have the same D and code_dtype;
- * sequences * G <= 65535 * 32, sequences * prefix_BH * G <= 2^27.
+ * sequences * G <= 65535 * 32, sequences * prefix_BH * G <= 2^27, |scale| <= 2^127.
  * Precision as fathom_rows8_chunk_attention's with a weight of 22 bits for the
  * prefix, fathom_rows8_attention's for the rest.
  * workspace: fathom_rows8_shared_attention_workspace_bytes(prefix_BH, sequences,

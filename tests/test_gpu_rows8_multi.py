@@ -744,3 +744,14 @@ def test_a_prefix_without_rows_is_refused():
     none = RowStore8.empty(0, 100, torch.float8_e4m3fn, 128, DEV)
     with pytest.raises(ValueError):
         st.shared_attention(torch.zeros(4, 2, 128, device=DEV), 100, none, 100)
+
+
+def test_scales_that_are_not_finite_are_refused():
+    st, _ = _filled(4, 100, 128, "e4m3")
+    pst, _ = _filled(2, 100, 128, "e4m3")
+    q = torch.zeros(4, 2, 8, 128, dtype=torch.bfloat16, device=DEV)
+    for scale in (float("nan"), float("inf"), -float("inf"), 3e38, 1e39):
+        with pytest.raises(ValueError):
+            st.chunk_attention(q, 100, scale=scale)
+        with pytest.raises(ValueError):
+            st.shared_attention(q[:, :, 0].contiguous(), 100, pst, 100, scale=scale)

@@ -174,3 +174,10 @@ def test_a_workspace_serves_every_kind_of_call(entry, BH, G, T):
             _refused(f"fathom_rows8_{entry}_attention", {**call, "wsb": need}, _lib.ERR_INVALID, b"aligned")
             refused += getattr(L, f"fathom_rows8_{entry}_attention")(*{**call, "wsb": need // 4}.values()) == _lib.ERR_WORKSPACE
     assert refused
+
+
+@pytest.mark.parametrize("entry", ["chunk", "shared"])
+@pytest.mark.parametrize("scale", [float("nan"), float("inf"), -float("inf"), 3e38])
+def test_scales_that_are_not_finite_are_refused(entry, scale):
+    args = _chunk(scale=scale) if entry == "chunk" else _shared(scale=scale)
+    _refused(f"fathom_rows8_{entry}_attention", args, _lib.ERR_INVALID, b"scale")

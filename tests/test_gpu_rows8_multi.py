@@ -755,3 +755,37 @@ def test_scales_that_are_not_finite_are_refused():
             st.chunk_attention(q, 100, scale=scale)
         with pytest.raises(ValueError):
             st.shared_attention(q[:, :, 0].contiguous(), 100, pst, 100, scale=scale)
+
+
+def test_biased_rows_behind_whole_blocks_of_a_prefix():
+    """With a bias and prefixes that end with a block, the joined row has the stores' blocks, so that the bound is the oracle's own."""
+    B, H, G, D = 5, 2, 3, 128
+    lens, plens = [40, 0, 7, 64, 100, 3, 0, 0, 99, 1], [128, 64]
+    for code in ("int8", "e4m3"):
+        pst, po = _filled(H, 192, D, code, seed=173)
+        st, o = _filled(B * H, 100, D, code, seed=174)
+        sl = 2.0 ** -torch.arange(1.0, B * H * G + 1).fmod(9).view(B * H, G)
+        for dtype in (torch.bfloat16, torch.float32):
+            q = _rand((B * H, G, D), 6, dtype)
+            for softcap, scale in ((20.0, None), (0.0, 0.2)):
+                got = st.shared_attention(q.to(DEV), torch.tensor(lens, device=DEV), pst, torch.tensor(plens, device=DEV), scale=scale,
+                                          softcap=softcap, slopes=sl.to(DEV))
+                _check_shared(got, q, o, po, code, lens, plens, scale, softcap, sl)
+
+
+def test_capped_plain_and_biased_calls_in_turn():
+    """The same shapes with a cap, without one and with a bias take kernels and tiles of their own: each call repeats its own bits with
+    the others in between, and a cap that no score feels changes a result by roundings alone."""
+    st, o = _filled(6, 1700, 128, "e4m3", seed=96)
+    q = _rand((48, 300, 128), 6, torch.bfloat16).view(6, 8, 300, 128)
+    lens = [1700, 1300, 900, 500, 310, 300]
+    on, length = q.to(DEV), torch.tensor(lens, dtype=torch.int32, device=DEV)
+    zeros = torch.zeros(8, device=DEV)
+    calls = [dict(), dict(softcap=1e4), dict(slopes=zeros), dict(softcap=5.0), dict(softcap=1e4, slopes=zeros)]
+    first = [st.chunk_attention(on, length, **kw) for kw in calls]
+    assert not torch.equal(first[0], first[3])
+    for kw, ref in zip(calls, first):
+        _check_chunk(ref, q, o, "e4m3", lens, softcap=kw.get("softcap", 0.0), slopes=torch.zeros(6, 8) if "slopes" in kw else None, every=97)
+    for _ in range(3):
+        for kw, ref in zip(calls, first):
+            assert torch.equal(st.chunk_attention(on, length, **kw), ref)

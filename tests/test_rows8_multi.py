@@ -181,3 +181,28 @@ def test_a_workspace_serves_every_kind_of_call(entry, BH, G, T):
 def test_scales_that_are_not_finite_are_refused(entry, scale):
     args = _chunk(scale=scale) if entry == "chunk" else _shared(scale=scale)
     _refused(f"fathom_rows8_{entry}_attention", args, _lib.ERR_INVALID, b"scale")
+
+
+@pytest.mark.parametrize("lens", [None, 1 << 29])
+def test_the_shared_workspace_holds_the_rows_own_part_too(lens):
+    """Sizes from what the prefix's part takes up to one byte less than both take are refused by the check of the rows' own part, before
+    any launch; what the query answers holds both.  (The least size that the prefix's part takes is found with an address that is 8
+    bytes off, which is refused behind that check.)"""
+    L = _lib.lib()
+    args = _shared(cap=100000, n=100000, lens=lens)
+
+    def status(wsb, ws=1 << 28):
+        return L.fathom_rows8_shared_attention(*{**args, "ws": ws, "wsb": wsb}.values())
+
+    need = L.fathom_rows8_shared_attention_workspace_bytes(2, 3, 4, 128, 10000, 100000)
+    low, high = 0, need  # refused for its size, and not
+    while high - low > 1:
+        mid = (low + high) // 2
+        low, high = (mid, high) if status(mid, (1 << 28) + 8) == _lib.ERR_WORKSPACE else (low, mid)
+    assert status(high) == _lib.ERR_WORKSPACE
+    message = L.fathom_last_error()
+    assert b"more than" not in message and b"workspace 0 bytes" in message
+    own = int(message.split()[-1])
+    assert own > 0 and need >= high + own
+    for wsb in (high + 1, high + own // 2, high + own - 1):
+        _refused("fathom_rows8_shared_attention", {**args, "wsb": wsb}, _lib.ERR_WORKSPACE, b"workspace %d bytes, need %d" % (wsb - high, own))

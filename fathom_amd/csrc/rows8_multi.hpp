@@ -238,7 +238,8 @@ constexpr bool kWide = RW == 1 && D == 128 && (EXTRA || QT == FATHOM_DT_F32);
 // queries: four, or eight (one workgroup per CU).  Where a row has no more than 32, RW is one: all four waves of a workgroup
 // have them all, and take blocks in turn.  Per 64-token block:
 //   the codes are requested a block ahead.  Several waves convert them once and keep them in LDS as 16-bit numbers (exact): K
-//     by tokens, V transposed, both with their 16-byte pieces in an order that keeps the lanes' reads on different banks.
+//     by tokens, V transposed, both with their 16-byte pieces in an order that spreads the lanes' reads over the banks (cycles lost
+//     to conflicts per LDS instruction: 0.84 in 8 x 4 x 2048 queries over 65536 tokens, 2.2 at D = 64 with a cap and a bias).
 //     A wave by itself takes its operands straight from the codes: the order of the channels inside K's contraction is
 //     free, and so is that of V's channels over the tiles of the result, lane c's being kTiles c ..
 //   S^T = K q^T (v_mfma_f32_32x32x16): lane l holds query l & 31 and 32 of the block's scores, so that maximum and sum

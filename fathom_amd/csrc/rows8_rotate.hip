@@ -177,9 +177,10 @@ __device__ __forceinline__ void turn(float (&x)[16], Pairs c, const float (&cs)[
 // largest value and its codes.  A workgroup's query tokens are as many as there are, up to its rows, and its heads the rest, so that
 // a token's angles are formed once for up to four heads (fewer where the call would not fill the device).
 //
-// Bound: HBM.  8 x 32768 tokens of 4 heads in bf16, D = 128, keys returned (0.81 GB in and out) 163 us, 4.9 TB/s, what a copy
-// reaches (4.97); norms and angles by themselves take less.  16 x 1777 of 7 heads, D = 64 (77 MB, much of it from L2) 19 us.
-// One token of 32 rows 8 us: the launch, the weights and frequencies on their way, then the row.
+// Bound: HBM.  8 x 32768 tokens of 4 heads in bf16, D = 128, keys returned (0.81 GB in and out) 163 us at the least of 20 under
+// a trace, 4.9 TB/s, what a copy reaches (4.97), 175 in the median; norms and angles by themselves take less.  16 x 1777 of 7
+// heads, D = 64 (77 MB, much of it from L2) 19 us.  One token of 32 rows 8 us: the launch, the frequencies on their way to LDS and
+// the barrier, then the weights and the row.
 template <int D, int DT, bool I8>
 __global__ __launch_bounds__(kThreads) void rotate_kernel(RotateArgs a) {
   typedef Lane<D> L;

@@ -222,7 +222,8 @@ class RowStore8:
         r <= d a multiple of 16; None: no rotation) channels c and c + r / 2 become (x_c cos - x_{c+r/2} sin,
         x_{c+r/2} cos + x_c sin) of the angle t inv_freq[c], whose whole turns are dropped exactly at any t; channels
         behind r stay.  offset is an int or integers [BH]: what stands before the store's first token, as a shared prefix
-        does.  Views as in `write`; with a tensor `pos`, rows whose tokens do not all fit are rotated but not written."""
+        does, of 32 bits (of a tensor's others the nearest).  Types other than float32, float16 and bfloat16 are taken, and given
+        back, as float32.  Views as in `write`; with a tensor `pos`, rows whose tokens do not all fit are rotated but not written."""
         gpu, BH, d = self._gpu, self.BH, self.d
         for t in (q, K, V):
             if t.get_device() != gpu:
@@ -359,8 +360,9 @@ class RowStore8:
         over the tokens up to its own: a prompt, a piece of one, or drafted tokens, once `write` or `write_rotated` has
         their keys and values.  Token i of a row of `length` tokens stands at place p = length - T + i and sees tokens
         t <= p, with a window only the last `window` of them and the first `sinks`.  Scores as in `attention`, with the
-        bias slopes[bh, g] (t - p).  [BH, G, T, d] in q's type; a token before the row's first (p < 0) gives zeros, so
-        rows of fewer than T tokens are padded in front."""
+        bias slopes[bh, g] (t - p); the scale is at most 2^127 in size, here and in `shared_attention`.  [BH, G, T, d] in
+        q's type (float32 for types other than those three); a token before the row's first (p < 0) gives zeros, so rows of
+        fewer than T tokens are padded in front."""
         if q.get_device() != self._gpu:
             self._elsewhere(q)
         shape = q.shape
@@ -384,7 +386,8 @@ class RowStore8:
         """`attention` for a batch whose sequences begin with the same tokens: `prefix`, a RowStore8 of H rows, holds
         them once, this store's rows [B, H] hold what follows (`length` tokens, ints or integers [B H]).  Row (b, h) attends to
         the first prefix_length (int, or integers [H]) tokens of the prefix's row h and then its own, in one
-        softmax; the prefix is read once for all B.  q [B H, G, d]; [B H, G, d] float32."""
+        softmax; the prefix is read once for all B.  One token a row: several behind a prefix need it in their own rows.
+        q [B H, G, d]; [B H, G, d] float32."""
         if not isinstance(prefix, RowStore8) or prefix.device != self.device:
             raise ValueError(f"the prefix must be a RowStore8 on {self.device}")
         H = prefix.BH

@@ -392,7 +392,8 @@ int fathom_rows8_write(const void *K, const void *V, int dtype, int64_t k_row_st
  * channels c and c + rotated / 2, c < rotated / 2, are turned by the angle t *
  * inv_freq[c] (inv_freq [rotated / 2] float32, finite and below 2^50 in size;
  * rotated a multiple of 16, 0: no rotation), whose whole turns are dropped exactly
- * at any t: (x_c cos - x_{c + rotated/2} sin, x_{c + rotated/2} cos + x_c sin).  q_out [BH, G, T, D] and, unless NULL, k_out
+ * at any t: (x_c cos - x_{c + rotated/2} sin, x_{c + rotated/2} cos + x_c sin);
+ * the others keep their values.  q_out [BH, G, T, D] and, unless NULL, k_out
  * [BH, T, D] of dtype take the results; K's codes are made from the float32 values.
  * Rows of `pos` that do not fit are rotated but not written.  T <= 2^27.
  */
@@ -470,7 +471,7 @@ int fathom_rows8_gather_attention(const void *q, int q_dtype, const int64_t *idx
  * above, query (bh, g, i) (at bh * q_row_stride + g * q_head_stride + i *
  * q_tok_stride elements; base and strides multiples of 16 bytes) stands at place
  * p = len - T + i of its row and sees tokens t <= p, with a window only those t >
- * p - window and t < sinks.  Scores, cap, bias (slopes[bh, g] * (t - p)) as
+ * p - window or t < sinks.  Scores, cap, bias (slopes[bh, g] * (t - p)) as
  * above; a query that sees nothing (p < 0) gives zeros.  out [BH, G, T, D] of
  * q_dtype (16-byte aligned).  bf16 and f16 queries take part exactly, float32 ones
  * with 22 bits, channels below 2^-18 of their head's largest too where a score could
@@ -479,9 +480,9 @@ int fathom_rows8_gather_attention(const void *q, int q_dtype, const int64_t *idx
  * times scale of V.
  * G * T <= 65535 * 32, BH * G * T <= 2^27, |scale| <= 2^127.
  * workspace: fathom_rows8_chunk_attention_workspace_bytes(BH, G, T, D, positions)
- * bytes, 16-byte aligned, positions = the longest length the host knows, or with a
- * window the smaller of that and window + T + sinks, sinks rounded up to a multiple
- * of 64.  The query never falls as positions grow.
+ * bytes, 16-byte aligned, positions = the longest length the host knows (cap, where
+ * lens is given), or with a window the smaller of that and window + T + sinks, sinks
+ * rounded up to a multiple of 64.  The query never falls as positions grow.
  */
 size_t fathom_rows8_chunk_attention_workspace_bytes(int64_t BH, int64_t G, int64_t T, int64_t D, int64_t positions);
 int fathom_rows8_chunk_attention(const void *q, int q_dtype, int64_t q_row_stride, int64_t q_head_stride,
@@ -503,7 +504,8 @@ int fathom_rows8_chunk_attention(const void *q, int q_dtype, int64_t q_row_strid
  * prefix, fathom_rows8_attention's for the rest.
  * workspace: fathom_rows8_shared_attention_workspace_bytes(prefix_BH, sequences,
  * G, D, prefix_positions, positions) bytes, 16-byte aligned, of the longest
- * lengths that the host knows.  The query falls with neither.
+ * lengths that the host knows (the caps, where lengths are on the device).  The
+ * query falls with neither.
  */
 size_t fathom_rows8_shared_attention_workspace_bytes(int64_t prefix_BH, int64_t sequences, int64_t G, int64_t D,
                                                      int64_t prefix_positions, int64_t positions);

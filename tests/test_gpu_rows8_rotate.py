@@ -256,3 +256,14 @@ def test_a_batch_from_prompt_to_tokens():
                 for g in range(G):
                     ref, tol = R.attention(rot[r, g].double().cpu().numpy(), k[r], v[r], R.sees(i, i + 1, 8, 2), i + 1, D ** -0.5)
                     assert (np.abs(outs[2][r, g].double().cpu().numpy() - ref) <= tol).all()
+
+
+def test_offsets_beyond_32_bits():
+    """An int is refused, a tensor's values count as the nearest of 32 bits."""
+    q, K, V = (x.to(DEV) for x in _inputs(2, 2, 5, 64, torch.float32))
+    inv = _inv(64).to(DEV)
+    st = RowStore8.empty(2, 200, torch.int8, 64, DEV)
+    with pytest.raises(ValueError):
+        st.write_rotated(q, K, V, inv, 0, 1 << 31)
+    far, near = torch.tensor([1 << 40, -(1 << 40)], device=DEV), torch.tensor([(1 << 31) - 1, -(1 << 31)], device=DEV)
+    assert torch.equal(st.write_rotated(q, K, V, inv, 0, far), st.write_rotated(q, K, V, inv, 0, near))
